@@ -45,6 +45,12 @@ extern "C" {
 #define MM_GPU_TF32 0   /* one TF32 pass: ~1e-3 relative error per product */
 #define MM_GPU_3XTF32 1 /* hi*hi + hi*lo + lo*hi: close to f32 accuracy */
 
+/* Activations of mm_gpu_linear_*. */
+#define MM_GPU_ACT_NONE 0
+#define MM_GPU_ACT_RELU 1 /* max(z, 0), slope 0 at 0 */
+#define MM_GPU_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
+#define MM_GPU_ACT_SILU 3 /* z / (1 + exp(-z)) */
+
 /* Message of the last failing call on this thread (NUL-terminated, static until
  * the next call). */
 MM_GPU_EXPORT const char *mm_gpu_last_error(void);
@@ -162,6 +168,74 @@ MM_GPU_EXPORT int32_t mm_gpu_embedding_backward(int32_t rows, const int32_t *ids
 MM_GPU_EXPORT int32_t mm_gpu_cross_entropy(int32_t rows, int32_t vocab, float *logits, int64_t ld,
                                            const int32_t *targets, float grad_scale, float *row_loss,
                                            double *mean_loss, void *stream);
+
+/* ---- Products with what follows them, dropout, and the loss over a vocabulary.
+ * The reference has no counterpart (its Linear has no bias, its model no dropout,
+ * and its loss takes whole logits). These calls allocate nothing and keep nothing
+ * between calls: temporaries live in `workspace` (device memory, 256-byte aligned,
+ * at least what the call's _workspace function returns for the same sizes; it may
+ * be reused as soon as the call's work on `stream` is done, and two calls that
+ * may run at the same time need two). After one earlier call of any entry point on
+ * the device they may be captured into a graph. Matrices have a row stride that is
+ * a multiple of 4 and start on 16-byte boundaries; widths are arbitrary, and
+ * columns past the width are neither read nor written. Outputs must not overlap
+ * inputs except where said. An infinite or NaN operand entry makes the outputs that
+ * depend on it NaN or infinite, no others.
+ *
+ * Dropout: element (i, j) of a [rows, cols] tensor is dropped where word j % 4 of
+ * the Philox4x32-10 block with counter (i * ceil(cols / 4) + j / 4, offset) and key
+ * seed is below floor(p * 2^32), and scaled by 1 / (1 - p) elsewhere. rng points
+ * to the two words {seed, offset} on the device, read when the kernel runs, so a
+ * captured graph draws anew when they change; it may be NULL when p is 0. The
+ * mask depends on rows, columns and the words alone (not on strides), so a
+ * backward with the same words meets the forward's mask. */
+
+/* y = r + dropout(x), over [rows, cols] with any row strides >= cols and any
+ * alignment; r may be NULL, y may be x or r. The gradient of x is the same call on
+ * dy (r NULL); that of r is dy. */
+MM_GPU_EXPORT int32_t mm_gpu_dropout(int64_t rows, int32_t cols, const float *x, int64_t ldx, const float *r,
+                                     int64_t ldr, float *y, int64_t ldy, double p, const uint64_t *rng, void *stream);
+
+/* z = A B (+ bias), c = r + dropout(activation(z)).
+ * A [m, k] row-major; B [k, n] (b_mn_major != 0) or its transpose [n, k] (0);
+ * bias [n] (any alignment) or NULL; r [m, n] or NULL, may be c; z [m, n] receives
+ * A B + bias for the backward, or NULL. m may be 0. */
+MM_GPU_EXPORT int64_t mm_gpu_linear_workspace(int32_t m, int32_t n, int32_t k, int32_t backward, int32_t precision);
+MM_GPU_EXPORT int32_t mm_gpu_linear_forward(int32_t m, int32_t n, int32_t k, const float *a, int64_t lda,
+                                            const float *b, int64_t ldb, int32_t b_mn_major, const float *bias,
+                                            int32_t activation, double p, const uint64_t *rng, const float *r,
+                                            int64_t ldr, float *z, int64_t ldz, float *c, int64_t ldc,
+                                            int32_t precision, void *workspace, int64_t workspace_bytes, void *stream);
+/* Its gradients from dc: dz = mask / (1 - p) * dc * activation'(z), da = dz B^T,
+ * db = A^T dz (in B's layout), dbias[j] = sum of column j of dz, summed in a fixed
+ * order. Each of da, db, dbias may be NULL (then what it alone needs may be NULL
+ * too); z may be NULL without an activation. accumulate != 0 adds to them instead of
+ * overwriting. r's gradient is dc itself. */
+MM_GPU_EXPORT int32_t mm_gpu_linear_backward(int32_t m, int32_t n, int32_t k, const float *a, int64_t lda,
+                                             const float *b, int64_t ldb, int32_t b_mn_major, int32_t activation,
+                                             double p, const uint64_t *rng, const float *z, int64_t ldz,
+                                             const float *dc, int64_t lddc, float *da, int64_t ldda, float *db,
+                                             int64_t lddb, float *dbias, int32_t accumulate, int32_t precision,
+                                             void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Softmax cross-entropy of the logits x W^T without storing them: x [rows, dim], W
+ * [vocab, dim] (w_mn_major 0, the tied embedding) or [dim, vocab] (1); targets on
+ * the device. row_loss[i] = ln(sum_j exp z_ij) - z_i,target. A row with target -1
+ * is left out: loss 0, dx 0, no share in dw, whatever its x holds. Another target
+ * outside [0, vocab) gives a NaN row loss, no gradient, and the device error flag.
+ * mean_loss (may be NULL): the mean over the rows not left out (0 when there are
+ * none), summed in f64. dx [rows, dim] and dw (W's layout) receive, where not NULL,
+ * the gradients of grad_scale * (sum of the row losses), added to what they hold
+ * when accumulate != 0. The workspace does not grow with rows * vocab: with
+ * gradients it holds the logits of as many rows as fit 256 MiB (256 rows at least). */
+MM_GPU_EXPORT int64_t mm_gpu_linear_cross_entropy_workspace(int32_t rows, int32_t vocab, int32_t dim,
+                                                            int32_t gradients, int32_t precision);
+MM_GPU_EXPORT int32_t mm_gpu_linear_cross_entropy(int32_t rows, int32_t vocab, int32_t dim, const float *x,
+                                                  int64_t ldx, const float *w, int64_t ldw, int32_t w_mn_major,
+                                                  const int32_t *targets, float grad_scale, float *row_loss,
+                                                  float *mean_loss, float *dx, int64_t lddx, float *dw, int64_t lddw,
+                                                  int32_t accumulate, int32_t precision, void *workspace,
+                                                  int64_t workspace_bytes, void *stream);
 
 /* Failure-path self-test of the bounded waits (no counterpart in the
  * reference): launches one thread that waits on a barrier nothing completes,

@@ -79,6 +79,24 @@ MM_GPU_EXPORT uint64_t mm_op_swiglu(uint32_t tape, uint64_t gate, uint64_t up);
  * tensor; the loss is summed in f64 (ops_reduce.rs:236-276). */
 MM_GPU_EXPORT uint64_t mm_op_cross_entropy(uint32_t tape, uint64_t logits, const int32_t *targets_host, int64_t rows);
 
+/* Operations the reference has no counterpart for (the kernels and the dropout
+ * mask are those of mm_gpu_dropout, mm_gpu_linear_* and
+ * mm_gpu_linear_cross_entropy, midman_gpu.h). */
+/* Dropout of x with probability p, the mask a function of (seed, offset) and the
+ * place in x seen as rows of its last dimension; give every use its own offset. */
+MM_GPU_EXPORT uint64_t mm_op_dropout(uint32_t tape, uint64_t x, double p, uint64_t seed, uint64_t offset);
+/* residual + dropout(activation(x w + bias)) in one kernel: x [m, k], w [k, n] (or
+ * [n, k] when w_transposed != 0), bias [n] or 0, residual [m, n] or 0, activation
+ * MM_GPU_ACT_*. p = 0 drops nothing. */
+MM_GPU_EXPORT uint64_t mm_op_linear(uint32_t tape, uint64_t x, uint64_t w, int32_t w_transposed, uint64_t bias,
+                                    int32_t activation, double p, uint64_t seed, uint64_t offset, uint64_t residual);
+/* Mean cross-entropy of x w (w [dim, classes], or [classes, dim] when w_transposed
+ * != 0, the tied head) against targets (HOST), a [1] tensor, without a tensor of
+ * logits: mm_op_matmul and mm_op_cross_entropy in one. Rows with target -1 are
+ * left out of the mean. */
+MM_GPU_EXPORT uint64_t mm_op_linear_cross_entropy(uint32_t tape, uint64_t x, uint64_t w, int32_t w_transposed,
+                                                  const int32_t *targets_host, int64_t rows);
+
 #ifdef __cplusplus
 }
 #endif

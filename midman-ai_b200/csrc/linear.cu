@@ -1,0 +1,700 @@
+// Products with an epilogue for sm_100a:
+//
+//   z = A B^T (+ bias),  c = r + dropout(act(z))         (LinearEpilogue)
+//   z = A B^T, per row and 128 columns max z and sum exp(z - max)  (LossEpilogue)
+//
+// Exact mode: A B = (Ah + Al)(Bh + Bl) ~ Al Bh + Ah Bl + Ah Bh, hi the bits the
+// tensor core reads of an f32 (11 significant bits), lo what they leave out
+// rounded to as many: the dropped Al Bl is 2^-22 of the product. The tensor
+// core's f32 accumulation loses a little on every UMMA, always in the same
+// direction, so every 64 of K start a fresh TMEM accumulation and the chunks are
+// summed in f32 registers.
+//
+// direct_kernel: one 128 x BN tile per cluster of `splits` CTAs, each CTA a part
+// of K. TMA brings the f32 operands; four converter warps write the lo part of
+// each stage beside it (elementwise, so the swizzled layout is kept), which
+// saves the passes and the workspace of copies made beforehand: what short
+// products are bound by is latency and one reading of the weights. The parts'
+// sums meet in shared memory over the cluster (each CTA sums 128 / splits rows
+// of all parts, in part order: bit-identical run to run) and go through the
+// epilogue in whole rows.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "device.h"
+#include "gemm.h"
+#include "linear.h"
+#include "ptx.cuh"
+#include "tma.h"
+
+namespace mm {
+namespace {
+
+constexpr int BM = 128;
+constexpr int BK = 32;  // 32 f32 = 128 bytes = one swizzle row
+constexpr uint32_t MN_BLOCK_BYTES = BK * 128;
+constexpr int kEpiWarps = 8;
+
+// ------------------------------------------------------------------ epilogues
+__device__ __forceinline__ float activate(float z, int act) {
+  switch (act) {
+    case kActRelu: return fmaxf(z, 0.0f);
+    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case kActSilu: return z / (1.0f + expf(-z));
+    default: return z;
+  }
+}
+
+// d act / dz
+__device__ __forceinline__ float activate_slope(float z, int act) {
+  switch (act) {
+    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+    case kActGelu:
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case kActSilu: {
+      const float s = 1.0f / (1.0f + expf(-z));
+      return s * (1.0f + z * (1.0f - s));
+    }
+    default: return 1.0f;
+  }
+}
+
+// Four columns of a row; those at n and past it are not touched.
+__device__ __forceinline__ float4 load_quad(const float* row, int col, int n) {
+  if (col + 3 < n) return *reinterpret_cast<const float4*>(row + col);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < n) v.x = row[col];
+  if (col + 1 < n) v.y = row[col + 1];
+  if (col + 2 < n) v.z = row[col + 2];
+  return v;
+}
+__device__ __forceinline__ void store_quad(float* row, int col, int n, float4 v) {
+  if (col + 3 < n) {
+    *reinterpret_cast<float4*>(row + col) = v;
+    return;
+  }
+  if (col < n) row[col] = v.x;
+  if (col + 1 < n) row[col + 1] = v.y;
+  if (col + 2 < n) row[col + 2] = v.z;
+}
+__device__ __forceinline__ float4 load_each(const float* row, int col, int n) {  // any alignment
+  return make_float4(col < n ? row[col] : 0.f, col + 1 < n ? row[col + 1] : 0.f, col + 2 < n ? row[col + 2] : 0.f,
+                     col + 3 < n ? row[col + 3] : 0.f);
+}
+__device__ __forceinline__ void store_each(float* row, int col, int n, float4 v) {
+  if (col < n) row[col] = v.x;
+  if (col + 1 < n) row[col + 1] = v.y;
+  if (col + 2 < n) row[col + 2] = v.z;
+  if (col + 3 < n) row[col + 3] = v.w;
+}
+// v: the product's four columns; r: the residual's (loaded by the caller before
+// anything of the batch is stored, so that r may be c).
+__device__ __forceinline__ void linear_quad(const LinearEpilogue& e, uint64_t seed, uint64_t offset, long long row,
+                                            int col, int n, float4 v, float4 r) {
+  if (e.bias) {
+    const float4 b = load_each(e.bias, col, n);
+    v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
+  }
+  if (e.Z) store_quad(e.Z + row * e.ldz, col, n, v);
+  if (e.act != kActNone) {
+    v.x = activate(v.x, e.act); v.y = activate(v.y, e.act); v.z = activate(v.z, e.act); v.w = activate(v.w, e.act);
+  }
+  if (e.drop.rng) v = dropout_quad(v, e.drop, seed, offset, row, col >> 2);
+  v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
+  store_quad(e.C + row * e.ldc, col, n, v);
+}
+
+__device__ __forceinline__ float quad_max(float4 v, int col, int n) {  // col < n
+  float m = v.x;
+  if (col + 1 < n) m = fmaxf(m, v.y);
+  if (col + 2 < n) m = fmaxf(m, v.z);
+  if (col + 3 < n) m = fmaxf(m, v.w);
+  return m;
+}
+
+// ------------------------------------------------------------------ direct kernel
+template <int TERMS, int BN>
+struct DirectTile {
+  static constexpr int A_BYTES = BM * BK * 4;
+  static constexpr int HI_BYTES = A_BYTES + BN * BK * 4;  // A, then B
+  static constexpr int STAGE = TERMS == 3 ? 2 * HI_BYTES : HI_BYTES;  // then their lo parts
+  static constexpr int STAGES = 196608 / STAGE > 8 ? 8 : 196608 / STAGE;
+  static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
+  static constexpr int CONVERTERS = TERMS == 3 ? 4 : 0;
+  static constexpr int THREADS = 32 * (2 + kEpiWarps + CONVERTERS);
+  static constexpr int CHUNK = TERMS == 3 ? 2 : 32;  // K steps per TMEM accumulation (24 or 128 UMMAs)
+  static_assert(BM * BN * 4 <= STAGES * STAGE, "the partial tile reuses the stages");
+};
+
+__device__ __forceinline__ float4 ld_cluster_quad(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float lo_part(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x - __uint_as_float(__float_as_uint(x) & 0xffffe000u)));
+  return __uint_as_float(r);
+}
+
+// Tiles in groups of 8 row blocks, the row block fastest inside a group: the
+// tiles at work at one time then share rows of A and columns of B in L2.
+__device__ __forceinline__ void tile_mn(int t, int tm, int tn, int& mt, int& nt) {
+  const int per_group = 8 * tn;
+  const int g = t / per_group, r = t - g * per_group;
+  const int rows = min(8, tm - g * 8);
+  mt = g * 8 + r % rows;
+  nt = r / rows;
+}
+
+template <int TERMS, bool A_MN, bool B_MN, int BN, class Epi>
+__global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
+    direct_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Epi epi,
+                  int M, int N, int K, int splits, int mn3d, int* err) {
+  using TL = DirectTile<TERMS, BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw_addr);
+  const uint32_t bar_base = base + TL::STAGES * TL::STAGE;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (TL::STAGES + s); };
+  auto lo_bar = [&](int s) { return bar_base + 8u * (2 * TL::STAGES + s); };
+  auto acc_full = [&](int b) { return bar_base + 8u * (3 * TL::STAGES + b); };
+  auto acc_empty = [&](int b) { return bar_base + 8u * (3 * TL::STAGES + 2 + b); };
+  constexpr int kBars = 3 * TL::STAGES + 4;
+  static_assert(8 * kBars + 16 <= 256, "barriers and counters fit their 256 bytes");
+  uint8_t* tail = smem + TL::STAGES * TL::STAGE + 8 * kBars;
+  const uint32_t tmem_slot = bar_base + 8u * kBars;
+  int* loads_issued = reinterpret_cast<int*>(tail + 8);
+  int* loads_consumed = loads_issued + 1;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int part = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
+  int mt, nt;
+  tile_mn(static_cast<int>(blockIdx.x) / splits, tm, tn, mt, nt);
+  const int m0 = mt * BM, n0 = nt * BN;
+  const int n_k = (K + BK - 1) / BK;
+  const int kb = static_cast<int>(static_cast<long long>(n_k) * part / splits);
+  const int ke = static_cast<int>(static_cast<long long>(n_k) * (part + 1) / splits);
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    for (int s = 0; s < TL::STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+      mbar_init(lo_bar(s), TERMS == 3 ? TL::CONVERTERS : 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), kEpiWarps);
+    }
+    *loads_issued = 0;
+    *loads_consumed = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 2 * BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer
+      for (int i = kb; i < ke; ++i) {
+        const int it = i - kb, s = it % TL::STAGES, round = it / TL::STAGES;
+        if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, err, kErrWaitEmpty)) break;
+        const uint32_t sa = base + s * TL::STAGE, sb = sa + TL::A_BYTES;
+        mbar_arrive_expect_tx(full_bar(s), TL::HI_BYTES);
+        const int k0 = i * BK;
+        if (!A_MN) {
+          tma_load_2d(sa, &tmA, full_bar(s), k0, m0);
+        } else if (mn3d & 1) {
+          tma_load_3d(sa, &tmA, full_bar(s), 0, k0, m0 / 32);
+        } else {
+#pragma unroll
+          for (int j = 0; j < BM / 32; ++j) tma_load_2d(sa + j * MN_BLOCK_BYTES, &tmA, full_bar(s), m0 + 32 * j, k0);
+        }
+        if (!B_MN) {
+          tma_load_2d(sb, &tmB, full_bar(s), k0, n0);
+        } else if (mn3d & 2) {
+          tma_load_3d(sb, &tmB, full_bar(s), 0, k0, n0 / 32);
+        } else {
+#pragma unroll
+          for (int j = 0; j < BN / 32; ++j) tma_load_2d(sb + j * MN_BLOCK_BYTES, &tmB, full_bar(s), n0 + 32 * j, k0);
+        }
+        *loads_issued = it + 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---------------- UMMA issuer
+      constexpr uint32_t idesc = idesc_tf32(BM, BN, A_MN, B_MN);
+      int j = 0;
+      bool ok = true;
+      for (int cb = kb; cb < ke && ok; cb += TL::CHUNK, ++j) {
+        const int ce = min(ke, cb + TL::CHUNK), buf = j & 1;
+        if (j >= 2 && !mbar_wait(acc_empty(buf), ((j >> 1) - 1) & 1, err, kErrWaitAccum)) break;
+        tc_fence_after();
+        const uint32_t acc = tmem_base + buf * BN;
+        for (int i = cb; i < ce; ++i) {
+          const int it = i - kb, s = it % TL::STAGES, round = it / TL::STAGES;
+          if (!mbar_wait(full_bar(s), round & 1, err, kErrWaitFull) ||
+              (TERMS == 3 && !mbar_wait(lo_bar(s), round & 1, err, kErrWaitFull))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          *loads_consumed = it + 1;
+          const uint32_t sa = base + s * TL::STAGE, sb = sa + TL::A_BYTES;
+          // the terms, small ones first: Al Bh, Ah Bl, Ah Bh (or Ah Bh alone)
+#pragma unroll
+          for (int term = 0; term < TERMS; ++term) {
+            const uint32_t at = sa + (TERMS == 3 && term == 0 ? TL::HI_BYTES : 0);
+            const uint32_t bt = sb + (TERMS == 3 && term == 1 ? TL::HI_BYTES : 0);
+#pragma unroll
+            for (int k = 0; k < BK / 8; ++k) {
+              const uint64_t adesc = A_MN ? smem_desc(at + k * 1024, MN_BLOCK_BYTES, 512, kLayoutSw128Base32)
+                                          : smem_desc(at + k * 32, 16, 1024, kLayoutSw128);
+              const uint64_t bdesc = B_MN ? smem_desc(bt + k * 1024, MN_BLOCK_BYTES, 512, kLayoutSw128Base32)
+                                          : smem_desc(bt + k * 32, 16, 1024, kLayoutSw128);
+              umma_tf32(acc, adesc, bdesc, idesc, (i != cb || term != 0 || k != 0) ? 1u : 0u);
+            }
+          }
+          umma_commit(empty_bar(s));
+        }
+        if (ok) umma_commit(acc_full(buf));
+      }
+    }
+  } else if (warp < 2 + kEpiWarps) {
+    // ---------------- chunk sums: 32 rows x BN / 2 columns per warp, then the partial tile
+    constexpr int NC = BN / 2;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    float sum[NC];
+#pragma unroll
+    for (int e = 0; e < NC; ++e) sum[e] = 0.0f;
+    int j = 0;
+    bool ok = true;
+    for (int cb = kb; cb < ke; cb += TL::CHUNK, ++j) {
+      const int buf = j & 1;
+      if (!mbar_wait(acc_full(buf), (j >> 1) & 1, err, kErrWaitAccum)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t acc = tmem_base + buf * BN + (static_cast<uint32_t>(quarter * 32) << 16) + half * NC;
+#pragma unroll
+      for (int c = 0; c < NC / 16; ++c) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(acc + c * 16, r);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[c * 16 + e] += __uint_as_float(r[e]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(buf));
+    }
+    if (ok) {
+      // Every UMMA of the tile is done, so every stage has landed and been read:
+      // the partial tile takes their place, row r's quad q at r BN/4 + (q ^ (r & 7))
+      // (eight rows of one quad lie in different banks).
+      float4* tile = reinterpret_cast<float4*>(smem);
+      const int row = quarter * 32 + lane;
+#pragma unroll
+      for (int q = 0; q < NC / 4; ++q)
+        tile[row * (BN / 4) + ((half * (NC / 4) + q) ^ (row & 7))] =
+            make_float4(sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]);
+    }
+  } else if (TERMS == 3) {
+    // ---------------- converters: the lo part of every stage, in the stage's own layout
+    for (int i = kb; i < ke; ++i) {
+      const int it = i - kb, s = it % TL::STAGES, round = it / TL::STAGES;
+      if (!mbar_wait(full_bar(s), round & 1, err, kErrWaitFull)) break;
+      const float4* hi = reinterpret_cast<const float4*>(smem + s * TL::STAGE);
+      float4* lo = reinterpret_cast<float4*>(smem + s * TL::STAGE + TL::HI_BYTES);
+      const int t = threadIdx.x - 32 * (2 + kEpiWarps);
+#pragma unroll 8
+      for (int e = t; e < TL::HI_BYTES / 16; e += 32 * TL::CONVERTERS) {
+        const float4 v = hi[e];
+        lo[e] = make_float4(lo_part(v.x), lo_part(v.y), lo_part(v.z), lo_part(v.w));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(lo_bar(s));
+    }
+  }
+
+  // ---------------- the parts' sums and the epilogue, 128 / splits rows per CTA
+  tc_fence_before();
+  if (splits > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  epi.template rows<BN>(base, m0, n0, part * (BM / splits), BM / splits, splits, M, N, warp, lane,
+                        TL::THREADS / 32);
+  if (splits > 1)
+    cluster_sync();  // a peer may still be reading this CTA's part
+  else
+    __syncthreads();
+  if (threadIdx.x == 0) {
+    // only after a timed-out wait can a stage still be in flight: let it land (bounded)
+    for (int i = *loads_consumed; i < *loads_issued; ++i)
+      if (!mbar_wait(full_bar(i % TL::STAGES), (i / TL::STAGES) & 1, err, kErrWaitDrain, 1000000000ull)) break;
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * BN);
+  }
+  __syncthreads();
+}
+
+// The sum over the cluster's parts, in part order, of quad q of tile row r.
+template <int BN>
+__device__ __forceinline__ float4 sum_quad(uint32_t tile, int r, int q, int splits) {
+  const uint32_t at = tile + 16u * static_cast<uint32_t>(r * (BN / 4) + (q ^ (r & 7)));
+  if (splits == 1) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at)
+                 : "memory");
+    return v;
+  }
+  float4 v = ld_cluster_quad(mapa_shared(at, 0));
+  for (int p = 1; p < splits; ++p) {
+    const float4 w = ld_cluster_quad(mapa_shared(at, p));
+    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+  }
+  return v;
+}
+
+struct LinearDirect {
+  LinearEpilogue e;
+  // Rows [r0, r0 + nr) of the tile; BN / 4 lanes per row, four rows of a lane at
+  // a time so that their residual loads are in flight together.
+  template <int BN>
+  __device__ __forceinline__ void rows(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
+                                       int warp, int lane, int warps) const {
+    constexpr int PER = 128 / BN;  // rows a warp covers at once
+    const int q = lane % (BN / 4), col = n0 + 4 * q;
+    uint64_t seed = 0, offset = 0;
+    if (e.drop.rng) {
+      seed = e.drop.rng[0];
+      offset = e.drop.rng[1];
+    }
+    constexpr int U = 4;
+    for (int i = warp * PER + lane / (BN / 4); i < nr; i += U * warps * PER) {
+      float4 v[U], r[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = i + u * warps * PER;
+        const long long row = m0 + r0 + j;
+        const bool live = j < nr && row < M && col < N;
+        v[u] = live ? sum_quad<BN>(tile, r0 + j, q, splits) : make_float4(0.f, 0.f, 0.f, 0.f);
+        r[u] = live && e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = i + u * warps * PER;
+        const long long row = m0 + r0 + j;
+        if (j < nr && row < M && col < N) linear_quad(e, seed, offset, row, col, N, v[u], r[u]);
+      }
+    }
+  }
+};
+
+struct LossDirect {
+  LossEpilogue e;
+  // A warp per row: its 128 columns' maximum and sum by shuffles.
+  template <int BN>
+  __device__ __forceinline__ void rows(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
+                                       int warp, int lane, int warps) const {
+    static_assert(BN == 128, "one partial per 128 columns");
+    const int col = n0 + 4 * lane;
+    for (int i = warp; i < nr; i += warps) {
+      const long long row = m0 + r0 + i;
+      if (row >= M) break;  // uniform over the warp
+      const float4 v = sum_quad<BN>(tile, r0 + i, lane, splits);
+      float m = col < N ? quad_max(v, col, N) : -INFINITY;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float s = 0.0f;
+      if (col < N) s += expf(v.x - m);
+      if (col + 1 < N) s += expf(v.y - m);
+      if (col + 2 < N) s += expf(v.z - m);
+      if (col + 3 < N) s += expf(v.w - m);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) e.part[row * e.tiles + n0 / 128] = make_float2(m, s);
+      const int t = e.targets[row] - col;
+      if (t >= 0 && t < 4 && col + t < N) e.zt[row] = t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w;
+      if (e.Z && col < N) store_quad(e.Z + row * e.ldz, col, N, v);
+    }
+  }
+};
+
+// ------------------------------------------------------------------ backward of the epilogue
+// dz and the column sums' partials: 64 rows x 128 columns per block, a warp per
+// row, so every access covers 512 contiguous bytes. Bound by HBM: 4 (dc) + 4 (z)
+// + 4 (dz) bytes an element.
+constexpr int kActRows = 64;
+
+__global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long long lddc, const float* z,
+                                                           long long ldz, int act, DropoutArgs drop, int rows,
+                                                           int cols, float* dz, long long lddz, float* part) {
+  __shared__ float4 sums[8][32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int col = (blockIdx.x * 32 + lane) * 4;
+  const int row0 = blockIdx.y * kActRows;
+  uint64_t seed = 0, offset = 0;
+  if (drop.rng) {
+    seed = drop.rng[0];
+    offset = drop.rng[1];
+  }
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < cols) {
+#pragma unroll 4
+    for (int i = warp; i < kActRows; i += 8) {
+      const long long row = row0 + i;
+      if (row >= rows) break;
+      float4 g = load_quad(dc + row * lddc, col, cols);
+      if (drop.rng) g = dropout_quad(g, drop, seed, offset, row, col >> 2);
+      if (act != kActNone) {
+        const float4 v = load_quad(z + row * ldz, col, cols);
+        g.x *= activate_slope(v.x, act); g.y *= activate_slope(v.y, act);
+        g.z *= activate_slope(v.z, act); g.w *= activate_slope(v.w, act);
+      }
+      if (dz) store_quad(dz + row * lddz, col, cols, g);
+      sum.x += g.x; sum.y += g.y; sum.z += g.z; sum.w += g.w;
+    }
+  }
+  if (!part) return;  // uniform
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && col < cols) {
+    for (int w = 1; w < 8; ++w) {
+      const float4 o = sums[w][lane];
+      sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
+    }
+    float* p = part + static_cast<long long>(blockIdx.y) * cols;  // rows of `cols`: any alignment
+    p[col] = sum.x;
+    if (col + 1 < cols) p[col + 1] = sum.y;
+    if (col + 2 < cols) p[col + 2] = sum.z;
+    if (col + 3 < cols) p[col + 3] = sum.w;
+  }
+}
+
+// 32 columns per block, eight rows of partials at a time, joined in a fixed order.
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int parts, int cols, float* out,
+                                                        int accumulate) {
+  __shared__ double sums[8][32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, col = blockIdx.x * 32 + lane;
+  double s = 0.0;
+  if (col < cols)
+    for (int p = warp; p < parts; p += 8) s += part[static_cast<long long>(p) * cols + col];
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && col < cols) {
+    for (int w = 1; w < 8; ++w) s += sums[w][lane];
+    out[col] = static_cast<float>(accumulate ? out[col] + s : s);
+  }
+}
+
+// ------------------------------------------------------------------ dropout
+// y = r + dropout(x): a thread per quad, bound by HBM (8 bytes an element, 12
+// with r): the ten rounds cost about 70 integer instructions for four elements.
+__global__ void __launch_bounds__(256) dropout_kernel(const float* x, long long ldx, const float* r, long long ldr,
+                                                      float* y, long long ldy, long long quads, int cols,
+                                                      DropoutArgs drop, int vec) {
+  const uint64_t seed = drop.rng ? drop.rng[0] : 0, offset = drop.rng ? drop.rng[1] : 0;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < quads; i += gridDim.x * 256ll) {
+    const long long row = i / drop.blocks;
+    const int quad = static_cast<int>(i - row * drop.blocks), col = 4 * quad;
+    const float* xp = x + row * ldx;
+    const float* rp = r ? r + row * ldr : nullptr;
+    float* yp = y + row * ldy;
+    float4 v = vec ? load_quad(xp, col, cols) : load_each(xp, col, cols);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (rp) a = vec ? load_quad(rp, col, cols) : load_each(rp, col, cols);
+    if (drop.rng) v = dropout_quad(v, drop, seed, offset, row, quad);
+    v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+    if (vec)
+      store_quad(yp, col, cols, v);
+    else
+      store_each(yp, col, cols, v);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// The operand's tensor map: `mn` rows (or columns) of the product, `box` of them
+// per tile. MN-major operands of a width that is a multiple of 32 load a stage in
+// one 3-D box (32 wide, BK rows, box / 32 blocks), others in 32-wide 2-D boxes.
+int operand_map(CUtensorMap* map, const GemmOperand& o, int mn, int k, int box, bool* box3d) {
+  if ((o.ld & 3) || !aligned16(o.ptr)) return kGemmMisaligned;
+  *box3d = false;
+  int rc;
+  if (!o.mn_major) {
+    const long long dims[2] = {k, mn}, strides[1] = {o.ld};
+    const int b[2] = {BK, box};
+    rc = encode_tensor_map(map, o.ptr, 2, dims, strides, b, false);
+  } else if (mn % 32 == 0) {
+    const long long dims[3] = {32, k, mn / 32}, strides[2] = {o.ld, 32};
+    const int b[3] = {32, BK, box / 32};
+    *box3d = true;
+    rc = encode_tensor_map(map, o.ptr, 3, dims, strides, b, true);
+  } else {
+    const long long dims[2] = {mn, k}, strides[1] = {o.ld};
+    const int b[2] = {32, BK};
+    rc = encode_tensor_map(map, o.ptr, 2, dims, strides, b, true);
+  }
+  return rc ? kGemmTensorMap : 0;
+}
+
+// How a product is cut: 128 x 64 tiles when even with K in eight parts the wider
+// ones would leave half of the SMs idle, and K in as many parts (a cluster's
+// CTAs) as fit the SMs beside one another, each at least four K steps.
+struct DirectPlan {
+  int bn, splits;
+};
+DirectPlan direct_plan(int M, int N, int K, bool any_bn) {
+  const int sms = 148, n_k = (K + BK - 1) / BK;
+  const long long tm = (M + BM - 1) / BM;
+  DirectPlan p{128, 1};
+  auto splits_of = [&](long long tiles) {
+    int s = 1;
+    while (s < 8 && tiles * s * 2 <= sms && n_k / (2 * s) >= 4) s *= 2;
+    return s;
+  };
+  const long long t128 = tm * ((N + 127) / 128), t64 = tm * ((N + 63) / 64);
+  if (any_bn && (N <= 64 || 2 * t128 * splits_of(t128) <= sms)) p.bn = 64;
+  p.splits = splits_of(p.bn == 128 ? t128 : t64);
+  return p;
+}
+
+template <int TERMS, bool A_MN, bool B_MN, int BN, class Epi>
+int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, int splits,
+                  int* d_err, cudaStream_t s) {
+  using TL = DirectTile<TERMS, BN>;
+  CUtensorMap ta{}, tb{};
+  bool a3 = false, b3 = false;
+  int rc = operand_map(&ta, A, M, K, BM, &a3);
+  if (!rc) rc = operand_map(&tb, B, N, K, BN, &b3);
+  if (rc) return rc;
+  auto kern = direct_kernel<TERMS, A_MN, B_MN, BN, Epi>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (configured_device != dev) {
+    check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TL::SMEM), "shared memory");
+    configured_device = dev;
+  }
+  const long long tiles = static_cast<long long>((M + BM - 1) / BM) * ((N + BN - 1) / BN);
+  if (tiles * splits > 0x7fffffffll) return kGemmBadArgument;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(splits);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+  cfg.blockDim = dim3(TL::THREADS);
+  cfg.dynamicSmemBytes = TL::SMEM;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kern, ta, tb, epi, M, N, K, splits, (a3 ? 1 : 0) | (b3 ? 2 : 0), d_err),
+             "linear");
+  return 0;
+}
+
+template <int TERMS, int BN, class Epi>
+int direct_majors(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, int splits,
+                  int* d_err, cudaStream_t s) {
+  if (!A.mn_major && !B.mn_major) return launch_direct<TERMS, false, false, BN>(M, N, K, A, B, epi, splits, d_err, s);
+  if (!A.mn_major) return launch_direct<TERMS, false, true, BN>(M, N, K, A, B, epi, splits, d_err, s);
+  if (B.mn_major) return launch_direct<TERMS, true, true, BN>(M, N, K, A, B, epi, splits, d_err, s);
+  return kGemmBadArgument;  // no caller has an MN-major A with a K-major B
+}
+
+}  // namespace
+
+DropoutArgs dropout_args(double p, const uint64_t* rng, int cols) {
+  DropoutArgs d;
+  d.blocks = static_cast<uint32_t>((static_cast<long long>(cols) + 3) / 4);
+  if (p > 0.0) {
+    d.rng = rng;
+    d.threshold = static_cast<uint32_t>(p * 4294967296.0);
+    d.scale = static_cast<float>(1.0 / (1.0 - p));
+  }
+  return d;
+}
+
+int linear_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, int* d_err,
+                   cudaStream_t s) {
+  if (M <= 0 || N <= 0) return 0;
+  const DirectPlan p = direct_plan(M, N, K, true);
+  const LinearDirect epi{e};
+  if (exact)
+    return p.bn == 128 ? direct_majors<3, 128>(M, N, K, A, B, epi, p.splits, d_err, s)
+                       : direct_majors<3, 64>(M, N, K, A, B, epi, p.splits, d_err, s);
+  return p.bn == 128 ? direct_majors<1, 128>(M, N, K, A, B, epi, p.splits, d_err, s)
+                     : direct_majors<1, 64>(M, N, K, A, B, epi, p.splits, d_err, s);
+}
+
+int loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
+                 cudaStream_t s) {
+  if (M <= 0 || N <= 0) return 0;
+  if (A.mn_major) return kGemmBadArgument;
+  const DirectPlan p = direct_plan(M, N, K, false);
+  const LossDirect epi{e};
+  if (exact)
+    return B.mn_major ? launch_direct<3, false, true, 128>(M, N, K, A, B, epi, p.splits, d_err, s)
+                      : launch_direct<3, false, false, 128>(M, N, K, A, B, epi, p.splits, d_err, s);
+  return B.mn_major ? launch_direct<1, false, true, 128>(M, N, K, A, B, epi, p.splits, d_err, s)
+                    : launch_direct<1, false, false, 128>(M, N, K, A, B, epi, p.splits, d_err, s);
+}
+
+int act_backward_parts(int rows) { return (rows + kActRows - 1) / kActRows; }
+
+void act_backward(const float* dc, long long lddc, const float* z, long long ldz, int act, const DropoutArgs& d,
+                  int rows, int cols, float* dz, long long lddz, float* part, cudaStream_t s) {
+  if (rows <= 0 || cols <= 0) return;
+  const dim3 grid((cols + 127) / 128, act_backward_parts(rows));
+  act_backward_kernel<<<grid, 256, 0, s>>>(dc, lddc, z, ldz, act, d, rows, cols, dz, lddz, part);
+  check_cuda(cudaGetLastError(), "linear backward");
+}
+
+void sum_parts(const float* part, int parts, int cols, float* out, bool accumulate, cudaStream_t s) {
+  if (cols <= 0) return;
+  sum_parts_kernel<<<(cols + 31) / 32, 256, 0, s>>>(part, parts, cols, out, accumulate ? 1 : 0);
+  check_cuda(cudaGetLastError(), "bias gradient");
+}
+
+void dropout(const float* x, long long ldx, const float* r, long long ldr, float* y, long long ldy, long long rows,
+             int cols, const DropoutArgs& d, cudaStream_t s) {
+  const long long quads = rows * d.blocks;
+  if (quads <= 0) return;
+  const bool vec = !((ldx | ldy | (r ? ldr : 0)) & 3) && aligned16(x) && aligned16(y) && (!r || aligned16(r));
+  const long long blocks = (quads + 255) / 256;
+  dropout_kernel<<<static_cast<int>(std::min(blocks, 148ll * 32)), 256, 0, s>>>(x, ldx, r, ldr, y, ldy, quads, cols, d,
+                                                                               vec ? 1 : 0);
+  check_cuda(cudaGetLastError(), "dropout");
+}
+
+}  // namespace mm

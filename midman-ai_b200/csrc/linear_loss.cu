@@ -1,0 +1,264 @@
+// Softmax cross-entropy of z = x w^T over a vocabulary, without the [rows, vocab]
+// logits: loss_i = lse_i - z_i,t, and on request dx = G w, dw = G^T x with
+// G = grad_scale (softmax(z) - onehot(t)). Rows with target -1 are left out: loss
+// 0, dx 0, no share in dw whatever their x holds.
+//
+// The loss alone: the product's epilogue reduces each row's 128 columns to their
+// maximum and sum of exponentials, so the logits never leave the chip; a warp per
+// row joins the vocab / 128 pairs. With gradients the rows go in blocks whose
+// logits fit a fixed part of the workspace: the product (6 N V D operations in
+// all, as with the logits kept; pieces of the vocabulary would have to form each
+// logit twice, 8 N V D), then z -> G in place, dx = G w, dw += G^T x.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "device.h"
+#include "linear.h"
+#include "ptx.cuh"
+
+namespace mm {
+namespace {
+
+constexpr long long kLogitBytes = 256ll << 20;  // a block's logits
+constexpr long long kPartBytes = 64ll << 20;    // a block's (max, sum) pairs, the loss alone
+
+long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
+
+struct Plan {
+  int tiles, rows;  // (max, sum) pairs per row; rows of a block
+  long long ldz, ldx;
+  long long part, zt, z, x, total;  // byte offsets into the workspace
+};
+
+Plan plan_of(int rows, int vocab, int dim, bool grad) {
+  Plan p{};
+  p.tiles = (vocab + 127) / 128;
+  p.ldz = round_up(vocab, 4);
+  p.ldx = round_up(dim, 4);
+  long long r = grad ? kLogitBytes / (p.ldz * 4) : kPartBytes / (p.tiles * 8ll);
+  r = std::max(256ll, r / 256 * 256);  // whole tiles of rows
+  p.rows = static_cast<int>(std::min<long long>(r, std::max(rows, 1)));
+  long long at = 0;
+  auto take = [&](long long bytes) {
+    const long long here = at;
+    at += round_up(bytes, 256);
+    return here;
+  };
+  p.part = take(static_cast<long long>(p.rows) * p.tiles * 8);
+  p.zt = take(p.rows * 4ll);
+  if (grad) {
+    p.z = take(p.rows * p.ldz * 4);
+    p.x = take(p.rows * p.ldx * 4);
+  }
+  p.total = at;
+  return p;
+}
+
+struct MaxSum {
+  float m, s;
+};
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
+  const float m = fmaxf(a.m, b.m);
+  if (m == -INFINITY) return {m, a.s + b.s};  // both empty (sums 0), or NaN logits: the NaN stays
+  return {m, a.s * expf(a.m - m) + b.s * expf(b.m - m)};
+}
+__device__ __forceinline__ MaxSum warp_join(MaxSum a) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+  return a;
+}
+
+// The row's loss; a target that is neither -1 nor a class sets the error flag.
+__device__ __forceinline__ float loss_of(MaxSum a, int t, int vocab, const float* zt, int* err) {
+  if (t >= 0 && t < vocab) return a.m + logf(a.s) - *zt;
+  if (t == -1) return 0.0f;
+  if (err) atomicCAS(err, 0, kErrIndex);
+  return NAN;
+}
+
+__global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int tiles, const float* zt,
+                                                       const int32_t* targets, int rows, int vocab, float* row_loss,
+                                                       int* err) {
+  const int r = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (r >= rows) return;
+  MaxSum a{-INFINITY, 0.0f};
+  for (int i = lane; i < tiles; i += 32) {
+    const float2 p = part[static_cast<long long>(r) * tiles + i];
+    a = join(a, {p.x, p.y});
+  }
+  a = warp_join(a);
+  if (lane == 0) row_loss[r] = loss_of(a, targets[r], vocab, zt + r, err);
+}
+
+// One row's kSegment logits -> gradients, in place; every block of a row joins
+// the row's pairs itself (vocab / 128 of them, from L2), the first writes the loss.
+constexpr int kSegment = 8192;
+
+__global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz, const float2* part, int tiles,
+                                                        const float* zt, const int32_t* targets, int vocab,
+                                                        float grad_scale, float* row_loss, int* err) {
+  __shared__ MaxSum warps[8];
+  const int r = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int t = targets[r];
+  const bool live = t >= 0 && t < vocab;
+  MaxSum a{-INFINITY, 0.0f};
+  for (int i = threadIdx.x; i < tiles; i += 256) {
+    const float2 p = part[static_cast<long long>(r) * tiles + i];
+    a = join(a, {p.x, p.y});
+  }
+  a = warp_join(a);
+  if (lane == 0) warps[warp] = a;
+  __syncthreads();
+  a = warps[0];
+  for (int w = 1; w < 8; ++w) a = join(a, warps[w]);
+  if (blockIdx.y == 0 && threadIdx.x == 0) row_loss[r] = loss_of(a, t, vocab, zt + r, err);
+  const float coef = grad_scale / a.s;
+  float4* row = reinterpret_cast<float4*>(z + r * ldz);
+  const int q_end = static_cast<int>(ldz / 4), q0 = blockIdx.y * (kSegment / 4);
+  for (int q = q0 + threadIdx.x; q < min(q_end, q0 + kSegment / 4); q += 256) {
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+      const float4 v = row[q];
+      g = make_float4(expf(v.x - a.m) * coef, expf(v.y - a.m) * coef, expf(v.z - a.m) * coef, expf(v.w - a.m) * coef);
+      if ((t >> 2) == q) {
+        if ((t & 3) == 0) g.x -= grad_scale;
+        if ((t & 3) == 1) g.y -= grad_scale;
+        if ((t & 3) == 2) g.z -= grad_scale;
+        if ((t & 3) == 3) g.w -= grad_scale;
+      }
+    }
+    row[q] = g;
+  }
+}
+
+// x with the rows that have no target as zeros: dw sums over all rows, and 0 times
+// what such a row holds may be NaN. A warp per row.
+__global__ void __launch_bounds__(256) live_rows_kernel(const float* x, long long ldx, const int32_t* targets,
+                                                        int rows, int dim, int vocab, float* out, long long ldo) {
+  const int r = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (r >= rows) return;
+  const int t = targets[r];
+  const bool live = t >= 0 && t < vocab;
+  const float* src = x + r * ldx;
+  float* dst = out + r * ldo;
+  for (int c = 4 * lane; c < dim; c += 128) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+      if (c + 3 < dim) {
+        v = *reinterpret_cast<const float4*>(src + c);
+      } else {
+        v.x = src[c];
+        if (c + 1 < dim) v.y = src[c + 1];
+        if (c + 2 < dim) v.z = src[c + 2];
+      }
+    }
+    *reinterpret_cast<float4*>(dst + c) = v;  // ldo is dim rounded up to 4
+  }
+}
+
+// The mean over the rows that have a target (0 when none has), in f64.
+__global__ void __launch_bounds__(1024) mean_live_kernel(const float* row_loss, const int32_t* targets, int rows,
+                                                         float* mean) {
+  __shared__ double sums[32];
+  __shared__ int counts[32];
+  double s = 0.0;
+  int n = 0;
+  for (int r = threadIdx.x; r < rows; r += 1024)
+    if (targets[r] != -1) {
+      s += row_loss[r];
+      ++n;
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if (threadIdx.x % 32 == 0) {
+    sums[threadIdx.x / 32] = s;
+    counts[threadIdx.x / 32] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) {
+      s += sums[w];
+      n += counts[w];
+    }
+    *mean = static_cast<float>(n ? s / n : 0.0);
+  }
+}
+
+}  // namespace
+
+long long linear_loss_ws_bytes(int rows, int vocab, int dim, bool grad, bool exact) {
+  (void)exact;
+  return plan_of(rows, vocab, dim, grad).total;
+}
+
+int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
+  const bool grad = a.dx || a.dw;
+  const Plan p = plan_of(a.rows, a.vocab, a.dim, grad);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  float2* part = reinterpret_cast<float2*>(base + p.part);
+  float* zt = reinterpret_cast<float*>(base + p.zt);
+  float* z = grad ? reinterpret_cast<float*>(base + p.z) : nullptr;
+  float* xl = grad ? reinterpret_cast<float*>(base + p.x) : nullptr;
+  for (int r0 = 0; r0 < a.rows; r0 += p.rows) {
+    const int n = std::min(p.rows, a.rows - r0);
+    const float* x = a.x + r0 * a.ldx;
+    const int32_t* t = a.targets + r0;
+    LossEpilogue e;
+    e.Z = z;
+    e.ldz = p.ldz;
+    e.part = part;
+    e.tiles = p.tiles;
+    e.targets = t;
+    e.zt = zt;
+    int rc = loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
+    if (rc) return rc;
+    if (!grad) {
+      row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(part, p.tiles, zt, t, n, a.vocab, a.row_loss + r0, d_err);
+      check_cuda(cudaGetLastError(), "row loss");
+      continue;
+    }
+    const dim3 grid(n, static_cast<unsigned>((p.ldz + kSegment - 1) / kSegment));
+    loss_grad_kernel<<<grid, 256, 0, s>>>(z, p.ldz, part, p.tiles, zt, t, a.vocab, a.grad_scale, a.row_loss + r0,
+                                          d_err);
+    check_cuda(cudaGetLastError(), "loss gradient");
+    if (a.dx) {
+      LinearEpilogue o;
+      o.C = a.dx + r0 * a.lddx;
+      o.ldc = a.lddx;
+      if (a.accumulate) {
+        o.R = o.C;
+        o.ldr = a.lddx;
+      }
+      rc = linear_product(n, a.dim, a.vocab, {z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, d_err, s);
+      if (rc) return rc;
+    }
+    if (a.dw) {
+      live_rows_kernel<<<(n + 7) / 8, 256, 0, s>>>(x, a.ldx, t, n, a.dim, a.vocab, xl, p.ldx);
+      check_cuda(cudaGetLastError(), "live rows");
+      LinearEpilogue o;
+      o.C = a.dw;
+      o.ldc = a.lddw;
+      if (a.accumulate || r0 > 0) {
+        o.R = a.dw;
+        o.ldr = a.lddw;
+      }
+      const GemmOperand g{z, p.ldz, true}, xo{xl, p.ldx, true};
+      rc = a.w_mn_major ? linear_product(a.dim, a.vocab, n, xo, g, o, a.exact, d_err, s)
+                        : linear_product(a.vocab, a.dim, n, g, xo, o, a.exact, d_err, s);
+      if (rc) return rc;
+    }
+  }
+  if (a.mean_loss) {
+    mean_live_kernel<<<1, 1024, 0, s>>>(a.row_loss, a.targets, a.rows, a.mean_loss);
+    check_cuda(cudaGetLastError(), "mean loss");
+  }
+  return 0;
+}
+
+}  // namespace mm

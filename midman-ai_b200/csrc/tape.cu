@@ -36,6 +36,7 @@
 #include "gemm.h"
 #include "host.h"
 #include "kernels.h"
+#include "linear.h"
 
 namespace mm {
 namespace {
@@ -273,6 +274,25 @@ R guarded(R on_error, F&& body) {
 }
 
 bool multiple4(int64_t v) { return v % 4 == 0; }
+
+// The words {seed, offset} that a dropout's kernels read, kept with the node.
+Buf rng_words(Tape& tp, uint64_t seed, uint64_t offset) {
+  const uint64_t words[2] = {seed, offset};
+  Buf b = tp.alloc(4);
+  check_cuda(cudaMemcpyAsync(b->ptr, words, sizeof words, cudaMemcpyHostToDevice, tp.stream), "dropout words");
+  check_cuda(cudaStreamSynchronize(tp.stream), "dropout words");  // `words` dies here
+  return b;
+}
+
+DropoutArgs dropout_of(const Buf& words, double p, int cols) {
+  return dropout_args(p, words ? reinterpret_cast<const uint64_t*>(words->ptr) : nullptr, cols);
+}
+
+void linear_status(int rc) {
+  if (rc) throw std::runtime_error(std::string("linear: ") + gemm_status_string(rc));
+}
+
+Buf workspace(Tape& tp, int64_t bytes) { return tp.alloc(static_cast<size_t>((bytes + 3) / 4)); }
 
 }  // namespace
 }  // namespace mm
@@ -653,6 +673,162 @@ uint64_t mm_op_cross_entropy(uint32_t tape, uint64_t logits_h, const int32_t* ta
         axpy_dev_kernel<<<blocks_for(n), 256, 0, tpp->stream>>>(dl, grad->ptr, dz, n);
         check_cuda(cudaGetLastError(), "cross_entropy backward");
       }
+    })->id;
+  });
+}
+
+uint64_t mm_op_dropout(uint32_t tape, uint64_t x_h, double p, uint64_t seed, uint64_t offset) {
+  return guarded<uint64_t>(0, [&]() -> uint64_t {
+    Tape& tp = tape_of(tape);
+    T x = tp.get(x_h);
+    require(p >= 0.0 && p < 1.0, MM_GPU_ERR_ARGUMENT, "dropout: p must lie in [0, 1)");
+    const int64_t cols = x->shape.back(), rows = x->numel() / cols;
+    require(cols <= INT32_MAX, MM_GPU_ERR_SHAPE, "dropout: the last dimension is too long");
+    Buf y = tp.alloc(static_cast<size_t>(x->numel()));
+    Buf words = p > 0.0 ? rng_words(tp, seed, offset) : nullptr;
+    const int n = static_cast<int>(cols);
+    dropout(x->data->ptr, n, nullptr, 0, y->ptr, n, rows, n, dropout_of(words, p, n), tp.stream);
+    Tape* tpp = &tp;
+    return tp.make(x->shape, y, {x}, [tpp, words, p, rows, n](const float* dy, const GradOf& grad_of) {
+      if (float* dx = grad_of(0))  // dx += mask / (1 - p) * dy
+        dropout(dy, n, dx, n, dx, n, rows, n, dropout_of(words, p, n), tpp->stream);
+    })->id;
+  });
+}
+
+uint64_t mm_op_linear(uint32_t tape, uint64_t x_h, uint64_t w_h, int32_t w_transposed, uint64_t bias_h,
+                      int32_t activation, double p, uint64_t seed, uint64_t offset, uint64_t residual_h) {
+  return guarded<uint64_t>(0, [&]() -> uint64_t {
+    Tape& tp = tape_of(tape);
+    T x = tp.get(x_h), w = tp.get(w_h);
+    T bias = bias_h ? tp.get(bias_h) : nullptr, res = residual_h ? tp.get(residual_h) : nullptr;
+    require(x->shape.size() == 2 && w->shape.size() == 2, MM_GPU_ERR_SHAPE, "linear: two 2-D tensors");
+    const bool wt = w_transposed != 0;
+    const int64_t m = x->shape[0], k = x->shape[1], n = w->shape[wt ? 0 : 1];
+    require(w->shape[wt ? 1 : 0] == k, MM_GPU_ERR_SHAPE, "linear: inner dimensions differ");
+    require(multiple4(k) && multiple4(n), MM_GPU_ERR_SHAPE, "linear: inner and output widths must be multiples of 4");
+    require(m <= INT32_MAX && k <= INT32_MAX && n <= INT32_MAX, MM_GPU_ERR_SHAPE, "linear: a dimension is too long");
+    require(!bias || bias->shape == std::vector<int64_t>{n}, MM_GPU_ERR_SHAPE, "linear: bias [n]");
+    require(!res || res->shape == std::vector<int64_t>({m, n}), MM_GPU_ERR_SHAPE, "linear: residual [m, n]");
+    require(activation >= 0 && activation < kActivations, MM_GPU_ERR_ARGUMENT, "linear: unknown activation");
+    require(p >= 0.0 && p < 1.0, MM_GPU_ERR_ARGUMENT, "dropout: p must lie in [0, 1)");
+    const bool exact = tp.precision == MM_GPU_3XTF32;
+    const int im = static_cast<int>(m), ik = static_cast<int>(k), in = static_cast<int>(n);
+    Buf words = p > 0.0 ? rng_words(tp, seed, offset) : nullptr;
+    Buf c = tp.alloc(static_cast<size_t>(m * n));
+    const bool tracks = x->tracks() || w->tracks() || (bias && bias->tracks());
+    Buf z = tracks && activation != kActNone ? tp.alloc(static_cast<size_t>(m * n)) : nullptr;  // for the slope
+    LinearEpilogue e;
+    e.bias = bias ? bias->data->ptr : nullptr;
+    e.act = activation;
+    e.drop = dropout_of(words, p, in);
+    e.R = res ? res->data->ptr : nullptr;
+    e.ldr = n;
+    e.Z = z ? z->ptr : nullptr;
+    e.ldz = n;
+    e.C = c->ptr;
+    e.ldc = n;
+    // W(n, k) = W[k][n] (MN-major, ld n) or Wt[n][k] (K-major, ld k)
+    linear_status(linear_product(im, in, ik, {x->data->ptr, k, false}, {w->data->ptr, wt ? k : n, !wt}, e, exact,
+                                 device_context().d_err, tp.stream));
+    std::vector<T> parents{x, w};
+    size_t at_bias = 0, at_res = 0;
+    if (bias) {
+      at_bias = parents.size();
+      parents.push_back(bias);
+    }
+    if (res) {
+      at_res = parents.size();
+      parents.push_back(res);
+    }
+    Tape* tpp = &tp;
+    return tp.make({m, n}, c, std::move(parents), [=](const float* dc, const GradOf& grad_of) {
+      float* dr = at_res ? grad_of(at_res) : nullptr;
+      if (dr) tpp->add_into(dr, dc, m * n);
+      float* dx = grad_of(0);
+      float* dw = grad_of(1);
+      float* db = at_bias ? grad_of(at_bias) : nullptr;
+      const bool plain = activation == kActNone && p == 0.0;
+      Buf dz = plain ? nullptr : tpp->alloc(static_cast<size_t>(m * n));
+      Buf part = db ? tpp->alloc(static_cast<size_t>(act_backward_parts(im)) * n) : nullptr;
+      if (dz || part) {
+        act_backward(dc, n, z ? z->ptr : nullptr, n, activation, dropout_of(words, p, in), im, in,
+                     dz ? dz->ptr : nullptr, n, part ? part->ptr : nullptr, tpp->stream);
+        if (part) sum_parts(part->ptr, act_backward_parts(im), in, db, true, tpp->stream);
+      }
+      const float* g = dz ? dz->ptr : dc;
+      auto product = [&](int M, int N, int K, GemmOperand A, GemmOperand B, float* out) {  // out += A B
+        LinearEpilogue o;
+        o.C = out;
+        o.R = out;
+        o.ldc = o.ldr = N;
+        linear_status(linear_product(M, N, K, A, B, o, exact, device_context().d_err, tpp->stream));
+      };
+      if (dx) product(im, ik, in, {g, n, false}, {w->data->ptr, wt ? k : n, wt}, dx);
+      if (dw && !wt) product(ik, in, im, {x->data->ptr, k, true}, {g, n, true}, dw);
+      if (dw && wt) product(in, ik, im, {g, n, true}, {x->data->ptr, k, true}, dw);
+    })->id;
+  });
+}
+
+uint64_t mm_op_linear_cross_entropy(uint32_t tape, uint64_t x_h, uint64_t w_h, int32_t w_transposed,
+                                    const int32_t* targets_host, int64_t rows) {
+  return guarded<uint64_t>(0, [&]() -> uint64_t {
+    Tape& tp = tape_of(tape);
+    T x = tp.get(x_h), w = tp.get(w_h);
+    require(x->shape.size() == 2 && w->shape.size() == 2 && x->shape[0] == rows && targets_host, MM_GPU_ERR_SHAPE,
+            "linear_cross_entropy: x [rows, dim], w and one target per row");
+    const bool wt = w_transposed != 0;
+    const int64_t dim = x->shape[1], vocab = w->shape[wt ? 0 : 1];
+    require(w->shape[wt ? 1 : 0] == dim, MM_GPU_ERR_SHAPE, "linear_cross_entropy: inner dimensions differ");
+    require(multiple4(dim) && multiple4(vocab), MM_GPU_ERR_SHAPE,
+            "linear_cross_entropy: the inner width and the classes must be multiples of 4");
+    require(rows <= INT32_MAX && dim <= INT32_MAX && vocab <= INT32_MAX, MM_GPU_ERR_SHAPE,
+            "linear_cross_entropy: a dimension is too long");
+    int64_t live = 0;
+    for (int64_t r = 0; r < rows; ++r) {
+      require(targets_host[r] >= -1 && targets_host[r] < vocab, MM_GPU_ERR_INDEX,
+              "linear_cross_entropy: target " + std::to_string(targets_host[r]) + " is outside the " +
+                  std::to_string(vocab) + " classes");
+      live += targets_host[r] >= 0 ? 1 : 0;
+    }
+    const bool exact = tp.precision == MM_GPU_3XTF32;
+    // The gradients of the mean come with the loss (one pass over the logits);
+    // backward scales them by the upstream gradient.
+    Buf dx = x->tracks() ? tp.alloc(static_cast<size_t>(rows * dim)) : nullptr;
+    Buf dw = w->tracks() ? tp.alloc(static_cast<size_t>(vocab * dim)) : nullptr;
+    Buf tgt = tp.alloc(static_cast<size_t>(rows)), row_loss = tp.alloc(static_cast<size_t>(rows)), loss = tp.alloc(1);
+    check_cuda(cudaMemcpyAsync(tgt->ptr, targets_host, rows * 4, cudaMemcpyHostToDevice, tp.stream), "targets");
+    LinearLoss a{};
+    a.rows = static_cast<int>(rows);
+    a.vocab = static_cast<int>(vocab);
+    a.dim = static_cast<int>(dim);
+    a.x = x->data->ptr;
+    a.ldx = dim;
+    a.w = w->data->ptr;
+    a.ldw = wt ? dim : vocab;
+    a.w_mn_major = !wt;
+    a.targets = reinterpret_cast<const int32_t*>(tgt->ptr);
+    a.grad_scale = live ? static_cast<float>(1.0 / static_cast<double>(live)) : 0.0f;
+    a.row_loss = row_loss->ptr;
+    a.mean_loss = loss->ptr;
+    a.dx = dx ? dx->ptr : nullptr;
+    a.lddx = dim;
+    a.dw = dw ? dw->ptr : nullptr;
+    a.lddw = a.ldw;
+    a.exact = exact;
+    Buf ws = workspace(tp, linear_loss_ws_bytes(a.rows, a.vocab, a.dim, dx || dw, exact));
+    linear_status(linear_loss(a, ws->ptr, device_context().d_err, tp.stream));
+    check_cuda(cudaStreamSynchronize(tp.stream), "targets");  // the caller's targets may go
+    Tape* tpp = &tp;
+    return tp.make({1}, loss, {x, w}, [tpp, dx, dw](const float* dl, const GradOf& grad_of) {
+      const Buf parts[2] = {dx, dw};
+      for (size_t i = 0; i < 2; ++i)
+        if (float* d = grad_of(i)) {
+          const long long n = static_cast<long long>(parts[i]->n);
+          axpy_dev_kernel<<<blocks_for(n), 256, 0, tpp->stream>>>(dl, parts[i]->ptr, d, n);
+          check_cuda(cudaGetLastError(), "linear_cross_entropy backward");
+        }
     })->id;
   });
 }

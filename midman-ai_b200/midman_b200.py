@@ -19,12 +19,15 @@ GPU_SYMBOLS = [
     "mm_gpu_attention_backward", "mm_gpu_attention_forward_noalloc", "mm_gpu_rmsnorm_forward",
     "mm_gpu_rmsnorm_backward", "mm_gpu_rope", "mm_gpu_swiglu_forward", "mm_gpu_swiglu_backward",
     "mm_gpu_embedding_forward", "mm_gpu_embedding_backward", "mm_gpu_cross_entropy", "mm_gpu_comm_create",
-    "mm_gpu_comm_destroy", "mm_gpu_allreduce_bucket", "mm_gpu_comm_wait", "mm_gpu_wait_selftest",
+    "mm_gpu_comm_destroy", "mm_gpu_allreduce_bucket", "mm_gpu_comm_wait", "mm_gpu_wait_selftest", "mm_gpu_dropout",
+    "mm_gpu_linear_workspace", "mm_gpu_linear_forward", "mm_gpu_linear_backward",
+    "mm_gpu_linear_cross_entropy_workspace", "mm_gpu_linear_cross_entropy",
 ]
 TENSOR_SYMBOLS = [
     "mm_tape_create", "mm_tape_destroy", "mm_tensor_new", "mm_tensor_shape", "mm_tensor_read", "mm_tensor_grad",
     "mm_tensor_free", "mm_tape_backward", "mm_op_matmul", "mm_op_add", "mm_op_mul", "mm_op_embedding",
     "mm_op_rms_norm", "mm_op_rope", "mm_op_causal_attention", "mm_op_swiglu", "mm_op_cross_entropy",
+    "mm_op_dropout", "mm_op_linear", "mm_op_linear_cross_entropy",
 ]
 API_SYMBOLS = [
     "midman_abi_version", "midman_alloc", "midman_free", "midman_text_ptr", "midman_text_len",
@@ -88,6 +91,16 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
     _sig(lib, "mm_gpu_allreduce_bucket", i32, vp, vp, i64, i32, vp)
     _sig(lib, "mm_gpu_comm_wait", i32, vp, vp, i32)
     _sig(lib, "mm_gpu_wait_selftest", i32, i32, vp)
+    f64 = C.c_double
+    _sig(lib, "mm_gpu_dropout", i32, i64, i32, vp, i64, vp, i64, vp, i64, f64, vp, vp)
+    _sig(lib, "mm_gpu_linear_workspace", i64, i32, i32, i32, i32, i32)
+    _sig(lib, "mm_gpu_linear_forward", i32, i32, i32, i32, vp, i64, vp, i64, i32, vp, i32, f64, vp, vp, i64, vp, i64, vp,
+         i64, i32, vp, i64, vp)
+    _sig(lib, "mm_gpu_linear_backward", i32, i32, i32, i32, vp, i64, vp, i64, i32, i32, f64, vp, vp, i64, vp, i64, vp,
+         i64, vp, i64, vp, i32, i32, vp, i64, vp)
+    _sig(lib, "mm_gpu_linear_cross_entropy_workspace", i64, i32, i32, i32, i32, i32)
+    _sig(lib, "mm_gpu_linear_cross_entropy", i32, i32, i32, i32, vp, i64, vp, i64, i32, vp, C.c_float, vp, vp, vp, i64,
+         vp, i64, i32, i32, vp, i64, vp)
     u64, i64p = C.c_uint64, C.POINTER(C.c_int64)
     _sig(lib, "mm_tape_create", u32, i32)
     _sig(lib, "mm_tape_destroy", i32, u32)
@@ -106,6 +119,9 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
     _sig(lib, "mm_op_causal_attention", u64, u32, u64, u64, u64, i32, i32, i32, i32)
     _sig(lib, "mm_op_swiglu", u64, u32, u64, u64)
     _sig(lib, "mm_op_cross_entropy", u64, u32, u64, i32p, i64)
+    _sig(lib, "mm_op_dropout", u64, u32, u64, f64, u64, u64)
+    _sig(lib, "mm_op_linear", u64, u32, u64, u64, i32, u64, i32, f64, u64, u64, u64)
+    _sig(lib, "mm_op_linear_cross_entropy", u64, u32, u64, u64, i32, i32p, i64)
     _sig(lib, "midman_abi_version", u32)
     _sig(lib, "midman_alloc", u8p, u32)
     _sig(lib, "midman_free", None, u8p, u32)
@@ -277,6 +293,95 @@ def cross_entropy(logits, targets, row_loss, *, rows, vocab, ld, grad_scale, mea
                                              _ptr(row_loss), _ptr(mean_loss), _stream(stream)))
 
 
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = range(4)
+
+
+def _device_tensors(dtype_name, **tensors):
+    """Refuses tensors of another type, in host memory, or on another GPU than the current one."""
+    import torch
+    dtype, current = getattr(torch, dtype_name), torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.dtype is not dtype:
+            raise TypeError(f"{name} must be {dtype_name}, not {t.dtype}")
+        if t.get_device() != current:
+            raise ValueError(f"{name} is on {t.device}, and the current device is cuda:{current}")
+
+
+def _workspace(bytes_needed, given, like):
+    """The caller's workspace, or one from torch's allocator (stream-ordered on the current stream)."""
+    need = check(bytes_needed)
+    if given is not None or need == 0:
+        return given
+    import torch
+    return torch.empty(need, dtype=torch.uint8, device=like.device)
+
+
+def _bytes(t):
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def dropout(x, y, *, rows, cols, ldx, ldy, p, rng=None, r=None, ldr=0, stream=None):
+    """y = r + dropout(x); rng: a CUDA int64 tensor [seed, offset] (see include/midman_gpu.h)."""
+    _device_tensors("float32", x=x, y=y, r=r)
+    _device_tensors("int64", rng=rng)
+    return check(load().mm_gpu_dropout(rows, cols, _ptr(x), ldx, _ptr(r), ldr, _ptr(y), ldy, p, _ptr(rng),
+                                       _stream(stream)))
+
+
+def linear_workspace(m, n, k, *, backward=False, precision=0) -> int:
+    """Bytes of the workspace of linear_forward / linear_backward."""
+    return check(load().mm_gpu_linear_workspace(m, n, k, int(bool(backward)), precision))
+
+
+def linear_forward(a, b, c, *, m, n, k, lda, ldb, ldc, b_mn_major=True, bias=None, activation=ACT_NONE, p=0.0, rng=None,
+                   r=None, ldr=0, z=None, ldz=0, precision=0, workspace=None, stream=None):
+    """c = r + dropout(activation(a b + bias)), z = a b + bias where wanted. Without a workspace one is allocated,
+    which needs `stream` to be the current one."""
+    _device_tensors("float32", a=a, b=b, c=c, bias=bias, r=r, z=z)
+    _device_tensors("int64", rng=rng)
+    lib = load()
+    ws = _workspace(lib.mm_gpu_linear_workspace(m, n, k, 0, precision), workspace, c)
+    return check(lib.mm_gpu_linear_forward(m, n, k, _ptr(a), lda, _ptr(b), ldb, int(b_mn_major), _ptr(bias), activation,
+                                           p, _ptr(rng), _ptr(r), ldr, _ptr(z), ldz, _ptr(c), ldc, precision, _ptr(ws),
+                                           _bytes(ws), _stream(stream)))
+
+
+def linear_backward(a, b, dc, *, m, n, k, lda, ldb, lddc, b_mn_major=True, activation=ACT_NONE, p=0.0, rng=None, z=None,
+                    ldz=0, da=None, ldda=0, db=None, lddb=0, dbias=None, accumulate=False, precision=0, workspace=None,
+                    stream=None):
+    """The gradients da, db, dbias (those given) of linear_forward from dc and the z it kept."""
+    _device_tensors("float32", a=a, b=b, dc=dc, z=z, da=da, db=db, dbias=dbias)
+    _device_tensors("int64", rng=rng)
+    lib = load()
+    ws = _workspace(lib.mm_gpu_linear_workspace(m, n, k, 1, precision), workspace, dc)
+    return check(lib.mm_gpu_linear_backward(m, n, k, _ptr(a), lda, _ptr(b), ldb, int(b_mn_major), activation, p, _ptr(rng),
+                                            _ptr(z), ldz, _ptr(dc), lddc, _ptr(da), ldda, _ptr(db), lddb, _ptr(dbias),
+                                            int(bool(accumulate)), precision, _ptr(ws), _bytes(ws), _stream(stream)))
+
+
+def linear_cross_entropy_workspace(rows, vocab, dim, *, gradients=True, precision=0) -> int:
+    """Bytes of the workspace of linear_cross_entropy."""
+    return check(load().mm_gpu_linear_cross_entropy_workspace(rows, vocab, dim, int(bool(gradients)), precision))
+
+
+def linear_cross_entropy(x, w, targets, row_loss, *, rows, vocab, dim, ldx, ldw, w_mn_major=False, grad_scale=1.0,
+                         mean_loss=None, dx=None, lddx=0, dw=None, lddw=0, accumulate=False, precision=0,
+                         workspace=None, stream=None):
+    """Cross-entropy of x w^T without its logits; dx and dw (those given) get its gradients. targets: CUDA int32, -1
+    leaves a row out."""
+    _device_tensors("float32", x=x, w=w, row_loss=row_loss, mean_loss=mean_loss, dx=dx, dw=dw)
+    _device_tensors("int32", targets=targets)
+    lib = load()
+    ws = _workspace(lib.mm_gpu_linear_cross_entropy_workspace(rows, vocab, dim, int(dx is not None or dw is not None),
+                                                              precision), workspace, x)
+    return check(lib.mm_gpu_linear_cross_entropy(rows, vocab, dim, _ptr(x), ldx, _ptr(w), ldw, int(w_mn_major),
+                                                 _ptr(targets), grad_scale, _ptr(row_loss), _ptr(mean_loss), _ptr(dx),
+                                                 lddx, _ptr(dw), lddw, int(bool(accumulate)), precision, _ptr(ws),
+                                                 _bytes(ws), _stream(stream)))
+
+
 class Comm:
     """mm_gpu_comm_*: one data-parallel communicator of this process's GPU."""
 
@@ -370,6 +475,17 @@ class Tape:
     def cross_entropy(self, logits, targets):
         t = _np.ascontiguousarray(targets, _np.int32)
         return self._t(load().mm_op_cross_entropy(self.h, logits, _ip(t), t.size))
+
+    def dropout(self, x, p, seed=0, offset=0):
+        return self._t(load().mm_op_dropout(self.h, x, p, seed, offset))
+
+    def linear(self, x, w, w_transposed=False, bias=0, activation=ACT_NONE, p=0.0, seed=0, offset=0, residual=0):
+        return self._t(load().mm_op_linear(self.h, x, w, int(bool(w_transposed)), bias, activation, p, seed, offset,
+                                           residual))
+
+    def linear_cross_entropy(self, x, w, targets, w_transposed=False):
+        t = _np.ascontiguousarray(targets, _np.int32)
+        return self._t(load().mm_op_linear_cross_entropy(self.h, x, w, int(bool(w_transposed)), _ip(t), t.size))
 
     def close(self):
         if self.h:
