@@ -78,13 +78,6 @@ int32_t product_status(int rc) {
   return fail(rc == mm::kGemmLaunch ? MM_GPU_ERR_DEVICE : MM_GPU_ERR_ARGUMENT, mm::gemm_status_string(rc));
 }
 
-int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-
-int64_t backward_dz_bytes(int32_t m, int32_t n) { return round_up(static_cast<int64_t>(m) * round_up(n, 4) * 4, 256); }
-int64_t backward_bytes(int32_t m, int32_t n) {
-  return backward_dz_bytes(m, n) + static_cast<int64_t>(mm::act_backward_parts(m)) * n * 4;
-}
-
 }  // namespace
 
 #define MM_TRY(x)               \
@@ -111,7 +104,8 @@ int64_t mm_gpu_linear_workspace(int32_t m, int32_t n, int32_t k, int32_t backwar
   return guarded<int64_t>("linear", [&]() -> int64_t {
     if (m < 0 || n <= 0 || k <= 0) return fail(MM_GPU_ERR_SHAPE, "linear: need m >= 0, n > 0 and k > 0");
     MM_TRY(check_precision(precision));
-    return backward ? backward_bytes(m, n) : 0;
+    const bool exact = precision == MM_GPU_3XTF32;
+    return backward ? mm::linear_backward_ws_bytes(m, n, k, exact) : mm::linear_forward_ws_bytes(m, n, k, exact);
   });
 }
 
@@ -130,20 +124,19 @@ int32_t mm_gpu_linear_forward(int32_t m, int32_t n, int32_t k, const float* a, i
     MM_TRY(check_matrix("linear: c", c, ldc, n));
     if (r) MM_TRY(check_matrix("linear: r", r, ldr, n));
     if (z) MM_TRY(check_matrix("linear: z", z, ldz, n));
-    MM_TRY(check_workspace(workspace, workspace_bytes, 0));
-    mm::LinearEpilogue e;
-    e.bias = bias;
-    e.act = activation;
-    e.drop = mm::dropout_args(p, rng, n);
-    e.R = r;
-    e.ldr = ldr;
-    e.Z = z;
-    e.ldz = ldz;
-    e.C = c;
-    e.ldc = ldc;
-    return product_status(mm::linear_product(m, n, k, {a, lda, false}, {b, ldb, b_mn_major != 0}, e,
-                                             precision == MM_GPU_3XTF32, mm::device_context().d_err,
-                                             as_stream(stream)));
+    const bool exact = precision == MM_GPU_3XTF32;
+    MM_TRY(check_workspace(workspace, workspace_bytes, mm::linear_forward_ws_bytes(m, n, k, exact)));
+    mm::LinearForward f{m, n, k, a, lda, b, ldb, b_mn_major != 0, {}, exact};
+    f.e.bias = bias;
+    f.e.act = activation;
+    f.e.drop = mm::dropout_args(p, rng, n);
+    f.e.R = r;
+    f.e.ldr = ldr;
+    f.e.Z = z;
+    f.e.ldz = ldz;
+    f.e.C = c;
+    f.e.ldc = ldc;
+    return product_status(mm::linear_forward(f, workspace, mm::device_context().d_err, as_stream(stream)));
   });
 }
 
@@ -175,41 +168,12 @@ int32_t mm_gpu_linear_backward(int32_t m, int32_t n, int32_t k, const float* a, 
       if (dbias) mm::check_cuda(cudaMemsetAsync(dbias, 0, n * 4ull, st), "dbias");
       return MM_GPU_OK;
     }
-    MM_TRY(check_workspace(workspace, workspace_bytes, backward_bytes(m, n)));
-    const mm::DropoutArgs drop = mm::dropout_args(p, rng, n);
-    const bool plain = activation == MM_GPU_ACT_NONE && p == 0.0;  // dz is dc
-    float* dz = static_cast<float*>(workspace);
-    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + backward_dz_bytes(m, n));
-    const int64_t lddz = round_up(n, 4);
-    if (!plain || dbias) {
-      mm::act_backward(dc, lddc, z, ldz, activation, drop, m, n, plain ? nullptr : dz, lddz, dbias ? part : nullptr,
-                       st);
-      if (dbias) mm::sum_parts(part, mm::act_backward_parts(m), n, dbias, accumulate != 0, st);
-    }
-    const float* g = plain ? dc : dz;
-    const long long ldg = plain ? lddc : lddz;
     const bool exact = precision == MM_GPU_3XTF32;
-    int* d_err = mm::device_context().d_err;
-    if (da) {
-      mm::LinearEpilogue e;
-      e.C = da;
-      e.ldc = ldda;
-      e.R = accumulate ? da : nullptr;
-      e.ldr = ldda;
-      MM_TRY(product_status(
-          mm::linear_product(m, k, n, {g, ldg, false}, {b, ldb, b_mn_major == 0}, e, exact, d_err, st)));
-    }
-    if (db) {
-      mm::LinearEpilogue e;
-      e.C = db;
-      e.ldc = lddb;
-      e.R = accumulate ? db : nullptr;
-      e.ldr = lddb;
-      const mm::GemmOperand ao{a, lda, true}, go{g, ldg, true};
-      MM_TRY(product_status(b_mn_major ? mm::linear_product(k, n, m, ao, go, e, exact, d_err, st)
-                                       : mm::linear_product(n, k, m, go, ao, e, exact, d_err, st)));
-    }
-    return MM_GPU_OK;
+    MM_TRY(check_workspace(workspace, workspace_bytes, mm::linear_backward_ws_bytes(m, n, k, exact)));
+    const mm::LinearBackward f{m,  n,    k,  a,    lda,   b,    ldb, b_mn_major != 0, activation, mm::dropout_args(p, rng, n),
+                               z,  ldz,  dc, lddc, da,    ldda, db,  lddb,            dbias,      accumulate != 0,
+                               exact};
+    return product_status(mm::linear_backward(f, workspace, mm::device_context().d_err, st));
   });
 }
 

@@ -1636,6 +1636,27 @@ int encode_tensor_map(CUtensorMap* map, const float* ptr, int rank, const long l
   return encode(map, ptr, rank, dims, strides, box, mn_major);
 }
 
+int encode_tensor_map_f16(CUtensorMap* map, const void* ptr, int rank, const long long* dims,
+                          const long long* strides, const int* box) {
+  auto fn = get_encode_fn();
+  if (!fn) return -1;
+  if (rank < 2 || rank > 5) return -2;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], e[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    b[i] = static_cast<cuuint32_t>(box[i]);
+  }
+  for (int i = 0; i + 1 < rank; ++i) {
+    st[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+    if (st[i] % 16 != 0) return -2;
+  }
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(ptr), d, st, b, e,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
 namespace {
 
 // 2-D operand: `inner` contiguous elements per row, `outer` rows, `ld` apart.

@@ -28,6 +28,7 @@
 #include "device.h"
 #include "gemm.h"
 #include "linear.h"
+#include "linear_epi.cuh"
 #include "ptx.cuh"
 #include "tma.h"
 
@@ -38,83 +39,6 @@ constexpr int BM = 128;
 constexpr int BK = 32;  // 32 f32 = 128 bytes = one swizzle row
 constexpr uint32_t MN_BLOCK_BYTES = BK * 128;
 constexpr int kEpiWarps = 8;
-
-// ------------------------------------------------------------------ epilogues
-__device__ __forceinline__ float activate(float z, int act) {
-  switch (act) {
-    case kActRelu: return fmaxf(z, 0.0f);
-    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case kActSilu: return z / (1.0f + expf(-z));
-    default: return z;
-  }
-}
-
-// d act / dz
-__device__ __forceinline__ float activate_slope(float z, int act) {
-  switch (act) {
-    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
-    case kActGelu:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-    case kActSilu: {
-      const float s = 1.0f / (1.0f + expf(-z));
-      return s * (1.0f + z * (1.0f - s));
-    }
-    default: return 1.0f;
-  }
-}
-
-// Four columns of a row; those at n and past it are not touched.
-__device__ __forceinline__ float4 load_quad(const float* row, int col, int n) {
-  if (col + 3 < n) return *reinterpret_cast<const float4*>(row + col);
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (col < n) v.x = row[col];
-  if (col + 1 < n) v.y = row[col + 1];
-  if (col + 2 < n) v.z = row[col + 2];
-  return v;
-}
-__device__ __forceinline__ void store_quad(float* row, int col, int n, float4 v) {
-  if (col + 3 < n) {
-    *reinterpret_cast<float4*>(row + col) = v;
-    return;
-  }
-  if (col < n) row[col] = v.x;
-  if (col + 1 < n) row[col + 1] = v.y;
-  if (col + 2 < n) row[col + 2] = v.z;
-}
-__device__ __forceinline__ float4 load_each(const float* row, int col, int n) {  // any alignment
-  return make_float4(col < n ? row[col] : 0.f, col + 1 < n ? row[col + 1] : 0.f, col + 2 < n ? row[col + 2] : 0.f,
-                     col + 3 < n ? row[col + 3] : 0.f);
-}
-__device__ __forceinline__ void store_each(float* row, int col, int n, float4 v) {
-  if (col < n) row[col] = v.x;
-  if (col + 1 < n) row[col + 1] = v.y;
-  if (col + 2 < n) row[col + 2] = v.z;
-  if (col + 3 < n) row[col + 3] = v.w;
-}
-// v: the product's four columns; r: the residual's (loaded by the caller before
-// anything of the batch is stored, so that r may be c).
-__device__ __forceinline__ void linear_quad(const LinearEpilogue& e, uint64_t seed, uint64_t offset, long long row,
-                                            int col, int n, float4 v, float4 r) {
-  if (e.bias) {
-    const float4 b = load_each(e.bias, col, n);
-    v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
-  }
-  if (e.Z) store_quad(e.Z + row * e.ldz, col, n, v);
-  if (e.act != kActNone) {
-    v.x = activate(v.x, e.act); v.y = activate(v.y, e.act); v.z = activate(v.z, e.act); v.w = activate(v.w, e.act);
-  }
-  if (e.drop.rng) v = dropout_quad(v, e.drop, seed, offset, row, col >> 2);
-  v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
-  store_quad(e.C + row * e.ldc, col, n, v);
-}
-
-__device__ __forceinline__ float quad_max(float4 v, int col, int n) {  // col < n
-  float m = v.x;
-  if (col + 1 < n) m = fmaxf(m, v.y);
-  if (col + 2 < n) m = fmaxf(m, v.z);
-  if (col + 3 < n) m = fmaxf(m, v.w);
-  return m;
-}
 
 // ------------------------------------------------------------------ direct kernel
 template <int TERMS, int BN>
@@ -434,10 +358,10 @@ struct LossDirect {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       float s = 0.0f;
-      if (col < N) s += expf(v.x - m);
-      if (col + 1 < N) s += expf(v.y - m);
-      if (col + 2 < N) s += expf(v.z - m);
-      if (col + 3 < N) s += expf(v.w - m);
+      if (col < N) s += loss_exp(v.x - m);
+      if (col + 1 < N) s += loss_exp(v.y - m);
+      if (col + 2 < N) s += loss_exp(v.z - m);
+      if (col + 3 < N) s += loss_exp(v.w - m);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (lane == 0) e.part[row * e.tiles + n0 / 128] = make_float2(m, s);
@@ -645,7 +569,7 @@ DropoutArgs dropout_args(double p, const uint64_t* rng, int cols) {
   return d;
 }
 
-int linear_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, int* d_err,
+int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, int* d_err,
                    cudaStream_t s) {
   if (M <= 0 || N <= 0) return 0;
   const DirectPlan p = direct_plan(M, N, K, true);
@@ -657,7 +581,7 @@ int linear_product(int M, int N, int K, GemmOperand A, GemmOperand B, const Line
                      : direct_majors<1, 64>(M, N, K, A, B, epi, p.splits, d_err, s);
 }
 
-int loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
+int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
                  cudaStream_t s) {
   if (M <= 0 || N <= 0) return 0;
   if (A.mn_major) return kGemmBadArgument;

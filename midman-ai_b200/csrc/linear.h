@@ -37,18 +37,77 @@ struct LossEpilogue {
   float* zt = nullptr;  // [rows]: the target's logit
 };
 
+// ---- Large exact products (linear_pair.cu): f16 halves of operands scaled block
+// by block, three terms on CTA pairs.
+//
+// A copy of a [rows, k] operand, K-major: per row and chunk of 128 of k, 256 f16
+// values [hi 0..63, lo 0..63, hi 64..127, lo 64..127] (zeros past k), and per
+// chunk and row the inverse of the power of two that the chunk was scaled by.
+struct SplitCopy {
+  uint16_t* data = nullptr;
+  float* inv = nullptr;  // [chunks, inv_ld], whole 256-row tiles (what lies past rows is never used)
+  int rows = 0, k = 0;
+  __host__ __device__ long long chunks() const { return (k + 127) / 128; }
+  __host__ __device__ long long row_halves() const { return chunks() * 256; }
+  __host__ __device__ long long inv_ld() const { return (rows + 255ll) / 256 * 256; }
+};
+long long split_copy_bytes(int rows, int k);
+SplitCopy split_copy_at(void* ptr, int rows, int k);  // ptr 256-byte aligned
+
+// What a split reads: a matrix; the epilogue's backward (dz of act_backward); or
+// the loss's gradient G from its logits.
+struct SplitMatrix {
+  const float* x;
+  long long ld;
+  const int32_t* targets = nullptr;  // rows without a class as target count as zeros
+  int vocab = 0;
+};
+struct SplitBackward {
+  const float* dc;
+  long long lddc;
+  const float* z;
+  long long ldz;
+  int act;
+  DropoutArgs drop;
+};
+struct SplitLoss {
+  const float* z;
+  long long ldz;
+  const float2* stat;  // per row: maximum, grad_scale / sum
+  const int32_t* targets;
+  int vocab;
+  float grad_scale;
+};
+// [rows, cols] -> its copy by rows (K = cols), its transpose's copy (K = rows), and
+// the column sums' partials [split_parts(rows), cols]; each may be absent.
+void split(const SplitMatrix& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
+           cudaStream_t s);
+void split(const SplitBackward& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
+           float* part, cudaStream_t s);
+void split(const SplitLoss& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
+           cudaStream_t s);
+inline int split_parts(int rows) { return (rows + 127) / 128; }
+
+// ws: pair_ws_bytes(A.rows, B.rows, A.k) bytes (a partial last wave's K parts).
+long long pair_ws_bytes(int M, int N, int K);
+int pair_product(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e, void* ws, int* d_err,
+                 cudaStream_t s);
+int pair_loss_product(const SplitCopy& A, const SplitCopy& B, const LossEpilogue& e, int* d_err, cudaStream_t s);
+// Whether an exact product of this size is worth the copies.
+bool pair_product_suits(int M, int N, int K);
+
 DropoutArgs dropout_args(double p, const uint64_t* rng, int cols);
 
 // y = r + dropout(x) over [rows, cols]; r may be null, y may be x or r.
 void dropout(const float* x, long long ldx, const float* r, long long ldr, float* y, long long ldy, long long rows,
              int cols, const DropoutArgs& d, cudaStream_t s);
 
-// C = epilogue(sum_k A(m, k) B(n, k)); operands as in gemm.h, precision exact or
-// one TF32 pass. Returns a GemmStatus.
-int linear_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, int* d_err,
+// C = epilogue(sum_k A(m, k) B(n, k)) on single CTAs; operands as in gemm.h,
+// precision exact or one TF32 pass. Returns a GemmStatus.
+int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, int* d_err,
                    cudaStream_t s);
 // The same product with the loss's epilogue.
-int loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
+int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
                  cudaStream_t s);
 
 // dz = mask / (1 - p) * dc * act'(z) (dz null: only the column sums), and the
@@ -59,6 +118,45 @@ void act_backward(const float* dc, long long lddc, const float* z, long long ldz
 int act_backward_parts(int rows);
 // out[c] (+)= sum over p of part[p, c], in f64 and in a fixed order.
 void sum_parts(const float* part, int parts, int cols, float* out, bool accumulate, cudaStream_t s);
+
+// ---- The operators (linear_ops.cu): direct or pair products by size; workspaces
+// are 256-byte aligned.
+struct LinearForward {
+  int m, n, k;
+  const float* a;
+  long long lda;
+  const float* b;
+  long long ldb;
+  bool b_mn_major;
+  LinearEpilogue e;
+  bool exact;
+};
+long long linear_forward_ws_bytes(int m, int n, int k, bool exact);
+int linear_forward(const LinearForward& f, void* ws, int* d_err, cudaStream_t s);
+
+struct LinearBackward {
+  int m, n, k;
+  const float* a;
+  long long lda;
+  const float* b;
+  long long ldb;
+  bool b_mn_major;
+  int act;
+  DropoutArgs drop;
+  const float* z;  // may be null without an activation
+  long long ldz;
+  const float* dc;
+  long long lddc;
+  float* da;  // each may be null
+  long long ldda;
+  float* db;
+  long long lddb;
+  float* dbias;
+  bool accumulate;
+  bool exact;
+};
+long long linear_backward_ws_bytes(int m, int n, int k, bool exact);
+int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t s);
 
 struct LinearLoss {
   int rows, vocab, dim;

@@ -216,7 +216,7 @@ int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
     e.tiles = p.tiles;
     e.targets = t;
     e.zt = zt;
-    int rc = loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
+    int rc = direct_loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
     if (rc) return rc;
     if (!grad) {
       row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(part, p.tiles, zt, t, n, a.vocab, a.row_loss + r0, d_err);
@@ -235,7 +235,7 @@ int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
         o.R = o.C;
         o.ldr = a.lddx;
       }
-      rc = linear_product(n, a.dim, a.vocab, {z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, d_err, s);
+      rc = direct_product(n, a.dim, a.vocab, {z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, d_err, s);
       if (rc) return rc;
     }
     if (a.dw) {
@@ -249,8 +249,8 @@ int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
         o.ldr = a.lddw;
       }
       const GemmOperand g{z, p.ldz, true}, xo{xl, p.ldx, true};
-      rc = a.w_mn_major ? linear_product(a.dim, a.vocab, n, xo, g, o, a.exact, d_err, s)
-                        : linear_product(a.vocab, a.dim, n, g, xo, o, a.exact, d_err, s);
+      rc = a.w_mn_major ? direct_product(a.dim, a.vocab, n, xo, g, o, a.exact, d_err, s)
+                        : direct_product(a.vocab, a.dim, n, g, xo, o, a.exact, d_err, s);
       if (rc) return rc;
     }
   }

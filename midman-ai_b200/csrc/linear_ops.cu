@@ -1,0 +1,143 @@
+// The linear operators: which kernels a call runs, and its workspace.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "device.h"
+#include "linear.h"
+
+namespace mm {
+namespace {
+
+// Lays a workspace out front to back, in 256-byte steps; with a null base it only counts.
+struct Arena {
+  uint8_t* base;
+  long long at = 0;
+  void* take(long long bytes) {
+    void* p = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  }
+  SplitCopy copy(int rows, int k) { return split_copy_at(take(split_copy_bytes(rows, k)), rows, k); }
+};
+
+long long round4(long long n) { return (n + 3) & ~3ll; }
+
+struct ForwardPlan {
+  bool pair;
+  SplitCopy a, b;
+  void* parts;
+  long long bytes;
+};
+ForwardPlan forward_plan(int m, int n, int k, bool exact, void* ws) {
+  ForwardPlan p{};
+  Arena at{static_cast<uint8_t*>(ws)};
+  p.pair = exact && m > 0 && pair_product_suits(m, n, k);
+  if (p.pair) {
+    p.a = at.copy(m, k);
+    p.b = at.copy(n, k);
+    p.parts = at.take(pair_ws_bytes(m, n, k));
+  }
+  p.bytes = at.at;
+  return p;
+}
+
+struct BackwardPlan {
+  bool pair;
+  SplitCopy dz, dzt, at, b;  // [m, n], [n, m], [k, m], [k, n]
+  void* parts;               // of one product at a time
+  float* dz_f32;
+  float* sums;
+  long long bytes;
+};
+BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
+  BackwardPlan p{};
+  Arena at{static_cast<uint8_t*>(ws)};
+  p.pair = exact && m > 0 && pair_product_suits(m, k, n) && pair_product_suits(k, n, m);
+  if (p.pair) {
+    p.dz = at.copy(m, n);
+    p.dzt = at.copy(n, m);
+    p.at = at.copy(k, m);
+    p.b = at.copy(k, n);
+    p.parts = at.take(std::max(pair_ws_bytes(m, k, n), pair_ws_bytes(k, n, m)));
+  } else {
+    p.dz_f32 = static_cast<float*>(at.take(m * round4(n) * 4));
+  }
+  p.sums = static_cast<float*>(at.take(static_cast<long long>(std::max(act_backward_parts(m), split_parts(m))) * n * 4));
+  p.bytes = at.at;
+  return p;
+}
+
+}  // namespace
+
+long long linear_forward_ws_bytes(int m, int n, int k, bool exact) {
+  return forward_plan(m, n, k, exact, nullptr).bytes;
+}
+
+int linear_forward(const LinearForward& f, void* ws, int* d_err, cudaStream_t s) {
+  if (f.m <= 0) return 0;
+  const ForwardPlan p = forward_plan(f.m, f.n, f.k, f.exact, ws);
+  if (!p.pair)
+    return direct_product(f.m, f.n, f.k, {f.a, f.lda, false}, {f.b, f.ldb, f.b_mn_major}, f.e, f.exact, d_err, s);
+  split(SplitMatrix{f.a, f.lda}, f.m, f.k, &p.a, nullptr, s);
+  if (f.b_mn_major)
+    split(SplitMatrix{f.b, f.ldb}, f.k, f.n, nullptr, &p.b, s);
+  else
+    split(SplitMatrix{f.b, f.ldb}, f.n, f.k, &p.b, nullptr, s);
+  return pair_product(p.a, p.b, f.e, p.parts, d_err, s);
+}
+
+long long linear_backward_ws_bytes(int m, int n, int k, bool exact) {
+  return backward_plan(m, n, k, exact, nullptr).bytes;
+}
+
+int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t s) {
+  if (f.m <= 0) return 0;
+  const BackwardPlan p = backward_plan(f.m, f.n, f.k, f.exact, ws);
+  LinearEpilogue da, db;
+  da.C = f.da;
+  da.R = f.accumulate ? f.da : nullptr;
+  da.ldc = da.ldr = f.ldda;
+  db.C = f.db;
+  db.R = f.accumulate ? f.db : nullptr;
+  db.ldc = db.ldr = f.lddb;
+  int rc = 0;
+  if (p.pair) {
+    // dz goes from dc and z straight into its copies
+    if (f.da || f.db || f.dbias)
+      split(SplitBackward{f.dc, f.lddc, f.z, f.ldz, f.act, f.drop}, f.m, f.n, f.da ? &p.dz : nullptr,
+            f.db ? &p.dzt : nullptr, f.dbias ? p.sums : nullptr, s);
+    if (f.dbias) sum_parts(p.sums, split_parts(f.m), f.n, f.dbias, f.accumulate, s);
+    if (f.da) {
+      if (f.b_mn_major)
+        split(SplitMatrix{f.b, f.ldb}, f.k, f.n, &p.b, nullptr, s);
+      else
+        split(SplitMatrix{f.b, f.ldb}, f.n, f.k, nullptr, &p.b, s);
+      rc = pair_product(p.dz, p.b, da, p.parts, d_err, s);
+    }
+    if (f.db && !rc) {
+      split(SplitMatrix{f.a, f.lda}, f.m, f.k, nullptr, &p.at, s);
+      rc = f.b_mn_major ? pair_product(p.at, p.dzt, db, p.parts, d_err, s)
+                        : pair_product(p.dzt, p.at, db, p.parts, d_err, s);
+    }
+    return rc;
+  }
+  const bool plain = f.act == kActNone && !f.drop.rng;  // dz is dc
+  const long long ldz = round4(f.n);
+  if (!plain || f.dbias)
+    act_backward(f.dc, f.lddc, f.z, f.ldz, f.act, f.drop, f.m, f.n, plain ? nullptr : p.dz_f32, ldz,
+                 f.dbias ? p.sums : nullptr, s);
+  if (f.dbias) sum_parts(p.sums, act_backward_parts(f.m), f.n, f.dbias, f.accumulate, s);
+  const float* g = plain ? f.dc : p.dz_f32;
+  const long long ldg = plain ? f.lddc : ldz;
+  if (f.da)
+    rc = direct_product(f.m, f.k, f.n, {g, ldg, false}, {f.b, f.ldb, !f.b_mn_major}, da, f.exact, d_err, s);
+  if (f.db && !rc) {
+    const GemmOperand ao{f.a, f.lda, true}, go{g, ldg, true};
+    rc = f.b_mn_major ? direct_product(f.k, f.n, f.m, ao, go, db, f.exact, d_err, s)
+                      : direct_product(f.n, f.k, f.m, go, ao, db, f.exact, d_err, s);
+  }
+  return rc;
+}
+
+}  // namespace mm

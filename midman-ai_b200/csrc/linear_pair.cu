@@ -1,0 +1,691 @@
+// Large exact products with an epilogue, on CTA pairs.
+//
+// Arithmetic: f16 has TF32's 11 significant bits at twice its rate, but few
+// exponents. Every 128 of K of an operand's row are scaled by a power of two that
+// brings the largest of them to [2^14, 2^15) (exact), then x 2^e = hi + lo with
+// hi = f16(x 2^e), lo = f16(x 2^e - hi): 22 bits of x, or 2^-39 of the chunk's
+// largest entry where lo leaves f16's range. C = Al Bh + Ah Bl + Ah Bh; Al Bl
+// (2^-22) is left out. (The splitting into halves with scaling is that of H.
+// Ootomo and R. Yokota, "Recovering single precision accuracy from Tensor Cores
+// while surpassing the FP32 theoretical peak performance", IJHPCA 2022.) The
+// chunk is also what one TMEM accumulation covers: 24 UMMAs, few enough that the
+// tensor core's truncating sums stay below f32's own error, and the epilogue
+// warps undo both scales as they add the chunk to the running sum in registers,
+// so the scales cost one multiplication per value and no pass over the data.
+//
+// The copies are made by one pass over 128 x 128 tiles (split_kernel), from a
+// matrix or straight from what would have been written for it: dz from dc and z,
+// the loss's gradient from its logits; by rows, transposed, or both, so that every
+// product reads K-major operands. It is bound by HBM: 4 bytes read per value (8
+// for dz), 4 written per copy.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "device.h"
+#include "gemm.h"
+#include "linear.h"
+#include "linear_epi.cuh"
+#include "ptx.cuh"
+#include "tma.h"
+
+namespace mm {
+namespace {
+
+// ------------------------------------------------------------------ split
+constexpr int kTile = 128;
+constexpr int kTileLd = kTile + 1;  // odd: a column's rows lie in different banks
+constexpr int kSplitSums = (8 * kTile + kTile) * 4;  // warps' column maxima or sums, scales
+constexpr int kSplitSmem = kSplitSums + kTile * kTileLd * 4;
+
+// The power of two for a chunk whose largest magnitude is m: [2^14, 2^15) after
+// scaling; 1 for infinities, and clamped so that its inverse is a normal number.
+__device__ __forceinline__ float chunk_scale(float m, float* inv) {
+  const int ex = static_cast<int>(__float_as_uint(m) >> 23);  // biased; m >= 0
+  int se = ex == 255 ? 127 : 268 - max(ex, 1);
+  se = min(se, 253);
+  *inv = __uint_as_float(static_cast<uint32_t>(254 - se) << 23);
+  return __uint_as_float(static_cast<uint32_t>(se) << 23);
+}
+
+__device__ __forceinline__ uint32_t pack(__half a, __half b) {
+  return static_cast<uint32_t>(__half_as_ushort(a)) | (static_cast<uint32_t>(__half_as_ushort(b)) << 16);
+}
+
+// hi and lo of a pair of scaled values
+__device__ __forceinline__ void halves(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half hx = __float2half_rn(x), hy = __float2half_rn(y);
+  hi = pack(hx, hy);
+  lo = pack(__float2half_rn(x - __half2float(hx)), __float2half_rn(y - __half2float(hy)));
+}
+
+// Sources: begin_row once per row of a warp, then load of the lane's four columns.
+struct MatrixSource {
+  SplitMatrix a;
+  __device__ __forceinline__ void begin() {}
+  __device__ __forceinline__ float4 load(long long row, int col, int cols) const {
+    if (a.targets) {
+      const int t = a.targets[row];
+      if (t < 0 || t >= a.vocab) return make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    return load_quad(a.x + row * a.ld, col, cols);
+  }
+};
+struct BackwardSource {
+  SplitBackward a;
+  uint64_t seed, offset;
+  __device__ __forceinline__ void begin() {
+    seed = a.drop.rng ? a.drop.rng[0] : 0;
+    offset = a.drop.rng ? a.drop.rng[1] : 0;
+  }
+  __device__ __forceinline__ float4 load(long long row, int col, int cols) const {
+    float4 g = load_quad(a.dc + row * a.lddc, col, cols);
+    if (a.drop.rng) g = dropout_quad(g, a.drop, seed, offset, row, col >> 2);
+    if (a.act != kActNone) {
+      const float4 v = load_quad(a.z + row * a.ldz, col, cols);
+      g.x *= activate_slope(v.x, a.act); g.y *= activate_slope(v.y, a.act);
+      g.z *= activate_slope(v.z, a.act); g.w *= activate_slope(v.w, a.act);
+    }
+    return g;
+  }
+};
+struct LossSource {
+  SplitLoss a;
+  __device__ __forceinline__ void begin() {}
+  __device__ __forceinline__ float4 load(long long row, int col, int cols) const {
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int t = a.targets[row];
+    if (t < 0 || t >= a.vocab) return g;
+    const float2 st = a.stat[row];
+    const float4 v = load_quad(a.z + row * a.ldz, col, cols);
+    g.x = loss_exp(v.x - st.x) * st.y;
+    if (col + 1 < cols) g.y = loss_exp(v.y - st.x) * st.y;
+    if (col + 2 < cols) g.z = loss_exp(v.z - st.x) * st.y;
+    if (col + 3 < cols) g.w = loss_exp(v.w - st.x) * st.y;
+    const int d = t - col;
+    if (d == 0) g.x -= a.grad_scale;
+    if (d == 1) g.y -= a.grad_scale;
+    if (d == 2) g.z -= a.grad_scale;
+    if (d == 3) g.w -= a.grad_scale;
+    return g;
+  }
+};
+
+// One 128 x 128 tile per block: a warp per row (16 of them), a lane four columns.
+template <class Source>
+__global__ void __launch_bounds__(256) split_kernel(Source src, int rows, int cols, SplitCopy by_rows,
+                                                    SplitCopy by_cols, float* part) {
+  extern __shared__ float split_smem[];
+  float* warp_max = split_smem;             // [8][128] column maxima, or column sums
+  float* col_scale = warp_max + 8 * kTile;  // [128]
+  float* tile = col_scale + kTile;          // [128][129], where the transposed copy is wanted
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int r0 = blockIdx.y * kTile, c0 = blockIdx.x * kTile;
+  const int col = c0 + 4 * lane;
+  src.begin();
+  float4 top = make_float4(0.f, 0.f, 0.f, 0.f), sum = top;
+#pragma unroll 4
+  for (int i = 0; i < kTile / 8; ++i) {
+    const int r = 8 * i + warp;
+    const long long row = r0 + r;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < rows && col < cols) v = src.load(row, col, cols);
+    if (by_cols.data) {
+      float* t = tile + r * kTileLd + 4 * lane;
+      t[0] = v.x; t[1] = v.y; t[2] = v.z; t[3] = v.w;
+      top.x = fmaxf(top.x, fabsf(v.x)); top.y = fmaxf(top.y, fabsf(v.y));
+      top.z = fmaxf(top.z, fabsf(v.z)); top.w = fmaxf(top.w, fabsf(v.w));
+    }
+    if (part) {
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    if (by_rows.data) {
+      float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (row < rows) {
+        float inv;
+        const float s = chunk_scale(m, &inv);
+        uint2 hi, lo;
+        halves(v.x * s, v.y * s, hi.x, lo.x);
+        halves(v.z * s, v.w * s, hi.y, lo.y);
+        uint16_t* out = by_rows.data + row * by_rows.row_halves() + blockIdx.x * 256ll + (lane / 16) * 128 +
+                        (lane % 16) * 4;
+        *reinterpret_cast<uint2*>(out) = hi;
+        *reinterpret_cast<uint2*>(out + 64) = lo;
+        if (lane == 0) by_rows.inv[blockIdx.x * by_rows.inv_ld() + row] = inv;
+      }
+    }
+  }
+  if (part) {  // column sums over the tile's rows, warps in order
+    float4* w = reinterpret_cast<float4*>(warp_max + warp * kTile) + lane;
+    *w = sum;
+    __syncthreads();
+    if (threadIdx.x < kTile && c0 + static_cast<int>(threadIdx.x) < cols) {
+      float s = 0.0f;
+      for (int k = 0; k < 8; ++k) s += warp_max[k * kTile + threadIdx.x];
+      part[static_cast<long long>(blockIdx.y) * cols + c0 + threadIdx.x] = s;
+    }
+    __syncthreads();
+  }
+  if (!by_cols.data) return;
+  reinterpret_cast<float4*>(warp_max + warp * kTile)[lane] = top;
+  __syncthreads();
+  if (threadIdx.x < kTile) {
+    float m = 0.0f;
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, warp_max[k * kTile + threadIdx.x]);
+    float inv;
+    col_scale[threadIdx.x] = chunk_scale(m, &inv);
+    if (c0 + static_cast<int>(threadIdx.x) < cols)
+      by_cols.inv[blockIdx.y * by_cols.inv_ld() + c0 + threadIdx.x] = inv;
+  }
+  __syncthreads();
+  // a warp per column: rows 2 lane, 2 lane + 1 of each 64
+  for (int i = 0; i < kTile / 8; ++i) {
+    const int c = 8 * i + warp;
+    if (c0 + c >= cols) break;  // uniform over the warp
+    const float s = col_scale[c];
+    uint16_t* out = by_cols.data + (c0 + c) * by_cols.row_halves() + blockIdx.y * 256ll + 2 * lane;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float x = tile[(64 * h + 2 * lane) * kTileLd + c], y = tile[(64 * h + 2 * lane + 1) * kTileLd + c];
+      uint32_t hi, lo;
+      halves(x * s, y * s, hi, lo);
+      *reinterpret_cast<uint32_t*>(out + 128 * h) = hi;
+      *reinterpret_cast<uint32_t*>(out + 128 * h + 64) = lo;
+    }
+  }
+}
+
+template <class Source>
+void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
+                  float* part, cudaStream_t s) {
+  if (rows <= 0 || cols <= 0) return;
+  auto kern = split_kernel<Source>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (configured_device != dev) {
+    check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem), "shared memory");
+    configured_device = dev;
+  }
+  const dim3 grid((cols + kTile - 1) / kTile, (rows + kTile - 1) / kTile);
+  kern<<<grid, 256, by_cols ? kSplitSmem : kSplitSums, s>>>(src, rows, cols, by_rows ? *by_rows : SplitCopy{},
+                                     by_cols ? *by_cols : SplitCopy{}, part);
+  check_cuda(cudaGetLastError(), "split");
+}
+
+// ------------------------------------------------------------------ products
+// 256 x 256 tiles on CTA pairs (cta_group::2): CTA r of a pair holds rows 128 r..
+// of the tile's A and of its B; a stage is 64 of K: Ah, Al, Bh, Bl, 16 KB each, a
+// chunk two stages. Per stage a CTA takes in 64 KB and its tensor core reads 3 x
+// 48 KB in 1,536 cycles: 135 bytes a cycle of shared memory, so the tensor pipe
+// stays above 90% busy. Warp 0 TMA, warp 1 UMMA (the leader's), warps 2..9 the
+// running sums (TMEM lanes 32 (w % 4).., columns 128 ((w - 2) / 4)..) and the
+// epilogue; the chunks' two TMEM accumulators let the next tile's first two chunks
+// run beside it.
+constexpr int BM = 128, PN = 256;
+constexpr int P_THREADS = 320;
+constexpr int P_STAGES = 3;
+constexpr int P_TILE = 16384;
+constexpr int P_STAGE = 4 * P_TILE;
+constexpr int P_SMEM = P_STAGES * P_STAGE + 1024 + 256 + 8 * 32 * 32 * 4;
+static_assert(P_SMEM <= 232448, "shared memory of a CTA");
+
+// Tiles in groups of 8 row blocks, the row block fastest inside a group, so that the
+// pairs at work at one time share rows of A and columns of B in L2.
+__device__ __forceinline__ void pair_tile(int t, int tm, int tn, int& mt, int& nt) {
+  const int per_group = 8 * tn;
+  const int g = t / per_group, r = t - g * per_group;
+  const int rows = min(8, tm - g * 8);
+  mt = g * 8 + r % rows;
+  nt = r / rows;
+}
+
+// Work unit u. Tiles [0, full) are whole units; each of the rest (the last, partial
+// wave) is cut into `splits` parts of its chunks, whose sums go to workspace tiles
+// that reduce_kernel adds, in part order, before the epilogue.
+struct PairWork {
+  int full = 0, splits = 1;
+  float* ws = nullptr;  // [(tiles - full) * splits][256][256]
+};
+struct PairUnit {
+  int tile, cb, ce, slot;
+};
+__device__ __forceinline__ PairUnit unit_of(int u, const PairWork& w, int chunks) {
+  if (u < w.full) return {u, 0, chunks, -1};
+  const int v = u - w.full, part = v % w.splits;
+  return {w.full + v / w.splits, chunks * part / w.splits, chunks * (part + 1) / w.splits, v};
+}
+
+__device__ __forceinline__ void stage_rows(const float* v, float4* stage_tile, int lane);
+
+template <class Epi>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const float* inv_a,
+                long long ld_ia, const float* inv_b, long long ld_ib, const Epi epi, int M, int N, int chunks, int units, const PairWork work, int* err) {
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = static_cast<int>(blockIdx.x) / 2, npairs = static_cast<int>(gridDim.x) / 2;
+  const int tm = (M + 2 * BM - 1) / (2 * BM), tn = (N + PN - 1) / PN;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw_addr);
+  const uint32_t bar_base = base + P_STAGES * P_STAGE;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (P_STAGES + s); };
+  auto acc_full = [&](int b) { return bar_base + 8u * (2 * P_STAGES + b); };
+  auto acc_empty = [&](int b) { return bar_base + 8u * (2 * P_STAGES + 2 + b); };
+  constexpr int kBars = 2 * P_STAGES + 4;
+  const uint32_t tmem_slot = bar_base + 8u * kBars;
+  uint8_t* tail = smem + P_STAGES * P_STAGE + 8 * kBars;
+  int* loads_issued = reinterpret_cast<int*>(tail + 8);
+  int* loads_consumed = loads_issued + 1;
+  static_assert(8 * kBars + 16 <= 256, "barriers and counters fit their 256 bytes");
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    for (int s = 0; s < P_STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 16);  // eight epilogue warps in each CTA
+    }
+    *loads_issued = 0;
+    *loads_consumed = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 2 * PN);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer (both CTAs); completions land on the leader's barriers
+      int it = 0;
+      bool ok = true;
+      for (int u = pair; u < units && ok; u += npairs) {
+        const PairUnit w = unit_of(u, work, chunks);
+        int mt, nt;
+        pair_tile(w.tile, tm, tn, mt, nt);
+        const int my_m0 = mt * 2 * BM + static_cast<int>(rank) * BM;
+        const int my_n0 = nt * PN + static_cast<int>(rank) * (PN / 2);
+        for (int i = 2 * w.cb; i < 2 * w.ce; ++i, ++it) {  // a chunk is two stages
+          const int s = it % P_STAGES, round = it / P_STAGES;
+          if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, err, kErrWaitEmpty)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(full_bar(s), 2 * P_STAGE);
+          const uint32_t fb = mapa_shared(full_bar(s), 0);
+          const uint32_t sa = base + s * P_STAGE;
+          tma_load_3d_pair(sa, &tmA, fb, 0, my_m0, 2 * i);               // hi, lo of A
+          tma_load_3d_pair(sa + 2 * P_TILE, &tmB, fb, 0, my_n0, 2 * i);  // and of B
+          *loads_issued = it + 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ---------------- UMMA issuer (leader only), M = 256 across the pair
+      constexpr uint32_t idesc = idesc_f16(2 * BM, PN);
+      int it = 0, j = 0;
+      bool ok = true;
+      for (int u = pair; u < units && ok; u += npairs) {
+        const PairUnit w = unit_of(u, work, chunks);
+        for (int c = w.cb; c < w.ce && ok; ++c) {
+          const int buf = j & 1;
+          if (j >= 2 && !mbar_wait(acc_empty(buf), ((j >> 1) - 1) & 1, err, kErrWaitAccum)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t acc = tmem_base + buf * PN;
+          for (int h = 0; h < 2; ++h, ++it) {
+            const int s = it % P_STAGES, round = it / P_STAGES;
+            if (!mbar_wait(full_bar(s), round & 1, err, kErrWaitFull)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            *loads_consumed = it + 1;
+            const uint32_t sa = base + s * P_STAGE;
+            // the terms, small ones first: Al Bh, Ah Bl, Ah Bh
+#pragma unroll
+            for (int term = 0; term < 3; ++term) {
+              const uint32_t at = sa + (term == 0 ? P_TILE : 0);
+              const uint32_t bt = sa + (term == 1 ? 3 * P_TILE : 2 * P_TILE);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)  // 16 f16 = 32 bytes along the swizzled row
+                umma_f16_pair(acc, smem_desc(at + k * 32, 16, 1024, kLayoutSw128),
+                              smem_desc(bt + k * 32, 16, 1024, kLayoutSw128), idesc,
+                              (h != 0 || term != 0 || k != 0) ? 1u : 0u);
+            }
+            umma_commit_pair(empty_bar(s), 0x3);
+          }
+          if (!ok) break;
+          umma_commit_pair(acc_full(buf), 0x3);
+          ++j;
+        }
+      }
+    }
+  } else {
+    // ---------------- running sums and epilogue (both CTAs): 32 rows x 128 columns per warp
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    float4* stage_tile = reinterpret_cast<float4*>(smem + P_STAGES * P_STAGE + 256) + (warp - 2) * 256;
+    int j = 0;
+    bool ok = true;
+    for (int u = pair; u < units && ok; u += npairs) {
+      const PairUnit w = unit_of(u, work, chunks);
+      int mt, nt;
+      pair_tile(w.tile, tm, tn, mt, nt);
+      const int wrow0 = mt * 2 * BM + static_cast<int>(rank) * BM + quarter * 32, wcol0 = nt * PN + half * 128;
+      float sum[128];
+#pragma unroll
+      for (int e = 0; e < 128; ++e) sum[e] = 0.0f;
+      for (int c = w.cb; c < w.ce; ++c) {
+        const float ia = __ldg(inv_a + c * ld_ia + wrow0 + lane);
+        const float4* ib = reinterpret_cast<const float4*>(inv_b + c * ld_ib + wcol0);
+        const int buf = j & 1;
+        if (!mbar_wait(acc_full(buf), (j >> 1) & 1, err, kErrWaitAccum)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem_base + buf * PN + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          float4 b[4];  // the columns' inverse scales, the same for every lane
+#pragma unroll
+          for (int e = 0; e < 4; ++e) b[e] = __ldg(ib + q * 4 + e);
+          uint32_t r[16];
+          tmem_ld_32x32b_x16(acc + q * 16, r);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float* o = sum + q * 16 + 4 * e;
+            o[0] = fmaf(__uint_as_float(r[4 * e]) * ia, b[e].x, o[0]);
+            o[1] = fmaf(__uint_as_float(r[4 * e + 1]) * ia, b[e].y, o[1]);
+            o[2] = fmaf(__uint_as_float(r[4 * e + 2]) * ia, b[e].z, o[2]);
+            o[3] = fmaf(__uint_as_float(r[4 * e + 3]) * ia, b[e].w, o[3]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(mapa_shared(acc_empty(buf), 0));
+        ++j;
+      }
+      if (!ok) break;
+      if (w.slot < 0) {
+        epi.tile(sum, stage_tile, wrow0, wcol0, M, N, lane);
+      } else {  // a part: its sums as they are
+        float* out = work.ws + (static_cast<long long>(w.slot) * 2 * BM + rank * BM + quarter * 32) * PN + half * 128;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          stage_rows(sum + 32 * c, stage_tile, lane);
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < 8; ++i) {
+            const int rr = i * 4 + (lane >> 3);
+            *reinterpret_cast<float4*>(out + rr * PN + 32 * c + 4 * (lane & 7)) =
+                stage_tile[rr * 8 + ((lane & 7) ^ (rr & 7))];
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync();  // both CTAs are done with their TMEM and with each other's barriers
+  if (leader && threadIdx.x == 0) {
+    // after a timed-out wait, let the pair's copies in flight land (bounded)
+    for (int i = *loads_consumed; i < *loads_issued; ++i)
+      if (!mbar_wait(full_bar(i % P_STAGES), (i / P_STAGES) & 1, err, kErrWaitDrain, 1000000000ull)) break;
+  }
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * PN);
+  }
+}
+
+// A warp's 32 rows (lane = row) x 32 columns through its staging tile: 8 lanes per
+// row then hold its 32 columns, so loads and stores cover whole 128-byte segments.
+__device__ __forceinline__ void stage_rows(const float* v, float4* stage_tile, int lane) {
+#pragma unroll
+  for (int g = 0; g < 8; ++g)
+    stage_tile[lane * 8 + (g ^ (lane & 7))] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+}
+
+struct LinearPair {
+  LinearEpilogue e;
+  __device__ __forceinline__ void tile(const float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
+                                       int lane) const {
+    const int sub = lane & 7, rsub = lane >> 3;
+    uint64_t seed = 0, offset = 0;
+    if (e.drop.rng) {
+      seed = e.drop.rng[0];
+      offset = e.drop.rng[1];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      stage_rows(sum + 32 * c, stage_tile, lane);
+      __syncwarp();
+      const int col = n0 + 32 * c + 4 * sub;
+#pragma unroll 2
+      for (int it = 0; it < 8; ++it) {
+        const int rr = it * 4 + rsub;
+        const long long row = wrow0 + rr;
+        const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
+        if (row < M && col < N) {
+          const float4 r = e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
+          linear_quad(e, seed, offset, row, col, N, v, r);
+        }
+      }
+      __syncwarp();  // before the next slice overwrites the staging tile
+    }
+  }
+};
+
+// The split tiles: parts summed in order, then the epilogue. Four rows of a tile per block.
+__global__ void __launch_bounds__(256) reduce_kernel(const PairWork work, const LinearEpilogue e, int M, int N) {
+  const int tm = (M + 2 * BM - 1) / (2 * BM), tn = (N + PN - 1) / PN;
+  int mt, nt;
+  pair_tile(work.full + static_cast<int>(blockIdx.x), tm, tn, mt, nt);
+  const int r = blockIdx.y * 4 + threadIdx.x / 64, c = (threadIdx.x % 64) * 4;
+  const long long row = mt * 2 * BM + r;
+  const int col = nt * PN + c;
+  if (row >= M || col >= N) return;
+  const float* p = work.ws + (static_cast<long long>(blockIdx.x) * work.splits * 2 * BM + r) * PN + c;
+  float4 v = *reinterpret_cast<const float4*>(p);
+  for (int i = 1; i < work.splits; ++i) {
+    p += 2 * BM * PN;
+    const float4 o = *reinterpret_cast<const float4*>(p);
+    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+  }
+  const float4 res = e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
+  linear_quad(e, e.drop.rng ? e.drop.rng[0] : 0, e.drop.rng ? e.drop.rng[1] : 0, row, col, N, v, res);
+}
+
+struct LossPair {
+  LossEpilogue e;
+  __device__ __forceinline__ void tile(const float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
+                                       int lane) const {
+    if (n0 >= N) return;  // uniform over the warp
+    const long long my_row = wrow0 + lane;
+    const int live = min(128, N - n0);
+    float m = -INFINITY, s = 0.0f;
+    if (live == 128) {
+#pragma unroll
+      for (int i = 0; i < 128; ++i) m = fmaxf(m, sum[i]);
+#pragma unroll
+      for (int i = 0; i < 128; ++i) s += loss_exp(sum[i] - m);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 128; ++i) m = i < live ? fmaxf(m, sum[i]) : m;
+#pragma unroll
+      for (int i = 0; i < 128; ++i) s += i < live ? loss_exp(sum[i] - m) : 0.0f;
+    }
+    if (my_row < M) {
+      e.part[my_row * e.tiles + n0 / 128] = make_float2(m, s);
+      const int t = e.targets[my_row] - n0;
+      if (t >= 0 && t < live) {
+        float zt = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 128; ++i) zt = i == t ? sum[i] : zt;
+        e.zt[my_row] = zt;
+      }
+    }
+    if (!e.Z) return;
+    const int sub = lane & 7, rsub = lane >> 3;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      __syncwarp();
+      stage_rows(sum + 32 * c, stage_tile, lane);
+      __syncwarp();
+      const int col = n0 + 32 * c + 4 * sub;
+#pragma unroll 4
+      for (int it = 0; it < 8; ++it) {
+        const int rr = it * 4 + rsub;
+        const long long row = wrow0 + rr;
+        const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
+        if (row < M && col < N) store_quad(e.Z + row * e.ldz, col, N, v);
+      }
+    }
+    __syncwarp();
+  }
+};
+
+// (64 halves, rows, segments): one box of {64, 128, 2} is a stage's hi and lo tile.
+int copy_map(CUtensorMap* map, const SplitCopy& c) {
+  const long long dims[3] = {64, c.rows, 4 * c.chunks()}, strides[2] = {c.row_halves(), 64};
+  const int box[3] = {64, 128, 2};
+  return encode_tensor_map_f16(map, c.data, 3, dims, strides, box) ? kGemmTensorMap : 0;
+}
+
+// The last wave's tiles are cut into parts when that saves at least eight chunks of
+// its length (a chunk takes 1.7 us; writing, reading and summing the parts about 8
+// us). The grid is that of the full part: 74 pairs.
+constexpr int kPairs = 74;
+PairWork work_of(long long tiles, int chunks) {
+  PairWork w;
+  w.full = static_cast<int>(tiles);
+  const int tail = static_cast<int>(tiles % kPairs);
+  if (tail == 0) return w;
+  const int s = std::min(kPairs / tail, chunks);
+  if (s < 2 || chunks - (chunks + s - 1) / s < 8) return w;
+  w.full = static_cast<int>(tiles - tail);
+  w.splits = s;
+  return w;
+}
+
+long long tiles_of(int M, int N) { return static_cast<long long>((M + 255) / 256) * ((N + 255) / 256); }
+
+template <class Epi>
+int launch_pair(const SplitCopy& A, const SplitCopy& B, const Epi& epi, const PairWork& work, int* d_err,
+                cudaStream_t s) {
+  CUtensorMap ta{}, tb{};
+  int rc = copy_map(&ta, A);
+  if (!rc) rc = copy_map(&tb, B);
+  if (rc) return rc;
+  auto kern = pair_kernel<Epi>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (configured_device != dev) {
+    check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM), "shared memory");
+    configured_device = dev;
+  }
+  const long long tiles = tiles_of(A.rows, B.rows), units = work.full + (tiles - work.full) * work.splits;
+  const int grid = 2 * static_cast<int>(std::min<long long>(units, std::min(kPairs, sm_count() / 2)));
+  kern<<<grid, P_THREADS, P_SMEM, s>>>(ta, tb, A.inv, A.inv_ld(), B.inv, B.inv_ld(), epi, A.rows, B.rows,
+                                       static_cast<int>(A.chunks()), static_cast<int>(units), work, d_err);
+  check_cuda(cudaGetLastError(), "linear");
+  return 0;
+}
+
+bool same_k(const SplitCopy& A, const SplitCopy& B) {
+  return A.k == B.k && A.k > 0 && tiles_of(A.rows, B.rows) <= (1 << 26);
+}
+
+long long copy_data_bytes(int rows, int k) { return rows * ((k + 127ll) / 128) * 512; }
+
+}  // namespace
+
+long long split_copy_bytes(int rows, int k) {
+  return copy_data_bytes(rows, k) + ((k + 127ll) / 128) * ((rows + 255ll) / 256 * 256) * 4;
+}
+
+SplitCopy split_copy_at(void* ptr, int rows, int k) {
+  SplitCopy c;
+  c.data = static_cast<uint16_t*>(ptr);
+  c.inv = reinterpret_cast<float*>(static_cast<uint8_t*>(ptr) + copy_data_bytes(rows, k));
+  c.rows = rows;
+  c.k = k;
+  return c;
+}
+
+void split(const SplitMatrix& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
+           cudaStream_t s) {
+  launch_split(MatrixSource{src}, rows, cols, by_rows, by_cols, nullptr, s);
+}
+void split(const SplitBackward& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
+           float* part, cudaStream_t s) {
+  launch_split(BackwardSource{src, 0, 0}, rows, cols, by_rows, by_cols, part, s);
+}
+void split(const SplitLoss& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
+           cudaStream_t s) {
+  launch_split(LossSource{src}, rows, cols, by_rows, by_cols, nullptr, s);
+}
+
+long long pair_ws_bytes(int M, int N, int K) {
+  const long long tiles = tiles_of(M, N);
+  const PairWork w = work_of(tiles, (K + 127) / 128);
+  return (tiles - w.full) * w.splits * (2ll * BM * PN * 4);
+}
+
+int pair_product(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e, void* ws, int* d_err,
+                 cudaStream_t s) {
+  if (A.rows <= 0 || B.rows <= 0) return 0;
+  if (!same_k(A, B)) return kGemmBadArgument;
+  const long long tiles = tiles_of(A.rows, B.rows);
+  PairWork work = work_of(tiles, static_cast<int>(A.chunks()));
+  work.ws = static_cast<float*>(ws);
+  const int rc = launch_pair(A, B, LinearPair{e}, work, d_err, s);
+  if (rc || work.full == tiles) return rc;
+  reduce_kernel<<<dim3(static_cast<unsigned>(tiles - work.full), 2 * BM / 4), 256, 0, s>>>(work, e, A.rows, B.rows);
+  check_cuda(cudaGetLastError(), "linear");
+  return 0;
+}
+
+int pair_loss_product(const SplitCopy& A, const SplitCopy& B, const LossEpilogue& e, int* d_err, cudaStream_t s) {
+  if (A.rows <= 0 || B.rows <= 0) return 0;
+  if (!same_k(A, B)) return kGemmBadArgument;
+  PairWork work;  // every epilogue needs its whole row sums: no parts
+  work.full = static_cast<int>(tiles_of(A.rows, B.rows));
+  return launch_pair(A, B, LossPair{e}, work, d_err, s);
+}
+
+bool pair_product_suits(int M, int N, int K) {
+  const PairWork w = work_of(tiles_of(M, N), (K + 127) / 128);
+  const long long units = w.full + (tiles_of(M, N) - w.full) * w.splits;
+  return K >= 128 && units >= kPairs / 2;
+}
+
+}  // namespace mm

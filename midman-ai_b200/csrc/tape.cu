@@ -718,19 +718,16 @@ uint64_t mm_op_linear(uint32_t tape, uint64_t x_h, uint64_t w_h, int32_t w_trans
     Buf c = tp.alloc(static_cast<size_t>(m * n));
     const bool tracks = x->tracks() || w->tracks() || (bias && bias->tracks());
     Buf z = tracks && activation != kActNone ? tp.alloc(static_cast<size_t>(m * n)) : nullptr;  // for the slope
-    LinearEpilogue e;
-    e.bias = bias ? bias->data->ptr : nullptr;
-    e.act = activation;
-    e.drop = dropout_of(words, p, in);
-    e.R = res ? res->data->ptr : nullptr;
-    e.ldr = n;
-    e.Z = z ? z->ptr : nullptr;
-    e.ldz = n;
-    e.C = c->ptr;
-    e.ldc = n;
-    // W(n, k) = W[k][n] (MN-major, ld n) or Wt[n][k] (K-major, ld k)
-    linear_status(linear_product(im, in, ik, {x->data->ptr, k, false}, {w->data->ptr, wt ? k : n, !wt}, e, exact,
-                                 device_context().d_err, tp.stream));
+    LinearForward f{im, in, ik, x->data->ptr, k, w->data->ptr, wt ? k : n, !wt, {}, exact};
+    f.e.bias = bias ? bias->data->ptr : nullptr;
+    f.e.act = activation;
+    f.e.drop = dropout_of(words, p, in);
+    f.e.R = res ? res->data->ptr : nullptr;
+    f.e.Z = z ? z->ptr : nullptr;
+    f.e.C = c->ptr;
+    f.e.ldr = f.e.ldz = f.e.ldc = n;
+    Buf ws = workspace(tp, linear_forward_ws_bytes(im, in, ik, exact));
+    linear_status(linear_forward(f, ws->ptr, device_context().d_err, tp.stream));
     std::vector<T> parents{x, w};
     size_t at_bias = 0, at_res = 0;
     if (bias) {
@@ -743,30 +740,28 @@ uint64_t mm_op_linear(uint32_t tape, uint64_t x_h, uint64_t w_h, int32_t w_trans
     }
     Tape* tpp = &tp;
     return tp.make({m, n}, c, std::move(parents), [=](const float* dc, const GradOf& grad_of) {
-      float* dr = at_res ? grad_of(at_res) : nullptr;
-      if (dr) tpp->add_into(dr, dc, m * n);
-      float* dx = grad_of(0);
-      float* dw = grad_of(1);
-      float* db = at_bias ? grad_of(at_bias) : nullptr;
-      const bool plain = activation == kActNone && p == 0.0;
-      Buf dz = plain ? nullptr : tpp->alloc(static_cast<size_t>(m * n));
-      Buf part = db ? tpp->alloc(static_cast<size_t>(act_backward_parts(im)) * n) : nullptr;
-      if (dz || part) {
-        act_backward(dc, n, z ? z->ptr : nullptr, n, activation, dropout_of(words, p, in), im, in,
-                     dz ? dz->ptr : nullptr, n, part ? part->ptr : nullptr, tpp->stream);
-        if (part) sum_parts(part->ptr, act_backward_parts(im), in, db, true, tpp->stream);
-      }
-      const float* g = dz ? dz->ptr : dc;
-      auto product = [&](int M, int N, int K, GemmOperand A, GemmOperand B, float* out) {  // out += A B
-        LinearEpilogue o;
-        o.C = out;
-        o.R = out;
-        o.ldc = o.ldr = N;
-        linear_status(linear_product(M, N, K, A, B, o, exact, device_context().d_err, tpp->stream));
-      };
-      if (dx) product(im, ik, in, {g, n, false}, {w->data->ptr, wt ? k : n, wt}, dx);
-      if (dw && !wt) product(ik, in, im, {x->data->ptr, k, true}, {g, n, true}, dw);
-      if (dw && wt) product(in, ik, im, {g, n, true}, {x->data->ptr, k, true}, dw);
+      if (float* dr = at_res ? grad_of(at_res) : nullptr) tpp->add_into(dr, dc, m * n);
+      LinearBackward g{};
+      g.m = im;
+      g.n = in;
+      g.k = ik;
+      g.a = x->data->ptr;
+      g.lda = g.ldda = k;
+      g.b = w->data->ptr;
+      g.ldb = g.lddb = wt ? k : n;
+      g.b_mn_major = !wt;
+      g.act = activation;
+      g.drop = dropout_of(words, p, in);
+      g.z = z ? z->ptr : nullptr;
+      g.dc = dc;
+      g.ldz = g.lddc = n;
+      g.da = grad_of(0);
+      g.db = grad_of(1);
+      g.dbias = at_bias ? grad_of(at_bias) : nullptr;
+      g.accumulate = true;
+      g.exact = exact;
+      Buf ws = workspace(*tpp, linear_backward_ws_bytes(im, in, ik, exact));
+      linear_status(linear_backward(g, ws->ptr, device_context().d_err, tpp->stream));
     })->id;
   });
 }

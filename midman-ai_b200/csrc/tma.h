@@ -11,4 +11,8 @@ namespace mm {
 int encode_tensor_map(CUtensorMap* map, const float* ptr, int rank, const long long* dims, const long long* strides,
                       const int* box, bool mn_major);
 
+// The same for f16 values with a 128-byte swizzle of 16-byte chunks (K-major).
+int encode_tensor_map_f16(CUtensorMap* map, const void* ptr, int rank, const long long* dims,
+                          const long long* strides, const int* box);
+
 }  // namespace mm
