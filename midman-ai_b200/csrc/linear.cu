@@ -321,6 +321,7 @@ struct LinearDirect {
       seed = e.drop.rng[0];
       offset = e.drop.rng[1];
     }
+    const float4 bias = bias_quad(e, col, N);
     constexpr int U = 4;
     for (int i = warp * PER + lane / (BN / 4); i < nr; i += U * warps * PER) {
       float4 v[U], r[U];
@@ -336,7 +337,7 @@ struct LinearDirect {
       for (int u = 0; u < U; ++u) {
         const int j = i + u * warps * PER;
         const long long row = m0 + r0 + j;
-        if (j < nr && row < M && col < N) linear_quad(e, seed, offset, row, col, N, v[u], r[u]);
+        if (j < nr && row < M && col < N) linear_quad(e, e.act, e.drop.rng != nullptr, seed, offset, row, col, N, v[u], bias, r[u]);
       }
     }
   }

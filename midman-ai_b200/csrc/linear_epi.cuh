@@ -11,23 +11,45 @@
 
 namespace mm {
 
+// The normal distribution function and its density, branch-free (the epilogue runs on
+// few warps, so a divergent erff costs both of its paths): C. Hastings' rational
+// approximation of erfc (Abramowitz and Stegun, 7.1.26), at most 0.75e-7 off, taken
+// on the side where nothing cancels.
+__device__ __forceinline__ float normal_cdf(float z, float* density) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+  const float e = ex2_approx(z * z * -0.72134752044448170f);  // exp(-z^2 / 2)
+  const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
+                              0.254829592f);
+  const float tail = 0.5f * poly * e;
+  *density = 0.39894228040143268f * e;
+  return z >= 0.0f ? 1.0f - tail : tail;
+}
+__device__ __forceinline__ float logistic(float z) {
+  return __fdividef(1.0f, 1.0f + ex2_approx(z * -1.4426950408889634f));  // 0 where the exponential overflows
+}
+
 __device__ __forceinline__ float activate(float z, int act) {
+  float density;
   switch (act) {
     case kActRelu: return fmaxf(z, 0.0f);
-    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case kActSilu: return z / (1.0f + expf(-z));
+    case kActGelu: return z * normal_cdf(z, &density);
+    case kActSilu: return z * logistic(z);
     default: return z;
   }
 }
 
 // d act / dz
 __device__ __forceinline__ float activate_slope(float z, int act) {
+  float density;
   switch (act) {
     case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
-    case kActGelu:
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+    case kActGelu: {
+      const float cdf = normal_cdf(z, &density);
+      return fmaf(z, density, cdf);
+    }
     case kActSilu: {
-      const float s = 1.0f / (1.0f + expf(-z));
+      const float s = logistic(z);
       return s * (1.0f + z * (1.0f - s));
     }
     default: return 1.0f;
@@ -62,21 +84,22 @@ __device__ __forceinline__ void store_each(float* row, int col, int n, float4 v)
   if (col + 2 < n) row[col + 2] = v.z;
   if (col + 3 < n) row[col + 3] = v.w;
 }
-// v: the product's four columns; r: the residual's (loaded by the caller before
-// anything of the batch is stored, so that r may be c).
-__device__ __forceinline__ void linear_quad(const LinearEpilogue& e, uint64_t seed, uint64_t offset, long long row,
-                                            int col, int n, float4 v, float4 r) {
-  if (e.bias) {
-    const float4 b = load_each(e.bias, col, n);
-    v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
-  }
+// v: the product's four columns; bias and r: the bias's and the residual's (r loaded by
+// the caller before anything of the batch is stored, so that it may be c).
+__device__ __forceinline__ void linear_quad(const LinearEpilogue& e, int act, bool drop, uint64_t seed,
+                                            uint64_t offset, long long row, int col, int n, float4 v, float4 bias,
+                                            float4 r) {
+  v.x += bias.x; v.y += bias.y; v.z += bias.z; v.w += bias.w;
   if (e.Z) store_quad(e.Z + row * e.ldz, col, n, v);
-  if (e.act != kActNone) {
-    v.x = activate(v.x, e.act); v.y = activate(v.y, e.act); v.z = activate(v.z, e.act); v.w = activate(v.w, e.act);
+  if (act != kActNone) {
+    v.x = activate(v.x, act); v.y = activate(v.y, act); v.z = activate(v.z, act); v.w = activate(v.w, act);
   }
-  if (e.drop.rng) v = dropout_quad(v, e.drop, seed, offset, row, col >> 2);
+  if (drop) v = dropout_quad(v, e.drop, seed, offset, row, col >> 2);
   v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
   store_quad(e.C + row * e.ldc, col, n, v);
+}
+__device__ __forceinline__ float4 bias_quad(const LinearEpilogue& e, int col, int n) {
+  return e.bias ? load_each(e.bias, col, n) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 // e^x for the softmax: 2^(x log2 e) on the special-function unit, 2^-22 relative.

@@ -399,9 +399,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
       float sum[128];
 #pragma unroll
       for (int e = 0; e < 128; ++e) sum[e] = 0.0f;
+      // The chunks' inverse scales, one chunk ahead: this lane's row's in a register,
+      // the columns' through the staging tile (idle until the epilogue).
+      const float* pa = inv_a + w.cb * ld_ia + wrow0 + lane;
+      const float4* pb = reinterpret_cast<const float4*>(inv_b + w.cb * ld_ib + wcol0) + lane;
+      float ia = __ldg(pa);
+      stage_tile[lane] = __ldg(pb);
+      __syncwarp();
       for (int c = w.cb; c < w.ce; ++c) {
-        const float ia = __ldg(inv_a + c * ld_ia + wrow0 + lane);
-        const float4* ib = reinterpret_cast<const float4*>(inv_b + c * ld_ib + wcol0);
+        const float4* ib = stage_tile + 32 * ((c - w.cb) & 1);
+        const bool more = c + 1 < w.ce;
+        pa += ld_ia;
+        pb += ld_ib / 4;
+        const float ia_next = more ? __ldg(pa) : 0.0f;
+        const float4 ib_next = more ? __ldg(pb) : make_float4(0.f, 0.f, 0.f, 0.f);
         const int buf = j & 1;
         if (!mbar_wait(acc_full(buf), (j >> 1) & 1, err, kErrWaitAccum)) {
           ok = false;
@@ -413,7 +424,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         for (int q = 0; q < 8; ++q) {
           float4 b[4];  // the columns' inverse scales, the same for every lane
 #pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = __ldg(ib + q * 4 + e);
+          for (int e = 0; e < 4; ++e) b[e] = ib[q * 4 + e];
           uint32_t r[16];
           tmem_ld_32x32b_x16(acc + q * 16, r);
 #pragma unroll
@@ -429,6 +440,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_remote(mapa_shared(acc_empty(buf), 0));
         ++j;
+        ia = ia_next;
+        stage_tile[32 * ((c + 1 - w.cb) & 1) + lane] = ib_next;
+        __syncwarp();
       }
       if (!ok) break;
       if (w.slot < 0) {
@@ -473,29 +487,42 @@ __device__ __forceinline__ void stage_rows(const float* v, float4* stage_tile, i
     stage_tile[lane * 8 + (g ^ (lane & 7))] = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
 }
 
+template <int ACT, bool DROP>
 struct LinearPair {
   LinearEpilogue e;
-  __device__ __forceinline__ void tile(const float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
+  __device__ __forceinline__ void tile(float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
                                        int lane) const {
     const int sub = lane & 7, rsub = lane >> 3;
     uint64_t seed = 0, offset = 0;
-    if (e.drop.rng) {
+    if (DROP) {
       seed = e.drop.rng[0];
       offset = e.drop.rng[1];
     }
-#pragma unroll
+    // A rolled loop over slices of 32 columns (the unrolled one outgrows the
+    // instruction cache): the first slice goes through the staging tile, the rest
+    // move down. The staged slice's registers then hold residuals.
+#pragma unroll 1
     for (int c = 0; c < 4; ++c) {
-      stage_rows(sum + 32 * c, stage_tile, lane);
-      __syncwarp();
+      stage_rows(sum, stage_tile, lane);
+#pragma unroll
+      for (int i = 0; i < 96; ++i) sum[i] = sum[i + 32];
       const int col = n0 + 32 * c + 4 * sub;
-#pragma unroll 2
-      for (int it = 0; it < 8; ++it) {
-        const int rr = it * 4 + rsub;
-        const long long row = wrow0 + rr;
-        const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
-        if (row < M && col < N) {
-          const float4 r = e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
-          linear_quad(e, seed, offset, row, col, N, v, r);
+      const float4 bias = bias_quad(e, col, N);
+      __syncwarp();
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        float4 r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const long long row = wrow0 + (4 * h + i) * 4 + rsub;
+          r[i] = e.R && row < M && col < N ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rr = (4 * h + i) * 4 + rsub;
+          const long long row = wrow0 + rr;
+          const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
+          if (row < M && col < N) linear_quad(e, ACT, DROP, seed, offset, row, col, N, v, bias, r[i]);
         }
       }
       __syncwarp();  // before the next slice overwrites the staging tile
@@ -520,12 +547,14 @@ __global__ void __launch_bounds__(256) reduce_kernel(const PairWork work, const 
     v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
   }
   const float4 res = e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
-  linear_quad(e, e.drop.rng ? e.drop.rng[0] : 0, e.drop.rng ? e.drop.rng[1] : 0, row, col, N, v, res);
+  const bool drop = e.drop.rng != nullptr;
+  linear_quad(e, e.act, drop, drop ? e.drop.rng[0] : 0, drop ? e.drop.rng[1] : 0, row, col, N, v, bias_quad(e, col, N),
+              res);
 }
 
 struct LossPair {
   LossEpilogue e;
-  __device__ __forceinline__ void tile(const float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
+  __device__ __forceinline__ void tile(float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
                                        int lane) const {
     if (n0 >= N) return;  // uniform over the warp
     const long long my_row = wrow0 + lane;
@@ -620,6 +649,22 @@ int launch_pair(const SplitCopy& A, const SplitCopy& B, const Epi& epi, const Pa
   return 0;
 }
 
+template <int ACT>
+int launch_act(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e, const PairWork& work, int* d_err,
+               cudaStream_t s) {
+  return e.drop.rng ? launch_pair(A, B, LinearPair<ACT, true>{e}, work, d_err, s)
+                    : launch_pair(A, B, LinearPair<ACT, false>{e}, work, d_err, s);
+}
+int launch_linear(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e, const PairWork& work, int* d_err,
+                  cudaStream_t s) {
+  switch (e.act) {
+    case kActRelu: return launch_act<kActRelu>(A, B, e, work, d_err, s);
+    case kActGelu: return launch_act<kActGelu>(A, B, e, work, d_err, s);
+    case kActSilu: return launch_act<kActSilu>(A, B, e, work, d_err, s);
+    default: return launch_act<kActNone>(A, B, e, work, d_err, s);
+  }
+}
+
 bool same_k(const SplitCopy& A, const SplitCopy& B) {
   return A.k == B.k && A.k > 0 && tiles_of(A.rows, B.rows) <= (1 << 26);
 }
@@ -667,7 +712,7 @@ int pair_product(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e
   const long long tiles = tiles_of(A.rows, B.rows);
   PairWork work = work_of(tiles, static_cast<int>(A.chunks()));
   work.ws = static_cast<float*>(ws);
-  const int rc = launch_pair(A, B, LinearPair{e}, work, d_err, s);
+  const int rc = launch_linear(A, B, e, work, d_err, s);
   if (rc || work.full == tiles) return rc;
   reduce_kernel<<<dim3(static_cast<unsigned>(tiles - work.full), 2 * BM / 4), 256, 0, s>>>(work, e, A.rows, B.rows);
   check_cuda(cudaGetLastError(), "linear");
