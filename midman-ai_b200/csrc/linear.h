@@ -54,6 +54,18 @@ struct SplitCopy {
 long long split_copy_bytes(int rows, int k);
 SplitCopy split_copy_at(void* ptr, int rows, int k);  // ptr 256-byte aligned
 
+// Lays a workspace out front to back, in 256-byte steps; with a null base it only counts.
+struct Arena {
+  uint8_t* base;
+  long long at = 0;
+  void* take(long long bytes) {
+    void* p = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  }
+  SplitCopy copy(int rows, int k) { return split_copy_at(take(split_copy_bytes(rows, k)), rows, k); }
+};
+
 // What a split reads: a matrix; the epilogue's backward (dz of act_backward); or
 // the loss's gradient G from its logits.
 struct SplitMatrix {

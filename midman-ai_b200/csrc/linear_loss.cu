@@ -16,43 +16,71 @@
 
 #include "device.h"
 #include "linear.h"
+#include "linear_epi.cuh"
 #include "ptx.cuh"
 
 namespace mm {
 namespace {
 
-constexpr long long kLogitBytes = 256ll << 20;  // a block's logits
+constexpr long long kLogitBytes = 256ll << 20;  // a block's logits, or half as much as w if that is more
 constexpr long long kPartBytes = 64ll << 20;    // a block's (max, sum) pairs, the loss alone
 
 long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
 
 struct Plan {
+  bool pair;        // pair products on copies, or direct ones
   int tiles, rows;  // (max, sum) pairs per row; rows of a block
   long long ldz, ldx;
-  long long part, zt, z, x, total;  // byte offsets into the workspace
+  float2* part;
+  float2* stat;
+  float* zt;
+  float* z;
+  float* x;                                  // direct: the live rows of x
+  SplitCopy w, wt, xr, xt, g, gt;            // pair: [vocab, dim], [dim, vocab], and of a block [n, dim], [dim, n],
+  void *xr_at, *xt_at, *g_at, *gt_at, *parts;  // [n, vocab], [vocab, n] (a block may be shorter)
+  long long bytes;
 };
 
-Plan plan_of(int rows, int vocab, int dim, bool grad) {
+Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* ws) {
   Plan p{};
+  const bool grad = dx || dw;
+  Arena at{static_cast<uint8_t*>(ws)};
   p.tiles = (vocab + 127) / 128;
   p.ldz = round_up(vocab, 4);
   p.ldx = round_up(dim, 4);
-  long long r = grad ? kLogitBytes / (p.ldz * 4) : kPartBytes / (p.tiles * 8ll);
-  r = std::max(256ll, r / 256 * 256);  // whole tiles of rows
-  p.rows = static_cast<int>(std::min<long long>(r, std::max(rows, 1)));
-  long long at = 0;
-  auto take = [&](long long bytes) {
-    const long long here = at;
-    at += round_up(bytes, 256);
-    return here;
-  };
-  p.part = take(static_cast<long long>(p.rows) * p.tiles * 8);
-  p.zt = take(p.rows * 4ll);
-  if (grad) {
-    p.z = take(p.rows * p.ldz * 4);
-    p.x = take(p.rows * p.ldx * 4);
+  const long long logits = std::max(kLogitBytes, 2ll * vocab * dim);
+  const long long most = std::max(256ll, (grad ? logits / (p.ldz * 4) : kPartBytes / (p.tiles * 8ll)) / 256 * 256);
+  const long long n = std::max(rows, 1), blocks = (n + most - 1) / most;
+  p.rows = static_cast<int>(std::min(n, round_up((n + blocks - 1) / blocks, 256)));  // even blocks of whole tiles
+  p.pair = exact && pair_product_suits(p.rows, vocab, dim) &&
+           (!grad || (pair_product_suits(p.rows, dim, vocab) && pair_product_suits(vocab, dim, p.rows)));
+  p.part = static_cast<float2*>(at.take(static_cast<long long>(p.rows) * p.tiles * 8));
+  p.zt = static_cast<float*>(at.take(p.rows * 4ll));
+  p.stat = static_cast<float2*>(at.take(p.rows * 8ll));
+  if (grad) p.z = static_cast<float*>(at.take(p.rows * p.ldz * 4));
+  if (p.pair) {
+    p.w = at.copy(vocab, dim);
+    p.xr_at = at.take(split_copy_bytes(p.rows, dim));
+    if (dx) {
+      p.wt = at.copy(dim, vocab);
+      p.g_at = at.take(split_copy_bytes(p.rows, vocab));
+    }
+    if (dw) {
+      p.xt_at = at.take(split_copy_bytes(dim, p.rows));
+      p.gt_at = at.take(split_copy_bytes(vocab, p.rows));
+    }
+    // the last block may be shorter: its products may be cut into parts that the others are not
+    const int last = static_cast<int>(n - (blocks - 1) * p.rows);
+    long long parts = 0;
+    for (const int r : {p.rows, std::max(last, 1)}) {
+      if (dx) parts = std::max(parts, pair_ws_bytes(r, dim, vocab));
+      if (dw) parts = std::max({parts, pair_ws_bytes(vocab, dim, r), pair_ws_bytes(dim, vocab, r)});
+    }
+    p.parts = at.take(parts);
+  } else if (dw) {
+    p.x = static_cast<float*>(at.take(p.rows * p.ldx * 4));
   }
-  p.total = at;
+  p.bytes = at.at;
   return p;
 }
 
@@ -80,8 +108,8 @@ __device__ __forceinline__ float loss_of(MaxSum a, int t, int vocab, const float
 }
 
 __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int tiles, const float* zt,
-                                                       const int32_t* targets, int rows, int vocab, float* row_loss,
-                                                       int* err) {
+                                                       const int32_t* targets, int rows, int vocab,
+                                                       float grad_scale, float* row_loss, float2* stat, int* err) {
   const int r = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   if (r >= rows) return;
   MaxSum a{-INFINITY, 0.0f};
@@ -90,7 +118,10 @@ __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int t
     a = join(a, {p.x, p.y});
   }
   a = warp_join(a);
-  if (lane == 0) row_loss[r] = loss_of(a, targets[r], vocab, zt + r, err);
+  if (lane == 0) {
+    row_loss[r] = loss_of(a, targets[r], vocab, zt + r, err);
+    if (stat) stat[r] = make_float2(a.m, grad_scale / a.s);
+  }
 }
 
 // One row's kSegment logits -> gradients, in place; every block of a row joins
@@ -122,7 +153,7 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) {
       const float4 v = row[q];
-      g = make_float4(expf(v.x - a.m) * coef, expf(v.y - a.m) * coef, expf(v.z - a.m) * coef, expf(v.w - a.m) * coef);
+      g = make_float4(loss_exp(v.x - a.m) * coef, loss_exp(v.y - a.m) * coef, loss_exp(v.z - a.m) * coef, loss_exp(v.w - a.m) * coef);
       if ((t >> 2) == q) {
         if ((t & 3) == 0) g.x -= grad_scale;
         if ((t & 3) == 1) g.y -= grad_scale;
@@ -193,66 +224,103 @@ __global__ void __launch_bounds__(1024) mean_live_kernel(const float* row_loss, 
 }  // namespace
 
 long long linear_loss_ws_bytes(int rows, int vocab, int dim, bool grad, bool exact) {
-  (void)exact;
-  return plan_of(rows, vocab, dim, grad).total;
+  return plan_of(rows, vocab, dim, grad, grad, exact, nullptr).bytes;
 }
+
+namespace {
+
+// One block of rows on copies. The copies of w are made before the first block.
+int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStream_t s) {
+  const float* x = a.x + r0 * a.ldx;
+  const int32_t* t = a.targets + r0;
+  p.xr = split_copy_at(p.xr_at, n, a.dim);
+  split(SplitMatrix{x, a.ldx}, n, a.dim, &p.xr, nullptr, s);
+  const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt};
+  int rc = pair_loss_product(p.xr, p.w, e, d_err, s);
+  if (rc) return rc;
+  row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(p.part, p.tiles, p.zt, t, n, a.vocab, a.grad_scale, a.row_loss + r0,
+                                              p.stat, d_err);
+  check_cuda(cudaGetLastError(), "row loss");
+  if (!a.dx && !a.dw) return 0;
+  if (a.dx) p.g = split_copy_at(p.g_at, n, a.vocab);
+  if (a.dw) p.gt = split_copy_at(p.gt_at, a.vocab, n);
+  split(SplitLoss{p.z, p.ldz, p.stat, t, a.vocab, a.grad_scale}, n, a.vocab, a.dx ? &p.g : nullptr,
+        a.dw ? &p.gt : nullptr, s);
+  if (a.dx) {
+    LinearEpilogue o;
+    o.C = a.dx + r0 * a.lddx;
+    o.R = a.accumulate ? o.C : nullptr;
+    o.ldc = o.ldr = a.lddx;
+    rc = pair_product(p.g, p.wt, o, p.parts, d_err, s);
+    if (rc) return rc;
+  }
+  if (a.dw) {
+    p.xt = split_copy_at(p.xt_at, a.dim, n);
+    split(SplitMatrix{x, a.ldx, t, a.vocab}, n, a.dim, nullptr, &p.xt, s);
+    LinearEpilogue o;
+    o.C = a.dw;
+    o.R = a.accumulate || r0 > 0 ? a.dw : nullptr;
+    o.ldc = o.ldr = a.lddw;
+    rc = a.w_mn_major ? pair_product(p.xt, p.gt, o, p.parts, d_err, s) : pair_product(p.gt, p.xt, o, p.parts, d_err, s);
+  }
+  return rc;
+}
+
+// One block of rows on direct products: G takes the logits' place.
+int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, cudaStream_t s) {
+  const float* x = a.x + r0 * a.ldx;
+  const int32_t* t = a.targets + r0;
+  const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt};
+  int rc = direct_loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
+  if (rc) return rc;
+  if (!a.dx && !a.dw) {
+    row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(p.part, p.tiles, p.zt, t, n, a.vocab, 0.0f, a.row_loss + r0, nullptr,
+                                                d_err);
+    check_cuda(cudaGetLastError(), "row loss");
+    return 0;
+  }
+  const dim3 grid(n, static_cast<unsigned>((p.ldz + kSegment - 1) / kSegment));
+  loss_grad_kernel<<<grid, 256, 0, s>>>(p.z, p.ldz, p.part, p.tiles, p.zt, t, a.vocab, a.grad_scale, a.row_loss + r0,
+                                        d_err);
+  check_cuda(cudaGetLastError(), "loss gradient");
+  if (a.dx) {
+    LinearEpilogue o;
+    o.C = a.dx + r0 * a.lddx;
+    o.R = a.accumulate ? o.C : nullptr;
+    o.ldc = o.ldr = a.lddx;
+    rc = direct_product(n, a.dim, a.vocab, {p.z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, d_err, s);
+    if (rc) return rc;
+  }
+  if (a.dw) {
+    live_rows_kernel<<<(n + 7) / 8, 256, 0, s>>>(x, a.ldx, t, n, a.dim, a.vocab, p.x, p.ldx);
+    check_cuda(cudaGetLastError(), "live rows");
+    LinearEpilogue o;
+    o.C = a.dw;
+    o.R = a.accumulate || r0 > 0 ? a.dw : nullptr;
+    o.ldc = o.ldr = a.lddw;
+    const GemmOperand g{p.z, p.ldz, true}, xo{p.x, p.ldx, true};
+    rc = a.w_mn_major ? direct_product(a.dim, a.vocab, n, xo, g, o, a.exact, d_err, s)
+                      : direct_product(a.vocab, a.dim, n, g, xo, o, a.exact, d_err, s);
+  }
+  return rc;
+}
+
+}  // namespace
 
 int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
   const bool grad = a.dx || a.dw;
-  const Plan p = plan_of(a.rows, a.vocab, a.dim, grad);
-  uint8_t* base = static_cast<uint8_t*>(ws);
-  float2* part = reinterpret_cast<float2*>(base + p.part);
-  float* zt = reinterpret_cast<float*>(base + p.zt);
-  float* z = grad ? reinterpret_cast<float*>(base + p.z) : nullptr;
-  float* xl = grad ? reinterpret_cast<float*>(base + p.x) : nullptr;
+  Plan p = plan_of(a.rows, a.vocab, a.dim, grad, grad, a.exact, ws);
+  if (p.pair) {
+    const SplitCopy* wt = a.dx ? &p.wt : nullptr;
+    if (a.w_mn_major)  // w is [dim, vocab]
+      split(SplitMatrix{a.w, a.ldw}, a.dim, a.vocab, wt, &p.w, s);
+    else
+      split(SplitMatrix{a.w, a.ldw}, a.vocab, a.dim, &p.w, wt, s);
+  }
   for (int r0 = 0; r0 < a.rows; r0 += p.rows) {
     const int n = std::min(p.rows, a.rows - r0);
-    const float* x = a.x + r0 * a.ldx;
-    const int32_t* t = a.targets + r0;
-    LossEpilogue e;
-    e.Z = z;
-    e.ldz = p.ldz;
-    e.part = part;
-    e.tiles = p.tiles;
-    e.targets = t;
-    e.zt = zt;
-    int rc = direct_loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
+    const int rc = p.pair ? pair_block(a, p, r0, n, d_err, s) : direct_block(a, p, r0, n, d_err, s);
     if (rc) return rc;
-    if (!grad) {
-      row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(part, p.tiles, zt, t, n, a.vocab, a.row_loss + r0, d_err);
-      check_cuda(cudaGetLastError(), "row loss");
-      continue;
-    }
-    const dim3 grid(n, static_cast<unsigned>((p.ldz + kSegment - 1) / kSegment));
-    loss_grad_kernel<<<grid, 256, 0, s>>>(z, p.ldz, part, p.tiles, zt, t, a.vocab, a.grad_scale, a.row_loss + r0,
-                                          d_err);
-    check_cuda(cudaGetLastError(), "loss gradient");
-    if (a.dx) {
-      LinearEpilogue o;
-      o.C = a.dx + r0 * a.lddx;
-      o.ldc = a.lddx;
-      if (a.accumulate) {
-        o.R = o.C;
-        o.ldr = a.lddx;
-      }
-      rc = direct_product(n, a.dim, a.vocab, {z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, d_err, s);
-      if (rc) return rc;
-    }
-    if (a.dw) {
-      live_rows_kernel<<<(n + 7) / 8, 256, 0, s>>>(x, a.ldx, t, n, a.dim, a.vocab, xl, p.ldx);
-      check_cuda(cudaGetLastError(), "live rows");
-      LinearEpilogue o;
-      o.C = a.dw;
-      o.ldc = a.lddw;
-      if (a.accumulate || r0 > 0) {
-        o.R = a.dw;
-        o.ldr = a.lddw;
-      }
-      const GemmOperand g{z, p.ldz, true}, xo{xl, p.ldx, true};
-      rc = a.w_mn_major ? direct_product(a.dim, a.vocab, n, xo, g, o, a.exact, d_err, s)
-                        : direct_product(a.vocab, a.dim, n, g, xo, o, a.exact, d_err, s);
-      if (rc) return rc;
-    }
   }
   if (a.mean_loss) {
     mean_live_kernel<<<1, 1024, 0, s>>>(a.row_loss, a.targets, a.rows, a.mean_loss);

@@ -9,18 +9,6 @@
 namespace mm {
 namespace {
 
-// Lays a workspace out front to back, in 256-byte steps; with a null base it only counts.
-struct Arena {
-  uint8_t* base;
-  long long at = 0;
-  void* take(long long bytes) {
-    void* p = base ? base + at : nullptr;
-    at += (bytes + 255) / 256 * 256;
-    return p;
-  }
-  SplitCopy copy(int rows, int k) { return split_copy_at(take(split_copy_bytes(rows, k)), rows, k); }
-};
-
 long long round4(long long n) { return (n + 3) & ~3ll; }
 
 struct ForwardPlan {

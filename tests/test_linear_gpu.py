@@ -329,7 +329,7 @@ def loss_case(g, rows, vocab, dim, tied, extra):
 # rows, vocab, dim, tied, extra, rows left out
 LOSS = [(1, 1, 4, True, 0, 0), (1, 5, 8, True, 0, 0), (3, 130, 33, False, 4, 1), (64, 1000, 64, True, 4, 5), (129, 4099, 96, False, 0, 0),
         (200, 513, 1030, True, 0, 199), (37, 32003, 260, True, 8, 3), (2049, 512, 128, False, 0, 100), (2304, 2305, 512, True, 0, 0),
-        (700, 131072, 40, True, 0, 9), (600, 120001, 36, False, 4, 9)]
+        (700, 131072, 40, True, 0, 9), (600, 120001, 36, False, 4, 9), (1100, 131073, 132, True, 4, 9), (777, 65537, 260, False, 0, 9)]
 
 
 @pytest.mark.parametrize("precision", [1, 0])
