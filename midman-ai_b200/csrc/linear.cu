@@ -291,87 +291,252 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
 template <int BN>
 __device__ __forceinline__ float4 sum_quad(uint32_t tile, int r, int q, int splits) {
   const uint32_t at = tile + 16u * static_cast<uint32_t>(r * (BN / 4) + (q ^ (r & 7)));
+  float4 v;
   if (splits == 1) {
-    float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                  : "r"(at)
                  : "memory");
     return v;
   }
-  float4 v = ld_cluster_quad(mapa_shared(at, 0));
-  for (int p = 1; p < splits; ++p) {
-    const float4 w = ld_cluster_quad(mapa_shared(at, p));
+  v = ld_cluster_quad(mapa_shared(at, 0));
+  if (splits == 2) {
+    const float4 w = ld_cluster_quad(mapa_shared(at, 1));
     v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    return v;
+  }
+  for (int p = 1; p < splits; p += 3) {  // 4 or 8 parts, at most three loads in flight
+    float4 w[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      w[i] = p + i < splits ? ld_cluster_quad(mapa_shared(at, p + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      v.x += w[i].x; v.y += w[i].y; v.z += w[i].z; v.w += w[i].w;
+    }
   }
   return v;
 }
 
 struct LinearDirect {
   LinearEpilogue e;
-  // Rows [r0, r0 + nr) of the tile; BN / 4 lanes per row, four rows of a lane at
-  // a time so that their residual loads are in flight together.
-  template <int BN>
-  __device__ __forceinline__ void rows(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
-                                       int warp, int lane, int warps) const {
-    constexpr int PER = 128 / BN;  // rows a warp covers at once
-    const int q = lane % (BN / 4), col = n0 + 4 * q;
+  // Rows [r0, r0 + nr) of the tile; BN / 4 lanes per row, four rows of a lane at a
+  // time so that their loads are in flight together. The tile inside the matrix
+  // (FULL) runs without bounds checks: the loop is bound by its instructions.
+  template <int BN, bool FULL>
+  __device__ __forceinline__ void run(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
+                                      int first, int step, int q) const {
+    const int col = n0 + 4 * q, n = FULL ? INT32_MAX : N;
     uint64_t seed = 0, offset = 0;
-    if (e.drop.rng) {
+    const bool drop = e.drop.rng != nullptr;
+    if (drop) {
       seed = e.drop.rng[0];
       offset = e.drop.rng[1];
     }
     const float4 bias = bias_quad(e, col, N);
     constexpr int U = 4;
-    for (int i = warp * PER + lane / (BN / 4); i < nr; i += U * warps * PER) {
+    for (int i = first; i < nr; i += U * step) {
       float4 v[U], r[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = i + u * warps * PER;
+        const int j = i + u * step;
         const long long row = m0 + r0 + j;
-        const bool live = j < nr && row < M && col < N;
+        const bool live = j < nr && (FULL || (row < M && col < N));
         v[u] = live ? sum_quad<BN>(tile, r0 + j, q, splits) : make_float4(0.f, 0.f, 0.f, 0.f);
-        r[u] = live && e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
+        r[u] = live && e.R ? load_quad(e.R + row * e.ldr, col, n) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = i + u * warps * PER;
+        const int j = i + u * step;
         const long long row = m0 + r0 + j;
-        if (j < nr && row < M && col < N) linear_quad(e, e.act, e.drop.rng != nullptr, seed, offset, row, col, N, v[u], bias, r[u]);
+        if (j < nr && (FULL || (row < M && col < N)))
+          linear_quad(e, e.act, drop, seed, offset, row, col, n, v[u], bias, r[u]);
       }
     }
+  }
+  template <int BN>
+  __device__ __forceinline__ void rows(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
+                                       int warp, int lane, int warps) const {
+    constexpr int PER = 128 / BN;  // rows a warp covers at once
+    const int q = lane % (BN / 4), first = warp * PER + lane / (BN / 4), step = warps * PER;
+    if (m0 + r0 + nr <= M && n0 + BN <= N)
+      run<BN, true>(tile, m0, n0, r0, nr, splits, M, N, first, step, q);
+    else
+      run<BN, false>(tile, m0, n0, r0, nr, splits, M, N, first, step, q);
   }
 };
 
 struct LossDirect {
   LossEpilogue e;
-  // A warp per row: its 128 columns' maximum and sum by shuffles.
+  // A warp per row, its 128 columns' maximum and sum by shuffles; three rows at a time.
   template <int BN>
   __device__ __forceinline__ void rows(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
                                        int warp, int lane, int warps) const {
     static_assert(BN == 128, "one partial per 128 columns");
     const int col = n0 + 4 * lane;
-    for (int i = warp; i < nr; i += warps) {
-      const long long row = m0 + r0 + i;
-      if (row >= M) break;  // uniform over the warp
-      const float4 v = sum_quad<BN>(tile, r0 + i, lane, splits);
-      float m = col < N ? quad_max(v, col, N) : -INFINITY;
+    constexpr int U = 3;
+    for (int i = warp; i < nr && m0 + r0 + i < M; i += U * warps) {  // uniform over the warp
+      float4 v[U];
+      float m[U], s[U];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      float s = 0.0f;
-      if (col < N) s += loss_exp(v.x - m);
-      if (col + 1 < N) s += loss_exp(v.y - m);
-      if (col + 2 < N) s += loss_exp(v.z - m);
-      if (col + 3 < N) s += loss_exp(v.w - m);
+      for (int u = 0; u < U; ++u) {
+        const int j = min(i + u * warps, nr - 1);
+        v[u] = sum_quad<BN>(tile, r0 + j, lane, splits);
+        m[u] = col < N ? quad_max(v[u], col, N) : -INFINITY;
+      }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) e.part[row * e.tiles + n0 / 128] = make_float2(m, s);
-      const int t = e.targets[row] - col;
-      if (t >= 0 && t < 4 && col + t < N) e.zt[row] = t == 0 ? v.x : t == 1 ? v.y : t == 2 ? v.z : v.w;
-      if (e.Z && col < N) store_quad(e.Z + row * e.ldz, col, N, v);
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], o));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[u] = 0.0f;
+        if (col < N) s[u] += loss_exp(v[u].x - m[u]);
+        if (col + 1 < N) s[u] += loss_exp(v[u].y - m[u]);
+        if (col + 2 < N) s[u] += loss_exp(v[u].z - m[u]);
+        if (col + 3 < N) s[u] += loss_exp(v[u].w - m[u]);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], o);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = i + u * warps;
+        const long long row = m0 + r0 + j;
+        if (j >= nr || row >= M) break;
+        if (lane == 0) e.part[row * e.tiles + n0 / 128] = make_float2(m[u], s[u]);
+        const int t = e.targets[row] - col;
+        if (t >= 0 && t < 4 && col + t < N) e.zt[row] = t == 0 ? v[u].x : t == 1 ? v[u].y : t == 2 ? v[u].z : v[u].w;
+        if (e.Z && col < N) store_quad(e.Z + row * e.ldz, col, N, v[u]);
+      }
     }
   }
 };
+
+// ------------------------------------------------------------------ few rows
+// Up to eight rows: bound by one reading of B, so the products are plain f32
+// multiply-adds on B as it streams by (a 128-row tensor-core tile would convert and
+// multiply 120 rows of nothing: one row of 2048 x 5632 took 30 us in it). A CTA
+// takes 128 columns (B [k, n]: a lane four columns, warps every eighth k) or 32
+// (B [n, k]: a warp four columns, lanes along k) and a part of K; a cluster's parts
+// meet in shared memory, in part order. A's values of 512 k at a time are kept in
+// shared memory.
+constexpr int kFewRows = 8;
+constexpr int kFewPiece = 512;
+
+template <int MT, bool B_MN>
+__global__ void __launch_bounds__(256) few_rows_kernel(const float* a, long long lda, const float* b, long long ldb,
+                                                       const LinearEpilogue e, int M, int N, int K, int splits) {
+  constexpr int COLS = B_MN ? 128 : 32;
+  __shared__ __align__(16) float as[kFewPiece * MT];
+  __shared__ __align__(16) float sums[(B_MN ? 8 : 1) * MT * COLS];  // [warps][MT][COLS], then [MT][COLS]
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int part = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int n0 = static_cast<int>(blockIdx.x) / splits * COLS;
+  const int units = (K + 31) / 32;  // parts are cut at multiples of 32
+  const int kb = static_cast<int>(static_cast<long long>(units) * part / splits) * 32;
+  const int ke = min(K, static_cast<int>(static_cast<long long>(units) * (part + 1) / splits) * 32);
+  float acc[MT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.0f;
+
+  for (int k0 = kb; k0 < ke; k0 += kFewPiece) {
+    const int kn = min(kFewPiece, ke - k0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kFewPiece * MT; i += 256) {
+      // B [k, n]: the rows of one k side by side; B [n, k]: k side by side
+      const int m = B_MN ? i % MT : i / kFewPiece, k = B_MN ? i / MT : i % kFewPiece;
+      as[i] = m < M && k < kn ? a[m * lda + k0 + k] : 0.0f;
+    }
+    __syncthreads();
+    if (B_MN) {
+      const int col = n0 + 4 * lane;
+      const float* row = b + (k0 + warp) * ldb;
+      const bool full = col + 3 < N;
+      if (col < N) {
+#pragma unroll 8
+        for (int k = warp; k < kn; k += 8, row += 8 * ldb) {
+          const float4 w = full ? __ldg(reinterpret_cast<const float4*>(row + col)) : load_each(row, col, N);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const float x = as[k * MT + m];
+            acc[m][0] = fmaf(x, w.x, acc[m][0]);
+            acc[m][1] = fmaf(x, w.y, acc[m][1]);
+            acc[m][2] = fmaf(x, w.z, acc[m][2]);
+            acc[m][3] = fmaf(x, w.w, acc[m][3]);
+          }
+        }
+      }
+    } else {
+      const int c0 = n0 + 4 * warp;
+#pragma unroll 4
+      for (int k = 4 * lane; k < kn; k += 128) {
+        float4 w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          w[c] = c0 + c < N ? load_quad(b + (c0 + c) * ldb + k0, k, kn) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const float4 x = *reinterpret_cast<const float4*>(as + m * kFewPiece + k);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            acc[m][c] = fmaf(x.x, w[c].x, acc[m][c]);
+            acc[m][c] = fmaf(x.y, w[c].y, acc[m][c]);
+            acc[m][c] = fmaf(x.z, w[c].z, acc[m][c]);
+            acc[m][c] = fmaf(x.w, w[c].w, acc[m][c]);
+          }
+        }
+      }
+    }
+  }
+  if (B_MN) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      reinterpret_cast<float4*>(sums)[(warp * MT + m) * 32 + lane] =
+          make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * COLS; i += 256) {
+      float s = sums[i];
+      for (int w = 1; w < 8; ++w) s += sums[w * MT * COLS + i];
+      sums[i] = s;
+    }
+  } else {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) acc[m][c] += __shfl_xor_sync(0xffffffffu, acc[m][c], o);
+      }
+    if (lane == 0)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        reinterpret_cast<float4*>(sums)[m * 8 + warp] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+  }
+  if (splits > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  const bool drop = e.drop.rng != nullptr;
+  for (int i = threadIdx.x * splits + part; i < MT * (COLS / 4); i += 256 * splits) {
+    const int row = i / (COLS / 4), q = i % (COLS / 4), col = n0 + 4 * q;
+    if (row >= M || col >= N) continue;
+    const uint32_t at = smem_u32(sums) + 16u * i;
+    float4 v = reinterpret_cast<const float4*>(sums)[i];
+    if (splits > 1) {
+      v = ld_cluster_quad(mapa_shared(at, 0));
+      for (int p = 1; p < splits; ++p) {
+        const float4 w = ld_cluster_quad(mapa_shared(at, p));
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+      }
+    }
+    const float4 r = e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
+    linear_quad(e, e.act, drop, drop ? e.drop.rng[0] : 0, drop ? e.drop.rng[1] : 0, row, col, N, v,
+                bias_quad(e, col, N), r);
+  }
+  if (splits > 1) cluster_sync();  // a peer may still be reading this CTA's part
+}
 
 // ------------------------------------------------------------------ backward of the epilogue
 // dz and the column sums' partials: 64 rows x 128 columns per block, a warp per
@@ -492,9 +657,11 @@ int operand_map(CUtensorMap* map, const GemmOperand& o, int mn, int k, int box, 
   return rc ? kGemmTensorMap : 0;
 }
 
-// How a product is cut: 128 x 64 tiles when even with K in eight parts the wider
-// ones would leave half of the SMs idle, and K in as many parts (a cluster's
-// CTAs) as fit the SMs beside one another, each at least four K steps.
+// How a product is cut: 128 x 64 tiles when even with K in parts the wider ones would
+// leave half of the SMs idle, and K in as many parts (a cluster's CTAs) as fit the SMs
+// beside one another, each at least four K steps. A cluster lies in one GPC, and
+// of clusters of eight only about fourteen fit the device at once (with sixteen the
+// last start when the first have ended): 2048 x 4096 x 128 in eight parts took 40 us.
 struct DirectPlan {
   int bn, splits;
 };
@@ -504,13 +671,29 @@ DirectPlan direct_plan(int M, int N, int K, bool any_bn) {
   DirectPlan p{128, 1};
   auto splits_of = [&](long long tiles) {
     int s = 1;
-    while (s < 8 && tiles * s * 2 <= sms && n_k / (2 * s) >= 4) s *= 2;
+    while (s < 8 && tiles * s * 2 <= (s == 4 ? 112 : sms) && n_k / (2 * s) >= 4) s *= 2;
     return s;
   };
   const long long t128 = tm * ((N + 127) / 128), t64 = tm * ((N + 63) / 64);
   if (any_bn && (N <= 64 || 2 * t128 * splits_of(t128) <= sms)) p.bn = 64;
   p.splits = splits_of(p.bn == 128 ? t128 : t64);
   return p;
+}
+
+template <class Kernel, class... Args>
+void launch_clusters(Kernel kern, long long tiles, int splits, int threads, int smem, cudaStream_t s, Args... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(splits);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), "linear");
 }
 
 template <int TERMS, bool A_MN, bool B_MN, int BN, class Epi>
@@ -532,20 +715,22 @@ int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& 
   }
   const long long tiles = static_cast<long long>((M + BM - 1) / BM) * ((N + BN - 1) / BN);
   if (tiles * splits > 0x7fffffffll) return kGemmBadArgument;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(splits);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
-  cfg.blockDim = dim3(TL::THREADS);
-  cfg.dynamicSmemBytes = TL::SMEM;
-  cfg.stream = s;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kern, ta, tb, epi, M, N, K, splits, (a3 ? 1 : 0) | (b3 ? 2 : 0), d_err),
-             "linear");
+  launch_clusters(kern, tiles, splits, TL::THREADS, TL::SMEM, s, ta, tb, epi, M, N, K, splits,
+                  (a3 ? 1 : 0) | (b3 ? 2 : 0), d_err);
   return 0;
+}
+
+template <int MT>
+void launch_few(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e,
+                cudaStream_t s) {
+  const long long tiles = B.mn_major ? (N + 127) / 128 : (N + 31) / 32;
+  int splits = 1;  // about four CTAs an SM, each at least 128 of K
+  while (splits < 8 && tiles * splits < 4 * 148 && K / (2 * splits) >= 128) splits *= 2;
+  if (B.mn_major)
+    launch_clusters(few_rows_kernel<MT, true>, tiles, splits, 256, 0, s, A.ptr, A.ld, B.ptr, B.ld, e, M, N, K, splits);
+  else
+    launch_clusters(few_rows_kernel<MT, false>, tiles, splits, 256, 0, s, A.ptr, A.ld, B.ptr, B.ld, e, M, N, K,
+                    splits);
 }
 
 template <int TERMS, int BN, class Epi>
@@ -573,6 +758,13 @@ DropoutArgs dropout_args(double p, const uint64_t* rng, int cols) {
 int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, int* d_err,
                    cudaStream_t s) {
   if (M <= 0 || N <= 0) return 0;
+  if (M <= kFewRows && !A.mn_major) {
+    if (M == 1) launch_few<1>(M, N, K, A, B, e, s);
+    else if (M == 2) launch_few<2>(M, N, K, A, B, e, s);
+    else if (M <= 4) launch_few<4>(M, N, K, A, B, e, s);
+    else launch_few<8>(M, N, K, A, B, e, s);
+    return 0;
+  }
   const DirectPlan p = direct_plan(M, N, K, true);
   const LinearDirect epi{e};
   if (exact)

@@ -730,7 +730,7 @@ int pair_loss_product(const SplitCopy& A, const SplitCopy& B, const LossEpilogue
 bool pair_product_suits(int M, int N, int K) {
   const PairWork w = work_of(tiles_of(M, N), (K + 127) / 128);
   const long long units = w.full + (tiles_of(M, N) - w.full) * w.splits;
-  return K >= 128 && units >= kPairs / 2;
+  return K >= 128 && units >= kPairs / 2 && 2e-9 * M * N * K >= 8.0;
 }
 
 }  // namespace mm

@@ -197,7 +197,8 @@ def _ptr(t) -> int | None:
 def _stream(stream) -> int | None:
     if stream is None:
         import torch
-        return torch.cuda.current_stream().cuda_stream
+        # the number alone: torch.cuda.current_stream() builds an object, 3 us against 0.1
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream
 
 
@@ -301,11 +302,9 @@ def _device_tensors(dtype_name, **tensors):
     import torch
     dtype, current = getattr(torch, dtype_name), torch.cuda.current_device()
     for name, t in tensors.items():
-        if t is None:
-            continue
-        if t.dtype is not dtype:
-            raise TypeError(f"{name} must be {dtype_name}, not {t.dtype}")
-        if t.get_device() != current:
+        if t is not None and (t.dtype is not dtype or t.get_device() != current):
+            if t.dtype is not dtype:
+                raise TypeError(f"{name} must be {dtype_name}, not {t.dtype}")
             raise ValueError(f"{name} is on {t.device}, and the current device is cuda:{current}")
 
 
