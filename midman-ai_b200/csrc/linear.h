@@ -98,6 +98,10 @@ void split(const SplitBackward& src, int rows, int cols, const SplitCopy* by_row
            float* part, cudaStream_t s);
 void split(const SplitLoss& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
            cudaStream_t s);
+// Two matrices in one launch.
+void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_by_rows, const SplitCopy* x_by_cols,
+               const SplitMatrix& y, int y_rows, int y_cols, const SplitCopy* y_by_rows, const SplitCopy* y_by_cols,
+               cudaStream_t s);
 inline int split_parts(int rows) { return (rows + 127) / 128; }
 
 // ws: pair_ws_bytes(A.rows, B.rows, A.k) bytes (a partial last wave's K parts).

@@ -67,11 +67,8 @@ int linear_forward(const LinearForward& f, void* ws, int* d_err, cudaStream_t s)
   const ForwardPlan p = forward_plan(f.m, f.n, f.k, f.exact, ws);
   if (!p.pair)
     return direct_product(f.m, f.n, f.k, {f.a, f.lda, false}, {f.b, f.ldb, f.b_mn_major}, f.e, f.exact, d_err, s);
-  split(SplitMatrix{f.a, f.lda}, f.m, f.k, &p.a, nullptr, s);
-  if (f.b_mn_major)
-    split(SplitMatrix{f.b, f.ldb}, f.k, f.n, nullptr, &p.b, s);
-  else
-    split(SplitMatrix{f.b, f.ldb}, f.n, f.k, &p.b, nullptr, s);
+  split_two({f.a, f.lda}, f.m, f.k, &p.a, nullptr, {f.b, f.ldb}, f.b_mn_major ? f.k : f.n, f.b_mn_major ? f.n : f.k,
+            f.b_mn_major ? nullptr : &p.b, f.b_mn_major ? &p.b : nullptr, s);
   return pair_product(p.a, p.b, f.e, p.parts, d_err, s);
 }
 
@@ -96,18 +93,20 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
       split(SplitBackward{f.dc, f.lddc, f.z, f.ldz, f.act, f.drop}, f.m, f.n, f.da ? &p.dz : nullptr,
             f.db ? &p.dzt : nullptr, f.dbias ? p.sums : nullptr, s);
     if (f.dbias) sum_parts(p.sums, split_parts(f.m), f.n, f.dbias, f.accumulate, s);
-    if (f.da) {
-      if (f.b_mn_major)
-        split(SplitMatrix{f.b, f.ldb}, f.k, f.n, &p.b, nullptr, s);
-      else
-        split(SplitMatrix{f.b, f.ldb}, f.n, f.k, nullptr, &p.b, s);
-      rc = pair_product(p.dz, p.b, da, p.parts, d_err, s);
-    }
-    if (f.db && !rc) {
-      split(SplitMatrix{f.a, f.lda}, f.m, f.k, nullptr, &p.at, s);
+    // b [k, n] by rows, or [n, k] by columns, for da; a by columns for db
+    const SplitMatrix a{f.a, f.lda}, b{f.b, f.ldb};
+    const int br = f.b_mn_major ? f.k : f.n, bc = f.b_mn_major ? f.n : f.k;
+    const SplitCopy *b_rows = f.b_mn_major ? &p.b : nullptr, *b_cols = f.b_mn_major ? nullptr : &p.b;
+    if (f.da && f.db)
+      split_two(b, br, bc, b_rows, b_cols, a, f.m, f.k, nullptr, &p.at, s);
+    else if (f.da)
+      split(b, br, bc, b_rows, b_cols, s);
+    else if (f.db)
+      split(a, f.m, f.k, nullptr, &p.at, s);
+    if (f.da) rc = pair_product(p.dz, p.b, da, p.parts, d_err, s);
+    if (f.db && !rc)
       rc = f.b_mn_major ? pair_product(p.at, p.dzt, db, p.parts, d_err, s)
                         : pair_product(p.dzt, p.at, db, p.parts, d_err, s);
-    }
     return rc;
   }
   const bool plain = f.act == kActNone && !f.drop.rng;  // dz is dc

@@ -25,6 +25,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <stdexcept>
 
 #include "device.h"
 #include "gemm.h"
@@ -38,32 +39,33 @@ namespace {
 
 // ------------------------------------------------------------------ split
 constexpr int kTile = 128;
-constexpr int kTileLd = kTile + 1;  // odd: a column's rows lie in different banks
-constexpr int kSplitSums = (8 * kTile + kTile) * 4;  // warps' column maxima or sums, scales
-constexpr int kSplitSmem = kSplitSums + kTile * kTileLd * 4;
+constexpr int kSplitSums = 8 * kTile * 4;  // the warps' column sums
+constexpr int kSplitSmem = kSplitSums + kTile * kTile * 4;
 
-// The power of two for a chunk whose largest magnitude is m: [2^14, 2^15) after
-// scaling; 1 for infinities, and clamped so that its inverse is a normal number.
-__device__ __forceinline__ float chunk_scale(float m, float* inv) {
-  const int ex = static_cast<int>(__float_as_uint(m) >> 23);  // biased; m >= 0
+// The power of two for a chunk whose largest magnitude has the bits m: [2^14, 2^15)
+// after scaling; 1 for infinities and NaN, and clamped so that its inverse is a
+// normal number.
+__device__ __forceinline__ float chunk_scale(uint32_t m, float* inv) {
+  const int ex = static_cast<int>(m >> 23);
   int se = ex == 255 ? 127 : 268 - max(ex, 1);
   se = min(se, 253);
   *inv = __uint_as_float(static_cast<uint32_t>(254 - se) << 23);
   return __uint_as_float(static_cast<uint32_t>(se) << 23);
 }
 
-__device__ __forceinline__ uint32_t pack(__half a, __half b) {
-  return static_cast<uint32_t>(__half_as_ushort(a)) | (static_cast<uint32_t>(__half_as_ushort(b)) << 16);
-}
+// Magnitudes compare as their bits do (a NaN above everything).
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // hi and lo of a pair of scaled values
 __device__ __forceinline__ void halves(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half hx = __float2half_rn(x), hy = __float2half_rn(y);
-  hi = pack(hx, hy);
-  lo = pack(__float2half_rn(x - __half2float(hx)), __float2half_rn(y - __half2float(hy)));
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// Sources: begin_row once per row of a warp, then load of the lane's four columns.
+// Sources: begin once, then load of a row's four columns.
 struct MatrixSource {
   SplitMatrix a;
   __device__ __forceinline__ void begin() {}
@@ -115,90 +117,117 @@ struct LossSource {
   }
 };
 
-// One 128 x 128 tile per block: a warp per row (16 of them), a lane four columns.
+// One 128 x 128 tile per block. By rows: a warp per row (16 each), a lane four columns.
+// By columns: the tile goes through shared memory, quad q of row r at r 32 +
+// (q ^ (r / 8 & 7)); a warp then takes a quad of columns, lane (c, j) column c and rows
+// 8 j.. of each 64 (eight j in eight different bank groups, so neither side has
+// conflicts), which are the 16 bytes of hi and of lo that it stores.
 template <class Source>
-__global__ void __launch_bounds__(256) split_kernel(Source src, int rows, int cols, SplitCopy by_rows,
-                                                    SplitCopy by_cols, float* part) {
-  extern __shared__ float split_smem[];
-  float* warp_max = split_smem;             // [8][128] column maxima, or column sums
-  float* col_scale = warp_max + 8 * kTile;  // [128]
-  float* tile = col_scale + kTile;          // [128][129], where the transposed copy is wanted
+__device__ __forceinline__ void split_tile(Source& src, int rows, int cols, const SplitCopy& by_rows,
+                                           const SplitCopy& by_cols, float* part, int tile_r, int tile_c) {
+  extern __shared__ __align__(16) float split_smem[];
+  float* sums = split_smem;                                            // [8][128]
+  float4* tile = reinterpret_cast<float4*>(split_smem + 8 * kTile);    // where the columns are wanted
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int r0 = blockIdx.y * kTile, c0 = blockIdx.x * kTile;
+  const int r0 = tile_r * kTile, c0 = tile_c * kTile;
   const int col = c0 + 4 * lane;
   src.begin();
-  float4 top = make_float4(0.f, 0.f, 0.f, 0.f), sum = top;
-#pragma unroll 4
-  for (int i = 0; i < kTile / 8; ++i) {
-    const int r = 8 * i + warp;
-    const long long row = r0 + r;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < rows && col < cols) v = src.load(row, col, cols);
-    if (by_cols.data) {
-      float* t = tile + r * kTileLd + 4 * lane;
-      t[0] = v.x; t[1] = v.y; t[2] = v.z; t[3] = v.w;
-      top.x = fmaxf(top.x, fabsf(v.x)); top.y = fmaxf(top.y, fabsf(v.y));
-      top.z = fmaxf(top.z, fabsf(v.z)); top.w = fmaxf(top.w, fabsf(v.w));
-    }
-    if (part) {
-      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-    }
-    if (by_rows.data) {
-      float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int U = 4;
+#pragma unroll 1
+  for (int i0 = 0; i0 < kTile / 8; i0 += U) {
+    float4 v[U];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (row < rows) {
-        float inv;
-        const float s = chunk_scale(m, &inv);
-        uint2 hi, lo;
-        halves(v.x * s, v.y * s, hi.x, lo.x);
-        halves(v.z * s, v.w * s, hi.y, lo.y);
-        uint16_t* out = by_rows.data + row * by_rows.row_halves() + blockIdx.x * 256ll + (lane / 16) * 128 +
-                        (lane % 16) * 4;
-        *reinterpret_cast<uint2*>(out) = hi;
-        *reinterpret_cast<uint2*>(out + 64) = lo;
-        if (lane == 0) by_rows.inv[blockIdx.x * by_rows.inv_ld() + row] = inv;
+    for (int u = 0; u < U; ++u) {
+      const long long row = r0 + 8 * (i0 + u) + warp;
+      v[u] = row < rows && col < cols ? src.load(row, col, cols) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = 8 * (i0 + u) + warp;
+      const long long row = r0 + r;
+      if (by_cols.data) tile[r * 32 + (lane ^ ((r >> 3) & 7))] = v[u];
+      if (part) {
+        sum.x += v[u].x; sum.y += v[u].y; sum.z += v[u].z; sum.w += v[u].w;
+      }
+      if (by_rows.data) {
+        const uint32_t m = __reduce_max_sync(
+            0xffffffffu, max(max(magnitude(v[u].x), magnitude(v[u].y)), max(magnitude(v[u].z), magnitude(v[u].w))));
+        if (row < rows) {
+          float inv;
+          const float s = chunk_scale(m, &inv);
+          uint2 hi, lo;
+          halves(v[u].x * s, v[u].y * s, hi.x, lo.x);
+          halves(v[u].z * s, v[u].w * s, hi.y, lo.y);
+          uint16_t* out =
+              by_rows.data + row * by_rows.row_halves() + tile_c * 256ll + (lane / 16) * 128 + (lane % 16) * 4;
+          *reinterpret_cast<uint2*>(out) = hi;
+          *reinterpret_cast<uint2*>(out + 64) = lo;
+          if (lane == 0) by_rows.inv[tile_c * by_rows.inv_ld() + row] = inv;
+        }
       }
     }
   }
   if (part) {  // column sums over the tile's rows, warps in order
-    float4* w = reinterpret_cast<float4*>(warp_max + warp * kTile) + lane;
-    *w = sum;
+    reinterpret_cast<float4*>(sums + warp * kTile)[lane] = sum;
     __syncthreads();
     if (threadIdx.x < kTile && c0 + static_cast<int>(threadIdx.x) < cols) {
       float s = 0.0f;
-      for (int k = 0; k < 8; ++k) s += warp_max[k * kTile + threadIdx.x];
-      part[static_cast<long long>(blockIdx.y) * cols + c0 + threadIdx.x] = s;
+      for (int k = 0; k < 8; ++k) s += sums[k * kTile + threadIdx.x];
+      part[static_cast<long long>(tile_r) * cols + c0 + threadIdx.x] = s;
     }
-    __syncthreads();
   }
   if (!by_cols.data) return;
-  reinterpret_cast<float4*>(warp_max + warp * kTile)[lane] = top;
   __syncthreads();
-  if (threadIdx.x < kTile) {
-    float m = 0.0f;
-    for (int k = 0; k < 8; ++k) m = fmaxf(m, warp_max[k * kTile + threadIdx.x]);
+  const int c = lane & 3, j = lane >> 2;
+#pragma unroll 1
+  for (int q = warp; q < 32 && c0 + 4 * q < cols; q += 8) {
+    const float* t = split_smem + 8 * kTile + 4 * (q ^ j) + c;
+    float v[16];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {  // row 64 (i / 8) + 8 j + i % 8: r / 8 & 7 is j
+      v[i] = t[(64 * (i / 8) + 8 * j + i % 8) * kTile];
+      m = max(m, magnitude(v[i]));
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     float inv;
-    col_scale[threadIdx.x] = chunk_scale(m, &inv);
-    if (c0 + static_cast<int>(threadIdx.x) < cols)
-      by_cols.inv[blockIdx.y * by_cols.inv_ld() + c0 + threadIdx.x] = inv;
-  }
-  __syncthreads();
-  // a warp per column: rows 2 lane, 2 lane + 1 of each 64
-  for (int i = 0; i < kTile / 8; ++i) {
-    const int c = 8 * i + warp;
-    if (c0 + c >= cols) break;  // uniform over the warp
-    const float s = col_scale[c];
-    uint16_t* out = by_cols.data + (c0 + c) * by_cols.row_halves() + blockIdx.y * 256ll + 2 * lane;
+    const float s = chunk_scale(m, &inv);
+    const int mine = c0 + 4 * q + c;
+    if (mine >= cols) continue;
+    uint16_t* out = by_cols.data + mine * by_cols.row_halves() + tile_r * 256ll + 8 * j;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float x = tile[(64 * h + 2 * lane) * kTileLd + c], y = tile[(64 * h + 2 * lane + 1) * kTileLd + c];
-      uint32_t hi, lo;
-      halves(x * s, y * s, hi, lo);
-      *reinterpret_cast<uint32_t*>(out + 128 * h) = hi;
-      *reinterpret_cast<uint32_t*>(out + 128 * h + 64) = lo;
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) halves(v[8 * h + 2 * i] * s, v[8 * h + 2 * i + 1] * s, hi[i], lo[i]);
+      *reinterpret_cast<uint4*>(out + 128 * h) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(out + 128 * h + 64) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
+    if (j == 0) by_cols.inv[tile_r * by_cols.inv_ld() + mine] = inv;
   }
+}
+
+template <class Source>
+__global__ void __launch_bounds__(256, 3) split_kernel(Source src, int rows, int cols, SplitCopy by_rows,
+                                                       SplitCopy by_cols, float* part) {
+  split_tile(src, rows, cols, by_rows, by_cols, part, blockIdx.y, blockIdx.x);
+}
+
+// Two matrices in one launch (a product's operands): the first's tiles, then the second's.
+struct MatrixJob {
+  MatrixSource src;
+  int rows, cols;
+  SplitCopy by_rows, by_cols;
+};
+__global__ void __launch_bounds__(256, 3) split_two_kernel(MatrixJob x, MatrixJob y) {
+  const int tiles_x = ((x.rows + kTile - 1) / kTile) * ((x.cols + kTile - 1) / kTile);
+  const bool first = static_cast<int>(blockIdx.x) < tiles_x;
+  MatrixJob& job = first ? x : y;
+  const int t = static_cast<int>(blockIdx.x) - (first ? 0 : tiles_x);
+  const int tc = (job.cols + kTile - 1) / kTile;
+  split_tile(job.src, job.rows, job.cols, job.by_rows, job.by_cols, nullptr, t / tc, t % tc);
 }
 
 template <class Source>
@@ -703,6 +732,29 @@ long long pair_ws_bytes(int M, int N, int K) {
   const long long tiles = tiles_of(M, N);
   const PairWork w = work_of(tiles, (K + 127) / 128);
   return (tiles - w.full) * w.splits * (2ll * BM * PN * 4);
+}
+
+void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_by_rows, const SplitCopy* x_by_cols,
+               const SplitMatrix& y, int y_rows, int y_cols, const SplitCopy* y_by_rows, const SplitCopy* y_by_cols,
+               cudaStream_t s) {
+  auto job = [](const SplitMatrix& m, int rows, int cols, const SplitCopy* r, const SplitCopy* c) {
+    return MatrixJob{{m}, rows, cols, r ? *r : SplitCopy{}, c ? *c : SplitCopy{}};
+  };
+  auto tiles = [](int rows, int cols) { return ((rows + 127ll) / 128) * ((cols + 127ll) / 128); };
+  const int smem = x_by_cols || y_by_cols ? kSplitSmem : kSplitSums;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (configured_device != dev) {
+    check_cuda(cudaFuncSetAttribute(split_two_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem),
+               "shared memory");
+    configured_device = dev;
+  }
+  const long long n = tiles(x_rows, x_cols) + tiles(y_rows, y_cols);
+  if (n > INT32_MAX) throw std::invalid_argument("a matrix is too large");
+  split_two_kernel<<<static_cast<unsigned>(n), 256, smem, s>>>(job(x, x_rows, x_cols, x_by_rows, x_by_cols),
+                                                               job(y, y_rows, y_cols, y_by_rows, y_by_cols));
+  check_cuda(cudaGetLastError(), "split");
 }
 
 int pair_product(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e, void* ws, int* d_err,
