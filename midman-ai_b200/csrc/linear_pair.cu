@@ -70,11 +70,12 @@ struct MatrixSource {
   SplitMatrix a;
   __device__ __forceinline__ void begin() {}
   __device__ __forceinline__ float4 load(long long row, int col, int cols) const {
+    const float4 v = load_quad(a.x + row * a.ld, col, cols);
     if (a.targets) {
       const int t = a.targets[row];
       if (t < 0 || t >= a.vocab) return make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    return load_quad(a.x + row * a.ld, col, cols);
+    return v;
   }
 };
 struct BackwardSource {
@@ -99,20 +100,23 @@ struct LossSource {
   SplitLoss a;
   __device__ __forceinline__ void begin() {}
   __device__ __forceinline__ float4 load(long long row, int col, int cols) const {
-    float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+    // the three loads side by side, whatever the target says
     const int t = a.targets[row];
-    if (t < 0 || t >= a.vocab) return g;
     const float2 st = a.stat[row];
     const float4 v = load_quad(a.z + row * a.ldz, col, cols);
-    g.x = loss_exp(v.x - st.x) * st.y;
-    if (col + 1 < cols) g.y = loss_exp(v.y - st.x) * st.y;
-    if (col + 2 < cols) g.z = loss_exp(v.z - st.x) * st.y;
-    if (col + 3 < cols) g.w = loss_exp(v.w - st.x) * st.y;
+    const bool live = t >= 0 && t < a.vocab;
+    float4 g;
+    g.x = live ? loss_exp(v.x - st.x) * st.y : 0.0f;
+    g.y = live && col + 1 < cols ? loss_exp(v.y - st.x) * st.y : 0.0f;
+    g.z = live && col + 2 < cols ? loss_exp(v.z - st.x) * st.y : 0.0f;
+    g.w = live && col + 3 < cols ? loss_exp(v.w - st.x) * st.y : 0.0f;
     const int d = t - col;
-    if (d == 0) g.x -= a.grad_scale;
-    if (d == 1) g.y -= a.grad_scale;
-    if (d == 2) g.z -= a.grad_scale;
-    if (d == 3) g.w -= a.grad_scale;
+    if (live && d >= 0 && d < 4) {
+      if (d == 0) g.x -= a.grad_scale;
+      if (d == 1) g.y -= a.grad_scale;
+      if (d == 2) g.z -= a.grad_scale;
+      if (d == 3) g.w -= a.grad_scale;
+    }
     return g;
   }
 };
@@ -253,12 +257,18 @@ void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_row
 // of the tile's A and of its B; a stage is 64 of K: Ah, Al, Bh, Bl, 16 KB each, a
 // chunk two stages. Per stage a CTA takes in 64 KB and its tensor core reads 3 x
 // 48 KB in 1,536 cycles: 135 bytes a cycle of shared memory, so the tensor pipe
-// stays above 90% busy. Warp 0 TMA, warp 1 UMMA (the leader's), warps 2..9 the
-// running sums (TMEM lanes 32 (w % 4).., columns 128 ((w - 2) / 4)..) and the
+// stays above 90% busy. Warp 0 TMA, warp 1 UMMA (the leader's), warps 4..11 the
+// running sums (TMEM lanes 32 (w % 4).., columns 128 ((w - 4) / 4)..) and the
 // epilogue; the chunks' two TMEM accumulators let the next tile's first two chunks
 // run beside it.
 constexpr int BM = 128, PN = 256;
-constexpr int P_THREADS = 320;
+constexpr int P_THREADS = 384;
+constexpr int P_SUM_WARP = 4;  // the first of the eight warps that sum and write
+// Registers: a launch of 384 threads has 168 a thread; warps 0..3 (TMA, UMMA, two
+// idle) give up all but 40, and the summing warps take 232 (40 + 2 x 232 = 3 x 168),
+// which holds 128 sums, the residuals and the epilogue without spills.
+constexpr int P_REGS = 168, P_REGS_FEW = 40, P_REGS_SUM = 232;
+static_assert(P_REGS_FEW + 2 * P_REGS_SUM <= 3 * P_REGS, "setmaxnreg draws on the launch's registers");
 constexpr int P_STAGES = 3;
 constexpr int P_TILE = 16384;
 constexpr int P_STAGE = 4 * P_TILE;
@@ -344,8 +354,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < P_SUM_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P_REGS_FEW));
+    if (warp == 0 && lane == 0) {
       // ---------------- TMA producer (both CTAs); completions land on the leader's barriers
       int it = 0;
       bool ok = true;
@@ -369,9 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
           *loads_issued = it + 1;
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    } else if (warp == 1 && lane == 0 && leader) {
       // ---------------- UMMA issuer (leader only), M = 256 across the pair
       constexpr uint32_t idesc = idesc_f16(2 * BM, PN);
       int it = 0, j = 0;
@@ -415,9 +424,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P_REGS_SUM));
     // ---------------- running sums and epilogue (both CTAs): 32 rows x 128 columns per warp
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    float4* stage_tile = reinterpret_cast<float4*>(smem + P_STAGES * P_STAGE + 256) + (warp - 2) * 256;
+    const int quarter = warp & 3, half = (warp - P_SUM_WARP) >> 2;
+    float4* stage_tile = reinterpret_cast<float4*>(smem + P_STAGES * P_STAGE + 256) + (warp - P_SUM_WARP) * 256;
     int j = 0;
     bool ok = true;
     for (int u = pair; u < units && ok; u += npairs) {
@@ -435,6 +445,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
       float ia = __ldg(pa);
       stage_tile[lane] = __ldg(pb);
       __syncwarp();
+      if (w.slot < 0) epi.prefetch(wrow0, wcol0, M, N, lane);
       for (int c = w.cb; c < w.ce; ++c) {
         const float4* ib = stage_tile + 32 * ((c - w.cb) & 1);
         const bool more = c + 1 < w.ce;
@@ -450,19 +461,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         tc_fence_after();
         const uint32_t acc = tmem_base + buf * PN + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          float4 b[4];  // the columns' inverse scales, the same for every lane
+        for (int q = 0; q < 4; ++q) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(acc + q * 32, r);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = ib[q * 4 + e];
-          uint32_t r[16];
-          tmem_ld_32x32b_x16(acc + q * 16, r);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float* o = sum + q * 16 + 4 * e;
-            o[0] = fmaf(__uint_as_float(r[4 * e]) * ia, b[e].x, o[0]);
-            o[1] = fmaf(__uint_as_float(r[4 * e + 1]) * ia, b[e].y, o[1]);
-            o[2] = fmaf(__uint_as_float(r[4 * e + 2]) * ia, b[e].z, o[2]);
-            o[3] = fmaf(__uint_as_float(r[4 * e + 3]) * ia, b[e].w, o[3]);
+          for (int e = 0; e < 8; ++e) {
+            const float4 b = ib[q * 8 + e];  // the columns' inverse scales, the same for every lane
+            float* o = sum + q * 32 + 4 * e;
+            o[0] = fmaf(__uint_as_float(r[4 * e]) * ia, b.x, o[0]);
+            o[1] = fmaf(__uint_as_float(r[4 * e + 1]) * ia, b.y, o[1]);
+            o[2] = fmaf(__uint_as_float(r[4 * e + 2]) * ia, b.z, o[2]);
+            o[3] = fmaf(__uint_as_float(r[4 * e + 3]) * ia, b.w, o[3]);
           }
         }
         tc_fence_before();
@@ -519,6 +528,14 @@ __device__ __forceinline__ void stage_rows(const float* v, float4* stage_tile, i
 template <int ACT, bool DROP>
 struct LinearPair {
   LinearEpilogue e;
+  // The residual's rows into L2 while the sums form (a row's 128 columns: four lines).
+  __device__ __forceinline__ void prefetch(int wrow0, int n0, int M, int N, int lane) const {
+    if (!e.R || wrow0 + lane >= M) return;
+    const float* row = e.R + (wrow0 + lane) * e.ldr;
+#pragma unroll
+    for (int c = 0; c < 128; c += 32)
+      if (n0 + c < N) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + n0 + c));
+  }
   __device__ __forceinline__ void tile(float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
                                        int lane) const {
     const int sub = lane & 7, rsub = lane >> 3;
@@ -538,17 +555,18 @@ struct LinearPair {
       const int col = n0 + 32 * c + 4 * sub;
       const float4 bias = bias_quad(e, col, N);
       __syncwarp();
+      constexpr int U = 8;
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        float4 r[4];
+      for (int h = 0; h < 8 / U; ++h) {
+        float4 r[U];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const long long row = wrow0 + (4 * h + i) * 4 + rsub;
+        for (int i = 0; i < U; ++i) {
+          const long long row = wrow0 + (U * h + i) * 4 + rsub;
           r[i] = e.R && row < M && col < N ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rr = (4 * h + i) * 4 + rsub;
+        for (int i = 0; i < U; ++i) {
+          const int rr = (U * h + i) * 4 + rsub;
           const long long row = wrow0 + rr;
           const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
           if (row < M && col < N) linear_quad(e, ACT, DROP, seed, offset, row, col, N, v, bias, r[i]);
@@ -583,6 +601,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const PairWork work, const 
 
 struct LossPair {
   LossEpilogue e;
+  __device__ __forceinline__ void prefetch(int, int, int, int, int) const {}
   __device__ __forceinline__ void tile(float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
                                        int lane) const {
     if (n0 >= N) return;  // uniform over the warp
@@ -668,6 +687,10 @@ int launch_pair(const SplitCopy& A, const SplitCopy& B, const Epi& epi, const Pa
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   if (configured_device != dev) {
     check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM), "shared memory");
+    // fewer registers at launch than the kernel's setmaxnreg hands out would make it wait
+    cudaFuncAttributes fa{};
+    check_cuda(cudaFuncGetAttributes(&fa, kern), "kernel attributes");
+    if (fa.numRegs != P_REGS) throw std::runtime_error("linear: the pair kernel's registers do not match its split");
     configured_device = dev;
   }
   const long long tiles = tiles_of(A.rows, B.rows), units = work.full + (tiles - work.full) * work.splits;
