@@ -326,7 +326,7 @@ struct LinearDirect {
   template <int BN, bool FULL>
   __device__ __forceinline__ void run(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
                                       int first, int step, int q) const {
-    const int col = n0 + 4 * q, n = FULL ? INT32_MAX : N;
+    const int col = n0 + 4 * q;
     uint64_t seed = 0, offset = 0;
     const bool drop = e.drop.rng != nullptr;
     if (drop) {
@@ -343,14 +343,16 @@ struct LinearDirect {
         const long long row = m0 + r0 + j;
         const bool live = j < nr && (FULL || (row < M && col < N));
         v[u] = live ? sum_quad<BN>(tile, r0 + j, q, splits) : make_float4(0.f, 0.f, 0.f, 0.f);
-        r[u] = live && e.R ? load_quad(e.R + row * e.ldr, col, n) : make_float4(0.f, 0.f, 0.f, 0.f);
+        r[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live && e.R)
+          r[u] = FULL ? *reinterpret_cast<const float4*>(e.R + row * e.ldr + col) : load_quad(e.R + row * e.ldr, col, N);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = i + u * step;
         const long long row = m0 + r0 + j;
         if (j < nr && (FULL || (row < M && col < N)))
-          linear_quad(e, e.act, drop, seed, offset, row, col, n, v[u], bias, r[u]);
+          linear_quad<FULL>(e, e.act, drop, seed, offset, row, col, N, v[u], bias, r[u]);
       }
     }
   }

@@ -85,18 +85,27 @@ __device__ __forceinline__ void store_each(float* row, int col, int n, float4 v)
   if (col + 3 < n) row[col + 3] = v.w;
 }
 // v: the product's four columns; bias and r: the bias's and the residual's (r loaded by
-// the caller before anything of the batch is stored, so that it may be c).
+// the caller before anything of the batch is stored, so that it may be c). FULL: all
+// four columns lie inside, which leaves the unrolled loops one block of straight code.
+template <bool FULL>
+__device__ __forceinline__ void put_quad(float* row, int col, int n, float4 v) {
+  if (FULL)
+    *reinterpret_cast<float4*>(row + col) = v;
+  else
+    store_quad(row, col, n, v);
+}
+template <bool FULL = false>
 __device__ __forceinline__ void linear_quad(const LinearEpilogue& e, int act, bool drop, uint64_t seed,
                                             uint64_t offset, long long row, int col, int n, float4 v, float4 bias,
                                             float4 r) {
   v.x += bias.x; v.y += bias.y; v.z += bias.z; v.w += bias.w;
-  if (e.Z) store_quad(e.Z + row * e.ldz, col, n, v);
+  if (e.Z) put_quad<FULL>(e.Z + row * e.ldz, col, n, v);
   if (act != kActNone) {
     v.x = activate(v.x, act); v.y = activate(v.y, act); v.z = activate(v.z, act); v.w = activate(v.w, act);
   }
   if (drop) v = dropout_quad(v, e.drop, seed, offset, row, col >> 2);
   v.x += r.x; v.y += r.y; v.z += r.z; v.w += r.w;
-  store_quad(e.C + row * e.ldc, col, n, v);
+  put_quad<FULL>(e.C + row * e.ldc, col, n, v);
 }
 __device__ __forceinline__ float4 bias_quad(const LinearEpilogue& e, int col, int n) {
   return e.bias ? load_each(e.bias, col, n) : make_float4(0.f, 0.f, 0.f, 0.f);

@@ -536,17 +536,18 @@ struct LinearPair {
     for (int c = 0; c < 128; c += 32)
       if (n0 + c < N) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + n0 + c));
   }
-  __device__ __forceinline__ void tile(float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
-                                       int lane) const {
+  // A rolled loop over slices of 32 columns (the unrolled one outgrows the instruction
+  // cache): the first slice goes through the staging tile, the rest move down.
+  template <bool FULL>
+  __device__ __forceinline__ void slices(float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
+                                         int lane) const {
     const int sub = lane & 7, rsub = lane >> 3;
     uint64_t seed = 0, offset = 0;
     if (DROP) {
       seed = e.drop.rng[0];
       offset = e.drop.rng[1];
     }
-    // A rolled loop over slices of 32 columns (the unrolled one outgrows the
-    // instruction cache): the first slice goes through the staging tile, the rest
-    // move down. The staged slice's registers then hold residuals.
+    const long long row0 = wrow0 + rsub;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
       stage_rows(sum, stage_tile, lane);
@@ -554,26 +555,43 @@ struct LinearPair {
       for (int i = 0; i < 96; ++i) sum[i] = sum[i + 32];
       const int col = n0 + 32 * c + 4 * sub;
       const float4 bias = bias_quad(e, col, N);
+      float4 r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        r[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!e.R) continue;
+        const float* p = e.R + (row0 + 4 * i) * e.ldr;
+        if (FULL)
+          r[i] = *reinterpret_cast<const float4*>(p + col);
+        else if (row0 + 4 * i < M && col < N)
+          r[i] = load_quad(p, col, N);
+      }
       __syncwarp();
-      constexpr int U = 8;
-#pragma unroll 1
-      for (int h = 0; h < 8 / U; ++h) {
-        float4 r[U];
+      if (FULL) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-          const long long row = wrow0 + (U * h + i) * 4 + rsub;
-          r[i] = e.R && row < M && col < N ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-          const int rr = (U * h + i) * 4 + rsub;
-          const long long row = wrow0 + rr;
+        for (int i = 0; i < 8; ++i) {
+          const int rr = 4 * i + rsub;
           const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
-          if (row < M && col < N) linear_quad(e, ACT, DROP, seed, offset, row, col, N, v, bias, r[i]);
+          linear_quad<true>(e, ACT, DROP, seed, offset, row0 + 4 * i, col, N, v, bias, r[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = 4 * i + rsub;
+          const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
+          if (row0 + 4 * i < M && col < N)
+            linear_quad(e, ACT, DROP, seed, offset, row0 + 4 * i, col, N, v, bias, r[i]);
         }
       }
       __syncwarp();  // before the next slice overwrites the staging tile
     }
+  }
+  __device__ __forceinline__ void tile(float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
+                                       int lane) const {
+    if (wrow0 + 32 <= M && n0 + 128 <= N)
+      slices<true>(sum, stage_tile, wrow0, n0, M, N, lane);
+    else
+      slices<false>(sum, stage_tile, wrow0, n0, M, N, lane);
   }
 };
 
@@ -630,22 +648,29 @@ struct LossPair {
       }
     }
     if (!e.Z) return;
+    if (wrow0 + 32 <= M && n0 + 128 <= N)
+      store<true>(sum, stage_tile, wrow0, n0, M, N, lane);
+    else
+      store<false>(sum, stage_tile, wrow0, n0, M, N, lane);
+  }
+  template <bool FULL>
+  __device__ __forceinline__ void store(const float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
+                                        int lane) const {
     const int sub = lane & 7, rsub = lane >> 3;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      __syncwarp();
       stage_rows(sum + 32 * c, stage_tile, lane);
       __syncwarp();
       const int col = n0 + 32 * c + 4 * sub;
-#pragma unroll 4
-      for (int it = 0; it < 8; ++it) {
-        const int rr = it * 4 + rsub;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int rr = 4 * i + rsub;
         const long long row = wrow0 + rr;
         const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
-        if (row < M && col < N) store_quad(e.Z + row * e.ldz, col, N, v);
+        if (FULL || (row < M && col < N)) put_quad<FULL>(e.Z + row * e.ldz, col, N, v);
       }
+      __syncwarp();  // before the next slice overwrites the staging tile
     }
-    __syncwarp();
   }
 };
 
