@@ -420,73 +420,111 @@ struct LossDirect {
 // Up to eight rows: bound by one reading of B, so the products are plain f32
 // multiply-adds on B as it streams by (a 128-row tensor-core tile would convert and
 // multiply 120 rows of nothing: one row of 2048 x 5632 took 30 us in it). A CTA
-// takes 128 columns (B [k, n]: a lane four columns, warps every eighth k) or 32
-// (B [n, k]: a warp four columns, lanes along k) and a part of K; a cluster's parts
-// meet in shared memory, in part order. A's values of 512 k at a time are kept in
-// shared memory.
+// takes 32 columns and a part of K, a cluster's parts meet in shared memory, in part
+// order. B [k, n]: eight lanes hold the 32 columns of a k, a warp four k at a time,
+// eight loads in flight; B [n, k]: a warp takes four columns, its lanes lie along k.
+// A's values of 512 k at a time are kept in shared memory.
 constexpr int kFewRows = 8;
 constexpr int kFewPiece = 512;
+constexpr int kFewCols = 32;
+
+// v[0 .. n) summed over the warp's lanes; value i ends in the lanes whose top bits
+// (log2 n of them) spell i, in v[0]. Half of the values change hands at each step.
+template <int N_VALUES>
+__device__ __forceinline__ void warp_sums(float (&v)[N_VALUES], int lane) {
+  int o = 16;
+#pragma unroll
+  for (int n = N_VALUES; n > 1; n >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float give = up ? v[i] : v[i + n / 2], keep = up ? v[i + n / 2] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+#pragma unroll
+  for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+}
+
+constexpr int few_blocks(int mt) { return mt <= 4 ? 4 : 3; }  // CTAs of an SM, by registers
 
 template <int MT, bool B_MN>
-__global__ void __launch_bounds__(256) few_rows_kernel(const float* a, long long lda, const float* b, long long ldb,
+__global__ void __launch_bounds__(256, few_blocks(MT)) few_rows_kernel(const float* a, long long lda, const float* b, long long ldb,
                                                        const LinearEpilogue e, int M, int N, int K, int splits) {
-  constexpr int COLS = B_MN ? 128 : 32;
   __shared__ __align__(16) float as[kFewPiece * MT];
-  __shared__ __align__(16) float sums[(B_MN ? 8 : 1) * MT * COLS];  // [warps][MT][COLS], then [MT][COLS]
+  __shared__ __align__(16) float sums[(B_MN ? 8 : 1) * MT * kFewCols];  // [warps][MT][32], then [MT][32]
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int part = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int n0 = static_cast<int>(blockIdx.x) / splits * COLS;
+  const int n0 = static_cast<int>(blockIdx.x) / splits * kFewCols;
   const int units = (K + 31) / 32;  // parts are cut at multiples of 32
   const int kb = static_cast<int>(static_cast<long long>(units) * part / splits) * 32;
   const int ke = min(K, static_cast<int>(static_cast<long long>(units) * (part + 1) / splits) * 32);
-  float acc[MT][4];
+  float acc[4 * MT];  // [MT][4 columns]
 #pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.0f;
+  for (int i = 0; i < 4 * MT; ++i) acc[i] = 0.0f;
 
   for (int k0 = kb; k0 < ke; k0 += kFewPiece) {
     const int kn = min(kFewPiece, ke - k0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kFewPiece * MT; i += 256) {
-      // B [k, n]: the rows of one k side by side; B [n, k]: k side by side
-      const int m = B_MN ? i % MT : i / kFewPiece, k = B_MN ? i / MT : i % kFewPiece;
-      as[i] = m < M && k < kn ? a[m * lda + k0 + k] : 0.0f;
-    }
+    if (k0 > kb) __syncthreads();
+    // B [k, n]: the rows of one k side by side; B [n, k]: k side by side
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < kFewPiece / 256; ++h) {
+        const int k = threadIdx.x + 256 * h;
+        as[B_MN ? k * MT + m : m * kFewPiece + k] = m < M && k < kn ? a[m * lda + k0 + k] : 0.0f;
+      }
     __syncthreads();
     if (B_MN) {
-      const int col = n0 + 4 * lane;
-      const float* row = b + (k0 + warp) * ldb;
-      const bool full = col + 3 < N;
-      if (col < N) {
-#pragma unroll 8
-        for (int k = warp; k < kn; k += 8, row += 8 * ldb) {
-          const float4 w = full ? __ldg(reinterpret_cast<const float4*>(row + col)) : load_each(row, col, N);
+      const int col = n0 + 4 * (lane & 7), kl = 4 * warp + (lane >> 3);
+      auto add = [&](int k, float4 w) {
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            const float x = as[k * MT + m];
-            acc[m][0] = fmaf(x, w.x, acc[m][0]);
-            acc[m][1] = fmaf(x, w.y, acc[m][1]);
-            acc[m][2] = fmaf(x, w.z, acc[m][2]);
-            acc[m][3] = fmaf(x, w.w, acc[m][3]);
-          }
+        for (int m = 0; m < MT; ++m) {
+          const float x = as[k * MT + m];
+          acc[4 * m] = fmaf(x, w.x, acc[4 * m]);
+          acc[4 * m + 1] = fmaf(x, w.y, acc[4 * m + 1]);
+          acc[4 * m + 2] = fmaf(x, w.z, acc[4 * m + 2]);
+          acc[4 * m + 3] = fmaf(x, w.w, acc[4 * m + 3]);
         }
+      };
+      if (n0 + kFewCols <= N) {
+        for (int k = kl; k < kn; k += 256) {
+          float4 w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)  // past the piece: any row of it, not added
+            w[i] = __ldg(reinterpret_cast<const float4*>(b + (k0 + min(k + 32 * i, kn - 1)) * ldb + col));
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (k + 32 * i < kn) add(k + 32 * i, w[i]);
+        }
+      } else if (col < N) {
+        for (int k = kl; k < kn; k += 32) add(k, load_quad(b + (k0 + k) * ldb, col, N));
       }
     } else {
       const int c0 = n0 + 4 * warp;
-#pragma unroll 4
+      const bool whole = c0 + 4 <= N && kn % 128 == 0;
+      const float* col = b + c0 * ldb + k0;
+#pragma unroll 2
       for (int k = 4 * lane; k < kn; k += 128) {
         float4 w[4];
+        if (whole) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          w[c] = c0 + c < N ? load_quad(b + (c0 + c) * ldb + k0, k, kn) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c = 0; c < 4; ++c) w[c] = __ldg(reinterpret_cast<const float4*>(col + c * ldb + k));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            w[c] = c0 + c < N ? load_quad(col + c * ldb, k, kn) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const float4 x = *reinterpret_cast<const float4*>(as + m * kFewPiece + k);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            acc[m][c] = fmaf(x.x, w[c].x, acc[m][c]);
-            acc[m][c] = fmaf(x.y, w[c].y, acc[m][c]);
-            acc[m][c] = fmaf(x.z, w[c].z, acc[m][c]);
-            acc[m][c] = fmaf(x.w, w[c].w, acc[m][c]);
+            float& o = acc[4 * m + c];
+            o = fmaf(x.x, w[c].x, o);
+            o = fmaf(x.y, w[c].y, o);
+            o = fmaf(x.z, w[c].z, o);
+            o = fmaf(x.w, w[c].w, o);
           }
         }
       }
@@ -494,48 +532,51 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const float* a, long long
   }
   if (B_MN) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-      reinterpret_cast<float4*>(sums)[(warp * MT + m) * 32 + lane] =
-          make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+    for (int i = 0; i < 4 * MT; ++i) {  // the warp's four k
+      acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 8);
+      acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 16);
+    }
+    if (lane < 8)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        reinterpret_cast<float4*>(sums)[(warp * MT + m) * 8 + lane] =
+            make_float4(acc[4 * m], acc[4 * m + 1], acc[4 * m + 2], acc[4 * m + 3]);
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * COLS; i += 256) {
+    for (int i = threadIdx.x; i < MT * kFewCols; i += 256) {
       float s = sums[i];
-      for (int w = 1; w < 8; ++w) s += sums[w * MT * COLS + i];
+      for (int w = 1; w < 8; ++w) s += sums[w * MT * kFewCols + i];
       sums[i] = s;
     }
   } else {
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc[m][c] += __shfl_xor_sync(0xffffffffu, acc[m][c], o);
-      }
-    if (lane == 0)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        reinterpret_cast<float4*>(sums)[m * 8 + warp] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+    warp_sums(acc, lane);
+    constexpr int SAME = 32 / (4 * MT);  // lanes that hold the same value
+    const int i = lane / SAME;
+    if (lane % SAME == 0) sums[(i / 4) * kFewCols + 4 * warp + i % 4] = acc[0];
   }
   if (splits > 1)
     cluster_sync();
   else
     __syncthreads();
   const bool drop = e.drop.rng != nullptr;
-  for (int i = threadIdx.x * splits + part; i < MT * (COLS / 4); i += 256 * splits) {
-    const int row = i / (COLS / 4), q = i % (COLS / 4), col = n0 + 4 * q;
+  for (int i = threadIdx.x * splits + part; i < MT * (kFewCols / 4); i += 256 * splits) {
+    const int row = i / (kFewCols / 4), q = i % (kFewCols / 4), col = n0 + 4 * q;
     if (row >= M || col >= N) continue;
-    const uint32_t at = smem_u32(sums) + 16u * i;
+    const float4 r = e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 bias = bias_quad(e, col, N);
     float4 v = reinterpret_cast<const float4*>(sums)[i];
     if (splits > 1) {
-      v = ld_cluster_quad(mapa_shared(at, 0));
-      for (int p = 1; p < splits; ++p) {
-        const float4 w = ld_cluster_quad(mapa_shared(at, p));
-        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+      const uint32_t at = smem_u32(sums) + 16u * i;
+      float4 w[8];
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        w[p] = p < splits ? ld_cluster_quad(mapa_shared(at, p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v = w[0];
+#pragma unroll
+      for (int p = 1; p < 8; ++p) {
+        v.x += w[p].x; v.y += w[p].y; v.z += w[p].z; v.w += w[p].w;
       }
     }
-    const float4 r = e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
-    linear_quad(e, e.act, drop, drop ? e.drop.rng[0] : 0, drop ? e.drop.rng[1] : 0, row, col, N, v,
-                bias_quad(e, col, N), r);
+    linear_quad(e, e.act, drop, drop ? e.drop.rng[0] : 0, drop ? e.drop.rng[1] : 0, row, col, N, v, bias, r);
   }
   if (splits > 1) cluster_sync();  // a peer may still be reading this CTA's part
 }
@@ -725,9 +766,9 @@ int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& 
 template <int MT>
 void launch_few(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e,
                 cudaStream_t s) {
-  const long long tiles = B.mn_major ? (N + 127) / 128 : (N + 31) / 32;
-  int splits = 1;  // about four CTAs an SM, each at least 128 of K
-  while (splits < 8 && tiles * splits < 4 * 148 && K / (2 * splits) >= 128) splits *= 2;
+  const long long tiles = (N + kFewCols - 1) / kFewCols;
+  int splits = 1;  // parts that all run at once, each at least 256 of K
+  while (splits < 8 && tiles * splits * 2 <= few_blocks(MT) * 148 && K / (2 * splits) >= 256) splits *= 2;
   if (B.mn_major)
     launch_clusters(few_rows_kernel<MT, true>, tiles, splits, 256, 0, s, A.ptr, A.ld, B.ptr, B.ld, e, M, N, K, splits);
   else
