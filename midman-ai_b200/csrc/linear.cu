@@ -11,13 +11,17 @@
 // summed in f32 registers.
 //
 // direct_kernel: one 128 x BN tile per cluster of `splits` CTAs, each CTA a part
-// of K. TMA brings the f32 operands; four converter warps write the lo part of
-// each stage beside it (elementwise, so the swizzled layout is kept), which
-// saves the passes and the workspace of copies made beforehand: what short
-// products are bound by is latency and one reading of the weights. The parts'
-// sums meet in shared memory over the cluster (each CTA sums 128 / splits rows
-// of all parts, in part order: bit-identical run to run) and go through the
-// epilogue in whole rows.
+// of K. TMA brings the f32 operands. Their lo parts are made on the way, which saves
+// the passes and the workspace of copies made beforehand (short products are bound by
+// latency and one reading of the operands): four warps take A's rows to tensor
+// memory, hi and lo, where the UMMAs read them; two write B's lo part beside it in
+// shared memory (elementwise, so the swizzled layout is kept). What bounds a K step
+// of 32 of a 128 x 128 tile is shared memory: 32 KB in by TMA, 48 KB through the
+// converters, 48 KB read by the UMMAs, 1,024 cycles at 128 bytes each; 1,140 measured
+// (with A's parts in shared memory too 1,536 and 1,600; with four warps on B's lo part
+// instead of two nothing changed). The parts' sums meet in shared memory over the
+// cluster (each CTA sums 128 / splits rows of all parts, in part order: bit-identical
+// run to run) and go through the epilogue in whole rows.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -41,15 +45,23 @@ constexpr uint32_t MN_BLOCK_BYTES = BK * 128;
 constexpr int kEpiWarps = 8;
 
 // ------------------------------------------------------------------ direct kernel
+// A stage: A, then B, then (three terms) B's lo part. Three terms: warps 2, 3 write
+// B's lo, 4..7 take A to tensor memory (the lanes of warp w are rows 32 (w % 4)..),
+// 8..15 sum; one term: warps 2..9 sum.
 template <int TERMS, int BN>
 struct DirectTile {
   static constexpr int A_BYTES = BM * BK * 4;
-  static constexpr int HI_BYTES = A_BYTES + BN * BK * 4;  // A, then B
-  static constexpr int STAGE = TERMS == 3 ? 2 * HI_BYTES : HI_BYTES;  // then their lo parts
-  static constexpr int STAGES = 196608 / STAGE > 8 ? 8 : 196608 / STAGE;
+  static constexpr int B_BYTES = BN * BK * 4;
+  static constexpr int IN_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGE = IN_BYTES + (TERMS == 3 ? B_BYTES : 0);
+  static constexpr int TMEM_STAGE = 2 * BK;  // columns of A's hi and lo
+  static constexpr int FIT = 196608 / STAGE > 8 ? 8 : 196608 / STAGE;
+  static constexpr int TMEM_FIT = (512 - 2 * BN) / TMEM_STAGE;
+  static constexpr int STAGES = TERMS == 3 && TMEM_FIT < FIT ? TMEM_FIT : FIT;
+  static constexpr int TMEM_COLS = TERMS == 3 ? 512 : 2 * BN;
   static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
-  static constexpr int CONVERTERS = TERMS == 3 ? 4 : 0;
-  static constexpr int THREADS = 32 * (2 + kEpiWarps + CONVERTERS);
+  static constexpr int SUM_WARP = TERMS == 3 ? 8 : 2;
+  static constexpr int THREADS = 32 * (SUM_WARP + kEpiWarps);
   static constexpr int CHUNK = TERMS == 3 ? 2 : 32;  // K steps per TMEM accumulation (24 or 128 UMMAs)
   static_assert(BM * BN * 4 <= STAGES * STAGE, "the partial tile reuses the stages");
 };
@@ -117,7 +129,7 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
     for (int s = 0; s < TL::STAGES; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
-      mbar_init(lo_bar(s), TERMS == 3 ? TL::CONVERTERS : 1);
+      mbar_init(lo_bar(s), 6);  // the converter warps
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
@@ -129,13 +141,14 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
     fence_proxy_async_smem();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 2 * BN);
+    tmem_alloc(tmem_slot, TL::TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
+  const uint32_t tmem_a = tmem_base + 2 * BN;  // three terms: A's stages
 
   if (warp == 0) {
     if (lane == 0) {
@@ -144,7 +157,7 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
         const int it = i - kb, s = it % TL::STAGES, round = it / TL::STAGES;
         if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, err, kErrWaitEmpty)) break;
         const uint32_t sa = base + s * TL::STAGE, sb = sa + TL::A_BYTES;
-        mbar_arrive_expect_tx(full_bar(s), TL::HI_BYTES);
+        mbar_arrive_expect_tx(full_bar(s), TL::IN_BYTES);
         const int k0 = i * BK;
         if (!A_MN) {
           tma_load_2d(sa, &tmA, full_bar(s), k0, m0);
@@ -168,7 +181,7 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       // ---------------- UMMA issuer
-      constexpr uint32_t idesc = idesc_tf32(BM, BN, A_MN, B_MN);
+      constexpr uint32_t idesc = idesc_tf32(BM, BN, TERMS == 1 && A_MN, B_MN);
       int j = 0;
       bool ok = true;
       for (int cb = kb; cb < ke && ok; cb += TL::CHUNK, ++j) {
@@ -189,15 +202,20 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
           // the terms, small ones first: Al Bh, Ah Bl, Ah Bh (or Ah Bh alone)
 #pragma unroll
           for (int term = 0; term < TERMS; ++term) {
-            const uint32_t at = sa + (TERMS == 3 && term == 0 ? TL::HI_BYTES : 0);
-            const uint32_t bt = sb + (TERMS == 3 && term == 1 ? TL::HI_BYTES : 0);
+            const uint32_t ta = tmem_a + s * TL::TMEM_STAGE + (term == 0 ? BK : 0);
+            const uint32_t bt = sb + (TERMS == 3 && term == 1 ? TL::B_BYTES : 0);
 #pragma unroll
             for (int k = 0; k < BK / 8; ++k) {
-              const uint64_t adesc = A_MN ? smem_desc(at + k * 1024, MN_BLOCK_BYTES, 512, kLayoutSw128Base32)
-                                          : smem_desc(at + k * 32, 16, 1024, kLayoutSw128);
               const uint64_t bdesc = B_MN ? smem_desc(bt + k * 1024, MN_BLOCK_BYTES, 512, kLayoutSw128Base32)
                                           : smem_desc(bt + k * 32, 16, 1024, kLayoutSw128);
-              umma_tf32(acc, adesc, bdesc, idesc, (i != cb || term != 0 || k != 0) ? 1u : 0u);
+              const uint32_t more = (i != cb || term != 0 || k != 0) ? 1u : 0u;
+              if (TERMS == 3) {
+                umma_tf32_ts(acc, ta + 8 * k, bdesc, idesc, more);
+              } else {
+                const uint64_t adesc = A_MN ? smem_desc(sa + k * 1024, MN_BLOCK_BYTES, 512, kLayoutSw128Base32)
+                                            : smem_desc(sa + k * 32, 16, 1024, kLayoutSw128);
+                umma_tf32(acc, adesc, bdesc, idesc, more);
+              }
             }
           }
           umma_commit(empty_bar(s));
@@ -205,10 +223,10 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
         if (ok) umma_commit(acc_full(buf));
       }
     }
-  } else if (warp < 2 + kEpiWarps) {
+  } else if (warp >= TL::SUM_WARP) {
     // ---------------- chunk sums: 32 rows x BN / 2 columns per warp, then the partial tile
     constexpr int NC = BN / 2;
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, half = (warp - TL::SUM_WARP) >> 2;
     float sum[NC];
 #pragma unroll
     for (int e = 0; e < NC; ++e) sum[e] = 0.0f;
@@ -244,20 +262,49 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
         tile[row * (BN / 4) + ((half * (NC / 4) + q) ^ (row & 7))] =
             make_float4(sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]);
     }
-  } else if (TERMS == 3) {
-    // ---------------- converters: the lo part of every stage, in the stage's own layout
+  } else if (TERMS == 3 && warp < 4) {
+    // ---------------- B's lo part, in the stage's own layout
     for (int i = kb; i < ke; ++i) {
       const int it = i - kb, s = it % TL::STAGES, round = it / TL::STAGES;
       if (!mbar_wait(full_bar(s), round & 1, err, kErrWaitFull)) break;
-      const float4* hi = reinterpret_cast<const float4*>(smem + s * TL::STAGE);
-      float4* lo = reinterpret_cast<float4*>(smem + s * TL::STAGE + TL::HI_BYTES);
-      const int t = threadIdx.x - 32 * (2 + kEpiWarps);
+      const float4* hi = reinterpret_cast<const float4*>(smem + s * TL::STAGE + TL::A_BYTES);
+      float4* lo = reinterpret_cast<float4*>(smem + s * TL::STAGE + TL::IN_BYTES);
 #pragma unroll 8
-      for (int e = t; e < TL::HI_BYTES / 16; e += 32 * TL::CONVERTERS) {
+      for (int e = threadIdx.x - 64; e < TL::B_BYTES / 16; e += 64) {
         const float4 v = hi[e];
         lo[e] = make_float4(lo_part(v.x), lo_part(v.y), lo_part(v.z), lo_part(v.w));
       }
       fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(lo_bar(s));
+    }
+  } else if (TERMS == 3) {
+    // ---------------- A's rows to tensor memory: lane = row, hi in 32 columns, lo in the next 32
+    const int row = 32 * (warp & 3) + lane;
+    for (int i = kb; i < ke; ++i) {
+      const int it = i - kb, s = it % TL::STAGES, round = it / TL::STAGES;
+      if (!mbar_wait(full_bar(s), round & 1, err, kErrWaitFull)) break;
+      tc_fence_after();  // the UMMAs that read this stage's columns before are done
+      const uint8_t* a = smem + s * TL::STAGE;
+      uint32_t hi[32], lo[32];
+      if (!A_MN) {  // 16-byte chunk c of row r at chunk c ^ (r & 7)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint4 v = *reinterpret_cast<const uint4*>(a + row * 128 + ((c ^ (row & 7)) << 4));
+          hi[4 * c] = v.x; hi[4 * c + 1] = v.y; hi[4 * c + 2] = v.z; hi[4 * c + 3] = v.w;
+        }
+      } else {  // 32-wide blocks of 32 K rows; 32-byte chunk c of K row k at chunk c ^ (k & 3)
+        const uint8_t* block = a + (warp & 3) * MN_BLOCK_BYTES + (lane & 7) * 4;
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          hi[k] = *reinterpret_cast<const uint32_t*>(block + k * 128 + (((lane >> 3) ^ (k & 3)) << 5));
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) lo[e] = __float_as_uint(lo_part(__uint_as_float(hi[e])));
+      const uint32_t at = tmem_a + s * TL::TMEM_STAGE + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+      tmem_st_32x32b_x32(at, hi);
+      tmem_st_32x32b_x32(at + BK, lo);
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(lo_bar(s));
     }
@@ -282,7 +329,7 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, 2 * BN);
+    tmem_dealloc(tmem_base, TL::TMEM_COLS);
   }
   __syncthreads();
 }
