@@ -723,30 +723,6 @@ __global__ void __launch_bounds__(256) dropout_kernel(const float* x, long long 
 // ------------------------------------------------------------------ host side
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// The operand's tensor map: `mn` rows (or columns) of the product, `box` of them
-// per tile. MN-major operands of a width that is a multiple of 32 load a stage in
-// one 3-D box (32 wide, BK rows, box / 32 blocks), others in 32-wide 2-D boxes.
-int operand_map(CUtensorMap* map, const GemmOperand& o, int mn, int k, int box, bool* box3d) {
-  if ((o.ld & 3) || !aligned16(o.ptr)) return kGemmMisaligned;
-  *box3d = false;
-  int rc;
-  if (!o.mn_major) {
-    const long long dims[2] = {k, mn}, strides[1] = {o.ld};
-    const int b[2] = {BK, box};
-    rc = encode_tensor_map(map, o.ptr, 2, dims, strides, b, false);
-  } else if (mn % 32 == 0) {
-    const long long dims[3] = {32, k, mn / 32}, strides[2] = {o.ld, 32};
-    const int b[3] = {32, BK, box / 32};
-    *box3d = true;
-    rc = encode_tensor_map(map, o.ptr, 3, dims, strides, b, true);
-  } else {
-    const long long dims[2] = {mn, k}, strides[1] = {o.ld};
-    const int b[2] = {32, BK};
-    rc = encode_tensor_map(map, o.ptr, 2, dims, strides, b, true);
-  }
-  return rc ? kGemmTensorMap : 0;
-}
-
 // How a product is cut: 128 x 64 tiles when even with K in parts the wider ones would
 // leave half of the SMs idle, and K in as many parts (a cluster's CTAs) as fit the SMs
 // beside one another, each at least four K steps. A cluster lies in one GPC, and
@@ -833,6 +809,27 @@ int direct_majors(int M, int N, int K, const GemmOperand& A, const GemmOperand& 
 }
 
 }  // namespace
+
+int operand_map(CUtensorMap* map, const GemmOperand& o, int mn, int k, int box, bool* box3d) {
+  if ((o.ld & 3) || !aligned16(o.ptr)) return kGemmMisaligned;
+  *box3d = false;
+  int rc;
+  if (!o.mn_major) {
+    const long long dims[2] = {k, mn}, strides[1] = {o.ld};
+    const int b[2] = {BK, box};
+    rc = encode_tensor_map(map, o.ptr, 2, dims, strides, b, false);
+  } else if (mn % 32 == 0) {
+    const long long dims[3] = {32, k, mn / 32}, strides[2] = {o.ld, 32};
+    const int b[3] = {32, BK, box / 32};
+    *box3d = true;
+    rc = encode_tensor_map(map, o.ptr, 3, dims, strides, b, true);
+  } else {
+    const long long dims[2] = {mn, k}, strides[1] = {o.ld};
+    const int b[2] = {32, BK};
+    rc = encode_tensor_map(map, o.ptr, 2, dims, strides, b, true);
+  }
+  return rc ? kGemmTensorMap : 0;
+}
 
 DropoutArgs dropout_args(double p, const uint64_t* rng, int cols) {
   DropoutArgs d;

@@ -6,6 +6,8 @@
 
 #include <cstdint>
 
+#include <cuda.h>
+
 #include "dropout.cuh"
 #include "gemm.h"
 
@@ -36,6 +38,11 @@ struct LossEpilogue {
   const int32_t* targets = nullptr;
   float* zt = nullptr;  // [rows]: the target's logit
 };
+
+// The operand's tensor map: `mn` rows (or columns) of the product, `box` of them
+// per tile. MN-major operands of a width that is a multiple of 32 load a stage in
+// one 3-D box (32 wide, 32 K rows, box / 32 blocks), others in 32-wide 2-D boxes.
+int operand_map(CUtensorMap* map, const GemmOperand& o, int mn, int k, int box, bool* box3d);
 
 // ---- Large exact products (linear_pair.cu): f16 halves of operands scaled block
 // by block, three terms on CTA pairs.
@@ -112,6 +119,15 @@ int pair_loss_product(const SplitCopy& A, const SplitCopy& B, const LossEpilogue
 // Whether an exact product of this size is worth the copies.
 bool pair_product_suits(int M, int N, int K);
 
+// Large TF32 products on the operands themselves (linear_pair.cu). An MN-major A
+// only with an MN-major B and no activation or dropout. ws: tf32_pair_ws_bytes bytes.
+long long tf32_pair_ws_bytes(int M, int N, int K);
+int tf32_pair_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e,
+                      void* ws, int* d_err, cudaStream_t s);
+int tf32_pair_loss_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LossEpilogue& e,
+                           int* d_err, cudaStream_t s);
+bool tf32_pair_suits(int M, int N, int K);
+
 DropoutArgs dropout_args(double p, const uint64_t* rng, int cols);
 
 // y = r + dropout(x) over [rows, cols]; r may be null, y may be x or r.
@@ -137,6 +153,13 @@ void sum_parts(const float* part, int parts, int cols, float* out, bool accumula
 
 // ---- The operators (linear_ops.cu): direct or pair products by size; workspaces
 // are 256-byte aligned.
+// A product on the operands themselves: TF32 on pairs where that suits, else direct.
+long long plain_ws_bytes(int M, int N, int K, bool exact);
+int plain_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e, bool exact,
+                  void* ws, int* d_err, cudaStream_t s);
+int plain_loss_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LossEpilogue& e,
+                       bool exact, int* d_err, cudaStream_t s);
+
 struct LinearForward {
   int m, n, k;
   const float* a;

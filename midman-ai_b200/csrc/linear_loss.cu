@@ -77,8 +77,15 @@ Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* w
       if (dw) parts = std::max({parts, pair_ws_bytes(vocab, dim, r), pair_ws_bytes(dim, vocab, r)});
     }
     p.parts = at.take(parts);
-  } else if (dw) {
-    p.x = static_cast<float*>(at.take(p.rows * p.ldx * 4));
+  } else {
+    if (dw) p.x = static_cast<float*>(at.take(p.rows * p.ldx * 4));
+    const int last = static_cast<int>(n - (blocks - 1) * p.rows);
+    long long parts = 0;
+    for (const int r : {p.rows, std::max(last, 1)}) {
+      if (dx) parts = std::max(parts, plain_ws_bytes(r, dim, vocab, exact));
+      if (dw) parts = std::max({parts, plain_ws_bytes(vocab, dim, r, exact), plain_ws_bytes(dim, vocab, r, exact)});
+    }
+    p.parts = at.take(parts);
   }
   p.bytes = at.at;
   return p;
@@ -271,7 +278,7 @@ int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, 
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
   const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt};
-  int rc = direct_loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
+  int rc = plain_loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
   if (rc) return rc;
   if (!a.dx && !a.dw) {
     row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(p.part, p.tiles, p.zt, t, n, a.vocab, 0.0f, a.row_loss + r0, nullptr,
@@ -288,7 +295,8 @@ int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, 
     o.C = a.dx + r0 * a.lddx;
     o.R = a.accumulate ? o.C : nullptr;
     o.ldc = o.ldr = a.lddx;
-    rc = direct_product(n, a.dim, a.vocab, {p.z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, d_err, s);
+    rc = plain_product(n, a.dim, a.vocab, {p.z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, p.parts, d_err,
+                       s);
     if (rc) return rc;
   }
   if (a.dw) {
@@ -299,8 +307,8 @@ int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, 
     o.R = a.accumulate || r0 > 0 ? a.dw : nullptr;
     o.ldc = o.ldr = a.lddw;
     const GemmOperand g{p.z, p.ldz, true}, xo{p.x, p.ldx, true};
-    rc = a.w_mn_major ? direct_product(a.dim, a.vocab, n, xo, g, o, a.exact, d_err, s)
-                      : direct_product(a.vocab, a.dim, n, g, xo, o, a.exact, d_err, s);
+    rc = a.w_mn_major ? plain_product(a.dim, a.vocab, n, xo, g, o, a.exact, p.parts, d_err, s)
+                      : plain_product(a.vocab, a.dim, n, g, xo, o, a.exact, p.parts, d_err, s);
   }
   return rc;
 }

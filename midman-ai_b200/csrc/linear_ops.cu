@@ -25,6 +25,8 @@ ForwardPlan forward_plan(int m, int n, int k, bool exact, void* ws) {
     p.a = at.copy(m, k);
     p.b = at.copy(n, k);
     p.parts = at.take(pair_ws_bytes(m, n, k));
+  } else {
+    p.parts = at.take(plain_ws_bytes(m, n, k, exact));
   }
   p.bytes = at.at;
   return p;
@@ -50,6 +52,7 @@ BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
     p.parts = at.take(std::max(pair_ws_bytes(m, k, n), pair_ws_bytes(k, n, m)));
   } else {
     p.dz_f32 = static_cast<float*>(at.take(m * round4(n) * 4));
+    p.parts = at.take(std::max({plain_ws_bytes(m, k, n, exact), plain_ws_bytes(k, n, m, exact), plain_ws_bytes(n, k, m, exact)}));
   }
   p.sums = static_cast<float*>(at.take(static_cast<long long>(std::max(act_backward_parts(m), split_parts(m))) * n * 4));
   p.bytes = at.at;
@@ -57,6 +60,20 @@ BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
 }
 
 }  // namespace
+
+long long plain_ws_bytes(int M, int N, int K, bool exact) {
+  return !exact && tf32_pair_suits(M, N, K) ? tf32_pair_ws_bytes(M, N, K) : 0;
+}
+int plain_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e, bool exact,
+                  void* ws, int* d_err, cudaStream_t s) {
+  if (!exact && tf32_pair_suits(M, N, K)) return tf32_pair_product(M, N, K, A, B, e, ws, d_err, s);
+  return direct_product(M, N, K, A, B, e, exact, d_err, s);
+}
+int plain_loss_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LossEpilogue& e,
+                       bool exact, int* d_err, cudaStream_t s) {
+  if (!exact && tf32_pair_suits(M, N, K)) return tf32_pair_loss_product(M, N, K, A, B, e, d_err, s);
+  return direct_loss_product(M, N, K, A, B, e, exact, d_err, s);
+}
 
 long long linear_forward_ws_bytes(int m, int n, int k, bool exact) {
   return forward_plan(m, n, k, exact, nullptr).bytes;
@@ -66,7 +83,8 @@ int linear_forward(const LinearForward& f, void* ws, int* d_err, cudaStream_t s)
   if (f.m <= 0) return 0;
   const ForwardPlan p = forward_plan(f.m, f.n, f.k, f.exact, ws);
   if (!p.pair)
-    return direct_product(f.m, f.n, f.k, {f.a, f.lda, false}, {f.b, f.ldb, f.b_mn_major}, f.e, f.exact, d_err, s);
+    return plain_product(f.m, f.n, f.k, {f.a, f.lda, false}, {f.b, f.ldb, f.b_mn_major}, f.e, f.exact, p.parts, d_err,
+                         s);
   split_two({f.a, f.lda}, f.m, f.k, &p.a, nullptr, {f.b, f.ldb}, f.b_mn_major ? f.k : f.n, f.b_mn_major ? f.n : f.k,
             f.b_mn_major ? nullptr : &p.b, f.b_mn_major ? &p.b : nullptr, s);
   return pair_product(p.a, p.b, f.e, p.parts, d_err, s);
@@ -118,11 +136,11 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
   const float* g = plain ? f.dc : p.dz_f32;
   const long long ldg = plain ? f.lddc : ldz;
   if (f.da)
-    rc = direct_product(f.m, f.k, f.n, {g, ldg, false}, {f.b, f.ldb, !f.b_mn_major}, da, f.exact, d_err, s);
+    rc = plain_product(f.m, f.k, f.n, {g, ldg, false}, {f.b, f.ldb, !f.b_mn_major}, da, f.exact, p.parts, d_err, s);
   if (f.db && !rc) {
     const GemmOperand ao{f.a, f.lda, true}, go{g, ldg, true};
-    rc = f.b_mn_major ? direct_product(f.k, f.n, f.m, ao, go, db, f.exact, d_err, s)
-                      : direct_product(f.n, f.k, f.m, go, ao, db, f.exact, d_err, s);
+    rc = f.b_mn_major ? plain_product(f.k, f.n, f.m, ao, go, db, f.exact, p.parts, d_err, s)
+                      : plain_product(f.n, f.k, f.m, go, ao, db, f.exact, p.parts, d_err, s);
   }
   return rc;
 }

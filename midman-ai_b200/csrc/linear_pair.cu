@@ -269,10 +269,9 @@ constexpr int P_SUM_WARP = 4;  // the first of the eight warps that sum and writ
 // which holds 128 sums, the residuals and the epilogue without spills.
 constexpr int P_REGS = 168, P_REGS_FEW = 40, P_REGS_SUM = 232;
 static_assert(P_REGS_FEW + 2 * P_REGS_SUM <= 3 * P_REGS, "setmaxnreg draws on the launch's registers");
-constexpr int P_STAGES = 3;
-constexpr int P_TILE = 16384;
-constexpr int P_STAGE = 4 * P_TILE;
-constexpr int P_SMEM = P_STAGES * P_STAGE + 1024 + 256 + 8 * 32 * 32 * 4;
+constexpr int P_RING = 196608;  // the stages' bytes
+constexpr int P_TILE = 16384;   // 128 rows of 128 bytes
+constexpr int P_SMEM = P_RING + 1024 + 256 + 8 * 32 * 32 * 4;
 static_assert(P_SMEM <= 232448, "shared memory of a CTA");
 
 // Tiles in groups of 8 row blocks, the row block fastest inside a group, so that the
@@ -295,18 +294,79 @@ struct PairWork {
 struct PairUnit {
   int tile, cb, ce, slot;
 };
-__device__ __forceinline__ PairUnit unit_of(int u, const PairWork& w, int chunks) {
-  if (u < w.full) return {u, 0, chunks, -1};
+__device__ __forceinline__ PairUnit unit_of(int u, const PairWork& w, int steps) {
+  if (u < w.full) return {u, 0, steps, -1};
   const int v = u - w.full, part = v % w.splits;
-  return {w.full + v / w.splits, chunks * part / w.splits, chunks * (part + 1) / w.splits, v};
+  return {w.full + v / w.splits, steps * part / w.splits, steps * (part + 1) / w.splits, v};
 }
 
 __device__ __forceinline__ void stage_rows(const float* v, float4* stage_tile, int lane);
 
-template <class Epi>
+// How operands reach the UMMAs. A work step is what a unit's K range counts: `LOADS`
+// stages; EACH: every work step is an accumulation of its own, scaled and summed in
+// registers, otherwise a unit is one accumulation.
+struct ExactFeed {  // split copies: hi and lo of A and B, 64 of K a stage, a chunk two
+  static constexpr int STAGE = 4 * P_TILE, LOADS = 2;
+  static constexpr bool EACH = true;
+  static constexpr uint32_t IDESC = idesc_f16(2 * BM, PN);
+  static __device__ __forceinline__ void load(uint32_t st, const CUtensorMap* a, const CUtensorMap* b, uint32_t bar,
+                                              int i, int m0, int n0, int) {
+    tma_load_3d_pair(st, a, bar, 0, m0, 2 * i);
+    tma_load_3d_pair(st + 2 * P_TILE, b, bar, 0, n0, 2 * i);
+  }
+  // the terms, small ones first: Al Bh, Ah Bl, Ah Bh; 16 f16 = 32 bytes along the swizzled row
+  static __device__ __forceinline__ void multiply(uint32_t acc, uint32_t st, bool first) {
+#pragma unroll
+    for (int term = 0; term < 3; ++term) {
+      const uint32_t a = st + (term == 0 ? P_TILE : 0), b = st + (term == 1 ? 3 * P_TILE : 2 * P_TILE);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        umma_f16_pair(acc, smem_desc(a + k * 32, 16, 1024, kLayoutSw128), smem_desc(b + k * 32, 16, 1024, kLayoutSw128),
+                      IDESC, (!first || term != 0 || k != 0) ? 1u : 0u);
+    }
+  }
+};
+// The f32 operands themselves, one TF32 pass: 32 of K a stage. Bits 1 and 2 of
+// `boxes`: an MN-major A, B loads its stage in one 3-D box, else in 32-wide ones.
+template <bool A_MN, bool B_MN>
+struct Tf32Feed {
+  static constexpr int STAGE = 2 * P_TILE, LOADS = 1;
+  static constexpr bool EACH = false;
+  static constexpr uint32_t IDESC = idesc_tf32(2 * BM, PN, A_MN, B_MN);
+  template <bool MN>
+  static __device__ __forceinline__ void side(uint32_t at, const CUtensorMap* map, uint32_t bar, int k0, int mn0,
+                                              bool box3d) {
+    if (!MN) {
+      tma_load_2d_pair(at, map, bar, k0, mn0);
+    } else if (box3d) {
+      tma_load_3d_pair(at, map, bar, 0, k0, mn0 / 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tma_load_2d_pair(at + j * 4096, map, bar, mn0 + 32 * j, k0);
+    }
+  }
+  static __device__ __forceinline__ void load(uint32_t st, const CUtensorMap* a, const CUtensorMap* b, uint32_t bar,
+                                              int i, int m0, int n0, int boxes) {
+    side<A_MN>(st, a, bar, 32 * i, m0, boxes & 1);
+    side<B_MN>(st + P_TILE, b, bar, 32 * i, n0, boxes & 2);
+  }
+  template <bool MN>
+  static __device__ __forceinline__ uint64_t desc(uint32_t at, int k) {  // 8 of K: 32 bytes, or 8 rows of 128
+    return MN ? smem_desc(at + k * 1024, 4096, 512, kLayoutSw128Base32) : smem_desc(at + k * 32, 16, 1024, kLayoutSw128);
+  }
+  static __device__ __forceinline__ void multiply(uint32_t acc, uint32_t st, bool first) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      umma_tf32_pair(acc, desc<A_MN>(st, k), desc<B_MN>(st + P_TILE, k), IDESC, (!first || k != 0) ? 1u : 0u);
+  }
+};
+
+template <class Feed, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const float* inv_a,
-                long long ld_ia, const float* inv_b, long long ld_ib, const Epi epi, int M, int N, int chunks, int units, const PairWork work, int* err) {
+                long long ld_ia, const float* inv_b, long long ld_ib, const Epi epi, int M, int N, int steps, int boxes,
+                int units, const PairWork work, int* err) {
+  constexpr int P_STAGE = Feed::STAGE, P_STAGES = P_RING / P_STAGE;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int pair = static_cast<int>(blockIdx.x) / 2, npairs = static_cast<int>(gridDim.x) / 2;
@@ -361,41 +421,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
       int it = 0;
       bool ok = true;
       for (int u = pair; u < units && ok; u += npairs) {
-        const PairUnit w = unit_of(u, work, chunks);
+        const PairUnit w = unit_of(u, work, steps);
         int mt, nt;
         pair_tile(w.tile, tm, tn, mt, nt);
         const int my_m0 = mt * 2 * BM + static_cast<int>(rank) * BM;
         const int my_n0 = nt * PN + static_cast<int>(rank) * (PN / 2);
-        for (int i = 2 * w.cb; i < 2 * w.ce; ++i, ++it) {  // a chunk is two stages
+        for (int i = Feed::LOADS * w.cb; i < Feed::LOADS * w.ce; ++i, ++it) {
           const int s = it % P_STAGES, round = it / P_STAGES;
           if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, err, kErrWaitEmpty)) {
             ok = false;
             break;
           }
           if (leader) mbar_arrive_expect_tx(full_bar(s), 2 * P_STAGE);
-          const uint32_t fb = mapa_shared(full_bar(s), 0);
-          const uint32_t sa = base + s * P_STAGE;
-          tma_load_3d_pair(sa, &tmA, fb, 0, my_m0, 2 * i);               // hi, lo of A
-          tma_load_3d_pair(sa + 2 * P_TILE, &tmB, fb, 0, my_n0, 2 * i);  // and of B
+          Feed::load(base + s * P_STAGE, &tmA, &tmB, mapa_shared(full_bar(s), 0), i, my_m0, my_n0, boxes);
           *loads_issued = it + 1;
         }
       }
     } else if (warp == 1 && lane == 0 && leader) {
       // ---------------- UMMA issuer (leader only), M = 256 across the pair
-      constexpr uint32_t idesc = idesc_f16(2 * BM, PN);
       int it = 0, j = 0;
       bool ok = true;
       for (int u = pair; u < units && ok; u += npairs) {
-        const PairUnit w = unit_of(u, work, chunks);
-        for (int c = w.cb; c < w.ce && ok; ++c) {
+        const PairUnit w = unit_of(u, work, steps);
+        for (int c = w.cb; c < w.ce && ok; c = Feed::EACH ? c + 1 : w.ce) {
           const int buf = j & 1;
           if (j >= 2 && !mbar_wait(acc_empty(buf), ((j >> 1) - 1) & 1, err, kErrWaitAccum)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t acc = tmem_base + buf * PN;
-          for (int h = 0; h < 2; ++h, ++it) {
+          const int loads = Feed::LOADS * (Feed::EACH ? 1 : w.ce - c);
+          for (int h = 0; h < loads; ++h, ++it) {
             const int s = it % P_STAGES, round = it / P_STAGES;
             if (!mbar_wait(full_bar(s), round & 1, err, kErrWaitFull)) {
               ok = false;
@@ -403,18 +459,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
             }
             tc_fence_after();
             *loads_consumed = it + 1;
-            const uint32_t sa = base + s * P_STAGE;
-            // the terms, small ones first: Al Bh, Ah Bl, Ah Bh
-#pragma unroll
-            for (int term = 0; term < 3; ++term) {
-              const uint32_t at = sa + (term == 0 ? P_TILE : 0);
-              const uint32_t bt = sa + (term == 1 ? 3 * P_TILE : 2 * P_TILE);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)  // 16 f16 = 32 bytes along the swizzled row
-                umma_f16_pair(acc, smem_desc(at + k * 32, 16, 1024, kLayoutSw128),
-                              smem_desc(bt + k * 32, 16, 1024, kLayoutSw128), idesc,
-                              (h != 0 || term != 0 || k != 0) ? 1u : 0u);
-            }
+            Feed::multiply(tmem_base + buf * PN, base + s * P_STAGE, h == 0);
             umma_commit_pair(empty_bar(s), 0x3);
           }
           if (!ok) break;
@@ -431,56 +476,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     int j = 0;
     bool ok = true;
     for (int u = pair; u < units && ok; u += npairs) {
-      const PairUnit w = unit_of(u, work, chunks);
+      const PairUnit w = unit_of(u, work, steps);
       int mt, nt;
       pair_tile(w.tile, tm, tn, mt, nt);
       const int wrow0 = mt * 2 * BM + static_cast<int>(rank) * BM + quarter * 32, wcol0 = nt * PN + half * 128;
       float sum[128];
 #pragma unroll
       for (int e = 0; e < 128; ++e) sum[e] = 0.0f;
-      // The chunks' inverse scales, one chunk ahead: this lane's row's in a register,
-      // the columns' through the staging tile (idle until the epilogue).
-      const float* pa = inv_a + w.cb * ld_ia + wrow0 + lane;
-      const float4* pb = reinterpret_cast<const float4*>(inv_b + w.cb * ld_ib + wcol0) + lane;
-      float ia = __ldg(pa);
-      stage_tile[lane] = __ldg(pb);
-      __syncwarp();
       if (w.slot < 0) epi.prefetch(wrow0, wcol0, M, N, lane);
-      for (int c = w.cb; c < w.ce; ++c) {
-        const float4* ib = stage_tile + 32 * ((c - w.cb) & 1);
-        const bool more = c + 1 < w.ce;
-        pa += ld_ia;
-        pb += ld_ib / 4;
-        const float ia_next = more ? __ldg(pa) : 0.0f;
-        const float4 ib_next = more ? __ldg(pb) : make_float4(0.f, 0.f, 0.f, 0.f);
+      // The accumulation's columns [32 q, 32 q + 32) of this warp; `release` hands it back.
+      auto wait_acc = [&](uint32_t* acc) {
         const int buf = j & 1;
-        if (!mbar_wait(acc_full(buf), (j >> 1) & 1, err, kErrWaitAccum)) {
-          ok = false;
-          break;
-        }
+        if (!mbar_wait(acc_full(buf), (j >> 1) & 1, err, kErrWaitAccum)) return false;
         tc_fence_after();
-        const uint32_t acc = tmem_base + buf * PN + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+        *acc = tmem_base + buf * PN + (static_cast<uint32_t>(quarter * 32) << 16) + half * 128;
+        return true;
+      };
+      auto release_acc = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(mapa_shared(acc_empty(j & 1), 0));
+        ++j;
+      };
+      uint32_t acc = 0;
+      if (!Feed::EACH) {
+        ok = wait_acc(&acc);
+        if (!ok) break;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint32_t r[32];
           tmem_ld_32x32b_x32(acc + q * 32, r);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 b = ib[q * 8 + e];  // the columns' inverse scales, the same for every lane
-            float* o = sum + q * 32 + 4 * e;
-            o[0] = fmaf(__uint_as_float(r[4 * e]) * ia, b.x, o[0]);
-            o[1] = fmaf(__uint_as_float(r[4 * e + 1]) * ia, b.y, o[1]);
-            o[2] = fmaf(__uint_as_float(r[4 * e + 2]) * ia, b.z, o[2]);
-            o[3] = fmaf(__uint_as_float(r[4 * e + 3]) * ia, b.w, o[3]);
-          }
+          for (int e = 0; e < 32; ++e) sum[q * 32 + e] = __uint_as_float(r[e]);
         }
-        tc_fence_before();
+        release_acc();
+      } else {
+        // The chunks' inverse scales, one chunk ahead: this lane's row's in a register,
+        // the columns' through the staging tile (idle until the epilogue).
+        const float* pa = inv_a + w.cb * ld_ia + wrow0 + lane;
+        const float4* pb = reinterpret_cast<const float4*>(inv_b + w.cb * ld_ib + wcol0) + lane;
+        float ia = __ldg(pa);
+        stage_tile[lane] = __ldg(pb);
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(mapa_shared(acc_empty(buf), 0));
-        ++j;
-        ia = ia_next;
-        stage_tile[32 * ((c + 1 - w.cb) & 1) + lane] = ib_next;
-        __syncwarp();
+        for (int c = w.cb; c < w.ce; ++c) {
+          const float4* ib = stage_tile + 32 * ((c - w.cb) & 1);
+          const bool more = c + 1 < w.ce;
+          pa += ld_ia;
+          pb += ld_ib / 4;
+          const float ia_next = more ? __ldg(pa) : 0.0f;
+          const float4 ib_next = more ? __ldg(pb) : make_float4(0.f, 0.f, 0.f, 0.f);
+          ok = wait_acc(&acc);
+          if (!ok) break;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(acc + q * 32, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 b = ib[q * 8 + e];  // the columns' inverse scales, the same for every lane
+              float* o = sum + q * 32 + 4 * e;
+              o[0] = fmaf(__uint_as_float(r[4 * e]) * ia, b.x, o[0]);
+              o[1] = fmaf(__uint_as_float(r[4 * e + 1]) * ia, b.y, o[1]);
+              o[2] = fmaf(__uint_as_float(r[4 * e + 2]) * ia, b.z, o[2]);
+              o[3] = fmaf(__uint_as_float(r[4 * e + 3]) * ia, b.w, o[3]);
+            }
+          }
+          release_acc();
+          ia = ia_next;
+          stage_tile[32 * ((c + 1 - w.cb) & 1) + lane] = ib_next;
+          __syncwarp();
+        }
       }
       if (!ok) break;
       if (w.slot < 0) {
@@ -681,17 +746,18 @@ int copy_map(CUtensorMap* map, const SplitCopy& c) {
   return encode_tensor_map_f16(map, c.data, 3, dims, strides, box) ? kGemmTensorMap : 0;
 }
 
-// The last wave's tiles are cut into parts when that saves at least eight chunks of
-// its length (a chunk takes 1.7 us; writing, reading and summing the parts about 8
-// us). The grid is that of the full part: 74 pairs.
+// The last wave's tiles are cut into parts when that saves at least `worth` work steps
+// of its length: writing, reading and summing the parts takes about 8 us, a chunk of
+// the exact mode 1.7 us, a TF32 step 0.45 us. The grid is that of the full part: 74 pairs.
 constexpr int kPairs = 74;
-PairWork work_of(long long tiles, int chunks) {
+constexpr int kWorthExact = 8, kWorthTf32 = 28;
+PairWork work_of(long long tiles, int steps, int worth) {
   PairWork w;
   w.full = static_cast<int>(tiles);
   const int tail = static_cast<int>(tiles % kPairs);
   if (tail == 0) return w;
-  const int s = std::min(kPairs / tail, chunks);
-  if (s < 2 || chunks - (chunks + s - 1) / s < 8) return w;
+  const int s = std::min(kPairs / tail, steps);
+  if (s < 2 || steps - (steps + s - 1) / s < worth) return w;
   w.full = static_cast<int>(tiles - tail);
   w.splits = s;
   return w;
@@ -699,14 +765,17 @@ PairWork work_of(long long tiles, int chunks) {
 
 long long tiles_of(int M, int N) { return static_cast<long long>((M + 255) / 256) * ((N + 255) / 256); }
 
-template <class Epi>
-int launch_pair(const SplitCopy& A, const SplitCopy& B, const Epi& epi, const PairWork& work, int* d_err,
-                cudaStream_t s) {
-  CUtensorMap ta{}, tb{};
-  int rc = copy_map(&ta, A);
-  if (!rc) rc = copy_map(&tb, B);
-  if (rc) return rc;
-  auto kern = pair_kernel<Epi>;
+// One launch's operands: tensor maps, and the copies' scales or the box flags.
+struct PairInput {
+  CUtensorMap a{}, b{};
+  const float *inv_a = nullptr, *inv_b = nullptr;
+  long long ld_ia = 0, ld_ib = 0;
+  int M, N, steps, boxes = 0;
+};
+
+template <class Feed, class Epi>
+int launch_pair(const PairInput& in, const Epi& epi, const PairWork& work, int* d_err, cudaStream_t s) {
+  auto kern = pair_kernel<Feed, Epi>;
   static thread_local int configured_device = -1;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
@@ -718,32 +787,72 @@ int launch_pair(const SplitCopy& A, const SplitCopy& B, const Epi& epi, const Pa
     if (fa.numRegs != P_REGS) throw std::runtime_error("linear: the pair kernel's registers do not match its split");
     configured_device = dev;
   }
-  const long long tiles = tiles_of(A.rows, B.rows), units = work.full + (tiles - work.full) * work.splits;
+  const long long tiles = tiles_of(in.M, in.N), units = work.full + (tiles - work.full) * work.splits;
   const int grid = 2 * static_cast<int>(std::min<long long>(units, std::min(kPairs, sm_count() / 2)));
-  kern<<<grid, P_THREADS, P_SMEM, s>>>(ta, tb, A.inv, A.inv_ld(), B.inv, B.inv_ld(), epi, A.rows, B.rows,
-                                       static_cast<int>(A.chunks()), static_cast<int>(units), work, d_err);
+  kern<<<grid, P_THREADS, P_SMEM, s>>>(in.a, in.b, in.inv_a, in.ld_ia, in.inv_b, in.ld_ib, epi, in.M, in.N, in.steps,
+                                       in.boxes, static_cast<int>(units), work, d_err);
   check_cuda(cudaGetLastError(), "linear");
   return 0;
 }
 
-template <int ACT>
-int launch_act(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e, const PairWork& work, int* d_err,
-               cudaStream_t s) {
-  return e.drop.rng ? launch_pair(A, B, LinearPair<ACT, true>{e}, work, d_err, s)
-                    : launch_pair(A, B, LinearPair<ACT, false>{e}, work, d_err, s);
+template <class Feed, int ACT>
+int launch_act(const PairInput& in, const LinearEpilogue& e, const PairWork& work, int* d_err, cudaStream_t s) {
+  return e.drop.rng ? launch_pair<Feed>(in, LinearPair<ACT, true>{e}, work, d_err, s)
+                    : launch_pair<Feed>(in, LinearPair<ACT, false>{e}, work, d_err, s);
 }
-int launch_linear(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e, const PairWork& work, int* d_err,
-                  cudaStream_t s) {
+template <class Feed>
+int launch_linear(const PairInput& in, const LinearEpilogue& e, const PairWork& work, int* d_err, cudaStream_t s) {
   switch (e.act) {
-    case kActRelu: return launch_act<kActRelu>(A, B, e, work, d_err, s);
-    case kActGelu: return launch_act<kActGelu>(A, B, e, work, d_err, s);
-    case kActSilu: return launch_act<kActSilu>(A, B, e, work, d_err, s);
-    default: return launch_act<kActNone>(A, B, e, work, d_err, s);
+    case kActRelu: return launch_act<Feed, kActRelu>(in, e, work, d_err, s);
+    case kActGelu: return launch_act<Feed, kActGelu>(in, e, work, d_err, s);
+    case kActSilu: return launch_act<Feed, kActSilu>(in, e, work, d_err, s);
+    default: return launch_act<Feed, kActNone>(in, e, work, d_err, s);
   }
 }
 
-bool same_k(const SplitCopy& A, const SplitCopy& B) {
-  return A.k == B.k && A.k > 0 && tiles_of(A.rows, B.rows) <= (1 << 26);
+int exact_input(const SplitCopy& A, const SplitCopy& B, PairInput* in) {
+  if (A.k != B.k || A.k <= 0 || tiles_of(A.rows, B.rows) > (1 << 26)) return kGemmBadArgument;
+  int rc = copy_map(&in->a, A);
+  if (!rc) rc = copy_map(&in->b, B);
+  in->inv_a = A.inv;
+  in->ld_ia = A.inv_ld();
+  in->inv_b = B.inv;
+  in->ld_ib = B.inv_ld();
+  in->M = A.rows;
+  in->N = B.rows;
+  in->steps = static_cast<int>(A.chunks());
+  return rc;
+}
+
+int tf32_input(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, PairInput* in) {
+  if (K <= 0 || tiles_of(M, N) > (1 << 26)) return kGemmBadArgument;
+  bool a3 = false, b3 = false;
+  int rc = operand_map(&in->a, A, M, K, 128, &a3);
+  if (!rc) rc = operand_map(&in->b, B, N, K, 128, &b3);
+  in->M = M;
+  in->N = N;
+  in->steps = (K + 31) / 32;
+  in->boxes = (a3 ? 1 : 0) | (b3 ? 2 : 0);
+  return rc;
+}
+
+long long parts_bytes(int M, int N, int steps, int worth) {
+  const PairWork w = work_of(tiles_of(M, N), steps, worth);
+  return (tiles_of(M, N) - w.full) * w.splits * (2ll * BM * PN * 4);
+}
+
+// Whether a product keeps half of the pairs busy, with tiles at least a quarter full.
+bool fills(int M, int N, int steps, int worth) {
+  if (M < 64 || N < 64) return false;
+  const PairWork w = work_of(tiles_of(M, N), steps, worth);
+  return 2 * (w.full + (tiles_of(M, N) - w.full) * w.splits) >= kPairs;
+}
+
+void reduce_parts(const PairInput& in, const PairWork& work, const LinearEpilogue& e, cudaStream_t s) {
+  const long long tail = tiles_of(in.M, in.N) - work.full;
+  if (!tail) return;
+  reduce_kernel<<<dim3(static_cast<unsigned>(tail), 2 * BM / 4), 256, 0, s>>>(work, e, in.M, in.N);
+  check_cuda(cudaGetLastError(), "linear");
 }
 
 long long copy_data_bytes(int rows, int k) { return rows * ((k + 127ll) / 128) * 512; }
@@ -776,12 +885,6 @@ void split(const SplitLoss& src, int rows, int cols, const SplitCopy* by_rows, c
   launch_split(LossSource{src}, rows, cols, by_rows, by_cols, nullptr, s);
 }
 
-long long pair_ws_bytes(int M, int N, int K) {
-  const long long tiles = tiles_of(M, N);
-  const PairWork w = work_of(tiles, (K + 127) / 128);
-  return (tiles - w.full) * w.splits * (2ll * BM * PN * 4);
-}
-
 void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_by_rows, const SplitCopy* x_by_cols,
                const SplitMatrix& y, int y_rows, int y_cols, const SplitCopy* y_by_rows, const SplitCopy* y_by_cols,
                cudaStream_t s) {
@@ -805,32 +908,69 @@ void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_
   check_cuda(cudaGetLastError(), "split");
 }
 
+long long pair_ws_bytes(int M, int N, int K) { return parts_bytes(M, N, (K + 127) / 128, kWorthExact); }
+
 int pair_product(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e, void* ws, int* d_err,
                  cudaStream_t s) {
   if (A.rows <= 0 || B.rows <= 0) return 0;
-  if (!same_k(A, B)) return kGemmBadArgument;
-  const long long tiles = tiles_of(A.rows, B.rows);
-  PairWork work = work_of(tiles, static_cast<int>(A.chunks()));
+  PairInput in;
+  int rc = exact_input(A, B, &in);
+  if (rc) return rc;
+  PairWork work = work_of(tiles_of(in.M, in.N), in.steps, kWorthExact);
   work.ws = static_cast<float*>(ws);
-  const int rc = launch_linear(A, B, e, work, d_err, s);
-  if (rc || work.full == tiles) return rc;
-  reduce_kernel<<<dim3(static_cast<unsigned>(tiles - work.full), 2 * BM / 4), 256, 0, s>>>(work, e, A.rows, B.rows);
-  check_cuda(cudaGetLastError(), "linear");
-  return 0;
+  rc = launch_linear<ExactFeed>(in, e, work, d_err, s);
+  if (!rc) reduce_parts(in, work, e, s);
+  return rc;
 }
 
 int pair_loss_product(const SplitCopy& A, const SplitCopy& B, const LossEpilogue& e, int* d_err, cudaStream_t s) {
   if (A.rows <= 0 || B.rows <= 0) return 0;
-  if (!same_k(A, B)) return kGemmBadArgument;
-  PairWork work;  // every epilogue needs its whole row sums: no parts
-  work.full = static_cast<int>(tiles_of(A.rows, B.rows));
-  return launch_pair(A, B, LossPair{e}, work, d_err, s);
+  PairInput in;
+  const int rc = exact_input(A, B, &in);
+  if (rc) return rc;
+  PairWork work;  // the epilogue needs a tile's whole sums: no parts
+  work.full = static_cast<int>(tiles_of(in.M, in.N));
+  return launch_pair<ExactFeed>(in, LossPair{e}, work, d_err, s);
 }
 
 bool pair_product_suits(int M, int N, int K) {
-  const PairWork w = work_of(tiles_of(M, N), (K + 127) / 128);
-  const long long units = w.full + (tiles_of(M, N) - w.full) * w.splits;
-  return K >= 128 && units >= kPairs / 2 && 2e-9 * M * N * K >= 8.0;
+  return K >= 128 && fills(M, N, (K + 127) / 128, kWorthExact) && 2e-9 * M * N * K >= 8.0;
 }
+
+long long tf32_pair_ws_bytes(int M, int N, int K) { return parts_bytes(M, N, (K + 31) / 32, kWorthTf32); }
+
+int tf32_pair_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e,
+                      void* ws, int* d_err, cudaStream_t s) {
+  if (M <= 0 || N <= 0) return 0;
+  PairInput in;
+  int rc = tf32_input(M, N, K, A, B, &in);
+  if (rc) return rc;
+  PairWork work = work_of(tiles_of(M, N), in.steps, kWorthTf32);
+  work.ws = static_cast<float*>(ws);
+  if (!A.mn_major)
+    rc = B.mn_major ? launch_linear<Tf32Feed<false, true>>(in, e, work, d_err, s)
+                    : launch_linear<Tf32Feed<false, false>>(in, e, work, d_err, s);
+  else if (B.mn_major && e.act == kActNone && !e.drop.rng)  // a weight's gradient
+    rc = launch_pair<Tf32Feed<true, true>>(in, LinearPair<kActNone, false>{e}, work, d_err, s);
+  else
+    return kGemmBadArgument;
+  if (!rc) reduce_parts(in, work, e, s);
+  return rc;
+}
+
+int tf32_pair_loss_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LossEpilogue& e,
+                           int* d_err, cudaStream_t s) {
+  if (M <= 0 || N <= 0) return 0;
+  if (A.mn_major) return kGemmBadArgument;
+  PairInput in;
+  const int rc = tf32_input(M, N, K, A, B, &in);
+  if (rc) return rc;
+  PairWork work;
+  work.full = static_cast<int>(tiles_of(M, N));
+  return B.mn_major ? launch_pair<Tf32Feed<false, true>>(in, LossPair{e}, work, d_err, s)
+                    : launch_pair<Tf32Feed<false, false>>(in, LossPair{e}, work, d_err, s);
+}
+
+bool tf32_pair_suits(int M, int N, int K) { return fills(M, N, (K + 31) / 32, kWorthTf32) && 2e-9 * M * N * K >= 2.0; }
 
 }  // namespace mm
