@@ -63,7 +63,7 @@ struct DirectTile {
   static constexpr int SUM_WARP = TERMS == 3 ? 8 : 2;
   static constexpr int THREADS = 32 * (SUM_WARP + kEpiWarps);
   static constexpr int CHUNK = TERMS == 3 ? 2 : 32;  // K steps per TMEM accumulation (24 or 128 UMMAs)
-  static_assert(BM * BN * 4 <= STAGES * STAGE, "the partial tile reuses the stages");
+  static_assert(BM * BN * 4 + 2 * BM * 8 <= STAGES * STAGE, "the partial tile and its halves reuse the stages");
 };
 
 __device__ __forceinline__ float4 ld_cluster_quad(uint32_t addr) {
@@ -72,6 +72,37 @@ __device__ __forceinline__ float4 ld_cluster_quad(uint32_t addr) {
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                : "r"(addr)
                : "memory");
+  return v;
+}
+
+// The sum over the cluster's parts, in part order, of quad q of tile row r.
+template <int BN>
+__device__ __forceinline__ float4 sum_quad(uint32_t tile, int r, int q, int splits) {
+  const uint32_t at = tile + 16u * static_cast<uint32_t>(r * (BN / 4) + (q ^ (r & 7)));
+  float4 v;
+  if (splits == 1) {
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at)
+                 : "memory");
+    return v;
+  }
+  v = ld_cluster_quad(mapa_shared(at, 0));
+  if (splits == 2) {
+    const float4 w = ld_cluster_quad(mapa_shared(at, 1));
+    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+    return v;
+  }
+  for (int p = 1; p < splits; p += 3) {  // 4 or 8 parts, at most three loads in flight
+    float4 w[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      w[i] = p + i < splits ? ld_cluster_quad(mapa_shared(at, p + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      v.x += w[i].x; v.y += w[i].y; v.z += w[i].z; v.w += w[i].w;
+    }
+  }
   return v;
 }
 
@@ -149,6 +180,7 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
   const uint32_t tmem_a = tmem_base + 2 * BN;  // three terms: A's stages
+  float2* halves = reinterpret_cast<float2*>(smem + BM * BN * 4);  // behind the partial tile
 
   if (warp == 0) {
     if (lane == 0) {
@@ -261,6 +293,8 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
       for (int q = 0; q < NC / 4; ++q)
         tile[row * (BN / 4) + ((half * (NC / 4) + q) ^ (row & 7))] =
             make_float4(sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]);
+      if constexpr (Epi::kOwnSums)
+        if (splits == 1) epi.own(sum, m0 + row, n0 + half * NC, M, N, halves + half * BM + row);
     }
   } else if (TERMS == 3 && warp < 4) {
     // ---------------- B's lo part, in the stage's own layout
@@ -316,7 +350,7 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
     cluster_sync();
   else
     __syncthreads();
-  epi.template rows<BN>(base, m0, n0, part * (BM / splits), BM / splits, splits, M, N, warp, lane,
+  epi.template rows<BN>(base, halves, m0, n0, part * (BM / splits), BM / splits, splits, M, N, warp, lane,
                         TL::THREADS / 32);
   if (splits > 1)
     cluster_sync();  // a peer may still be reading this CTA's part
@@ -334,39 +368,9 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
   __syncthreads();
 }
 
-// The sum over the cluster's parts, in part order, of quad q of tile row r.
-template <int BN>
-__device__ __forceinline__ float4 sum_quad(uint32_t tile, int r, int q, int splits) {
-  const uint32_t at = tile + 16u * static_cast<uint32_t>(r * (BN / 4) + (q ^ (r & 7)));
-  float4 v;
-  if (splits == 1) {
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(at)
-                 : "memory");
-    return v;
-  }
-  v = ld_cluster_quad(mapa_shared(at, 0));
-  if (splits == 2) {
-    const float4 w = ld_cluster_quad(mapa_shared(at, 1));
-    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-    return v;
-  }
-  for (int p = 1; p < splits; p += 3) {  // 4 or 8 parts, at most three loads in flight
-    float4 w[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      w[i] = p + i < splits ? ld_cluster_quad(mapa_shared(at, p + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      v.x += w[i].x; v.y += w[i].y; v.z += w[i].z; v.w += w[i].w;
-    }
-  }
-  return v;
-}
-
 struct LinearDirect {
   LinearEpilogue e;
+  static constexpr bool kOwnSums = false;
   // Rows [r0, r0 + nr) of the tile; BN / 4 lanes per row, four rows of a lane at a
   // time so that their loads are in flight together. The tile inside the matrix
   // (FULL) runs without bounds checks: the loop is bound by its instructions.
@@ -394,18 +398,37 @@ struct LinearDirect {
         if (live && e.R)
           r[u] = FULL ? *reinterpret_cast<const float4*>(e.R + row * e.ldr + col) : load_quad(e.R + row * e.ldr, col, N);
       }
+      // Part by part over the batch, so that the path through the code is short and
+      // straight: a CTA runs it once, and what it costs is fetching it.
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = i + u * step;
-        const long long row = m0 + r0 + j;
-        if (j < nr && (FULL || (row < M && col < N)))
-          linear_quad<FULL>(e, e.act, drop, seed, offset, row, col, N, v[u], bias, r[u]);
+        v[u].x += bias.x; v[u].y += bias.y; v[u].z += bias.z; v[u].w += bias.w;
       }
+      auto put = [&](float* base, long long ld) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int j = i + u * step;
+          const long long row = m0 + r0 + j;
+          if (j < nr && (FULL || (row < M && col < N))) put_quad<FULL>(base + row * ld, col, N, v[u]);
+        }
+      };
+      if (e.Z) put(e.Z, e.ldz);
+      activate_quads<U>(v, e.act);
+      if (drop)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          v[u] = dropout_quad(v[u], e.drop, seed, offset, m0 + r0 + i + u * step, col >> 2);
+      if (e.R)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          v[u].x += r[u].x; v[u].y += r[u].y; v[u].z += r[u].z; v[u].w += r[u].w;
+        }
+      put(e.C, e.ldc);
     }
   }
   template <int BN>
-  __device__ __forceinline__ void rows(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
-                                       int warp, int lane, int warps) const {
+  __device__ __forceinline__ void rows(uint32_t tile, const float2*, int m0, int n0, int r0, int nr, int splits, int M,
+                                       int N, int warp, int lane, int warps) const {
     constexpr int PER = 128 / BN;  // rows a warp covers at once
     const int q = lane % (BN / 4), first = warp * PER + lane / (BN / 4), step = warps * PER;
     if (m0 + r0 + nr <= M && n0 + BN <= N)
@@ -417,11 +440,70 @@ struct LinearDirect {
 
 struct LossDirect {
   LossEpilogue e;
-  // A warp per row, its 128 columns' maximum and sum by shuffles; three rows at a time.
+  static constexpr bool kOwnSums = true;
+  // One part: the summing warps hold the row already, half of it each (lane = row): their
+  // maximum and sum in registers, the halves joined through shared memory.
+  template <int NC>
+  __device__ __forceinline__ void own(const float (&sum)[NC], int row, int n0, int M, int N, float2* half_of) const {
+    const int live = min(NC, N - n0);
+    float m = -INFINITY, s = 0.0f;
+    if (live == NC) {
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, all[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NC; ++i) top[i % 4] = fmaxf(top[i % 4], sum[i]);
+      m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+#pragma unroll
+      for (int i = 0; i < NC; ++i) all[i % 4] += loss_exp(sum[i] - m);
+      s = (all[0] + all[1]) + (all[2] + all[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) m = i < live ? fmaxf(m, sum[i]) : m;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) s += i < live ? loss_exp(sum[i] - m) : 0.0f;
+    }
+    *half_of = make_float2(m, s);
+    if (row < M) {
+      const int t = e.targets[row] - n0;
+      if (t >= 0 && t < live) {
+        float zt = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) zt = i == t ? sum[i] : zt;
+        e.zt[row] = zt;
+      }
+    }
+  }
+  __device__ __forceinline__ void join(float2 a, float2 b, long long row, int n0) const {
+    const float m = fmaxf(a.x, b.x);  // the first half has a column, so b = (-inf, 0) adds nothing
+    e.part[row * e.tiles + n0 / 128] = make_float2(m, a.y * loss_exp(a.x - m) + b.y * loss_exp(b.x - m));
+  }
+  // and the logits, where they are wanted
+  __device__ __forceinline__ void store(uint32_t tile, int m0, int n0, int M, int N, int warp, int lane,
+                                        int warps) const {
+    const int col = n0 + 4 * lane;
+    const bool full = col + 3 < N;
+#pragma unroll 4
+    for (int r = warp; r < BM; r += warps) {
+      if (m0 + r >= M) break;  // uniform over the warp
+      const float4 v = sum_quad<128>(tile, r, lane, 1);
+      float* row = e.Z + static_cast<long long>(m0 + r) * e.ldz;
+      if (full)
+        *reinterpret_cast<float4*>(row + col) = v;
+      else
+        store_quad(row, col, N, v);
+    }
+  }
+  // Several parts: a warp per joined row, its 128 columns' maximum and sum by shuffles;
+  // three rows at a time.
   template <int BN>
-  __device__ __forceinline__ void rows(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
-                                       int warp, int lane, int warps) const {
+  __device__ __forceinline__ void rows(uint32_t tile, const float2* halves, int m0, int n0, int r0, int nr, int splits,
+                                       int M, int N, int warp, int lane, int warps) const {
     static_assert(BN == 128, "one partial per 128 columns");
+    if (splits == 1) {
+      const int r = warp * 32 + lane;
+      if (r < BM && m0 + r < M) join(halves[r], halves[BM + r], m0 + r, n0);
+      if (e.Z) store(tile, m0, n0, M, N, warp, lane, warps);
+      return;
+    }
     const int col = n0 + 4 * lane;
     constexpr int U = 3;
     for (int i = warp; i < nr && m0 + r0 + i < M; i += U * warps) {  // uniform over the warp

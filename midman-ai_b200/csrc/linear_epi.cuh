@@ -56,6 +56,23 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
   }
 }
 
+// The activation of U quads, one branch for all of them.
+template <int U>
+__device__ __forceinline__ void activate_quads(float4 (&v)[U], int act) {
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u].x = f(v[u].x); v[u].y = f(v[u].y); v[u].z = f(v[u].z); v[u].w = f(v[u].w);
+    }
+  };
+  switch (act) {
+    case kActRelu: each([](float z) { return activate(z, kActRelu); }); break;
+    case kActGelu: each([](float z) { return activate(z, kActGelu); }); break;
+    case kActSilu: each([](float z) { return activate(z, kActSilu); }); break;
+    default: break;
+  }
+}
+
 // Four columns of a row; those at n and past it are not touched.
 __device__ __forceinline__ float4 load_quad(const float* row, int col, int n) {
   if (col + 3 < n) return *reinterpret_cast<const float4*>(row + col);

@@ -132,12 +132,16 @@ __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int t
 }
 
 // One row's kSegment logits -> gradients, in place; every block of a row joins
-// the row's pairs itself (vocab / 128 of them, from L2), the first writes the loss.
+// the row's pairs itself (vocab / 128 of them, from L2), the first writes the loss and,
+// where dw is wanted, copies the row of x (zeros for a row without a target: dw sums
+// over all rows, and 0 times what such a row holds may be NaN).
 constexpr int kSegment = 8192;
 
 __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz, const float2* part, int tiles,
                                                         const float* zt, const int32_t* targets, int vocab,
-                                                        float grad_scale, float* row_loss, int* err) {
+                                                        float grad_scale, float* row_loss, const float* x,
+                                                        long long ldx, int dim, float* live_x, long long ldl,
+                                                        int* err) {
   __shared__ MaxSum warps[8];
   const int r = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int t = targets[r];
@@ -153,6 +157,10 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
   a = warps[0];
   for (int w = 1; w < 8; ++w) a = join(a, warps[w]);
   if (blockIdx.y == 0 && threadIdx.x == 0) row_loss[r] = loss_of(a, t, vocab, zt + r, err);
+  if (blockIdx.y == 0 && live_x)
+    for (int c = 4 * threadIdx.x; c < dim; c += 1024)  // ldl is dim rounded up to 4
+      *reinterpret_cast<float4*>(live_x + r * ldl + c) =
+          live ? load_quad(x + r * ldx, c, dim) : make_float4(0.f, 0.f, 0.f, 0.f);
   const float coef = grad_scale / a.s;
   float4* row = reinterpret_cast<float4*>(z + r * ldz);
   const int q_end = static_cast<int>(ldz / 4), q0 = blockIdx.y * (kSegment / 4);
@@ -169,31 +177,6 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
       }
     }
     row[q] = g;
-  }
-}
-
-// x with the rows that have no target as zeros: dw sums over all rows, and 0 times
-// what such a row holds may be NaN. A warp per row.
-__global__ void __launch_bounds__(256) live_rows_kernel(const float* x, long long ldx, const int32_t* targets,
-                                                        int rows, int dim, int vocab, float* out, long long ldo) {
-  const int r = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (r >= rows) return;
-  const int t = targets[r];
-  const bool live = t >= 0 && t < vocab;
-  const float* src = x + r * ldx;
-  float* dst = out + r * ldo;
-  for (int c = 4 * lane; c < dim; c += 128) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) {
-      if (c + 3 < dim) {
-        v = *reinterpret_cast<const float4*>(src + c);
-      } else {
-        v.x = src[c];
-        if (c + 1 < dim) v.y = src[c + 1];
-        if (c + 2 < dim) v.z = src[c + 2];
-      }
-    }
-    *reinterpret_cast<float4*>(dst + c) = v;  // ldo is dim rounded up to 4
   }
 }
 
@@ -240,8 +223,11 @@ namespace {
 int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStream_t s) {
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
+  // x's rows without a target count as zeros: their logits are not used, and dw sums over
+  // all rows, where 0 times what such a row holds may be NaN
   p.xr = split_copy_at(p.xr_at, n, a.dim);
-  split(SplitMatrix{x, a.ldx}, n, a.dim, &p.xr, nullptr, s);
+  if (a.dw) p.xt = split_copy_at(p.xt_at, a.dim, n);
+  split(SplitMatrix{x, a.ldx, t, a.vocab}, n, a.dim, &p.xr, a.dw ? &p.xt : nullptr, s);
   const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt};
   int rc = pair_loss_product(p.xr, p.w, e, d_err, s);
   if (rc) return rc;
@@ -262,8 +248,6 @@ int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStre
     if (rc) return rc;
   }
   if (a.dw) {
-    p.xt = split_copy_at(p.xt_at, a.dim, n);
-    split(SplitMatrix{x, a.ldx, t, a.vocab}, n, a.dim, nullptr, &p.xt, s);
     LinearEpilogue o;
     o.C = a.dw;
     o.R = a.accumulate || r0 > 0 ? a.dw : nullptr;
@@ -288,7 +272,7 @@ int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, 
   }
   const dim3 grid(n, static_cast<unsigned>((p.ldz + kSegment - 1) / kSegment));
   loss_grad_kernel<<<grid, 256, 0, s>>>(p.z, p.ldz, p.part, p.tiles, p.zt, t, a.vocab, a.grad_scale, a.row_loss + r0,
-                                        d_err);
+                                        x, a.ldx, a.dim, a.dw ? p.x : nullptr, p.ldx, d_err);
   check_cuda(cudaGetLastError(), "loss gradient");
   if (a.dx) {
     LinearEpilogue o;
@@ -300,8 +284,6 @@ int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, 
     if (rc) return rc;
   }
   if (a.dw) {
-    live_rows_kernel<<<(n + 7) / 8, 256, 0, s>>>(x, a.ldx, t, n, a.dim, a.vocab, p.x, p.ldx);
-    check_cuda(cudaGetLastError(), "live rows");
     LinearEpilogue o;
     o.C = a.dw;
     o.R = a.accumulate || r0 > 0 ? a.dw : nullptr;
