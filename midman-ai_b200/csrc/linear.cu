@@ -93,7 +93,7 @@ __device__ __forceinline__ float4 sum_quad(uint32_t tile, int r, int q, int spli
     v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
     return v;
   }
-  for (int p = 1; p < splits; p += 3) {  // 4 or 8 parts, at most three loads in flight
+  for (int p = 1; p < splits; p += 3) {  // at most three loads in flight
     float4 w[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i)
@@ -350,7 +350,8 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
     cluster_sync();
   else
     __syncthreads();
-  epi.template rows<BN>(base, halves, m0, n0, part * (BM / splits), BM / splits, splits, M, N, warp, lane,
+  const int r0 = BM * part / splits;
+  epi.template rows<BN>(base, halves, m0, n0, r0, BM * (part + 1) / splits - r0, splits, M, N, warp, lane,
                         TL::THREADS / 32);
   if (splits > 1)
     cluster_sync();  // a peer may still be reading this CTA's part
@@ -805,27 +806,27 @@ __global__ void __launch_bounds__(256) dropout_kernel(const float* x, long long 
 // ------------------------------------------------------------------ host side
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// How a product is cut: 128 x 64 tiles when even with K in parts the wider ones would
-// leave half of the SMs idle, and K in as many parts (a cluster's CTAs) as fit the SMs
-// beside one another, each at least four K steps. A cluster lies in one GPC, and
-// of clusters of eight only about fourteen fit the device at once (with sixteen the
-// last start when the first have ended): 2048 x 4096 x 128 in eight parts took 40 us.
-struct DirectPlan {
-  int bn, splits;
-};
-DirectPlan direct_plan(int M, int N, int K, bool any_bn) {
-  const int sms = 148, n_k = (K + BK - 1) / BK;
-  const long long tm = (M + BM - 1) / BM;
-  DirectPlan p{128, 1};
-  auto splits_of = [&](long long tiles) {
-    int s = 1;
-    while (s < 8 && tiles * s * 2 <= (s == 4 ? 112 : sms) && n_k / (2 * s) >= 4) s *= 2;
-    return s;
-  };
-  const long long t128 = tm * ((N + 127) / 128), t64 = tm * ((N + 63) / 64);
-  if (any_bn && (N <= 64 || 2 * t128 * splits_of(t128) <= sms)) p.bn = 64;
-  p.splits = splits_of(p.bn == 128 ? t128 : t64);
-  return p;
+// How many parts K is cut into (a cluster's CTAs): the count with the shortest time by
+// waves of clusters, steps of a part and a tile's fixed cost. A cluster lies in one
+// GPC, so fewer CTAs run at once in larger ones (the occupancy query's counts for this
+// kernel on a B200; a device with other GPCs runs the same plan in other waves). A step
+// takes 0.6 us, a tile's start and end about 5, the parts' join 1. (128 x 64 tiles, tried
+// for more CTAs, took 0.69 us a step: a UMMA of half the width is no shorter.)
+int direct_splits(int M, int N, int K) {
+  constexpr int kFit[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+  const long long tiles = static_cast<long long>((M + BM - 1) / BM) * ((N + 127) / 128);
+  const int n_k = (K + BK - 1) / BK;
+  int best = 1;
+  double best_us = 0.0;
+  for (int s = 1; s <= 8 && (s == 1 || n_k >= 4 * s); ++s) {
+    const double waves = static_cast<double>((tiles + kFit[s] - 1) / kFit[s]);
+    const double us = waves * ((n_k + s - 1) / s * 0.6 + 5.0 + (s > 1 ? 1.0 : 0.0));
+    if (s == 1 || us < best_us) {
+      best = s;
+      best_us = us;
+    }
+  }
+  return best;
 }
 
 template <class Kernel, class... Args>
@@ -881,12 +882,12 @@ void launch_few(int M, int N, int K, const GemmOperand& A, const GemmOperand& B,
                     splits);
 }
 
-template <int TERMS, int BN, class Epi>
+template <int TERMS, class Epi>
 int direct_majors(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, int splits,
                   int* d_err, cudaStream_t s) {
-  if (!A.mn_major && !B.mn_major) return launch_direct<TERMS, false, false, BN>(M, N, K, A, B, epi, splits, d_err, s);
-  if (!A.mn_major) return launch_direct<TERMS, false, true, BN>(M, N, K, A, B, epi, splits, d_err, s);
-  if (B.mn_major) return launch_direct<TERMS, true, true, BN>(M, N, K, A, B, epi, splits, d_err, s);
+  if (!A.mn_major && !B.mn_major) return launch_direct<TERMS, false, false, 128>(M, N, K, A, B, epi, splits, d_err, s);
+  if (!A.mn_major) return launch_direct<TERMS, false, true, 128>(M, N, K, A, B, epi, splits, d_err, s);
+  if (B.mn_major) return launch_direct<TERMS, true, true, 128>(M, N, K, A, B, epi, splits, d_err, s);
   return kGemmBadArgument;  // no caller has an MN-major A with a K-major B
 }
 
@@ -934,26 +935,23 @@ int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const Line
     else launch_few<8>(M, N, K, A, B, e, s);
     return 0;
   }
-  const DirectPlan p = direct_plan(M, N, K, true);
   const LinearDirect epi{e};
-  if (exact)
-    return p.bn == 128 ? direct_majors<3, 128>(M, N, K, A, B, epi, p.splits, d_err, s)
-                       : direct_majors<3, 64>(M, N, K, A, B, epi, p.splits, d_err, s);
-  return p.bn == 128 ? direct_majors<1, 128>(M, N, K, A, B, epi, p.splits, d_err, s)
-                     : direct_majors<1, 64>(M, N, K, A, B, epi, p.splits, d_err, s);
+  const int splits = direct_splits(M, N, K);
+  return exact ? direct_majors<3>(M, N, K, A, B, epi, splits, d_err, s)
+               : direct_majors<1>(M, N, K, A, B, epi, splits, d_err, s);
 }
 
 int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
                  cudaStream_t s) {
   if (M <= 0 || N <= 0) return 0;
   if (A.mn_major) return kGemmBadArgument;
-  const DirectPlan p = direct_plan(M, N, K, false);
   const LossDirect epi{e};
+  const int splits = direct_splits(M, N, K);
   if (exact)
-    return B.mn_major ? launch_direct<3, false, true, 128>(M, N, K, A, B, epi, p.splits, d_err, s)
-                      : launch_direct<3, false, false, 128>(M, N, K, A, B, epi, p.splits, d_err, s);
-  return B.mn_major ? launch_direct<1, false, true, 128>(M, N, K, A, B, epi, p.splits, d_err, s)
-                    : launch_direct<1, false, false, 128>(M, N, K, A, B, epi, p.splits, d_err, s);
+    return B.mn_major ? launch_direct<3, false, true, 128>(M, N, K, A, B, epi, splits, d_err, s)
+                      : launch_direct<3, false, false, 128>(M, N, K, A, B, epi, splits, d_err, s);
+  return B.mn_major ? launch_direct<1, false, true, 128>(M, N, K, A, B, epi, splits, d_err, s)
+                    : launch_direct<1, false, false, 128>(M, N, K, A, B, epi, splits, d_err, s);
 }
 
 int act_backward_parts(int rows) { return (rows + kActRows - 1) / kActRows; }
