@@ -10,8 +10,9 @@
 // direction, so every 64 of K start a fresh TMEM accumulation and the chunks are
 // summed in f32 registers.
 //
-// direct_kernel: one 128 x BN tile per cluster of `splits` CTAs, each CTA a part
-// of K. TMA brings the f32 operands. Their lo parts are made on the way, which saves
+// direct_kernel: one 128 x 128 tile per cluster of `splits` CTAs, each CTA a part
+// of K (and where few tiles share a long K, clusters for its slices, whose sums go to
+// the workspace and join_kernel). TMA brings the f32 operands. Their lo parts are made on the way, which saves
 // the passes and the workspace of copies made beforehand (short products are bound by
 // latency and one reading of the operands): four warps take A's rows to tensor
 // memory, hi and lo, where the UMMAs read them; two write B's lo part beside it in
@@ -125,7 +126,7 @@ __device__ __forceinline__ void tile_mn(int t, int tm, int tn, int& mt, int& nt)
 template <int TERMS, bool A_MN, bool B_MN, int BN, class Epi>
 __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
     direct_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Epi epi,
-                  int M, int N, int K, int splits, int mn3d, int* err) {
+                  int M, int N, int K, int splits, int slices, long long slice_stride, int mn3d, int* err) {
   using TL = DirectTile<TERMS, BN>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -147,12 +148,13 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int part = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN;
+  const int cluster = static_cast<int>(blockIdx.x) / splits, slice = cluster / (tm * tn);
   int mt, nt;
-  tile_mn(static_cast<int>(blockIdx.x) / splits, tm, tn, mt, nt);
+  tile_mn(cluster - slice * (tm * tn), tm, tn, mt, nt);
   const int m0 = mt * BM, n0 = nt * BN;
   const int n_k = (K + BK - 1) / BK;
-  const int kb = static_cast<int>(static_cast<long long>(n_k) * part / splits);
-  const int ke = static_cast<int>(static_cast<long long>(n_k) * (part + 1) / splits);
+  const long long kpart = static_cast<long long>(slice) * splits + part, kparts = static_cast<long long>(slices) * splits;
+  const int kb = static_cast<int>(n_k * kpart / kparts), ke = static_cast<int>(n_k * (kpart + 1) / kparts);
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmA);
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
   else
     __syncthreads();
   const int r0 = BM * part / splits;
-  epi.template rows<BN>(base, halves, m0, n0, r0, BM * (part + 1) / splits - r0, splits, M, N, warp, lane,
+  epi.slice(slice * slice_stride).template rows<BN>(base, halves, m0, n0, r0, BM * (part + 1) / splits - r0, splits, M, N, warp, lane,
                         TL::THREADS / 32);
   if (splits > 1)
     cluster_sync();  // a peer may still be reading this CTA's part
@@ -372,6 +374,11 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
 struct LinearDirect {
   LinearEpilogue e;
   static constexpr bool kOwnSums = false;
+  __device__ __forceinline__ LinearDirect slice(long long offset) const {
+    LinearDirect d = *this;
+    d.e.C += offset;
+    return d;
+  }
   // Rows [r0, r0 + nr) of the tile; BN / 4 lanes per row, four rows of a lane at a
   // time so that their loads are in flight together. The tile inside the matrix
   // (FULL) runs without bounds checks: the loop is bound by its instructions.
@@ -442,6 +449,7 @@ struct LinearDirect {
 struct LossDirect {
   LossEpilogue e;
   static constexpr bool kOwnSums = true;
+  __device__ __forceinline__ LossDirect slice(long long) const { return *this; }
   // One part: the summing warps hold the row already, half of it each (lane = row): their
   // maximum and sum in registers, the halves joined through shared memory.
   template <int NC>
@@ -580,15 +588,19 @@ constexpr int few_blocks(int mt) { return mt <= 4 ? 4 : 3; }  // CTAs of an SM, 
 
 template <int MT, bool B_MN>
 __global__ void __launch_bounds__(256, few_blocks(MT)) few_rows_kernel(const float* a, long long lda, const float* b, long long ldb,
-                                                       const LinearEpilogue e, int M, int N, int K, int splits) {
+                                                       LinearEpilogue e, int M, int N, int K, int splits,
+                                                       int slices, long long slice_stride) {
   __shared__ __align__(16) float as[kFewPiece * MT];
   __shared__ __align__(16) float sums[(B_MN ? 8 : 1) * MT * kFewCols];  // [warps][MT][32], then [MT][32]
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int part = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int n0 = static_cast<int>(blockIdx.x) / splits * kFewCols;
+  const int tiles = (N + kFewCols - 1) / kFewCols, cluster = static_cast<int>(blockIdx.x) / splits;
+  const int slice = cluster / tiles, n0 = (cluster - slice * tiles) * kFewCols;
+  e.C += slice * slice_stride;
   const int units = (K + 31) / 32;  // parts are cut at multiples of 32
-  const int kb = static_cast<int>(static_cast<long long>(units) * part / splits) * 32;
-  const int ke = min(K, static_cast<int>(static_cast<long long>(units) * (part + 1) / splits) * 32);
+  const long long kpart = static_cast<long long>(slice) * splits + part, kparts = static_cast<long long>(slices) * splits;
+  const int kb = static_cast<int>(units * kpart / kparts) * 32;
+  const int ke = min(K, static_cast<int>(units * (kpart + 1) / kparts) * 32);
   float acc[4 * MT];  // [MT][4 columns]
 #pragma unroll
   for (int i = 0; i < 4 * MT; ++i) acc[i] = 0.0f;
@@ -711,6 +723,27 @@ __global__ void __launch_bounds__(256, few_blocks(MT)) few_rows_kernel(const flo
   if (splits > 1) cluster_sync();  // a peer may still be reading this CTA's part
 }
 
+// ------------------------------------------------------------------ K slices
+// The slices' sums [slices][M, ld], in slice order, and the epilogue: a thread per quad.
+__global__ void __launch_bounds__(256) join_kernel(const float* parts, int slices, long long slice_stride,
+                                                   long long ld, const LinearEpilogue e, int M, int N) {
+  const int quads = (N + 3) / 4;
+  const long long i = blockIdx.x * 256ll + threadIdx.x, row = i / quads;
+  const int col = 4 * static_cast<int>(i - row * quads);
+  if (row >= M) return;
+  const float* p = parts + row * ld + col;
+  float4 v = *reinterpret_cast<const float4*>(p);  // ld is N rounded up to 4
+#pragma unroll 4
+  for (int k = 1; k < slices; ++k) {
+    const float4 o = *reinterpret_cast<const float4*>(p + k * slice_stride);
+    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+  }
+  const bool drop = e.drop.rng != nullptr;
+  const float4 r = e.R ? load_quad(e.R + row * e.ldr, col, N) : make_float4(0.f, 0.f, 0.f, 0.f);
+  linear_quad(e, e.act, drop, drop ? e.drop.rng[0] : 0, drop ? e.drop.rng[1] : 0, row, col, N, v, bias_quad(e, col, N),
+              r);
+}
+
 // ------------------------------------------------------------------ backward of the epilogue
 // dz and the column sums' partials: 64 rows x 128 columns per block, a warp per
 // row, so every access covers 512 contiguous bytes. Bound by HBM: 4 (dc) + 4 (z)
@@ -806,28 +839,51 @@ __global__ void __launch_bounds__(256) dropout_kernel(const float* x, long long 
 // ------------------------------------------------------------------ host side
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// How many parts K is cut into (a cluster's CTAs): the count with the shortest time by
-// waves of clusters, steps of a part and a tile's fixed cost. A cluster lies in one
-// GPC, so fewer CTAs run at once in larger ones (the occupancy query's counts for this
-// kernel on a B200; a device with other GPCs runs the same plan in other waves). A step
-// takes 0.6 us, a tile's start and end about 5, the parts' join 1. (128 x 64 tiles, tried
-// for more CTAs, took 0.69 us a step: a UMMA of half the width is no shorter.)
-int direct_splits(int M, int N, int K) {
+// How K is cut: into parts (a cluster's CTAs) and slices (clusters), by the shortest
+// time from waves of clusters, steps of a part and a tile's fixed cost. A cluster lies
+// in one GPC, so fewer CTAs run at once in larger ones (the occupancy query's counts for
+// this kernel on a B200; a device with other GPCs runs the same plan in other waves). A
+// step takes 0.6 us, a tile's start and end about 5, the parts' join 1, writing,
+// reading and joining slices 6 (64 x 32000 -> 512 in eight parts alone took 80 us, in
+// four slices of eight 25). (128 x 64 tiles, tried for more CTAs, took 0.69 us a step: a
+// UMMA of half the width is no shorter.)
+struct Cut {
+  int splits = 1, slices = 1;
+};
+Cut direct_cut(int M, int N, int K, bool sliced) {
   constexpr int kFit[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
   const long long tiles = static_cast<long long>((M + BM - 1) / BM) * ((N + 127) / 128);
   const int n_k = (K + BK - 1) / BK;
-  int best = 1;
-  double best_us = 0.0;
-  for (int s = 1; s <= 8 && (s == 1 || n_k >= 4 * s); ++s) {
-    const double waves = static_cast<double>((tiles + kFit[s] - 1) / kFit[s]);
-    const double us = waves * ((n_k + s - 1) / s * 0.6 + 5.0 + (s > 1 ? 1.0 : 0.0));
-    if (s == 1 || us < best_us) {
-      best = s;
-      best_us = us;
+  Cut best;
+  double best_us = 1e30;
+  for (int s = 1; s <= 8 && (s == 1 || n_k >= 4 * s); ++s)
+    for (int l = 1; l <= (sliced ? 32 : 1) && (l == 1 || (n_k >= 8 * s * l && tiles * l <= kFit[s])); ++l) {
+      const double waves = static_cast<double>((tiles * l + kFit[s] - 1) / kFit[s]);
+      const double us = waves * ((n_k + s * l - 1) / (s * l) * 0.6 + 5.0 + (s > 1 ? 1.0 : 0.0)) + (l > 1 ? 6.0 : 0.0);
+      if (us < best_us) {
+        best = {s, l};
+        best_us = us;
+      }
     }
-  }
   return best;
 }
+
+// Few rows: parts that all run at once, each at least 256 of K, then slices while one
+// has more than 2048 of it.
+Cut few_cut(int M, int N, int K) {
+  const int fit = few_blocks(M <= 4 ? 4 : 8) * 148;
+  const long long tiles = (N + kFewCols - 1) / kFewCols;
+  Cut c;
+  while (c.splits < 8 && tiles * c.splits * 2 <= fit && K / (2 * c.splits) >= 256) c.splits *= 2;
+  while (tiles * c.splits * c.slices * 2 <= fit && K / (c.splits * c.slices * 2) >= 1024) c.slices *= 2;
+  return c;
+}
+
+Cut cut_of(int M, int N, int K, bool a_mn_major) {
+  return M <= kFewRows && !a_mn_major ? few_cut(M, N, K) : direct_cut(M, N, K, true);
+}
+
+long long slice_floats(int M, int N) { return M * ((N + 3ll) & ~3ll); }
 
 template <class Kernel, class... Args>
 void launch_clusters(Kernel kern, long long tiles, int splits, int threads, int smem, cudaStream_t s, Args... args) {
@@ -846,7 +902,7 @@ void launch_clusters(Kernel kern, long long tiles, int splits, int threads, int 
 }
 
 template <int TERMS, bool A_MN, bool B_MN, int BN, class Epi>
-int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, int splits,
+int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, Cut cut,
                   int* d_err, cudaStream_t s) {
   using TL = DirectTile<TERMS, BN>;
   CUtensorMap ta{}, tb{};
@@ -863,31 +919,27 @@ int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& 
     configured_device = dev;
   }
   const long long tiles = static_cast<long long>((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-  if (tiles * splits > 0x7fffffffll) return kGemmBadArgument;
-  launch_clusters(kern, tiles, splits, TL::THREADS, TL::SMEM, s, ta, tb, epi, M, N, K, splits,
-                  (a3 ? 1 : 0) | (b3 ? 2 : 0), d_err);
+  if (tiles * cut.splits * cut.slices > 0x7fffffffll) return kGemmBadArgument;
+  launch_clusters(kern, tiles * cut.slices, cut.splits, TL::THREADS, TL::SMEM, s, ta, tb, epi, M, N, K, cut.splits,
+                  cut.slices, slice_floats(M, N), (a3 ? 1 : 0) | (b3 ? 2 : 0), d_err);
   return 0;
 }
 
 template <int MT>
-void launch_few(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e,
+void launch_few(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e, Cut cut,
                 cudaStream_t s) {
-  const long long tiles = (N + kFewCols - 1) / kFewCols;
-  int splits = 1;  // parts that all run at once, each at least 256 of K
-  while (splits < 8 && tiles * splits * 2 <= few_blocks(MT) * 148 && K / (2 * splits) >= 256) splits *= 2;
-  if (B.mn_major)
-    launch_clusters(few_rows_kernel<MT, true>, tiles, splits, 256, 0, s, A.ptr, A.ld, B.ptr, B.ld, e, M, N, K, splits);
-  else
-    launch_clusters(few_rows_kernel<MT, false>, tiles, splits, 256, 0, s, A.ptr, A.ld, B.ptr, B.ld, e, M, N, K,
-                    splits);
+  const long long clusters = (N + kFewCols - 1) / kFewCols * static_cast<long long>(cut.slices);
+  auto kern = B.mn_major ? few_rows_kernel<MT, true> : few_rows_kernel<MT, false>;
+  launch_clusters(kern, clusters, cut.splits, 256, 0, s, A.ptr, A.ld, B.ptr, B.ld, e, M, N, K, cut.splits, cut.slices,
+                  slice_floats(M, N));
 }
 
 template <int TERMS, class Epi>
-int direct_majors(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, int splits,
+int direct_majors(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, Cut cut,
                   int* d_err, cudaStream_t s) {
-  if (!A.mn_major && !B.mn_major) return launch_direct<TERMS, false, false, 128>(M, N, K, A, B, epi, splits, d_err, s);
-  if (!A.mn_major) return launch_direct<TERMS, false, true, 128>(M, N, K, A, B, epi, splits, d_err, s);
-  if (B.mn_major) return launch_direct<TERMS, true, true, 128>(M, N, K, A, B, epi, splits, d_err, s);
+  if (!A.mn_major && !B.mn_major) return launch_direct<TERMS, false, false, 128>(M, N, K, A, B, epi, cut, d_err, s);
+  if (!A.mn_major) return launch_direct<TERMS, false, true, 128>(M, N, K, A, B, epi, cut, d_err, s);
+  if (B.mn_major) return launch_direct<TERMS, true, true, 128>(M, N, K, A, B, epi, cut, d_err, s);
   return kGemmBadArgument;  // no caller has an MN-major A with a K-major B
 }
 
@@ -925,33 +977,50 @@ DropoutArgs dropout_args(double p, const uint64_t* rng, int cols) {
   return d;
 }
 
-int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, int* d_err,
-                   cudaStream_t s) {
+long long direct_ws_bytes(int M, int N, int K, bool a_mn_major) {
   if (M <= 0 || N <= 0) return 0;
+  const Cut c = cut_of(M, N, K, a_mn_major);
+  return c.slices > 1 ? c.slices * slice_floats(M, N) * 4 : 0;
+}
+
+int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, void* ws,
+                   int* d_err, cudaStream_t s) {
+  if (M <= 0 || N <= 0) return 0;
+  const Cut cut = cut_of(M, N, K, A.mn_major);
+  LinearEpilogue raw;  // a slice's sums as they are
+  raw.C = static_cast<float*>(ws);
+  raw.ldc = (N + 3ll) & ~3ll;
+  const LinearEpilogue& out = cut.slices > 1 ? raw : e;
   if (M <= kFewRows && !A.mn_major) {
-    if (M == 1) launch_few<1>(M, N, K, A, B, e, s);
-    else if (M == 2) launch_few<2>(M, N, K, A, B, e, s);
-    else if (M <= 4) launch_few<4>(M, N, K, A, B, e, s);
-    else launch_few<8>(M, N, K, A, B, e, s);
-    return 0;
+    if (M == 1) launch_few<1>(M, N, K, A, B, out, cut, s);
+    else if (M == 2) launch_few<2>(M, N, K, A, B, out, cut, s);
+    else if (M <= 4) launch_few<4>(M, N, K, A, B, out, cut, s);
+    else launch_few<8>(M, N, K, A, B, out, cut, s);
+  } else {
+    const int rc = exact ? direct_majors<3>(M, N, K, A, B, LinearDirect{out}, cut, d_err, s)
+                         : direct_majors<1>(M, N, K, A, B, LinearDirect{out}, cut, d_err, s);
+    if (rc) return rc;
   }
-  const LinearDirect epi{e};
-  const int splits = direct_splits(M, N, K);
-  return exact ? direct_majors<3>(M, N, K, A, B, epi, splits, d_err, s)
-               : direct_majors<1>(M, N, K, A, B, epi, splits, d_err, s);
+  if (cut.slices > 1) {
+    const long long quads = M * ((N + 3ll) / 4);
+    join_kernel<<<static_cast<unsigned>((quads + 255) / 256), 256, 0, s>>>(raw.C, cut.slices, slice_floats(M, N),
+                                                                         raw.ldc, e, M, N);
+    check_cuda(cudaGetLastError(), "linear");
+  }
+  return 0;
 }
 
 int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
-                 cudaStream_t s) {
+                        cudaStream_t s) {
   if (M <= 0 || N <= 0) return 0;
   if (A.mn_major) return kGemmBadArgument;
   const LossDirect epi{e};
-  const int splits = direct_splits(M, N, K);
+  const Cut cut = direct_cut(M, N, K, false);
   if (exact)
-    return B.mn_major ? launch_direct<3, false, true, 128>(M, N, K, A, B, epi, splits, d_err, s)
-                      : launch_direct<3, false, false, 128>(M, N, K, A, B, epi, splits, d_err, s);
-  return B.mn_major ? launch_direct<1, false, true, 128>(M, N, K, A, B, epi, splits, d_err, s)
-                    : launch_direct<1, false, false, 128>(M, N, K, A, B, epi, splits, d_err, s);
+    return B.mn_major ? launch_direct<3, false, true, 128>(M, N, K, A, B, epi, cut, d_err, s)
+                      : launch_direct<3, false, false, 128>(M, N, K, A, B, epi, cut, d_err, s);
+  return B.mn_major ? launch_direct<1, false, true, 128>(M, N, K, A, B, epi, cut, d_err, s)
+                    : launch_direct<1, false, false, 128>(M, N, K, A, B, epi, cut, d_err, s);
 }
 
 int act_backward_parts(int rows) { return (rows + kActRows - 1) / kActRows; }

@@ -136,8 +136,10 @@ void dropout(const float* x, long long ldx, const float* r, long long ldr, float
 
 // C = epilogue(sum_k A(m, k) B(n, k)) on single CTAs; operands as in gemm.h,
 // precision exact or one TF32 pass. Returns a GemmStatus.
-int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, int* d_err,
-                   cudaStream_t s);
+// ws: direct_ws_bytes bytes (the sums of a long K's slices).
+long long direct_ws_bytes(int M, int N, int K, bool a_mn_major);
+int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, void* ws,
+                   int* d_err, cudaStream_t s);
 // The same product with the loss's epilogue.
 int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
                  cudaStream_t s);
@@ -154,7 +156,7 @@ void sum_parts(const float* part, int parts, int cols, float* out, bool accumula
 // ---- The operators (linear_ops.cu): direct or pair products by size; workspaces
 // are 256-byte aligned.
 // A product on the operands themselves: TF32 on pairs where that suits, else direct.
-long long plain_ws_bytes(int M, int N, int K, bool exact);
+long long plain_ws_bytes(int M, int N, int K, bool a_mn_major, bool exact);
 int plain_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e, bool exact,
                   void* ws, int* d_err, cudaStream_t s);
 int plain_loss_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LossEpilogue& e,

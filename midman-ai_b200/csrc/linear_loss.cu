@@ -82,8 +82,8 @@ Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* w
     const int last = static_cast<int>(n - (blocks - 1) * p.rows);
     long long parts = 0;
     for (const int r : {p.rows, std::max(last, 1)}) {
-      if (dx) parts = std::max(parts, plain_ws_bytes(r, dim, vocab, exact));
-      if (dw) parts = std::max({parts, plain_ws_bytes(vocab, dim, r, exact), plain_ws_bytes(dim, vocab, r, exact)});
+      if (dx) parts = std::max(parts, plain_ws_bytes(r, dim, vocab, false, exact));
+      if (dw) parts = std::max({parts, plain_ws_bytes(vocab, dim, r, true, exact), plain_ws_bytes(dim, vocab, r, true, exact)});
     }
     p.parts = at.take(parts);
   }

@@ -26,7 +26,7 @@ ForwardPlan forward_plan(int m, int n, int k, bool exact, void* ws) {
     p.b = at.copy(n, k);
     p.parts = at.take(pair_ws_bytes(m, n, k));
   } else {
-    p.parts = at.take(plain_ws_bytes(m, n, k, exact));
+    p.parts = at.take(plain_ws_bytes(m, n, k, false, exact));
   }
   p.bytes = at.at;
   return p;
@@ -52,7 +52,8 @@ BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
     p.parts = at.take(std::max(pair_ws_bytes(m, k, n), pair_ws_bytes(k, n, m)));
   } else {
     p.dz_f32 = static_cast<float*>(at.take(m * round4(n) * 4));
-    p.parts = at.take(std::max({plain_ws_bytes(m, k, n, exact), plain_ws_bytes(k, n, m, exact), plain_ws_bytes(n, k, m, exact)}));
+    p.parts = at.take(std::max({plain_ws_bytes(m, k, n, false, exact), plain_ws_bytes(k, n, m, true, exact),
+                                plain_ws_bytes(n, k, m, true, exact)}));
   }
   p.sums = static_cast<float*>(at.take(static_cast<long long>(std::max(act_backward_parts(m), split_parts(m))) * n * 4));
   p.bytes = at.at;
@@ -61,13 +62,13 @@ BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
 
 }  // namespace
 
-long long plain_ws_bytes(int M, int N, int K, bool exact) {
-  return !exact && tf32_pair_suits(M, N, K) ? tf32_pair_ws_bytes(M, N, K) : 0;
+long long plain_ws_bytes(int M, int N, int K, bool a_mn_major, bool exact) {
+  return !exact && tf32_pair_suits(M, N, K) ? tf32_pair_ws_bytes(M, N, K) : direct_ws_bytes(M, N, K, a_mn_major);
 }
 int plain_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e, bool exact,
                   void* ws, int* d_err, cudaStream_t s) {
   if (!exact && tf32_pair_suits(M, N, K)) return tf32_pair_product(M, N, K, A, B, e, ws, d_err, s);
-  return direct_product(M, N, K, A, B, e, exact, d_err, s);
+  return direct_product(M, N, K, A, B, e, exact, ws, d_err, s);
 }
 int plain_loss_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LossEpilogue& e,
                        bool exact, int* d_err, cudaStream_t s) {

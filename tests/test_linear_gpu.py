@@ -89,6 +89,12 @@ FORWARD = [
     (1537, 2052, 1031, True, "gelu", True, 0.1, True, True, 4),
     (2304, 768, 2304, False, "gelu", True, 0.05, True, True, 0),
     (4096, 4099, 513, True, "none", True, 0.0, True, False, 0),
+    # few outputs over a long k
+    (3, 20001, 41, False, "silu", True, 0.1, True, True, 4),
+    (8, 9000, 64, True, "gelu", True, 0.1, True, True, 0),
+    (8, 9001, 1000, False, "none", False, 0.0, False, False, 0),
+    (37, 8196, 101, False, "gelu", True, 0.1, True, True, 4),
+    (130, 16390, 70, True, "none", True, 0.0, True, False, 0),
 ]
 
 
@@ -142,6 +148,7 @@ def test_the_residual_may_be_the_output(mm):
 BACKWARD = [(1, 8, 8, False, "none", True, 0.0, 0), (1, 1, 1, True, "silu", True, 0.0, 0), (3, 7, 5, True, "relu", True, 0.5, 4),
             (37, 501, 1003, True, "gelu", True, 0.1, 8), (65, 40, 129, False, "silu", True, 0.0, 4),
             (129, 2048, 352, False, "none", True, 0.25, 0), (2048, 128, 344, False, "gelu", True, 0.1, 0),
+            (20000, 36, 68, False, "gelu", True, 0.1, 4), (9001, 3, 5, True, "relu", True, 0.1, 0), (20, 40, 12001, False, "silu", True, 0.0, 0),
             (2305, 1031, 1537, False, "gelu", True, 0.1, 4), (2305, 1031, 1537, True, "silu", False, 0.0, 4),
             (4096, 2304, 1536, False, "none", True, 0.0, 0)]
 
@@ -329,7 +336,7 @@ def loss_case(g, rows, vocab, dim, tied, extra):
 # rows, vocab, dim, tied, extra, rows left out
 LOSS = [(1, 1, 4, True, 0, 0), (1, 5, 8, True, 0, 0), (3, 130, 33, False, 4, 1), (64, 1000, 64, True, 4, 5), (129, 4099, 96, False, 0, 0),
         (200, 513, 1030, True, 0, 199), (37, 32003, 260, True, 8, 3), (2049, 512, 128, False, 0, 100), (2304, 2305, 512, True, 0, 0),
-        (700, 131072, 40, True, 0, 9), (600, 120001, 36, False, 4, 9), (1100, 131073, 132, True, 4, 9), (777, 65537, 260, False, 0, 9)]
+        (700, 131072, 40, True, 0, 9), (600, 120001, 36, False, 4, 9), (5, 20001, 40, True, 4, 1), (64, 32000, 64, True, 0, 3), (1100, 131073, 132, True, 4, 9), (777, 65537, 260, False, 0, 9)]
 
 
 @pytest.mark.parametrize("precision", [1, 0])
