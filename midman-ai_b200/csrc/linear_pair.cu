@@ -841,9 +841,19 @@ long long parts_bytes(int M, int N, int steps, int worth) {
   return (tiles_of(M, N) - w.full) * w.splits * (2ll * BM * PN * 4);
 }
 
-// Whether a product keeps half of the pairs busy, with tiles at least a quarter full.
-bool fills(int M, int N, int steps, int worth) {
-  if (M < 64 || N < 64) return false;
+// Whether a product is better on pairs than direct: its units keep half of the pairs
+// busy, its tiles are mostly full, and it is long enough (`least` GFLOP, 2.9 where both
+// sides have two tiles) or has so many tiles that direct ones, which do not overlap
+// their starts and ends, would take three waves. Both sides, device time (us, direct /
+// pair with its copies; exact, then TF32): 1024 x 1024 x 1024 21 / 28, 13 / 18; 256 x 2048 x
+// 5632 49 / 49, 29 / 21; 512 x 1024 x 2816 32 / 30, 18 / 19; 2048 x 512 x 1408 37 / 22,
+// 23 / 14; 1024 x 128 x 8192 37 / 21, 30 / 14; 4096 x 2048 x 5632 525 / 225, 250 / 133; 128 x
+// 2048 x 5632 26 / 47, 15 / 19.
+bool suits(int M, int N, int K, int steps, int worth, double least) {
+  const int side = std::min(M, N);
+  const double gflop = 2e-9 * M * N * K;
+  const long long direct_tiles = ((M + 127ll) / 128) * ((N + 127ll) / 128);
+  if (side < 192 || !(gflop >= least || (side >= 512 && gflop >= 2.9) || direct_tiles >= 3 * 148)) return false;
   const PairWork w = work_of(tiles_of(M, N), steps, worth);
   return 2 * (w.full + (tiles_of(M, N) - w.full) * w.splits) >= kPairs;
 }
@@ -933,9 +943,7 @@ int pair_loss_product(const SplitCopy& A, const SplitCopy& B, const LossEpilogue
   return launch_pair<ExactFeed>(in, LossPair{e}, work, d_err, s);
 }
 
-bool pair_product_suits(int M, int N, int K) {
-  return K >= 128 && fills(M, N, (K + 127) / 128, kWorthExact) && 2e-9 * M * N * K >= 8.0;
-}
+bool pair_product_suits(int M, int N, int K) { return K >= 128 && suits(M, N, K, (K + 127) / 128, kWorthExact, 6.0); }
 
 long long tf32_pair_ws_bytes(int M, int N, int K) { return parts_bytes(M, N, (K + 31) / 32, kWorthTf32); }
 
@@ -971,6 +979,6 @@ int tf32_pair_loss_product(int M, int N, int K, const GemmOperand& A, const Gemm
                     : launch_pair<Tf32Feed<false, false>>(in, LossPair{e}, work, d_err, s);
 }
 
-bool tf32_pair_suits(int M, int N, int K) { return fills(M, N, (K + 31) / 32, kWorthTf32) && 2e-9 * M * N * K >= 2.0; }
+bool tf32_pair_suits(int M, int N, int K) { return suits(M, N, K, (K + 31) / 32, kWorthTf32, 5.0); }
 
 }  // namespace mm
