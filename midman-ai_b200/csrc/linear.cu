@@ -745,18 +745,21 @@ __global__ void __launch_bounds__(256) join_kernel(const float* parts, int slice
 }
 
 // ------------------------------------------------------------------ backward of the epilogue
-// dz and the column sums' partials: 64 rows x 128 columns per block, a warp per
-// row, so every access covers 512 contiguous bytes. Bound by HBM: 4 (dc) + 4 (z)
-// + 4 (dz) bytes an element.
-constexpr int kActRows = 64;
+// dz and the column sums' partials: 64 rows (16 of a small matrix, for enough blocks) x
+// 128 columns per block, a warp per row, so every access covers 512 contiguous bytes.
+// Bound by HBM: 4 (dc) + 4 (z) + 4 (dz) bytes an element.
+int act_rows(int rows, int cols) {
+  return ((rows + 63ll) / 64) * ((cols + 127ll) / 128) >= 2 * 148 ? 64 : 16;
+}
 
 __global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long long lddc, const float* z,
                                                            long long ldz, int act, DropoutArgs drop, int rows,
-                                                           int cols, float* dz, long long lddz, float* part) {
+                                                           int cols, int block_rows, float* dz, long long lddz,
+                                                           float* part) {
   __shared__ float4 sums[8][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int col = (blockIdx.x * 32 + lane) * 4;
-  const int row0 = blockIdx.y * kActRows;
+  const int row0 = blockIdx.y * block_rows;
   uint64_t seed = 0, offset = 0;
   if (drop.rng) {
     seed = drop.rng[0];
@@ -765,7 +768,7 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   if (col < cols) {
 #pragma unroll 4
-    for (int i = warp; i < kActRows; i += 8) {
+    for (int i = warp; i < block_rows; i += 8) {
       const long long row = row0 + i;
       if (row >= rows) break;
       float4 g = load_quad(dc + row * lddc, col, cols);
@@ -1023,13 +1026,16 @@ int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const
                     : launch_direct<1, false, false, 128>(M, N, K, A, B, epi, cut, d_err, s);
 }
 
-int act_backward_parts(int rows) { return (rows + kActRows - 1) / kActRows; }
+int act_backward_parts(int rows, int cols) {
+  const int r = act_rows(rows, cols);
+  return (rows + r - 1) / r;
+}
 
 void act_backward(const float* dc, long long lddc, const float* z, long long ldz, int act, const DropoutArgs& d,
                   int rows, int cols, float* dz, long long lddz, float* part, cudaStream_t s) {
   if (rows <= 0 || cols <= 0) return;
-  const dim3 grid((cols + 127) / 128, act_backward_parts(rows));
-  act_backward_kernel<<<grid, 256, 0, s>>>(dc, lddc, z, ldz, act, d, rows, cols, dz, lddz, part);
+  const dim3 grid((cols + 127) / 128, act_backward_parts(rows, cols));
+  act_backward_kernel<<<grid, 256, 0, s>>>(dc, lddc, z, ldz, act, d, rows, cols, act_rows(rows, cols), dz, lddz, part);
   check_cuda(cudaGetLastError(), "linear backward");
 }
 

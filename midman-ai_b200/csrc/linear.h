@@ -146,10 +146,10 @@ int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const
 
 // dz = mask / (1 - p) * dc * act'(z) (dz null: only the column sums), and the
 // column sums' partials for dbias where part is not null: part must hold
-// act_backward_parts(rows) * cols floats.
+// act_backward_parts(rows, cols) * cols floats.
 void act_backward(const float* dc, long long lddc, const float* z, long long ldz, int act, const DropoutArgs& d,
                   int rows, int cols, float* dz, long long lddz, float* part, cudaStream_t s);
-int act_backward_parts(int rows);
+int act_backward_parts(int rows, int cols);
 // out[c] (+)= sum over p of part[p, c], in f64 and in a fixed order.
 void sum_parts(const float* part, int parts, int cols, float* out, bool accumulate, cudaStream_t s);
 

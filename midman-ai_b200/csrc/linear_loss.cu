@@ -120,9 +120,13 @@ __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int t
   const int r = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   if (r >= rows) return;
   MaxSum a{-INFINITY, 0.0f};
-  for (int i = lane; i < tiles; i += 32) {
-    const float2 p = part[static_cast<long long>(r) * tiles + i];
-    a = join(a, {p.x, p.y});
+  const float2* mine = part + static_cast<long long>(r) * tiles;
+  for (int i = lane; i < tiles; i += 256) {  // eight loads in flight
+    float2 p[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) p[u] = i + 32 * u < tiles ? mine[i + 32 * u] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) a = join(a, {p[u].x, p[u].y});
   }
   a = warp_join(a);
   if (lane == 0) {
@@ -219,7 +223,7 @@ long long linear_loss_ws_bytes(int rows, int vocab, int dim, bool grad, bool exa
 
 namespace {
 
-// One block of rows on copies. The copies of w are made before the first block.
+// One block of rows on copies; the first makes those of w too.
 int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStream_t s) {
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
@@ -227,7 +231,18 @@ int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStre
   // all rows, where 0 times what such a row holds may be NaN
   p.xr = split_copy_at(p.xr_at, n, a.dim);
   if (a.dw) p.xt = split_copy_at(p.xt_at, a.dim, n);
-  split(SplitMatrix{x, a.ldx, t, a.vocab}, n, a.dim, &p.xr, a.dw ? &p.xt : nullptr, s);
+  const SplitMatrix xm{x, a.ldx, t, a.vocab};
+  const SplitCopy* xt = a.dw ? &p.xt : nullptr;
+  if (r0 == 0) {  // with w, [vocab, dim] or [dim, vocab]
+    const SplitCopy* wt = a.dx ? &p.wt : nullptr;
+    const SplitMatrix w{a.w, a.ldw};
+    if (a.w_mn_major)
+      split_two(w, a.dim, a.vocab, wt, &p.w, xm, n, a.dim, &p.xr, xt, s);
+    else
+      split_two(w, a.vocab, a.dim, &p.w, wt, xm, n, a.dim, &p.xr, xt, s);
+  } else {
+    split(xm, n, a.dim, &p.xr, xt, s);
+  }
   const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt};
   int rc = pair_loss_product(p.xr, p.w, e, d_err, s);
   if (rc) return rc;
@@ -300,13 +315,6 @@ int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, 
 int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
   const bool grad = a.dx || a.dw;
   Plan p = plan_of(a.rows, a.vocab, a.dim, grad, grad, a.exact, ws);
-  if (p.pair) {
-    const SplitCopy* wt = a.dx ? &p.wt : nullptr;
-    if (a.w_mn_major)  // w is [dim, vocab]
-      split(SplitMatrix{a.w, a.ldw}, a.dim, a.vocab, wt, &p.w, s);
-    else
-      split(SplitMatrix{a.w, a.ldw}, a.vocab, a.dim, &p.w, wt, s);
-  }
   for (int r0 = 0; r0 < a.rows; r0 += p.rows) {
     const int n = std::min(p.rows, a.rows - r0);
     const int rc = p.pair ? pair_block(a, p, r0, n, d_err, s) : direct_block(a, p, r0, n, d_err, s);

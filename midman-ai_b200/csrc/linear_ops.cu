@@ -55,7 +55,7 @@ BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
     p.parts = at.take(std::max({plain_ws_bytes(m, k, n, false, exact), plain_ws_bytes(k, n, m, true, exact),
                                 plain_ws_bytes(n, k, m, true, exact)}));
   }
-  p.sums = static_cast<float*>(at.take(static_cast<long long>(std::max(act_backward_parts(m), split_parts(m))) * n * 4));
+  p.sums = static_cast<float*>(at.take(static_cast<long long>(std::max(act_backward_parts(m, n), split_parts(m))) * n * 4));
   p.bytes = at.at;
   return p;
 }
@@ -133,7 +133,7 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
   if (!plain || f.dbias)
     act_backward(f.dc, f.lddc, f.z, f.ldz, f.act, f.drop, f.m, f.n, plain ? nullptr : p.dz_f32, ldz,
                  f.dbias ? p.sums : nullptr, s);
-  if (f.dbias) sum_parts(p.sums, act_backward_parts(f.m), f.n, f.dbias, f.accumulate, s);
+  if (f.dbias) sum_parts(p.sums, act_backward_parts(f.m, f.n), f.n, f.dbias, f.accumulate, s);
   const float* g = plain ? f.dc : p.dz_f32;
   const long long ldg = plain ? f.lddc : ldz;
   if (f.da)
