@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <stdexcept>
 
 #include "device.h"
 #include "gemm.h"
@@ -758,8 +759,9 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long
                                                            float* part) {
   __shared__ float4 sums[8][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int col = (blockIdx.x * 32 + lane) * 4;
-  const int row0 = blockIdx.y * block_rows;
+  const int across = (cols + 127) / 128, band = static_cast<int>(blockIdx.x) / across;
+  const int col = ((static_cast<int>(blockIdx.x) - band * across) * 32 + lane) * 4;
+  const int row0 = band * block_rows;
   uint64_t seed = 0, offset = 0;
   if (drop.rng) {
     seed = drop.rng[0];
@@ -790,7 +792,7 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long
       const float4 o = sums[w][lane];
       sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w;
     }
-    float* p = part + static_cast<long long>(blockIdx.y) * cols;  // rows of `cols`: any alignment
+    float* p = part + static_cast<long long>(band) * cols;  // rows of `cols`: any alignment
     p[col] = sum.x;
     if (col + 1 < cols) p[col + 1] = sum.y;
     if (col + 2 < cols) p[col + 2] = sum.z;
@@ -1034,8 +1036,9 @@ int act_backward_parts(int rows, int cols) {
 void act_backward(const float* dc, long long lddc, const float* z, long long ldz, int act, const DropoutArgs& d,
                   int rows, int cols, float* dz, long long lddz, float* part, cudaStream_t s) {
   if (rows <= 0 || cols <= 0) return;
-  const dim3 grid((cols + 127) / 128, act_backward_parts(rows, cols));
-  act_backward_kernel<<<grid, 256, 0, s>>>(dc, lddc, z, ldz, act, d, rows, cols, act_rows(rows, cols), dz, lddz, part);
+  const long long blocks = (cols + 127ll) / 128 * act_backward_parts(rows, cols);
+  if (blocks > INT32_MAX) throw std::invalid_argument("a matrix is too large");
+  act_backward_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(dc, lddc, z, ldz, act, d, rows, cols, act_rows(rows, cols), dz, lddz, part);
   check_cuda(cudaGetLastError(), "linear backward");
 }
 

@@ -37,6 +37,10 @@ struct LossEpilogue {
   int tiles = 0;
   const int32_t* targets = nullptr;
   float* zt = nullptr;  // [rows]: the target's logit
+  // Instead of the logits (pair_loss_product): each row's 128 columns' exp(logit -
+  // maximum) 2^14 as a split copy's halves, rows of copy_ld.
+  uint16_t* copy = nullptr;
+  long long copy_ld = 0;
 };
 
 // The operand's tensor map: `mn` rows (or columns) of the product, `box` of them
@@ -73,8 +77,7 @@ struct Arena {
   SplitCopy copy(int rows, int k) { return split_copy_at(take(split_copy_bytes(rows, k)), rows, k); }
 };
 
-// What a split reads: a matrix; the epilogue's backward (dz of act_backward); or
-// the loss's gradient G from its logits.
+// What a split reads: a matrix, or the epilogue's backward (dz of act_backward).
 struct SplitMatrix {
   const float* x;
   long long ld;
@@ -89,22 +92,18 @@ struct SplitBackward {
   int act;
   DropoutArgs drop;
 };
-struct SplitLoss {
-  const float* z;
-  long long ldz;
-  const float2* stat;  // per row: maximum, grad_scale / sum
-  const int32_t* targets;
-  int vocab;
-  float grad_scale;
-};
 // [rows, cols] -> its copy by rows (K = cols), its transpose's copy (K = rows), and
 // the column sums' partials [split_parts(rows), cols]; each may be absent.
 void split(const SplitMatrix& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
            cudaStream_t s);
 void split(const SplitBackward& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
            float* part, cudaStream_t s);
-void split(const SplitLoss& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
-           cudaStream_t s);
+// src [rows, k] -> its transpose's copy [k, rows].
+void split_transposed(const SplitCopy& src, const SplitCopy& by_cols, cudaStream_t s);
+// The copy that LossEpilogue wrote -> the loss's gradient: part as the epilogue left it,
+// stat per row its maximum and grad_scale / its sum.
+void loss_scales(const SplitCopy& g, const float2* part, const float2* stat, const int32_t* targets, int vocab,
+                 float grad_scale, cudaStream_t s);
 // Two matrices in one launch.
 void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_by_rows, const SplitCopy* x_by_cols,
                const SplitMatrix& y, int y_rows, int y_cols, const SplitCopy* y_by_rows, const SplitCopy* y_by_cols,

@@ -8,7 +8,12 @@
 // row joins the vocab / 128 pairs. With gradients the rows go in blocks whose
 // logits fit a fixed part of the workspace: the product (6 N V D operations in
 // all, as with the logits kept; pieces of the vocabulary would have to form each
-// logit twice, 8 N V D), then z -> G in place, dx = G w, dw += G^T x.
+// logit twice, 8 N V D), then z -> G in place, dx = G w, dw += G^T x. Large exact blocks
+// never hold z: the epilogue writes exp(z - its chunk's maximum) as the split copy that
+// dx's product reads, and what softmax still lacks, exp(that maximum - the row's)
+// grad_scale / the row's sum, is one number per row and chunk, which that product
+// multiplies by anyhow as the chunk's scale. So only dw needs a pass over the block, to
+// transpose (8 bytes a logit; forming both copies from z took 12).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -57,14 +62,11 @@ Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* w
   p.part = static_cast<float2*>(at.take(static_cast<long long>(p.rows) * p.tiles * 8));
   p.zt = static_cast<float*>(at.take(p.rows * 4ll));
   p.stat = static_cast<float2*>(at.take(p.rows * 8ll));
-  if (grad) p.z = static_cast<float*>(at.take(p.rows * p.ldz * 4));
   if (p.pair) {
     p.w = at.copy(vocab, dim);
     p.xr_at = at.take(split_copy_bytes(p.rows, dim));
-    if (dx) {
-      p.wt = at.copy(dim, vocab);
-      p.g_at = at.take(split_copy_bytes(p.rows, vocab));
-    }
+    if (grad) p.g_at = at.take(split_copy_bytes(p.rows, vocab));
+    if (dx) p.wt = at.copy(dim, vocab);
     if (dw) {
       p.xt_at = at.take(split_copy_bytes(dim, p.rows));
       p.gt_at = at.take(split_copy_bytes(vocab, p.rows));
@@ -78,6 +80,7 @@ Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* w
     }
     p.parts = at.take(parts);
   } else {
+    if (grad) p.z = static_cast<float*>(at.take(p.rows * p.ldz * 4));
     if (dw) p.x = static_cast<float*>(at.take(p.rows * p.ldx * 4));
     const int last = static_cast<int>(n - (blocks - 1) * p.rows);
     long long parts = 0;
@@ -243,17 +246,28 @@ int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStre
   } else {
     split(xm, n, a.dim, &p.xr, xt, s);
   }
-  const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt};
+  const bool grad = a.dx || a.dw;
+  LossEpilogue e;
+  e.part = p.part;
+  e.tiles = p.tiles;
+  e.targets = t;
+  e.zt = p.zt;
+  if (grad) {
+    p.g = split_copy_at(p.g_at, n, a.vocab);
+    e.copy = p.g.data;
+    e.copy_ld = p.g.row_halves();
+  }
   int rc = pair_loss_product(p.xr, p.w, e, d_err, s);
   if (rc) return rc;
   row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(p.part, p.tiles, p.zt, t, n, a.vocab, a.grad_scale, a.row_loss + r0,
                                               p.stat, d_err);
   check_cuda(cudaGetLastError(), "row loss");
-  if (!a.dx && !a.dw) return 0;
-  if (a.dx) p.g = split_copy_at(p.g_at, n, a.vocab);
-  if (a.dw) p.gt = split_copy_at(p.gt_at, a.vocab, n);
-  split(SplitLoss{p.z, p.ldz, p.stat, t, a.vocab, a.grad_scale}, n, a.vocab, a.dx ? &p.g : nullptr,
-        a.dw ? &p.gt : nullptr, s);
+  if (!grad) return 0;
+  loss_scales(p.g, p.part, p.stat, t, a.vocab, a.grad_scale, s);
+  if (a.dw) {
+    p.gt = split_copy_at(p.gt_at, a.vocab, n);
+    split_transposed(p.g, p.gt, s);
+  }
   if (a.dx) {
     LinearEpilogue o;
     o.C = a.dx + r0 * a.lddx;
@@ -276,7 +290,7 @@ int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStre
 int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, cudaStream_t s) {
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
-  const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt};
+  const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt, nullptr, 0};
   int rc = plain_loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
   if (rc) return rc;
   if (!a.dx && !a.dw) {

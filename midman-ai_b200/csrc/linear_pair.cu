@@ -67,6 +67,7 @@ __device__ __forceinline__ void halves(float x, float y, uint32_t& hi, uint32_t&
 
 // Sources: begin once, then load of a row's four columns.
 struct MatrixSource {
+  static constexpr int ROWS = 8;
   SplitMatrix a;
   __device__ __forceinline__ void begin() {}
   __device__ __forceinline__ float4 load(long long row, int col, int cols) const {
@@ -79,6 +80,7 @@ struct MatrixSource {
   }
 };
 struct BackwardSource {
+  static constexpr int ROWS = 4;
   SplitBackward a;
   uint64_t seed, offset;
   __device__ __forceinline__ void begin() {
@@ -96,28 +98,21 @@ struct BackwardSource {
     return g;
   }
 };
-struct LossSource {
-  SplitLoss a;
+struct CopySource {  // a copy's values again, scale and all
+  static constexpr int ROWS = 8;
+  SplitCopy a;
   __device__ __forceinline__ void begin() {}
-  __device__ __forceinline__ float4 load(long long row, int col, int cols) const {
-    // the three loads side by side, whatever the target says
-    const int t = a.targets[row];
-    const float2 st = a.stat[row];
-    const float4 v = load_quad(a.z + row * a.ldz, col, cols);
-    const bool live = t >= 0 && t < a.vocab;
-    float4 g;
-    g.x = live ? loss_exp(v.x - st.x) * st.y : 0.0f;
-    g.y = live && col + 1 < cols ? loss_exp(v.y - st.x) * st.y : 0.0f;
-    g.z = live && col + 2 < cols ? loss_exp(v.z - st.x) * st.y : 0.0f;
-    g.w = live && col + 3 < cols ? loss_exp(v.w - st.x) * st.y : 0.0f;
-    const int d = t - col;
-    if (live && d >= 0 && d < 4) {
-      if (d == 0) g.x -= a.grad_scale;
-      if (d == 1) g.y -= a.grad_scale;
-      if (d == 2) g.z -= a.grad_scale;
-      if (d == 3) g.w -= a.grad_scale;
-    }
-    return g;
+  __device__ __forceinline__ float4 load(long long row, int col, int) const {  // zeros past k, as the copy has
+    const uint16_t* p = a.data + row * a.row_halves() + (col >> 7) * 256 + ((col >> 6) & 1) * 128 + (col & 63);
+    const uint2 hi = *reinterpret_cast<const uint2*>(p), lo = *reinterpret_cast<const uint2*>(p + 64);
+    const float inv = a.inv[(col >> 7) * a.inv_ld() + row];
+    auto sum = [&](uint32_t h, uint32_t l) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&l));
+      return make_float2((x.x + y.x) * inv, (x.y + y.y) * inv);
+    };
+    const float2 v = sum(hi.x, lo.x), w = sum(hi.y, lo.y);
+    return make_float4(v.x, v.y, w.x, w.y);
   }
 };
 
@@ -137,7 +132,7 @@ __device__ __forceinline__ void split_tile(Source& src, int rows, int cols, cons
   const int col = c0 + 4 * lane;
   src.begin();
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  constexpr int U = 4;
+  constexpr int U = Source::ROWS;  // rows of a warp in flight
 #pragma unroll 1
   for (int i0 = 0; i0 < kTile / 8; i0 += U) {
     float4 v[U];
@@ -216,7 +211,8 @@ __device__ __forceinline__ void split_tile(Source& src, int rows, int cols, cons
 template <class Source>
 __global__ void __launch_bounds__(256, 3) split_kernel(Source src, int rows, int cols, SplitCopy by_rows,
                                                        SplitCopy by_cols, float* part) {
-  split_tile(src, rows, cols, by_rows, by_cols, part, blockIdx.y, blockIdx.x);
+  const int tc = (cols + kTile - 1) / kTile, t = static_cast<int>(blockIdx.x);
+  split_tile(src, rows, cols, by_rows, by_cols, part, t / tc, t % tc);
 }
 
 // Two matrices in one launch (a product's operands): the first's tiles, then the second's.
@@ -246,8 +242,9 @@ void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_row
     check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSplitSmem), "shared memory");
     configured_device = dev;
   }
-  const dim3 grid((cols + kTile - 1) / kTile, (rows + kTile - 1) / kTile);
-  kern<<<grid, 256, by_cols ? kSplitSmem : kSplitSums, s>>>(src, rows, cols, by_rows ? *by_rows : SplitCopy{},
+  const long long tiles = ((rows + kTile - 1ll) / kTile) * ((cols + kTile - 1ll) / kTile);
+  if (tiles > INT32_MAX) throw std::invalid_argument("a matrix is too large");
+  kern<<<static_cast<unsigned>(tiles), 256, by_cols ? kSplitSmem : kSplitSums, s>>>(src, rows, cols, by_rows ? *by_rows : SplitCopy{},
                                      by_cols ? *by_cols : SplitCopy{}, part);
   check_cuda(cudaGetLastError(), "split");
 }
@@ -690,33 +687,66 @@ struct LossPair {
     if (n0 >= N) return;  // uniform over the warp
     const long long my_row = wrow0 + lane;
     const int live = min(128, N - n0);
-    float m = -INFINITY, s = 0.0f;
-    if (live == 128) {
+    const int t = my_row < M ? e.targets[my_row] - n0 : -1;
+    if (t >= 0 && t < live) {
+      float zt = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 128; ++i) m = fmaxf(m, sum[i]);
+      for (int i = 0; i < 128; ++i) zt = i == t ? sum[i] : zt;
+      e.zt[my_row] = zt;
+    }
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, all[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 128; ++i) s += loss_exp(sum[i] - m);
+    for (int i = 0; i < 128; ++i) top[i % 4] = live == 128 || i < live ? fmaxf(top[i % 4], sum[i]) : top[i % 4];
+    const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    if (e.copy) {  // the exponentials take the logits' place
+#pragma unroll
+      for (int i = 0; i < 128; ++i) {
+        sum[i] = live == 128 || i < live ? loss_exp(sum[i] - m) : 0.0f;
+        all[i % 4] += sum[i];
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 128; ++i) m = i < live ? fmaxf(m, sum[i]) : m;
-#pragma unroll
-      for (int i = 0; i < 128; ++i) s += i < live ? loss_exp(sum[i] - m) : 0.0f;
+      for (int i = 0; i < 128; ++i) all[i % 4] += live == 128 || i < live ? loss_exp(sum[i] - m) : 0.0f;
     }
-    if (my_row < M) {
-      e.part[my_row * e.tiles + n0 / 128] = make_float2(m, s);
-      const int t = e.targets[my_row] - n0;
-      if (t >= 0 && t < live) {
-        float zt = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) zt = i == t ? sum[i] : zt;
-        e.zt[my_row] = zt;
-      }
+    if (my_row < M) e.part[my_row * e.tiles + n0 / 128] = make_float2(m, (all[0] + all[1]) + (all[2] + all[3]));
+    if (e.copy) {
+      if (wrow0 + 32 <= M)
+        store_copy<true>(sum, stage_tile, wrow0, n0, M, lane);
+      else
+        store_copy<false>(sum, stage_tile, wrow0, n0, M, lane);
+      return;
     }
     if (!e.Z) return;
     if (wrow0 + 32 <= M && n0 + 128 <= N)
       store<true>(sum, stage_tile, wrow0, n0, M, N, lane);
     else
       store<false>(sum, stage_tile, wrow0, n0, M, N, lane);
+  }
+  // The chunk's exponentials, in (0, 1], times 2^14 as hi and lo: the copy that dx's product
+  // reads once its scales (2^-14 exp(m - row maximum) grad_scale / row sum) are known.
+  template <bool FULL>
+  __device__ __forceinline__ void store_copy(const float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M,
+                                             int lane) const {
+    const int sub = lane & 7, rsub = lane >> 3;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      stage_rows(sum + 32 * c, stage_tile, lane);
+      __syncwarp();
+      uint16_t* out = e.copy + (wrow0 + rsub) * e.copy_ld + (n0 / 128) * 256ll + (c / 2) * 128 + (c % 2) * 32 + 4 * sub;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int rr = 4 * i + rsub;
+        const float4 v = stage_tile[rr * 8 + (sub ^ (rr & 7))];
+        uint2 hi, lo;
+        halves(v.x * 16384.0f, v.y * 16384.0f, hi.x, lo.x);
+        halves(v.z * 16384.0f, v.w * 16384.0f, hi.y, lo.y);
+        if (FULL || wrow0 + rr < M) {
+          *reinterpret_cast<uint2*>(out + 4 * i * e.copy_ld) = hi;
+          *reinterpret_cast<uint2*>(out + 4 * i * e.copy_ld + 64) = lo;
+        }
+      }
+      __syncwarp();  // before the next slice overwrites the staging tile
+    }
   }
   template <bool FULL>
   __device__ __forceinline__ void store(const float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
@@ -738,6 +768,53 @@ struct LossPair {
     }
   }
 };
+
+// G from the exponentials' copy: every chunk's scale becomes 2^-14 exp(its maximum - the
+// row's) grad_scale / the row's sum (0 for a row without a target), which the products
+// apply as they apply any scale, and the target's chunk is written anew with grad_scale
+// taken off. A warp per row.
+__global__ void __launch_bounds__(256) loss_scales_kernel(SplitCopy g, const float2* part, const float2* stat,
+                                                          const int32_t* targets, int vocab, float grad_scale) {
+  const int row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (row >= g.rows) return;
+  const int chunks = static_cast<int>(g.chunks());
+  const int t = targets[row];
+  const bool live = t >= 0 && t < vocab;
+  const float2 st = stat[row];
+  const float2* mine = part + static_cast<long long>(row) * chunks;
+  float* inv = g.inv + row;
+  const float unit = st.y * 6.103515625e-05f;  // 2^-14 grad_scale / sum
+#pragma unroll 8
+  for (int c = lane; c < chunks; c += 32) inv[c * g.inv_ld()] = live ? loss_exp(mine[c].x - st.x) * unit : 0.0f;
+  if (!live) return;
+  const int c = t >> 7;
+  const float f = loss_exp(mine[c].x - st.x) * unit;
+  uint16_t* p = g.data + row * g.row_halves() + c * 256ll + (lane / 16) * 128 + (lane % 16) * 4;  // columns 4 lane..
+  uint2 hi = *reinterpret_cast<const uint2*>(p), lo = *reinterpret_cast<const uint2*>(p + 64);
+  const uint32_t h[2] = {hi.x, hi.y}, l[2] = {lo.x, lo.y};
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&l[i]));
+    v[2 * i] = (a.x + b.x) * f;
+    v[2 * i + 1] = (a.y + b.y) * f;
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((t & 127) == 4 * lane + i) v[i] -= grad_scale;
+    m = max(m, magnitude(v[i]));
+  }
+  float back;
+  const float scale = chunk_scale(__reduce_max_sync(0xffffffffu, m), &back);
+  halves(v[0] * scale, v[1] * scale, hi.x, lo.x);
+  halves(v[2] * scale, v[3] * scale, hi.y, lo.y);
+  *reinterpret_cast<uint2*>(p) = hi;
+  *reinterpret_cast<uint2*>(p + 64) = lo;
+  __syncwarp();  // the loop above wrote this chunk's scale too
+  if (lane == 0) inv[c * g.inv_ld()] = back;
+}
 
 // (64 halves, rows, segments): one box of {64, 128, 2} is a stage's hi and lo tile.
 int copy_map(CUtensorMap* map, const SplitCopy& c) {
@@ -890,9 +967,15 @@ void split(const SplitBackward& src, int rows, int cols, const SplitCopy* by_row
            float* part, cudaStream_t s) {
   launch_split(BackwardSource{src, 0, 0}, rows, cols, by_rows, by_cols, part, s);
 }
-void split(const SplitLoss& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
-           cudaStream_t s) {
-  launch_split(LossSource{src}, rows, cols, by_rows, by_cols, nullptr, s);
+void loss_scales(const SplitCopy& g, const float2* part, const float2* stat, const int32_t* targets, int vocab,
+                 float grad_scale, cudaStream_t s) {
+  if (g.rows <= 0) return;
+  loss_scales_kernel<<<(g.rows + 7) / 8, 256, 0, s>>>(g, part, stat, targets, vocab, grad_scale);
+  check_cuda(cudaGetLastError(), "loss gradient");
+}
+
+void split_transposed(const SplitCopy& src, const SplitCopy& by_cols, cudaStream_t s) {
+  launch_split(CopySource{src}, src.rows, src.k, nullptr, &by_cols, nullptr, s);
 }
 
 void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_by_rows, const SplitCopy* x_by_cols,
