@@ -175,12 +175,19 @@ MM_GPU_EXPORT int32_t mm_gpu_cross_entropy(int32_t rows, int32_t vocab, float *l
  * between calls: temporaries live in `workspace` (device memory, 256-byte aligned,
  * at least what the call's _workspace function returns for the same sizes; it may
  * be reused as soon as the call's work on `stream` is done, and two calls that
- * may run at the same time need two). After one earlier call of any entry point on
- * the device they may be captured into a graph. Matrices have a row stride that is
- * a multiple of 4 and start on 16-byte boundaries; widths are arbitrary, and
- * columns past the width are neither read nor written. Outputs must not overlap
- * inputs except where said. An infinite or NaN operand entry makes the outputs that
- * depend on it NaN or infinite, no others.
+ * may run at the same time need two). They may be captured into a graph, once
+ * mm_gpu_device_status has been called on the device (the first use of its error flag
+ * allocates it). Matrices have a row stride that is a multiple of 4 and start on
+ * 16-byte boundaries; widths are arbitrary, and columns past the width are neither
+ * read nor written. Outputs must not overlap inputs, the workspace or one another
+ * except where said. An infinite or NaN operand entry makes the outputs that depend on
+ * it NaN or infinite, no others.
+ *
+ * Precision: MM_GPU_TF32 is one TF32 pass (up to eight rows: f32 multiply-adds).
+ * MM_GPU_3XTF32 is the exact mode, f32 accuracy: three products of 11-bit halves,
+ * TF32 ones, or for large products f16 ones of operands scaled by a power of two for
+ * every 128 entries along the sum (an entry more than 2^-17 below the largest of its
+ * 128 begins to lose bits, one 2^-39 below it is lost).
  *
  * Dropout: element (i, j) of a [rows, cols] tensor is dropped where word j % 4 of
  * the Philox4x32-10 block with counter (i * ceil(cols / 4) + j / 4, offset) and key
@@ -227,7 +234,10 @@ MM_GPU_EXPORT int32_t mm_gpu_linear_backward(int32_t m, int32_t n, int32_t k, co
  * none), summed in f64. dx [rows, dim] and dw (W's layout) receive, where not NULL,
  * the gradients of grad_scale * (sum of the row losses), added to what they hold
  * when accumulate != 0. The workspace does not grow with rows * vocab: with
- * gradients it holds the logits of as many rows as fit 256 MiB (256 rows at least). */
+ * gradients the rows go in blocks whose logits take at most 384 MiB, or half as much
+ * as W if that is more (256 rows at least); large calls in the exact mode hold a
+ * block's gradient twice (by rows and transposed) and copies of W, as large as W for
+ * the logits and once more for dx. */
 MM_GPU_EXPORT int64_t mm_gpu_linear_cross_entropy_workspace(int32_t rows, int32_t vocab, int32_t dim,
                                                             int32_t gradients, int32_t precision);
 MM_GPU_EXPORT int32_t mm_gpu_linear_cross_entropy(int32_t rows, int32_t vocab, int32_t dim, const float *x,

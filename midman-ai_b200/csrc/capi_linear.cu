@@ -94,6 +94,8 @@ int32_t mm_gpu_dropout(int64_t rows, int32_t cols, const float* x, int64_t ldx, 
     if (rows > 0 && (!x || !y)) return fail(MM_GPU_ERR_ARGUMENT, "dropout: null pointer");
     if (ldx < cols || ldy < cols || (r && ldr < cols))
       return fail(MM_GPU_ERR_SHAPE, "dropout: a row stride is smaller than the row");
+    if (rows > 0 && ((y == x && ldy != ldx) || (y == r && ldy != ldr)))
+      return fail(MM_GPU_ERR_SHAPE, "dropout: y may be x or r only with its row stride");
     MM_TRY(check_dropout(p, rng));
     mm::dropout(x, ldx, r, ldr, y, ldy, rows, cols, mm::dropout_args(p, rng, cols), as_stream(stream));
     return MM_GPU_OK;
@@ -124,6 +126,8 @@ int32_t mm_gpu_linear_forward(int32_t m, int32_t n, int32_t k, const float* a, i
     MM_TRY(check_matrix("linear: c", c, ldc, n));
     if (r) MM_TRY(check_matrix("linear: r", r, ldr, n));
     if (z) MM_TRY(check_matrix("linear: z", z, ldz, n));
+    if (r == c && ldr != ldc) return fail(MM_GPU_ERR_SHAPE, "linear: r may be c only with c's row stride");
+    if (z == c || (z && z == r)) return fail(MM_GPU_ERR_ARGUMENT, "linear: z must have a buffer of its own");
     const bool exact = precision == MM_GPU_3XTF32;
     MM_TRY(check_workspace(workspace, workspace_bytes, mm::linear_forward_ws_bytes(m, n, k, exact)));
     mm::LinearForward f{m, n, k, a, lda, b, ldb, b_mn_major != 0, {}, exact};

@@ -117,6 +117,8 @@ int pair_product(const SplitCopy& A, const SplitCopy& B, const LinearEpilogue& e
 int pair_loss_product(const SplitCopy& A, const SplitCopy& B, const LossEpilogue& e, int* d_err, cudaStream_t s);
 // Whether an exact product of this size is worth the copies.
 bool pair_product_suits(int M, int N, int K);
+// About how long it takes, copies aside; parts: whether its last wave may be cut.
+double pair_us(int M, int N, int K, bool parts);
 
 // Large TF32 products on the operands themselves (linear_pair.cu). An MN-major A
 // only with an MN-major B and no activation or dropout. ws: tf32_pair_ws_bytes bytes.

@@ -27,7 +27,7 @@
 namespace mm {
 namespace {
 
-constexpr long long kLogitBytes = 256ll << 20;  // a block's logits, or half as much as w if that is more
+constexpr long long kLogitBytes = 384ll << 20;  // a block's logits, or half as much as w if that is more
 constexpr long long kPartBytes = 64ll << 20;    // a block's (max, sum) pairs, the loss alone
 
 long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
@@ -46,6 +46,28 @@ struct Plan {
   long long bytes;
 };
 
+// Of `least` blocks and a few more, the count whose products take the shortest time: dx
+// has few tiles (2048 rows of the large preset's 64, for 74 pairs; 2816 have 88, the 14
+// past a wave cut into parts).
+long long best_blocks(long long n, long long least, int vocab, int dim) {
+  long long best = least;
+  double best_us = 1e30;
+  for (long long b = least; b <= 2 * least + 1; ++b) {
+    const long long rows = round_up((n + b - 1) / b, 256), last = n - rows * (b - 1);
+    if (last <= 0) break;
+    auto block_us = [&](long long r) {
+      const int m = static_cast<int>(r);
+      return pair_us(m, vocab, dim, false) + pair_us(m, dim, vocab, true) + pair_us(vocab, dim, m, true);
+    };
+    const double us = (b - 1) * block_us(rows) + block_us(last);
+    if (us < best_us) {
+      best_us = us;
+      best = b;
+    }
+  }
+  return best;
+}
+
 Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* ws) {
   Plan p{};
   const bool grad = dx || dw;
@@ -55,7 +77,9 @@ Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* w
   p.ldx = round_up(dim, 4);
   const long long logits = std::max(kLogitBytes, 2ll * vocab * dim);
   const long long most = std::max(256ll, (grad ? logits / (p.ldz * 4) : kPartBytes / (p.tiles * 8ll)) / 256 * 256);
-  const long long n = std::max(rows, 1), blocks = (n + most - 1) / most;
+  const long long n = std::max(rows, 1);
+  long long blocks = (n + most - 1) / most;
+  if (grad && exact && blocks > 1) blocks = best_blocks(n, blocks, vocab, dim);
   p.rows = static_cast<int>(std::min(n, round_up((n + blocks - 1) / blocks, 256)));  // even blocks of whole tiles
   p.pair = exact && pair_product_suits(p.rows, vocab, dim) &&
            (!grad || (pair_product_suits(p.rows, dim, vocab) && pair_product_suits(vocab, dim, p.rows)));
@@ -227,7 +251,7 @@ long long linear_loss_ws_bytes(int rows, int vocab, int dim, bool grad, bool exa
 namespace {
 
 // One block of rows on copies; the first makes those of w too.
-int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStream_t s) {
+int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cudaStream_t s) {
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
   // x's rows without a target count as zeros: their logits are not used, and dw sums over
@@ -287,7 +311,7 @@ int pair_block(const LinearLoss& a, Plan& p, int r0, int n, int* d_err, cudaStre
 }
 
 // One block of rows on direct products: G takes the logits' place.
-int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, cudaStream_t s) {
+int direct_block(const LinearLoss& a, const Plan& p, long long r0, int n, int* d_err, cudaStream_t s) {
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
   const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt, nullptr, 0};
@@ -329,8 +353,8 @@ int direct_block(const LinearLoss& a, const Plan& p, int r0, int n, int* d_err, 
 int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
   const bool grad = a.dx || a.dw;
   Plan p = plan_of(a.rows, a.vocab, a.dim, grad, grad, a.exact, ws);
-  for (int r0 = 0; r0 < a.rows; r0 += p.rows) {
-    const int n = std::min(p.rows, a.rows - r0);
+  for (long long r0 = 0; r0 < a.rows; r0 += p.rows) {
+    const int n = static_cast<int>(std::min<long long>(p.rows, a.rows - r0));
     const int rc = p.pair ? pair_block(a, p, r0, n, d_err, s) : direct_block(a, p, r0, n, d_err, s);
     if (rc) return rc;
   }

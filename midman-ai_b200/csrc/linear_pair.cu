@@ -1028,6 +1028,19 @@ int pair_loss_product(const SplitCopy& A, const SplitCopy& B, const LossEpilogue
 
 bool pair_product_suits(int M, int N, int K) { return K >= 128 && suits(M, N, K, (K + 127) / 128, kWorthExact, 6.0); }
 
+double pair_us(int M, int N, int K, bool parts) {
+  const int chunks = (K + 127) / 128;
+  const long long tiles = tiles_of(M, N);
+  PairWork w = work_of(tiles, chunks, kWorthExact);
+  if (!parts) {
+    w.full = static_cast<int>(tiles);
+    w.splits = 1;
+  }
+  const double whole = 2.05 * chunks + 2.5;
+  const long long waves = (w.full + kPairs - 1) / kPairs;
+  return waves * whole + (w.full < tiles ? 2.05 * ((chunks + w.splits - 1) / w.splits) + 10.0 : 0.0);
+}
+
 long long tf32_pair_ws_bytes(int M, int N, int K) { return parts_bytes(M, N, (K + 31) / 32, kWorthTf32); }
 
 int tf32_pair_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LinearEpilogue& e,

@@ -30,9 +30,10 @@ def test_the_mask_keeps_the_share_it_says():
 def test_workspaces(mm):
     assert mm.linear_workspace(0, 1, 1) >= 0
     assert mm.linear_workspace(100, 30, 8, backward=True) >= 100 * 32 * 4
-    small, large = (mm.linear_cross_entropy_workspace(rows, 32000, 256) for rows in (8192, 65536))
-    assert large < 8192 * 32000 * 4  # below one batch's logits,
-    assert large - small <= 1 << 20  # and no more for more rows
+    # A block's logits take 384 MiB at most: 3146 rows of 32000. A row needs besides 250 (maximum, sum) pairs, three
+    # numbers and its 256 inputs: 3036 bytes, under 10 MB in all. A last wave's parts: at most 74 tiles of 256 KiB.
+    for rows in (8192, 65536, 1 << 20):
+        assert mm.linear_cross_entropy_workspace(rows, 32000, 256) < (384 << 20) + 10_000_000 + 74 * (256 << 10)
     assert mm.linear_cross_entropy_workspace(8192, 32000, 256, gradients=False) < 128 << 20
     for bad in ((-1, 4, 4), (1, 0, 4), (1, 4, 0)):
         with pytest.raises(mm.MidmanGpuError):
@@ -84,7 +85,8 @@ SHAPE, ARGUMENT = -3, -1
     (forward, dict(act=4), ARGUMENT), (forward, dict(act=-1), ARGUMENT), (forward, dict(precision=2), ARGUMENT),
     (forward, dict(p=1.0), ARGUMENT), (forward, dict(p=-0.1), ARGUMENT), (forward, dict(p=NAN), ARGUMENT),
     (forward, dict(p=0.1), ARGUMENT), (forward, dict(p=0.1, rng=P + 4), ARGUMENT),
-    (forward, dict(n=16, mn=0, ldb=8, ldc=8), SHAPE),
+    (forward, dict(n=16, mn=0, ldb=8, ldc=8), SHAPE), (forward, dict(r=P, ldr=12), SHAPE),
+    (forward, dict(z=P, ldz=8), ARGUMENT), (forward, dict(z=2 * P, ldz=8, r=2 * P, ldr=8), ARGUMENT),
     (backward, dict(m=-1), SHAPE), (backward, dict(dc=None), ARGUMENT), (backward, dict(act=2), ARGUMENT),
     (backward, dict(act=2, z=P, ldz=4), SHAPE), (backward, dict(b=None), ARGUMENT), (backward, dict(a=None), ARGUMENT),
     (backward, dict(ldda=4), SHAPE), (backward, dict(db=P + 4), ARGUMENT), (backward, dict(ws=None), ARGUMENT),
@@ -96,7 +98,7 @@ SHAPE, ARGUMENT = -3, -1
     (loss, dict(precision=7), ARGUMENT),
     (dropout, dict(rows=-1), SHAPE), (dropout, dict(cols=0), SHAPE), (dropout, dict(x=None), ARGUMENT),
     (dropout, dict(ldx=7), SHAPE), (dropout, dict(r=P, ldr=7), SHAPE), (dropout, dict(p=1.0), ARGUMENT),
-    (dropout, dict(rng=None), ARGUMENT),
+    (dropout, dict(rng=None), ARGUMENT), (dropout, dict(ldy=9), SHAPE), (dropout, dict(r=2 * P, ldr=9, y=2 * P), SHAPE),
 ])
 def test_refusals(mm, call, change, status):
     rc, message = call(mm, **change)

@@ -336,7 +336,8 @@ def loss_case(g, rows, vocab, dim, tied, extra):
 # rows, vocab, dim, tied, extra, rows left out
 LOSS = [(1, 1, 4, True, 0, 0), (1, 5, 8, True, 0, 0), (3, 130, 33, False, 4, 1), (64, 1000, 64, True, 4, 5), (129, 4099, 96, False, 0, 0),
         (200, 513, 1030, True, 0, 199), (37, 32003, 260, True, 8, 3), (2049, 512, 128, False, 0, 100), (2304, 2305, 512, True, 0, 0),
-        (700, 131072, 40, True, 0, 9), (600, 120001, 36, False, 4, 9), (5, 20001, 40, True, 4, 1), (64, 32000, 64, True, 0, 3), (1100, 131073, 132, True, 4, 9), (777, 65537, 260, False, 0, 9)]
+        (700, 131072, 40, True, 0, 9), (600, 120001, 36, False, 4, 9), (5, 20001, 40, True, 4, 1), (64, 32000, 64, True, 0, 3), (1100, 131073, 132, True, 4, 9), (777, 65537, 260, False, 0, 9),
+        (1100, 131073, 260, True, 4, 9), (900, 131072, 196, False, 0, 0)]
 
 
 @pytest.mark.parametrize("precision", [1, 0])
@@ -452,31 +453,34 @@ def test_no_rows(mm):
 def all_of_them(mm, s, stream=None):
     """The operators one after another on the tensors of `s`; every output."""
     m, k, n, v = s["sizes"]
-    kw = dict(m=m, n=n, k=k, lda=k, ldb=n, activation=2, p=0.1, rng=s["rng"], z=s["z"], ldz=n, precision=1, stream=stream)
+    kw = dict(m=m, n=n, k=k, lda=k, ldb=n, activation=2, p=0.1, rng=s["rng"], z=s["z"], ldz=n, precision=s["precision"], stream=stream)
     mm.linear_forward(s["a"], s["b"], s["c"], ldc=n, bias=s["bias"], r=s["r"], ldr=n, **kw)
     mm.linear_cross_entropy(s["c"], s["w"], s["t"], s["loss"], rows=m, vocab=v, dim=n, ldx=n, ldw=n, grad_scale=1 / m,
-                            mean_loss=s["mean"], dx=s["dc"], lddx=n, dw=s["dw"], lddw=n, precision=1, workspace=s["ws"], stream=stream)
+                            mean_loss=s["mean"], dx=s["dc"], lddx=n, dw=s["dw"], lddw=n, precision=s["precision"], workspace=s["ws"],
+                            stream=stream)
     mm.linear_backward(s["a"], s["b"], s["dc"], lddc=n, da=s["da"], ldda=k, db=s["db"], lddb=n, dbias=s["dbias"],
                        workspace=s["ws"], **kw)
     mm.dropout(s["da"], s["y"], rows=m, cols=k, ldx=k, ldy=k, p=0.1, rng=s["rng"], stream=stream)
     return [s[o] for o in ("c", "z", "loss", "mean", "dc", "dw", "da", "db", "dbias", "y")]
 
 
-def tensors_for(mm, seed, m, k, n, v):
+def tensors_for(mm, seed, m, k, n, v, precision):
     g = torch.Generator(device="cuda").manual_seed(seed)
     new = lambda *shape: torch.randn(*shape, device="cuda", generator=g)  # noqa: E731
-    s = {"sizes": (m, k, n, v), "a": new(m, k), "b": new(k, n) * k ** -0.5, "bias": new(n), "r": new(m, n), "w": new(v, n) * 0.1,
+    s = {"sizes": (m, k, n, v), "precision": precision, "a": new(m, k), "b": new(k, n) * k ** -0.5, "bias": new(n), "r": new(m, n), "w": new(v, n) * 0.1,
          "t": torch.randint(0, v, (m,), device="cuda", generator=g, dtype=torch.int32), "rng": rng_words(seed, 7)}
     for name, shape in dict(c=(m, n), z=(m, n), loss=(m,), mean=(1,), dc=(m, n), dw=(v, n), da=(m, k), db=(k, n), dbias=(n,),
                             y=(m, k)).items():
         s[name] = torch.empty(*shape, device="cuda")
-    need = max(mm.linear_workspace(m, n, k, backward=True, precision=1), mm.linear_workspace(m, n, k, precision=1),
-               mm.linear_cross_entropy_workspace(m, v, n, precision=1))
+    need = max(mm.linear_workspace(m, n, k, backward=True, precision=precision), mm.linear_workspace(m, n, k, precision=precision),
+               mm.linear_cross_entropy_workspace(m, v, n, precision=precision))
     s["ws"] = torch.empty(need, dtype=torch.uint8, device="cuda")
     return s
 
 
-SIZES = [(300, 96, 200, 1000), (2304, 256, 2304, 2305)]
+# few rows, direct products, slices of a long sum, pairs; both precisions
+SIZES = [(5, 96, 200, 1000, 1), (300, 96, 200, 1000, 1), (300, 96, 200, 1000, 0), (40, 36, 68, 20001, 1), (2304, 256, 2304, 2305, 1),
+         (2304, 256, 2304, 2305, 0)]
 
 
 @pytest.mark.parametrize("sizes", SIZES)
