@@ -254,11 +254,13 @@ namespace {
 int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cudaStream_t s) {
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
-  // x's rows without a target count as zeros: their logits are not used, and dw sums over
-  // all rows, where 0 times what such a row holds may be NaN
+  // For gradients x's rows without a target count as zeros: their logits are not used, but
+  // their exponentials are multiplied by 0 for dx, and dw sums over all rows, and 0 times
+  // what such a row holds may be NaN
   p.xr = split_copy_at(p.xr_at, n, a.dim);
   if (a.dw) p.xt = split_copy_at(p.xt_at, a.dim, n);
-  const SplitMatrix xm{x, a.ldx, t, a.vocab};
+  const bool grad = a.dx || a.dw;
+  const SplitMatrix xm{x, a.ldx, grad ? t : nullptr, a.vocab};
   const SplitCopy* xt = a.dw ? &p.xt : nullptr;
   if (r0 == 0) {  // with w, [vocab, dim] or [dim, vocab]
     const SplitCopy* wt = a.dx ? &p.wt : nullptr;
@@ -270,7 +272,6 @@ int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cu
   } else {
     split(xm, n, a.dim, &p.xr, xt, s);
   }
-  const bool grad = a.dx || a.dw;
   LossEpilogue e;
   e.part = p.part;
   e.tiles = p.tiles;

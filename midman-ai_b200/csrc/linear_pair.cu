@@ -67,7 +67,7 @@ __device__ __forceinline__ void halves(float x, float y, uint32_t& hi, uint32_t&
 
 // Sources: begin once, then load of a row's four columns.
 struct MatrixSource {
-  static constexpr int ROWS = 8;
+  static constexpr int ROWS = 4;
   SplitMatrix a;
   __device__ __forceinline__ void begin() {}
   __device__ __forceinline__ float4 load(long long row, int col, int cols) const {

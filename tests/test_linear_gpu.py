@@ -383,6 +383,11 @@ def test_linear_cross_entropy(mm, rows, vocab, dim, tied, extra, out, precision)
     mm.linear_cross_entropy(x, w, t, alone, mean_loss=mean, **kw)
     mm.device_status()
     check(alone, loss, torch.where(live, t_exp + 4 * ULP * (lse.abs() + z.abs().max(1).values), 0.0), "the loss alone")
+    # each gradient alone is the same
+    bx, bw = torch.empty_like(dx), torch.empty_like(dw)
+    mm.linear_cross_entropy(x, w, t, alone, dx=bx, lddx=dx.stride(0), **kw)
+    mm.linear_cross_entropy(x, w, t, alone, dw=bw, lddw=dw.stride(0), **kw)
+    assert torch.equal(bx[:, :dim], dx[:, :dim]) and torch.equal(bw[:, :dim if tied else vocab], dw[:, :dim if tied else vocab])
     # added to what the gradients hold
     ax, aw = dx.clone(), dw.clone()
     mm.linear_cross_entropy(x, w, t, row_loss, dx=ax, lddx=dx.stride(0), dw=aw, lddw=dw.stride(0), accumulate=True, **kw)
