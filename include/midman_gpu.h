@@ -47,7 +47,7 @@ extern "C" {
 
 /* Activations of mm_gpu_linear_*. */
 #define MM_GPU_ACT_NONE 0
-#define MM_GPU_ACT_RELU 1 /* max(z, 0), slope 0 at 0 */
+#define MM_GPU_ACT_RELU 1 /* max(z, 0), slope 0 at 0, NaN for NaN */
 #define MM_GPU_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
 #define MM_GPU_ACT_SILU 3 /* z / (1 + exp(-z)) */
 
@@ -180,8 +180,9 @@ MM_GPU_EXPORT int32_t mm_gpu_cross_entropy(int32_t rows, int32_t vocab, float *l
  * allocates it). Matrices have a row stride that is a multiple of 4 and start on
  * 16-byte boundaries; widths are arbitrary, and columns past the width are neither
  * read nor written. Outputs must not overlap inputs, the workspace or one another
- * except where said. An infinite or NaN operand entry makes the outputs that depend on
- * it NaN or infinite, no others.
+ * except where said. An infinite or NaN operand entry makes the products that depend on
+ * it NaN or infinite, no others; activations keep a NaN, dropout drops it as it drops
+ * any element.
  *
  * Precision: MM_GPU_TF32 is one TF32 pass (up to eight rows: f32 multiply-adds).
  * MM_GPU_3XTF32 is the exact mode, f32 accuracy: three products of 11-bit halves,

@@ -32,7 +32,7 @@ __device__ __forceinline__ float logistic(float z) {
 __device__ __forceinline__ float activate(float z, int act) {
   float density;
   switch (act) {
-    case kActRelu: return fmaxf(z, 0.0f);
+    case kActRelu: return z < 0.0f ? 0.0f : z;  // a NaN stays
     case kActGelu: return z * normal_cdf(z, &density);
     case kActSilu: return z * logistic(z);
     default: return z;
@@ -43,7 +43,7 @@ __device__ __forceinline__ float activate(float z, int act) {
 __device__ __forceinline__ float activate_slope(float z, int act) {
   float density;
   switch (act) {
-    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+    case kActRelu: return z <= 0.0f ? 0.0f : 1.0f;
     case kActGelu: {
       const float cdf = normal_cdf(z, &density);
       return fmaf(z, density, cdf);

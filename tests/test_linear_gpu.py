@@ -247,6 +247,20 @@ def test_rows_that_are_not_finite_stay_alone(mm):
         check(d[m - 1], want, product_tol(1, bad[m - 1].to(F).abs() @ b.to(F).abs(), k) + 2 * ULP * want.abs(), "large row")
 
 
+@pytest.mark.parametrize("precision", [1, 0])
+@pytest.mark.parametrize("m,k,n", [(2, 64, 40), (40, 96, 72), (2304, 512, 2304)])
+def test_activations_keep_a_nan(mm, m, k, n, precision):
+    a, b = torch.ones(m, k, device="cuda"), torch.full((k, n), 0.5, device="cuda")
+    a[1, 3] = float("nan")
+    for act in range(4):
+        c, z = (torch.zeros(m, n, device="cuda") for _ in range(2))
+        mm.linear_forward(a, b, c, m=m, n=n, k=k, lda=k, ldb=n, ldc=n, activation=act, z=z, ldz=n, precision=precision)
+        mm.device_status()
+        assert torch.isnan(c[1]).all() and torch.isnan(z[1]).all(), ACTS[act]
+        rest = [i for i in range(m) if i != 1]
+        assert torch.isfinite(c[rest]).all()
+
+
 def test_entries_of_very_different_sizes(mm):
     """Rows of a and columns of b over 2^-40 .. 2^40: every element is held to its own row's and column's sizes."""
     g = torch.Generator(device="cuda").manual_seed(3)
