@@ -178,8 +178,8 @@ MM_GPU_EXPORT int32_t mm_gpu_cross_entropy(int32_t rows, int32_t vocab, float *l
  * may run at the same time need two). They may be captured into a graph, once
  * mm_gpu_device_status has been called on the device (the first use of its error flag
  * allocates it). Matrices have a row stride that is a multiple of 4 and start on
- * 16-byte boundaries; widths are arbitrary, and columns past the width are neither
- * read nor written. Outputs must not overlap inputs, the workspace or one another
+ * 16-byte boundaries; dimensions are arbitrary up to 2^31 - 512, and columns past the
+ * width are neither read nor written. Outputs must not overlap inputs, the workspace or one another
  * except where said. An infinite or NaN operand entry makes the products that depend on
  * it NaN or infinite, no others; activations keep a NaN, dropout drops it as it drops
  * any element.

@@ -48,6 +48,12 @@ int32_t check_matrix(const char* what, const void* p, int64_t ld, int64_t width)
   return MM_GPU_OK;
 }
 
+int32_t check_lengths(const char* what, int64_t a, int64_t b, int64_t c) {
+  if (a > mm::kLongest || b > mm::kLongest || c > mm::kLongest)
+    return fail(MM_GPU_ERR_SHAPE, std::string(what) + ": a dimension is longer than " + std::to_string(mm::kLongest));
+  return MM_GPU_OK;
+}
+
 int32_t check_precision(int32_t precision) {
   if (precision != MM_GPU_TF32 && precision != MM_GPU_3XTF32)
     return fail(MM_GPU_ERR_ARGUMENT, "precision must be MM_GPU_TF32 or MM_GPU_3XTF32");
@@ -91,6 +97,7 @@ int32_t mm_gpu_dropout(int64_t rows, int32_t cols, const float* x, int64_t ldx, 
                        int64_t ldy, double p, const uint64_t* rng, void* stream) {
   return guarded<int32_t>("dropout", [&]() -> int32_t {
     if (rows < 0 || cols <= 0) return fail(MM_GPU_ERR_SHAPE, "dropout: need rows >= 0 and cols > 0");
+    MM_TRY(check_lengths("dropout", 0, cols, 0));
     if (rows > 0 && (!x || !y)) return fail(MM_GPU_ERR_ARGUMENT, "dropout: null pointer");
     if (ldx < cols || ldy < cols || (r && ldr < cols))
       return fail(MM_GPU_ERR_SHAPE, "dropout: a row stride is smaller than the row");
@@ -105,6 +112,7 @@ int32_t mm_gpu_dropout(int64_t rows, int32_t cols, const float* x, int64_t ldx, 
 int64_t mm_gpu_linear_workspace(int32_t m, int32_t n, int32_t k, int32_t backward, int32_t precision) {
   return guarded<int64_t>("linear", [&]() -> int64_t {
     if (m < 0 || n <= 0 || k <= 0) return fail(MM_GPU_ERR_SHAPE, "linear: need m >= 0, n > 0 and k > 0");
+    MM_TRY(check_lengths("linear", m, n, k));
     MM_TRY(check_precision(precision));
     const bool exact = precision == MM_GPU_3XTF32;
     return backward ? mm::linear_backward_ws_bytes(m, n, k, exact) : mm::linear_forward_ws_bytes(m, n, k, exact);
@@ -117,6 +125,7 @@ int32_t mm_gpu_linear_forward(int32_t m, int32_t n, int32_t k, const float* a, i
                               int64_t ldc, int32_t precision, void* workspace, int64_t workspace_bytes, void* stream) {
   return guarded<int32_t>("linear", [&]() -> int32_t {
     if (m < 0 || n <= 0 || k <= 0) return fail(MM_GPU_ERR_SHAPE, "linear: need m >= 0, n > 0 and k > 0");
+    MM_TRY(check_lengths("linear", m, n, k));
     MM_TRY(check_precision(precision));
     MM_TRY(check_activation(activation));
     MM_TRY(check_dropout(p, rng));
@@ -151,6 +160,7 @@ int32_t mm_gpu_linear_backward(int32_t m, int32_t n, int32_t k, const float* a, 
                                void* workspace, int64_t workspace_bytes, void* stream) {
   return guarded<int32_t>("linear backward", [&]() -> int32_t {
     if (m < 0 || n <= 0 || k <= 0) return fail(MM_GPU_ERR_SHAPE, "linear backward: need m >= 0, n > 0 and k > 0");
+    MM_TRY(check_lengths("linear backward", m, n, k));
     MM_TRY(check_precision(precision));
     MM_TRY(check_activation(activation));
     MM_TRY(check_dropout(p, rng));
@@ -186,6 +196,7 @@ int64_t mm_gpu_linear_cross_entropy_workspace(int32_t rows, int32_t vocab, int32
   return guarded<int64_t>("linear_cross_entropy", [&]() -> int64_t {
     if (rows < 0 || vocab <= 0 || dim <= 0)
       return fail(MM_GPU_ERR_SHAPE, "linear_cross_entropy: need rows >= 0, vocab > 0 and dim > 0");
+    MM_TRY(check_lengths("linear_cross_entropy", rows, vocab, dim));
     MM_TRY(check_precision(precision));
     return mm::linear_loss_ws_bytes(rows, vocab, dim, gradients != 0, precision == MM_GPU_3XTF32);
   });
@@ -199,6 +210,7 @@ int32_t mm_gpu_linear_cross_entropy(int32_t rows, int32_t vocab, int32_t dim, co
   return guarded<int32_t>("linear_cross_entropy", [&]() -> int32_t {
     if (rows < 0 || vocab <= 0 || dim <= 0)
       return fail(MM_GPU_ERR_SHAPE, "linear_cross_entropy: need rows >= 0, vocab > 0 and dim > 0");
+    MM_TRY(check_lengths("linear_cross_entropy", rows, vocab, dim));
     MM_TRY(check_precision(precision));
     if (!std::isfinite(grad_scale)) return fail(MM_GPU_ERR_ARGUMENT, "linear_cross_entropy: grad_scale must be finite");
     if (rows > 0) {

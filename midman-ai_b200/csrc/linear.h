@@ -2,16 +2,18 @@
 // the linear cross-entropy (linear_loss.cu). All calls are asynchronous on
 // `stream`; every temporary lives in the caller's workspace.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
-
-#include <cuda.h>
 
 #include "dropout.cuh"
 #include "gemm.h"
 
 namespace mm {
+
+// The longest dimension: indices of the tile that holds the last row stay inside 32 bits.
+constexpr long long kLongest = 0x7fffffffll - 511;
 
 enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActivations = 4 };
 
@@ -142,8 +144,8 @@ long long direct_ws_bytes(int M, int N, int K, bool a_mn_major);
 int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LinearEpilogue& e, bool exact, void* ws,
                    int* d_err, cudaStream_t s);
 // The same product with the loss's epilogue.
-int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
-                 cudaStream_t s);
+int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact,
+                        int* d_err, cudaStream_t s);
 
 // dz = mask / (1 - p) * dc * act'(z) (dz null: only the column sums), and the
 // column sums' partials for dbias where part is not null: part must hold

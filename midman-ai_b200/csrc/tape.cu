@@ -683,7 +683,7 @@ uint64_t mm_op_dropout(uint32_t tape, uint64_t x_h, double p, uint64_t seed, uin
     T x = tp.get(x_h);
     require(p >= 0.0 && p < 1.0, MM_GPU_ERR_ARGUMENT, "dropout: p must lie in [0, 1)");
     const int64_t cols = x->shape.back(), rows = x->numel() / cols;
-    require(cols <= INT32_MAX, MM_GPU_ERR_SHAPE, "dropout: the last dimension is too long");
+    require(cols <= kLongest, MM_GPU_ERR_SHAPE, "dropout: the last dimension is too long");
     Buf y = tp.alloc(static_cast<size_t>(x->numel()));
     Buf words = p > 0.0 ? rng_words(tp, seed, offset) : nullptr;
     const int n = static_cast<int>(cols);
@@ -707,7 +707,7 @@ uint64_t mm_op_linear(uint32_t tape, uint64_t x_h, uint64_t w_h, int32_t w_trans
     const int64_t m = x->shape[0], k = x->shape[1], n = w->shape[wt ? 0 : 1];
     require(w->shape[wt ? 1 : 0] == k, MM_GPU_ERR_SHAPE, "linear: inner dimensions differ");
     require(multiple4(k) && multiple4(n), MM_GPU_ERR_SHAPE, "linear: inner and output widths must be multiples of 4");
-    require(m <= INT32_MAX && k <= INT32_MAX && n <= INT32_MAX, MM_GPU_ERR_SHAPE, "linear: a dimension is too long");
+    require(m <= kLongest && k <= kLongest && n <= kLongest, MM_GPU_ERR_SHAPE, "linear: a dimension is too long");
     require(!bias || bias->shape == std::vector<int64_t>{n}, MM_GPU_ERR_SHAPE, "linear: bias [n]");
     require(!res || res->shape == std::vector<int64_t>({m, n}), MM_GPU_ERR_SHAPE, "linear: residual [m, n]");
     require(activation >= 0 && activation < kActivations, MM_GPU_ERR_ARGUMENT, "linear: unknown activation");
@@ -778,7 +778,7 @@ uint64_t mm_op_linear_cross_entropy(uint32_t tape, uint64_t x_h, uint64_t w_h, i
     require(w->shape[wt ? 1 : 0] == dim, MM_GPU_ERR_SHAPE, "linear_cross_entropy: inner dimensions differ");
     require(multiple4(dim) && multiple4(vocab), MM_GPU_ERR_SHAPE,
             "linear_cross_entropy: the inner width and the classes must be multiples of 4");
-    require(rows <= INT32_MAX && dim <= INT32_MAX && vocab <= INT32_MAX, MM_GPU_ERR_SHAPE,
+    require(rows <= kLongest && dim <= kLongest && vocab <= kLongest, MM_GPU_ERR_SHAPE,
             "linear_cross_entropy: a dimension is too long");
     int64_t live = 0;
     for (int64_t r = 0; r < rows; ++r) {

@@ -105,5 +105,30 @@ def test_refusals(mm, call, change, status):
     assert rc == status and message
 
 
+LONG = 2 ** 31 - 511
+
+
+@pytest.mark.parametrize("call,change", [
+    (forward, dict(m=LONG)), (forward, dict(n=LONG, ldb=2 ** 31, ldc=2 ** 31)), (forward, dict(k=LONG, lda=2 ** 31)),
+    (backward, dict(m=LONG)), (loss, dict(rows=LONG)), (loss, dict(vocab=LONG)), (dropout, dict(cols=LONG, ldx=LONG, ldy=LONG)),
+])
+def test_dimensions_whose_tiles_pass_32_bits_are_refused(mm, call, change):
+    rc, message = call(mm, **change)
+    assert rc == SHAPE and "longer than" in message
+
+
+def test_workspaces_of_the_longest_dimensions(mm):
+    longest = LONG - 1
+    for sizes in ((longest, 4, 4), (4, longest, 4), (4, 4, longest)):
+        for backward_too in (False, True):
+            assert mm.linear_workspace(*sizes, backward=backward_too, precision=1) >= 0
+        assert mm.linear_cross_entropy_workspace(*sizes) > 0
+    for too_long in ((LONG, 4, 4), (4, LONG, 4), (4, 4, LONG)):
+        with pytest.raises(mm.MidmanGpuError):
+            mm.linear_workspace(*too_long)
+        with pytest.raises(mm.MidmanGpuError):
+            mm.linear_cross_entropy_workspace(*too_long)
+
+
 def test_no_rows_is_nothing_to_do(mm):
     assert forward(mm, m=0, a=None, c=None)[0] == 0
