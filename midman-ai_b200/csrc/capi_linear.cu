@@ -2,8 +2,10 @@
 // cross-entropy (include/midman_gpu.h): argument checks, then the launchers.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <exception>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/midman_gpu.h"
@@ -73,6 +75,19 @@ int32_t check_activation(int32_t activation) {
   return MM_GPU_OK;
 }
 
+// An output that is an input, or another output, would be read after it is written.
+// Compared by where they start: rows of two matrices may lie between one another's.
+int32_t check_distinct(const char* what, std::initializer_list<const void*> outputs,
+                       std::initializer_list<const void*> inputs) {
+  for (auto o = outputs.begin(); o != outputs.end(); ++o) {
+    if (!*o) continue;
+    if (std::find(o + 1, outputs.end(), *o) != outputs.end() ||
+        std::find(inputs.begin(), inputs.end(), *o) != inputs.end())
+      return fail(MM_GPU_ERR_ARGUMENT, std::string(what) + ": an output must have a buffer of its own");
+  }
+  return MM_GPU_OK;
+}
+
 int32_t check_workspace(const void* ws, int64_t bytes, int64_t need) {
   if (need > 0 && (!ws || bytes < need || !aligned(ws, 256)))
     return fail(MM_GPU_ERR_ARGUMENT, "workspace: needs " + std::to_string(need) + " bytes, 256-byte aligned");
@@ -136,7 +151,8 @@ int32_t mm_gpu_linear_forward(int32_t m, int32_t n, int32_t k, const float* a, i
     if (r) MM_TRY(check_matrix("linear: r", r, ldr, n));
     if (z) MM_TRY(check_matrix("linear: z", z, ldz, n));
     if (r == c && ldr != ldc) return fail(MM_GPU_ERR_SHAPE, "linear: r may be c only with c's row stride");
-    if (z == c || (z && z == r)) return fail(MM_GPU_ERR_ARGUMENT, "linear: z must have a buffer of its own");
+    MM_TRY(check_distinct("linear", {c, z}, {a, b, bias}));
+    if (z && z == r) return fail(MM_GPU_ERR_ARGUMENT, "linear: z must have a buffer of its own");
     const bool exact = precision == MM_GPU_3XTF32;
     MM_TRY(check_workspace(workspace, workspace_bytes, mm::linear_forward_ws_bytes(m, n, k, exact)));
     mm::LinearForward f{m, n, k, a, lda, b, ldb, b_mn_major != 0, {}, exact};
@@ -183,10 +199,11 @@ int32_t mm_gpu_linear_backward(int32_t m, int32_t n, int32_t k, const float* a, 
       return MM_GPU_OK;
     }
     const bool exact = precision == MM_GPU_3XTF32;
+    MM_TRY(check_distinct("linear backward", {da, db, dbias}, {a, b, z, dc}));
     MM_TRY(check_workspace(workspace, workspace_bytes, mm::linear_backward_ws_bytes(m, n, k, exact)));
-    const mm::LinearBackward f{m,  n,    k,  a,    lda,   b,    ldb, b_mn_major != 0, activation, mm::dropout_args(p, rng, n),
-                               z,  ldz,  dc, lddc, da,    ldda, db,  lddb,            dbias,      accumulate != 0,
-                               exact};
+    const mm::LinearBackward f{m,     n,    k,  a,    lda,        b,   ldb,  b_mn_major != 0,
+                               activation, mm::dropout_args(p, rng, n), z, ldz, dc, lddc,
+                               da,    ldda, db, lddb, dbias,      accumulate != 0, exact};
     return product_status(mm::linear_backward(f, workspace, mm::device_context().d_err, st));
   });
 }
@@ -230,6 +247,7 @@ int32_t mm_gpu_linear_cross_entropy(int32_t rows, int32_t vocab, int32_t dim, co
       return MM_GPU_OK;
     }
     const bool exact = precision == MM_GPU_3XTF32;
+    MM_TRY(check_distinct("linear_cross_entropy", {dx, dw, row_loss, mean_loss}, {x, w, targets}));
     MM_TRY(check_workspace(workspace, workspace_bytes, mm::linear_loss_ws_bytes(rows, vocab, dim, dx || dw, exact)));
     const mm::LinearLoss a{rows, vocab,     dim, x,    ldx, w,    ldw,  w_mn_major != 0,  targets,
                            grad_scale, row_loss, mean_loss, dx, lddx, dw, lddw, accumulate != 0, exact};

@@ -105,6 +105,24 @@ def test_refusals(mm, call, change, status):
     assert rc == status and message
 
 
+Q, R, S, T = (P * i for i in (2, 3, 4, 5))
+
+
+@pytest.mark.parametrize("call,change", [
+    (forward, dict(a=Q, b=R, c=Q)), (forward, dict(a=Q, b=R, c=R)), (forward, dict(a=Q, b=R, c=S, bias=S)),
+    (forward, dict(a=Q, b=R, c=S, z=S, ldz=8)), (forward, dict(a=Q, b=R, c=S, z=R, ldz=8)),
+    (backward, dict(a=Q, b=R, dc=S, da=S, db=T)), (backward, dict(a=Q, b=R, dc=S, da=T, db=T)),
+    (backward, dict(a=Q, b=R, dc=S, da=None, db=Q)), (backward, dict(a=Q, b=R, dc=S, da=R, db=None)),
+    (backward, dict(a=Q, b=R, dc=S, z=T, ldz=8, act=1, da=P, db=T)),
+    (backward, dict(a=Q, b=R, dc=S, da=P, db=T, dbias=T)),
+    (loss, dict(x=Q, w=R, targets=S, dx=Q, dw=T)), (loss, dict(x=Q, w=R, targets=S, dx=None, dw=R)),
+    (loss, dict(x=Q, w=R, targets=S, dx=T, dw=T)), (loss, dict(x=Q, w=R, targets=S, dx=T, dw=6 * P, mean=P)),
+])
+def test_outputs_that_are_inputs_or_one_another_are_refused(mm, call, change):
+    rc, message = call(mm, **change)
+    assert rc == ARGUMENT and "buffer of its own" in message
+
+
 LONG = 2 ** 31 - 511
 
 
