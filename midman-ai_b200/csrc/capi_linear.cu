@@ -199,8 +199,8 @@ int32_t mm_gpu_linear_backward(int32_t m, int32_t n, int32_t k, const float* a, 
       return MM_GPU_OK;
     }
     const bool exact = precision == MM_GPU_3XTF32;
-    MM_TRY(check_distinct("linear backward", {da, db, dbias}, {a, b, z, dc}));
     MM_TRY(check_workspace(workspace, workspace_bytes, mm::linear_backward_ws_bytes(m, n, k, exact)));
+    MM_TRY(check_distinct("linear backward", {da, db, dbias}, {a, b, z, dc}));
     const mm::LinearBackward f{m,     n,    k,  a,    lda,        b,   ldb,  b_mn_major != 0,
                                activation, mm::dropout_args(p, rng, n), z, ldz, dc, lddc,
                                da,    ldda, db, lddb, dbias,      accumulate != 0, exact};
@@ -247,8 +247,8 @@ int32_t mm_gpu_linear_cross_entropy(int32_t rows, int32_t vocab, int32_t dim, co
       return MM_GPU_OK;
     }
     const bool exact = precision == MM_GPU_3XTF32;
-    MM_TRY(check_distinct("linear_cross_entropy", {dx, dw, row_loss, mean_loss}, {x, w, targets}));
     MM_TRY(check_workspace(workspace, workspace_bytes, mm::linear_loss_ws_bytes(rows, vocab, dim, dx || dw, exact)));
+    MM_TRY(check_distinct("linear_cross_entropy", {dx, dw, row_loss, mean_loss}, {x, w, targets}));
     const mm::LinearLoss a{rows, vocab,     dim, x,    ldx, w,    ldw,  w_mn_major != 0,  targets,
                            grad_scale, row_loss, mean_loss, dx, lddx, dw, lddw, accumulate != 0, exact};
     return product_status(mm::linear_loss(a, workspace, mm::device_context().d_err, st));

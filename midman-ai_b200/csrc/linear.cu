@@ -12,17 +12,17 @@
 //
 // direct_kernel: one 128 x 128 tile per cluster of `splits` CTAs, each CTA a part
 // of K (and where few tiles share a long K, clusters for its slices, whose sums go to
-// the workspace and join_kernel). TMA brings the f32 operands. Their lo parts are made on the way, which saves
-// the passes and the workspace of copies made beforehand (short products are bound by
-// latency and one reading of the operands): four warps take A's rows to tensor
-// memory, hi and lo, where the UMMAs read them; two write B's lo part beside it in
-// shared memory (elementwise, so the swizzled layout is kept). What bounds a K step
-// of 32 of a 128 x 128 tile is shared memory: 32 KB in by TMA, 48 KB through the
-// converters, 48 KB read by the UMMAs, 1,024 cycles at 128 bytes each; 1,140 measured
-// (with A's parts in shared memory too 1,536 and 1,600; with four warps on B's lo part
-// instead of two nothing changed). The parts' sums meet in shared memory over the
-// cluster (each CTA sums 128 / splits rows of all parts, in part order: bit-identical
-// run to run) and go through the epilogue in whole rows.
+// the workspace and join_kernel). TMA brings the f32 operands. Their lo parts are made
+// on the way, which saves the passes and the workspace of copies made beforehand (short
+// products are bound by latency and one reading of the operands): four warps take A's
+// rows to tensor memory, hi and lo, where the UMMAs read them; two write B's lo part
+// beside it in shared memory (elementwise, so the swizzled layout is kept). What bounds
+// a K step of 32 of a 128 x 128 tile is shared memory: 32 KB in by TMA, 48 KB through
+// the converters, 48 KB read by the UMMAs, 1,024 cycles at 128 bytes each; 1,140
+// measured (with A's parts in shared memory too 1,536 and 1,600; with four warps on B's
+// lo part instead of two nothing changed). The parts' sums meet in shared memory over
+// the cluster (each CTA sums 128 / splits rows of all parts, in part order:
+// bit-identical run to run) and go through the epilogue in whole rows.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -41,7 +41,7 @@
 namespace mm {
 namespace {
 
-constexpr int BM = 128;
+constexpr int BM = 128, BN = 128;
 constexpr int BK = 32;  // 32 f32 = 128 bytes = one swizzle row
 constexpr uint32_t MN_BLOCK_BYTES = BK * 128;
 constexpr int kEpiWarps = 8;
@@ -50,7 +50,7 @@ constexpr int kEpiWarps = 8;
 // A stage: A, then B, then (three terms) B's lo part. Three terms: warps 2, 3 write
 // B's lo, 4..7 take A to tensor memory (the lanes of warp w are rows 32 (w % 4)..),
 // 8..15 sum; one term: warps 2..9 sum.
-template <int TERMS, int BN>
+template <int TERMS>
 struct DirectTile {
   static constexpr int A_BYTES = BM * BK * 4;
   static constexpr int B_BYTES = BN * BK * 4;
@@ -78,7 +78,6 @@ __device__ __forceinline__ float4 ld_cluster_quad(uint32_t addr) {
 }
 
 // The sum over the cluster's parts, in part order, of quad q of tile row r.
-template <int BN>
 __device__ __forceinline__ float4 sum_quad(uint32_t tile, int r, int q, int splits) {
   const uint32_t at = tile + 16u * static_cast<uint32_t>(r * (BN / 4) + (q ^ (r & 7)));
   float4 v;
@@ -124,11 +123,11 @@ __device__ __forceinline__ void tile_mn(int t, int tm, int tn, int& mt, int& nt)
   nt = r / rows;
 }
 
-template <int TERMS, bool A_MN, bool B_MN, int BN, class Epi>
-__global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
+template <int TERMS, bool A_MN, bool B_MN, class Epi>
+__global__ void __launch_bounds__(DirectTile<TERMS>::THREADS, 1)
     direct_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Epi epi,
                   int M, int N, int K, int splits, int slices, long long slice_stride, int mn3d, int* err) {
-  using TL = DirectTile<TERMS, BN>;
+  using TL = DirectTile<TERMS>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -154,7 +153,8 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
   tile_mn(cluster - slice * (tm * tn), tm, tn, mt, nt);
   const int m0 = mt * BM, n0 = nt * BN;
   const int n_k = (K + BK - 1) / BK;
-  const long long kpart = static_cast<long long>(slice) * splits + part, kparts = static_cast<long long>(slices) * splits;
+  const long long kpart = static_cast<long long>(slice) * splits + part;
+  const long long kparts = static_cast<long long>(slices) * splits;
   const int kb = static_cast<int>(n_k * kpart / kparts), ke = static_cast<int>(n_k * (kpart + 1) / kparts);
 
   if (threadIdx.x == 0) {
@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(DirectTile<TERMS, BN>::THREADS, 1)
   else
     __syncthreads();
   const int r0 = BM * part / splits;
-  epi.slice(slice * slice_stride).template rows<BN>(base, halves, m0, n0, r0, BM * (part + 1) / splits - r0, splits, M, N, warp, lane,
-                        TL::THREADS / 32);
+  epi.slice(slice * slice_stride)
+      .rows(base, halves, m0, n0, r0, BM * (part + 1) / splits - r0, splits, M, N, warp, lane, TL::THREADS / 32);
   if (splits > 1)
     cluster_sync();  // a peer may still be reading this CTA's part
   else
@@ -380,13 +380,13 @@ struct LinearDirect {
     d.e.C += offset;
     return d;
   }
-  // Rows [r0, r0 + nr) of the tile; BN / 4 lanes per row, four rows of a lane at a
-  // time so that their loads are in flight together. The tile inside the matrix
+  // Rows [r0, r0 + nr) of the tile; a warp per row, four rows of a warp at a time
+  // so that their loads are in flight together. The tile inside the matrix
   // (FULL) runs without bounds checks: the loop is bound by its instructions.
-  template <int BN, bool FULL>
+  template <bool FULL>
   __device__ __forceinline__ void run(uint32_t tile, int m0, int n0, int r0, int nr, int splits, int M, int N,
-                                      int first, int step, int q) const {
-    const int col = n0 + 4 * q;
+                                      int warp, int warps, int lane) const {
+    const int col = n0 + 4 * lane;
     uint64_t seed = 0, offset = 0;
     const bool drop = e.drop.rng != nullptr;
     if (drop) {
@@ -395,17 +395,18 @@ struct LinearDirect {
     }
     const float4 bias = bias_quad(e, col, N);
     constexpr int U = 4;
-    for (int i = first; i < nr; i += U * step) {
+    for (int i = warp; i < nr; i += U * warps) {
       float4 v[U], r[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = i + u * step;
+        const int j = i + u * warps;
         const long long row = m0 + r0 + j;
         const bool live = j < nr && (FULL || (row < M && col < N));
-        v[u] = live ? sum_quad<BN>(tile, r0 + j, q, splits) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[u] = live ? sum_quad(tile, r0 + j, lane, splits) : make_float4(0.f, 0.f, 0.f, 0.f);
         r[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (live && e.R)
-          r[u] = FULL ? *reinterpret_cast<const float4*>(e.R + row * e.ldr + col) : load_quad(e.R + row * e.ldr, col, N);
+          r[u] = FULL ? *reinterpret_cast<const float4*>(e.R + row * e.ldr + col)
+                      : load_quad(e.R + row * e.ldr, col, N);
       }
       // Part by part over the batch, so that the path through the code is short and
       // straight: a CTA runs it once, and what it costs is fetching it.
@@ -416,7 +417,7 @@ struct LinearDirect {
       auto put = [&](float* base, long long ld) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int j = i + u * step;
+          const int j = i + u * warps;
           const long long row = m0 + r0 + j;
           if (j < nr && (FULL || (row < M && col < N))) put_quad<FULL>(base + row * ld, col, N, v[u]);
         }
@@ -426,7 +427,7 @@ struct LinearDirect {
       if (drop)
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          v[u] = dropout_quad(v[u], e.drop, seed, offset, m0 + r0 + i + u * step, col >> 2);
+          v[u] = dropout_quad(v[u], e.drop, seed, offset, m0 + r0 + i + u * warps, col >> 2);
       if (e.R)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -435,15 +436,12 @@ struct LinearDirect {
       put(e.C, e.ldc);
     }
   }
-  template <int BN>
   __device__ __forceinline__ void rows(uint32_t tile, const float2*, int m0, int n0, int r0, int nr, int splits, int M,
                                        int N, int warp, int lane, int warps) const {
-    constexpr int PER = 128 / BN;  // rows a warp covers at once
-    const int q = lane % (BN / 4), first = warp * PER + lane / (BN / 4), step = warps * PER;
     if (m0 + r0 + nr <= M && n0 + BN <= N)
-      run<BN, true>(tile, m0, n0, r0, nr, splits, M, N, first, step, q);
+      run<true>(tile, m0, n0, r0, nr, splits, M, N, warp, warps, lane);
     else
-      run<BN, false>(tile, m0, n0, r0, nr, splits, M, N, first, step, q);
+      run<false>(tile, m0, n0, r0, nr, splits, M, N, warp, warps, lane);
   }
 };
 
@@ -494,7 +492,7 @@ struct LossDirect {
 #pragma unroll 4
     for (int r = warp; r < BM; r += warps) {
       if (m0 + r >= M) break;  // uniform over the warp
-      const float4 v = sum_quad<128>(tile, r, lane, 1);
+      const float4 v = sum_quad(tile, r, lane, 1);
       float* row = e.Z + static_cast<long long>(m0 + r) * e.ldz;
       if (full)
         *reinterpret_cast<float4*>(row + col) = v;
@@ -504,10 +502,8 @@ struct LossDirect {
   }
   // Several parts: a warp per joined row, its 128 columns' maximum and sum by shuffles;
   // three rows at a time.
-  template <int BN>
   __device__ __forceinline__ void rows(uint32_t tile, const float2* halves, int m0, int n0, int r0, int nr, int splits,
                                        int M, int N, int warp, int lane, int warps) const {
-    static_assert(BN == 128, "one partial per 128 columns");
     if (splits == 1) {
       const int r = warp * 32 + lane;
       if (r < BM && m0 + r < M) join(halves[r], halves[BM + r], m0 + r, n0);
@@ -522,7 +518,7 @@ struct LossDirect {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = min(i + u * warps, nr - 1);
-        v[u] = sum_quad<BN>(tile, r0 + j, lane, splits);
+        v[u] = sum_quad(tile, r0 + j, lane, splits);
         m[u] = col < N ? quad_max(v[u], col, N) : -INFINITY;
       }
 #pragma unroll
@@ -588,9 +584,9 @@ __device__ __forceinline__ void warp_sums(float (&v)[N_VALUES], int lane) {
 constexpr int few_blocks(int mt) { return mt <= 4 ? 4 : 3; }  // CTAs of an SM, by registers
 
 template <int MT, bool B_MN>
-__global__ void __launch_bounds__(256, few_blocks(MT)) few_rows_kernel(const float* a, long long lda, const float* b, long long ldb,
-                                                       LinearEpilogue e, int M, int N, int K, int splits,
-                                                       int slices, long long slice_stride) {
+__global__ void __launch_bounds__(256, few_blocks(MT))
+    few_rows_kernel(const float* a, long long lda, const float* b, long long ldb, LinearEpilogue e, int M, int N, int K,
+                    int splits, int slices, long long slice_stride) {
   __shared__ __align__(16) float as[kFewPiece * MT];
   __shared__ __align__(16) float sums[(B_MN ? 8 : 1) * MT * kFewCols];  // [warps][MT][32], then [MT][32]
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -599,7 +595,8 @@ __global__ void __launch_bounds__(256, few_blocks(MT)) few_rows_kernel(const flo
   const int slice = cluster / tiles, n0 = (cluster - slice * tiles) * kFewCols;
   e.C += slice * slice_stride;
   const int units = (K + 31) / 32;  // parts are cut at multiples of 32
-  const long long kpart = static_cast<long long>(slice) * splits + part, kparts = static_cast<long long>(slices) * splits;
+  const long long kpart = static_cast<long long>(slice) * splits + part;
+  const long long kparts = static_cast<long long>(slices) * splits;
   const int kb = static_cast<int>(units * kpart / kparts) * 32;
   const int ke = min(K, static_cast<int>(units * (kpart + 1) / kparts) * 32);
   float acc[4 * MT];  // [MT][4 columns]
@@ -925,16 +922,16 @@ void launch_clusters(Kernel kern, long long tiles, int splits, int threads, int 
   check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), "linear");
 }
 
-template <int TERMS, bool A_MN, bool B_MN, int BN, class Epi>
+template <int TERMS, bool A_MN, bool B_MN, class Epi>
 int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, Cut cut,
                   int* d_err, cudaStream_t s) {
-  using TL = DirectTile<TERMS, BN>;
+  using TL = DirectTile<TERMS>;
   CUtensorMap ta{}, tb{};
   bool a3 = false, b3 = false;
   int rc = operand_map(&ta, A, M, K, BM, &a3);
   if (!rc) rc = operand_map(&tb, B, N, K, BN, &b3);
   if (rc) return rc;
-  auto kern = direct_kernel<TERMS, A_MN, B_MN, BN, Epi>;
+  auto kern = direct_kernel<TERMS, A_MN, B_MN, Epi>;
   static thread_local int configured_device = -1;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
@@ -961,9 +958,9 @@ void launch_few(int M, int N, int K, const GemmOperand& A, const GemmOperand& B,
 template <int TERMS, class Epi>
 int direct_majors(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, Cut cut,
                   int* d_err, cudaStream_t s) {
-  if (!A.mn_major && !B.mn_major) return launch_direct<TERMS, false, false, 128>(M, N, K, A, B, epi, cut, d_err, s);
-  if (!A.mn_major) return launch_direct<TERMS, false, true, 128>(M, N, K, A, B, epi, cut, d_err, s);
-  if (B.mn_major) return launch_direct<TERMS, true, true, 128>(M, N, K, A, B, epi, cut, d_err, s);
+  if (!A.mn_major && !B.mn_major) return launch_direct<TERMS, false, false>(M, N, K, A, B, epi, cut, d_err, s);
+  if (!A.mn_major) return launch_direct<TERMS, false, true>(M, N, K, A, B, epi, cut, d_err, s);
+  if (B.mn_major) return launch_direct<TERMS, true, true>(M, N, K, A, B, epi, cut, d_err, s);
   return kGemmBadArgument;  // no caller has an MN-major A with a K-major B
 }
 
@@ -1034,17 +1031,17 @@ int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const Line
   return 0;
 }
 
-int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact, int* d_err,
-                        cudaStream_t s) {
+int direct_loss_product(int M, int N, int K, GemmOperand A, GemmOperand B, const LossEpilogue& e, bool exact,
+                        int* d_err, cudaStream_t s) {
   if (M <= 0 || N <= 0) return 0;
   if (A.mn_major) return kGemmBadArgument;
   const LossDirect epi{e};
   const Cut cut = direct_cut(M, N, K, false);
   if (exact)
-    return B.mn_major ? launch_direct<3, false, true, 128>(M, N, K, A, B, epi, cut, d_err, s)
-                      : launch_direct<3, false, false, 128>(M, N, K, A, B, epi, cut, d_err, s);
-  return B.mn_major ? launch_direct<1, false, true, 128>(M, N, K, A, B, epi, cut, d_err, s)
-                    : launch_direct<1, false, false, 128>(M, N, K, A, B, epi, cut, d_err, s);
+    return B.mn_major ? launch_direct<3, false, true>(M, N, K, A, B, epi, cut, d_err, s)
+                      : launch_direct<3, false, false>(M, N, K, A, B, epi, cut, d_err, s);
+  return B.mn_major ? launch_direct<1, false, true>(M, N, K, A, B, epi, cut, d_err, s)
+                    : launch_direct<1, false, false>(M, N, K, A, B, epi, cut, d_err, s);
 }
 
 int act_backward_parts(int rows, int cols) {
@@ -1057,7 +1054,8 @@ void act_backward(const float* dc, long long lddc, const float* z, long long ldz
   if (rows <= 0 || cols <= 0) return;
   const long long blocks = (cols + 127ll) / 128 * act_backward_parts(rows, cols);
   if (blocks > INT32_MAX) throw std::invalid_argument("a matrix is too large");
-  act_backward_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(dc, lddc, z, ldz, act, d, rows, cols, act_rows(rows, cols), dz, lddz, part);
+  act_backward_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(dc, lddc, z, ldz, act, d, rows, cols,
+                                                                    act_rows(rows, cols), dz, lddz, part);
   check_cuda(cudaGetLastError(), "linear backward");
 }
 

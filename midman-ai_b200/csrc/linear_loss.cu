@@ -110,7 +110,8 @@ Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* w
     long long parts = 0;
     for (const int r : {p.rows, std::max(last, 1)}) {
       if (dx) parts = std::max(parts, plain_ws_bytes(r, dim, vocab, false, exact));
-      if (dw) parts = std::max({parts, plain_ws_bytes(vocab, dim, r, true, exact), plain_ws_bytes(dim, vocab, r, true, exact)});
+      if (dw)
+        parts = std::max({parts, plain_ws_bytes(vocab, dim, r, true, exact), plain_ws_bytes(dim, vocab, r, true, exact)});
     }
     p.parts = at.take(parts);
   }
@@ -199,7 +200,8 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) {
       const float4 v = row[q];
-      g = make_float4(loss_exp(v.x - a.m) * coef, loss_exp(v.y - a.m) * coef, loss_exp(v.z - a.m) * coef, loss_exp(v.w - a.m) * coef);
+      g = make_float4(loss_exp(v.x - a.m) * coef, loss_exp(v.y - a.m) * coef, loss_exp(v.z - a.m) * coef,
+                      loss_exp(v.w - a.m) * coef);
       if ((t >> 2) == q) {
         if ((t & 3) == 0) g.x -= grad_scale;
         if ((t & 3) == 1) g.y -= grad_scale;

@@ -55,7 +55,8 @@ BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
     p.parts = at.take(std::max({plain_ws_bytes(m, k, n, false, exact), plain_ws_bytes(k, n, m, true, exact),
                                 plain_ws_bytes(n, k, m, true, exact)}));
   }
-  p.sums = static_cast<float*>(at.take(static_cast<long long>(std::max(act_backward_parts(m, n), split_parts(m))) * n * 4));
+  const long long parts = std::max(act_backward_parts(m, n), split_parts(m));
+  p.sums = static_cast<float*>(at.take(parts * n * 4));
   p.bytes = at.at;
   return p;
 }

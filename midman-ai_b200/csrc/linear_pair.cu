@@ -296,8 +296,9 @@ void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_row
   }
   const long long tiles = ((rows + kTile - 1ll) / kTile) * ((cols + kTile - 1ll) / kTile);
   if (tiles > INT32_MAX) throw std::invalid_argument("a matrix is too large");
-  kern<<<static_cast<unsigned>(tiles), 256, by_cols ? kSplitSmem : kSplitSums, s>>>(src, rows, cols, by_rows ? *by_rows : SplitCopy{},
-                                     by_cols ? *by_cols : SplitCopy{}, part);
+  const SplitCopy none{};
+  kern<<<static_cast<unsigned>(tiles), 256, by_cols ? kSplitSmem : kSplitSums, s>>>(
+      src, rows, cols, by_rows ? *by_rows : none, by_cols ? *by_cols : none, part);
   check_cuda(cudaGetLastError(), "split");
 }
 
