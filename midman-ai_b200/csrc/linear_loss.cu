@@ -34,6 +34,7 @@ long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
 
 struct Plan {
   bool pair;        // pair products on copies, or direct ones
+  bool pair_logits; // direct ones, but for the logits
   int tiles, rows;  // (max, sum) pairs per row; rows of a block
   long long ldz, ldx;
   float2* part;
@@ -83,12 +84,15 @@ Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* w
   p.rows = static_cast<int>(std::min(n, round_up((n + blocks - 1) / blocks, 256)));  // even blocks of whole tiles
   p.pair = exact && pair_product_suits(p.rows, vocab, dim) &&
            (!grad || (pair_product_suits(p.rows, dim, vocab) && pair_product_suits(vocab, dim, p.rows)));
+  p.pair_logits = exact && !p.pair && pair_product_suits(p.rows, vocab, dim);
   p.part = static_cast<float2*>(at.take(static_cast<long long>(p.rows) * p.tiles * 8));
   p.zt = static_cast<float*>(at.take(p.rows * 4ll));
   p.stat = static_cast<float2*>(at.take(p.rows * 8ll));
-  if (p.pair) {
+  if (p.pair || p.pair_logits) {
     p.w = at.copy(vocab, dim);
     p.xr_at = at.take(split_copy_bytes(p.rows, dim));
+  }
+  if (p.pair) {
     if (grad) p.g_at = at.take(split_copy_bytes(p.rows, vocab));
     if (dx) p.wt = at.copy(dim, vocab);
     if (dw) {
@@ -252,9 +256,21 @@ long long linear_loss_ws_bytes(int rows, int vocab, int dim, bool grad, bool exa
 
 namespace {
 
-// One block of rows on copies; the first makes those of w too.
+// The copies of a block's rows of x, transposed too where xt is given, and with the first
+// block's those of w. With `targets` rows without one count as zeros.
+void copy_operands(const LinearLoss& a, const Plan& p, long long r0, int n, const int32_t* targets, const SplitCopy* wt,
+                   const SplitCopy* xt, cudaStream_t s) {
+  const SplitMatrix x{a.x + r0 * a.ldx, a.ldx, targets, a.vocab}, w{a.w, a.ldw};
+  if (r0 > 0)
+    split(x, n, a.dim, &p.xr, xt, s);
+  else if (a.w_mn_major)  // [dim, vocab]
+    split_two(w, a.dim, a.vocab, wt, &p.w, x, n, a.dim, &p.xr, xt, s);
+  else
+    split_two(w, a.vocab, a.dim, &p.w, wt, x, n, a.dim, &p.xr, xt, s);
+}
+
+// One block of rows on copies.
 int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cudaStream_t s) {
-  const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
   // For gradients x's rows without a target count as zeros: their logits are not used, but
   // their exponentials are multiplied by 0 for dx, and dw sums over all rows, and 0 times
@@ -262,18 +278,7 @@ int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cu
   p.xr = split_copy_at(p.xr_at, n, a.dim);
   if (a.dw) p.xt = split_copy_at(p.xt_at, a.dim, n);
   const bool grad = a.dx || a.dw;
-  const SplitMatrix xm{x, a.ldx, grad ? t : nullptr, a.vocab};
-  const SplitCopy* xt = a.dw ? &p.xt : nullptr;
-  if (r0 == 0) {  // with w, [vocab, dim] or [dim, vocab]
-    const SplitCopy* wt = a.dx ? &p.wt : nullptr;
-    const SplitMatrix w{a.w, a.ldw};
-    if (a.w_mn_major)
-      split_two(w, a.dim, a.vocab, wt, &p.w, xm, n, a.dim, &p.xr, xt, s);
-    else
-      split_two(w, a.vocab, a.dim, &p.w, wt, xm, n, a.dim, &p.xr, xt, s);
-  } else {
-    split(xm, n, a.dim, &p.xr, xt, s);
-  }
+  copy_operands(a, p, r0, n, grad ? t : nullptr, a.dx ? &p.wt : nullptr, a.dw ? &p.xt : nullptr, s);
   LossEpilogue e;
   e.part = p.part;
   e.tiles = p.tiles;
@@ -313,12 +318,21 @@ int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cu
   return rc;
 }
 
-// One block of rows on direct products: G takes the logits' place.
-int direct_block(const LinearLoss& a, const Plan& p, long long r0, int n, int* d_err, cudaStream_t s) {
+// One block of rows on direct products: G takes the logits' place. Where rows and classes
+// are many but the rows short, the logits have the tiles for a pair product and the
+// gradients do not.
+int direct_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cudaStream_t s) {
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
   const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt, nullptr, 0};
-  int rc = plain_loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
+  int rc;
+  if (p.pair_logits) {
+    p.xr = split_copy_at(p.xr_at, n, a.dim);
+    copy_operands(a, p, r0, n, nullptr, nullptr, nullptr, s);
+    rc = pair_loss_product(p.xr, p.w, e, d_err, s);
+  } else {
+    rc = plain_loss_product(n, a.vocab, a.dim, {x, a.ldx, false}, {a.w, a.ldw, a.w_mn_major}, e, a.exact, d_err, s);
+  }
   if (rc) return rc;
   if (!a.dx && !a.dw) {
     row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(p.part, p.tiles, p.zt, t, n, a.vocab, 0.0f, a.row_loss + r0, nullptr,
