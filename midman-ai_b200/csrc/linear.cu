@@ -864,10 +864,12 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 // time from waves of clusters, steps of a part and a tile's fixed cost. A cluster lies
 // in one GPC, so fewer CTAs run at once in larger ones (the occupancy query's counts for
 // this kernel on a B200; a device with other GPCs runs the same plan in other waves). A
-// step takes 0.6 us, a tile's start and end about 5, the parts' join 1, writing,
-// reading and joining slices 6 (64 x 32000 -> 512 in eight parts alone took 80 us, in
-// four slices of eight 25). (128 x 64 tiles, tried for more CTAs, took 0.69 us a step: a
-// UMMA of half the width is no shorter.)
+// step takes 0.66 us, a tile's start and end 5.5, the parts' join 0.5, the slices' launch
+// and their sums 3, some of it the host's (2048 x 4096 -> 128 in six parts takes 24.7 us, in
+// nine slices 21.4, in four parts of two slices 22.0; 128 x 2048 -> 2048 16.8, 16.0 and 16.1;
+// 4096 x 2048 -> 128 in four parts 20.0, in four slices 21.6; 64 x 32000 -> 512 in eight
+// parts alone 80, in four of eight slices 34). (128 x 64 tiles, tried for more CTAs, took
+// 0.69 us a step: a UMMA of half the width is no shorter.)
 struct Cut {
   int splits = 1, slices = 1;
 };
@@ -880,7 +882,7 @@ Cut direct_cut(int M, int N, int K, bool sliced) {
   for (int s = 1; s <= 8 && (s == 1 || n_k >= 4 * s); ++s)
     for (int l = 1; l <= (sliced ? 32 : 1) && (l == 1 || (n_k >= 8 * s * l && tiles * l <= kFit[s])); ++l) {
       const double waves = static_cast<double>((tiles * l + kFit[s] - 1) / kFit[s]);
-      const double us = waves * ((n_k + s * l - 1) / (s * l) * 0.6 + 5.0 + (s > 1 ? 1.0 : 0.0)) + (l > 1 ? 6.0 : 0.0);
+      const double us = waves * ((n_k + s * l - 1) / (s * l) * 0.66 + 5.5 + (s > 1 ? 0.5 : 0.0)) + (l > 1 ? 3.0 : 0.0);
       if (us < best_us) {
         best = {s, l};
         best_us = us;

@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int t
 // the row's pairs itself (vocab / 128 of them, from L2), the first writes the loss and,
 // where dw is wanted, copies the row of x (zeros for a row without a target: dw sums
 // over all rows, and 0 times what such a row holds may be NaN).
-constexpr int kSegment = 8192;
+constexpr int kSegment = 4096;
 
 __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz, const float2* part, int tiles,
                                                         const float* zt, const int32_t* targets, int vocab,
@@ -182,6 +182,12 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
   const int r = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int t = targets[r];
   const bool live = t >= 0 && t < vocab;
+  float4* row = reinterpret_cast<float4*>(z + r * ldz);
+  const int q_end = static_cast<int>(ldz / 4), q0 = blockIdx.y * (kSegment / 4) + threadIdx.x;
+  float4 v[kSegment / 1024];  // on their way while the row's pairs are joined
+#pragma unroll
+  for (int u = 0; u < kSegment / 1024; ++u)
+    v[u] = q0 + 256 * u < q_end ? row[q0 + 256 * u] : make_float4(0.f, 0.f, 0.f, 0.f);
   MaxSum a{-INFINITY, 0.0f};
   for (int i = threadIdx.x; i < tiles; i += 256) {
     const float2 p = part[static_cast<long long>(r) * tiles + i];
@@ -198,14 +204,14 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
       *reinterpret_cast<float4*>(live_x + r * ldl + c) =
           live ? load_quad(x + r * ldx, c, dim) : make_float4(0.f, 0.f, 0.f, 0.f);
   const float coef = grad_scale / a.s;
-  float4* row = reinterpret_cast<float4*>(z + r * ldz);
-  const int q_end = static_cast<int>(ldz / 4), q0 = blockIdx.y * (kSegment / 4);
-  for (int q = q0 + threadIdx.x; q < min(q_end, q0 + kSegment / 4); q += 256) {
+#pragma unroll
+  for (int u = 0; u < kSegment / 1024; ++u) {
+    const int q = q0 + 256 * u;
+    if (q >= q_end) break;
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) {
-      const float4 v = row[q];
-      g = make_float4(loss_exp(v.x - a.m) * coef, loss_exp(v.y - a.m) * coef, loss_exp(v.z - a.m) * coef,
-                      loss_exp(v.w - a.m) * coef);
+      g = make_float4(loss_exp(v[u].x - a.m) * coef, loss_exp(v[u].y - a.m) * coef, loss_exp(v[u].z - a.m) * coef,
+                      loss_exp(v[u].w - a.m) * coef);
       if ((t >> 2) == q) {
         if ((t & 3) == 0) g.x -= grad_scale;
         if ((t & 3) == 1) g.y -= grad_scale;
