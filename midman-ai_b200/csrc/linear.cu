@@ -181,6 +181,8 @@ __global__ void __launch_bounds__(DirectTile<TERMS>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  let_next();
+  after_previous();
   const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
   const uint32_t tmem_a = tmem_base + 2 * BN;  // three terms: A's stages
   float2* halves = reinterpret_cast<float2*>(smem + BM * BN * 4);  // behind the partial tile
@@ -587,6 +589,8 @@ template <int MT, bool B_MN>
 __global__ void __launch_bounds__(256, few_blocks(MT))
     few_rows_kernel(const float* a, long long lda, const float* b, long long ldb, LinearEpilogue e, int M, int N, int K,
                     int splits, int slices, long long slice_stride) {
+  let_next();
+  after_previous();
   __shared__ __align__(16) float as[kFewPiece * MT];
   __shared__ __align__(16) float sums[(B_MN ? 8 : 1) * MT * kFewCols];  // [warps][MT][32], then [MT][32]
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -632,7 +636,7 @@ __global__ void __launch_bounds__(256, few_blocks(MT))
           float4 w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i)  // past the piece: any row of it, not added
-            w[i] = __ldg(reinterpret_cast<const float4*>(b + (k0 + min(k + 32 * i, kn - 1)) * ldb + col));
+            w[i] = *reinterpret_cast<const float4*>(b + (k0 + min(k + 32 * i, kn - 1)) * ldb + col);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (k + 32 * i < kn) add(k + 32 * i, w[i]);
@@ -649,7 +653,7 @@ __global__ void __launch_bounds__(256, few_blocks(MT))
         float4 w[4];
         if (whole) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) w[c] = __ldg(reinterpret_cast<const float4*>(col + c * ldb + k));
+          for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const float4*>(col + c * ldb + k);
         } else {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -725,6 +729,8 @@ __global__ void __launch_bounds__(256, few_blocks(MT))
 // The slices' sums [slices][M, ld], in slice order, and the epilogue: a thread per quad.
 __global__ void __launch_bounds__(256) join_kernel(const float* parts, int slices, long long slice_stride,
                                                    long long ld, const LinearEpilogue e, int M, int N) {
+  let_next();
+  after_previous();
   const int quads = (N + 3) / 4;
   const long long i = blockIdx.x * 256ll + threadIdx.x, row = i / quads;
   const int col = 4 * static_cast<int>(i - row * quads);
@@ -754,6 +760,8 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long
                                                            long long ldz, int act, DropoutArgs drop, int rows,
                                                            int cols, int block_rows, float* dz, long long lddz,
                                                            float* part) {
+  let_next();
+  after_previous();
   __shared__ float4 sums[8][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int across = (cols + 127) / 128, band = static_cast<int>(blockIdx.x) / across;
@@ -800,6 +808,8 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long
 // 32 columns per block, eight rows of partials at a time, joined in a fixed order.
 __global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int parts, int cols, float* out,
                                                         int accumulate) {
+  let_next();
+  after_previous();
   __shared__ double sums[8][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, col = blockIdx.x * 32 + lane;
   double s = 0.0;
@@ -825,6 +835,8 @@ template <bool VEC, int U, class Index>
 __global__ void __launch_bounds__(256) dropout_kernel(const float* x, long long ldx, const float* r, long long ldr,
                                                       float* y, long long ldy, Index quads, int cols,
                                                       DropoutArgs drop) {
+  let_next();
+  after_previous();
   const uint64_t seed = drop.rng ? drop.rng[0] : 0, offset = drop.rng ? drop.rng[1] : 0;
   const Index step = static_cast<Index>(gridDim.x) * 256;
   for (long long first = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; first < quads; first += U * step) {
@@ -908,22 +920,6 @@ Cut cut_of(int M, int N, int K, bool a_mn_major) {
 
 long long slice_floats(int M, int N) { return M * ((N + 3ll) & ~3ll); }
 
-template <class Kernel, class... Args>
-void launch_clusters(Kernel kern, long long tiles, int splits, int threads, int smem, cudaStream_t s, Args... args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(splits);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = &attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
-  check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), "linear");
-}
-
 template <int TERMS, bool A_MN, bool B_MN, class Epi>
 int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const Epi& epi, Cut cut,
                   int* d_err, cudaStream_t s) {
@@ -943,8 +939,9 @@ int launch_direct(int M, int N, int K, const GemmOperand& A, const GemmOperand& 
   }
   const long long tiles = static_cast<long long>((M + BM - 1) / BM) * ((N + BN - 1) / BN);
   if (tiles * cut.splits * cut.slices > 0x7fffffffll) return kGemmBadArgument;
-  launch_clusters(kern, tiles * cut.slices, cut.splits, TL::THREADS, TL::SMEM, s, ta, tb, epi, M, N, K, cut.splits,
-                  cut.slices, slice_floats(M, N), (a3 ? 1 : 0) | (b3 ? 2 : 0), d_err);
+  launch_next("linear", kern, dim3(static_cast<unsigned>(tiles * cut.slices * cut.splits)), TL::THREADS, TL::SMEM,
+              cut.splits, s, ta, tb, epi, M, N, K, cut.splits, cut.slices, slice_floats(M, N),
+              (a3 ? 1 : 0) | (b3 ? 2 : 0), d_err);
   return 0;
 }
 
@@ -953,8 +950,8 @@ void launch_few(int M, int N, int K, const GemmOperand& A, const GemmOperand& B,
                 cudaStream_t s) {
   const long long clusters = (N + kFewCols - 1) / kFewCols * static_cast<long long>(cut.slices);
   auto kern = B.mn_major ? few_rows_kernel<MT, true> : few_rows_kernel<MT, false>;
-  launch_clusters(kern, clusters, cut.splits, 256, 0, s, A.ptr, A.ld, B.ptr, B.ld, e, M, N, K, cut.splits, cut.slices,
-                  slice_floats(M, N));
+  launch_next("linear", kern, dim3(static_cast<unsigned>(clusters * cut.splits)), 256, 0, cut.splits, s, A.ptr, A.ld,
+              B.ptr, B.ld, e, M, N, K, cut.splits, cut.slices, slice_floats(M, N));
 }
 
 template <int TERMS, class Epi>
@@ -1026,9 +1023,8 @@ int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const Line
   }
   if (cut.slices > 1) {
     const long long quads = M * ((N + 3ll) / 4);
-    join_kernel<<<static_cast<unsigned>((quads + 255) / 256), 256, 0, s>>>(raw.C, cut.slices, slice_floats(M, N),
-                                                                         raw.ldc, e, M, N);
-    check_cuda(cudaGetLastError(), "linear");
+    launch_next("linear", join_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), 256, 0, 1, s, raw.C, cut.slices,
+                slice_floats(M, N), raw.ldc, e, M, N);
   }
   return 0;
 }
@@ -1056,15 +1052,14 @@ void act_backward(const float* dc, long long lddc, const float* z, long long ldz
   if (rows <= 0 || cols <= 0) return;
   const long long blocks = (cols + 127ll) / 128 * act_backward_parts(rows, cols);
   if (blocks > INT32_MAX) throw std::invalid_argument("a matrix is too large");
-  act_backward_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(dc, lddc, z, ldz, act, d, rows, cols,
-                                                                    act_rows(rows, cols), dz, lddz, part);
-  check_cuda(cudaGetLastError(), "linear backward");
+  launch_next("linear backward", act_backward_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, 1, s, dc, lddc, z, ldz,
+              act, d, rows, cols, act_rows(rows, cols), dz, lddz, part);
 }
 
 void sum_parts(const float* part, int parts, int cols, float* out, bool accumulate, cudaStream_t s) {
   if (cols <= 0) return;
-  sum_parts_kernel<<<(cols + 31) / 32, 256, 0, s>>>(part, parts, cols, out, accumulate ? 1 : 0);
-  check_cuda(cudaGetLastError(), "bias gradient");
+  launch_next("bias gradient", sum_parts_kernel, dim3((cols + 31) / 32), 256, 0, 1, s, part, parts, cols, out,
+              accumulate ? 1 : 0);
 }
 
 void dropout(const float* x, long long ldx, const float* r, long long ldr, float* y, long long ldy, long long rows,
@@ -1073,7 +1068,9 @@ void dropout(const float* x, long long ldx, const float* r, long long ldr, float
   if (quads <= 0) return;
   const bool vec = !((ldx | ldy | (r ? ldr : 0)) & 3) && aligned16(x) && aligned16(y) && (!r || aligned16(r));
   const int blocks = static_cast<int>(std::min((quads + 255) / 256, 148ll * 16));
-  auto run = [&](auto kernel, auto n) { kernel<<<blocks, 256, 0, s>>>(x, ldx, r, ldr, y, ldy, n, cols, d); };
+  auto run = [&](auto kernel, auto n) {
+    launch_next("dropout", kernel, dim3(blocks), 256, 0, 1, s, x, ldx, r, ldr, y, ldy, n, cols, d);
+  };
   if (quads > INT32_MAX)
     vec ? run(dropout_kernel<true, 4, long long>, quads) : run(dropout_kernel<false, 4, long long>, quads);
   else if (quads >= 1 << 21)
@@ -1082,7 +1079,6 @@ void dropout(const float* x, long long ldx, const float* r, long long ldr, float
   else
     vec ? run(dropout_kernel<true, 1, uint32_t>, static_cast<uint32_t>(quads))
         : run(dropout_kernel<false, 1, uint32_t>, static_cast<uint32_t>(quads));
-  check_cuda(cudaGetLastError(), "dropout");
 }
 
 }  // namespace mm

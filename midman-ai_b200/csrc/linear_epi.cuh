@@ -6,10 +6,41 @@
 #include <cstdint>
 
 #include "dropout.cuh"
+#include "device.h"
 #include "linear.h"
 #include "ptx.cuh"
 
 namespace mm {
+
+// Launches one after another on a stream: a kernel may start while the one before it
+// ends, so that its launch and its prologue are hidden (1 to 2 us a launch, of calls that
+// make four to eight short ones). Every thread of every kernel here waits for the one
+// before it to be complete and visible (`after_previous`) before it touches global
+// memory, so completion passes along the chain; kernels launched in any other way wait
+// for everything before them as ever. (So nothing is loaded as read-only for the
+// kernel's lifetime: that begins before the kernel that wrote it ends.) `let_next` comes once the CTA holds all that it
+// allocates, so a waiting CTA of the next kernel never holds what this one needs.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... Params, class... Args>
+void launch_next(const char* what, void (*kernel)(Params...), dim3 grid, int threads, int smem, int cluster,
+                 cudaStream_t s, const Args&... args) {
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
 
 // The normal distribution function and its density, branch-free (the epilogue runs on
 // few warps, so a divergent erff costs both of its paths): C. Hastings' rational

@@ -149,6 +149,8 @@ __device__ __forceinline__ float loss_of(MaxSum a, int t, int vocab, const float
 __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int tiles, const float* zt,
                                                        const int32_t* targets, int rows, int vocab,
                                                        float grad_scale, float* row_loss, float2* stat, int* err) {
+  let_next();
+  after_previous();
   const int r = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   if (r >= rows) return;
   MaxSum a{-INFINITY, 0.0f};
@@ -178,6 +180,8 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
                                                         float grad_scale, float* row_loss, const float* x,
                                                         long long ldx, int dim, float* live_x, long long ldl,
                                                         int* err) {
+  let_next();
+  after_previous();
   __shared__ MaxSum warps[8];
   const int r = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int t = targets[r];
@@ -226,6 +230,8 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
 // The mean over the rows that have a target (0 when none has), in f64.
 __global__ void __launch_bounds__(1024) mean_live_kernel(const float* row_loss, const int32_t* targets, int rows,
                                                          float* mean) {
+  let_next();
+  after_previous();
   __shared__ double sums[32];
   __shared__ int counts[32];
   double s = 0.0;
@@ -297,9 +303,8 @@ int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cu
   }
   int rc = pair_loss_product(p.xr, p.w, e, d_err, s);
   if (rc) return rc;
-  row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(p.part, p.tiles, p.zt, t, n, a.vocab, a.grad_scale, a.row_loss + r0,
-                                              p.stat, d_err);
-  check_cuda(cudaGetLastError(), "row loss");
+  launch_next("row loss", row_loss_kernel, dim3((n + 7) / 8), 256, 0, 1, s, p.part, p.tiles, p.zt, t, n, a.vocab,
+              a.grad_scale, a.row_loss + r0, p.stat, d_err);
   if (!grad) return 0;
   loss_scales(p.g, p.part, p.stat, t, a.vocab, a.grad_scale, s);
   if (a.dw) {
@@ -341,15 +346,13 @@ int direct_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, 
   }
   if (rc) return rc;
   if (!a.dx && !a.dw) {
-    row_loss_kernel<<<(n + 7) / 8, 256, 0, s>>>(p.part, p.tiles, p.zt, t, n, a.vocab, 0.0f, a.row_loss + r0, nullptr,
-                                                d_err);
-    check_cuda(cudaGetLastError(), "row loss");
+    launch_next("row loss", row_loss_kernel, dim3((n + 7) / 8), 256, 0, 1, s, p.part, p.tiles, p.zt, t, n, a.vocab, 0.0f,
+                a.row_loss + r0, nullptr, d_err);
     return 0;
   }
   const dim3 grid(n, static_cast<unsigned>((p.ldz + kSegment - 1) / kSegment));
-  loss_grad_kernel<<<grid, 256, 0, s>>>(p.z, p.ldz, p.part, p.tiles, p.zt, t, a.vocab, a.grad_scale, a.row_loss + r0,
-                                        x, a.ldx, a.dim, a.dw ? p.x : nullptr, p.ldx, d_err);
-  check_cuda(cudaGetLastError(), "loss gradient");
+  launch_next("loss gradient", loss_grad_kernel, grid, 256, 0, 1, s, p.z, p.ldz, p.part, p.tiles, p.zt, t, a.vocab,
+              a.grad_scale, a.row_loss + r0, x, a.ldx, a.dim, a.dw ? p.x : nullptr, p.ldx, d_err);
   if (a.dx) {
     LinearEpilogue o;
     o.C = a.dx + r0 * a.lddx;
@@ -382,8 +385,7 @@ int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
     if (rc) return rc;
   }
   if (a.mean_loss) {
-    mean_live_kernel<<<1, 1024, 0, s>>>(a.row_loss, a.targets, a.rows, a.mean_loss);
-    check_cuda(cudaGetLastError(), "mean loss");
+    launch_next("mean loss", mean_live_kernel, dim3(1), 1024, 0, 1, s, a.row_loss, a.targets, a.rows, a.mean_loss);
   }
   return 0;
 }

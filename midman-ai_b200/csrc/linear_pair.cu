@@ -225,6 +225,8 @@ __device__ __forceinline__ void split_tile(Source& src, int rows, int cols, cons
 template <class Source>
 __global__ void __launch_bounds__(256, 3) split_kernel(Source src, int rows, int cols, SplitCopy by_rows,
                                                        SplitCopy by_cols, float* part) {
+  let_next();
+  after_previous();
   const int tc = (cols + kTile - 1) / kTile, t = static_cast<int>(blockIdx.x);
   split_tile(src, rows, cols, by_rows, by_cols, part, t / tc, t % tc);
 }
@@ -236,6 +238,8 @@ __global__ void __launch_bounds__(256, 3) split_kernel(Source src, int rows, int
 constexpr int kHalf = 64;
 template <class Source>
 __global__ void __launch_bounds__(256, 6) split_transposed_kernel(Source src, int rows, int cols, SplitCopy by_cols) {
+  let_next();
+  after_previous();
   __shared__ __align__(16) float4 tile[kTile * kHalf / 4];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int tc = (cols + kHalf - 1) / kHalf, tile_r = static_cast<int>(blockIdx.x) / tc;
@@ -267,6 +271,8 @@ struct MatrixJob {
   SplitCopy by_rows, by_cols;
 };
 __global__ void __launch_bounds__(256, 3) split_two_kernel(MatrixJob x, MatrixJob y) {
+  let_next();
+  after_previous();
   const int tiles_x = ((x.rows + kTile - 1) / kTile) * ((x.cols + kTile - 1) / kTile);
   const bool first = static_cast<int>(blockIdx.x) < tiles_x;
   MatrixJob& job = first ? x : y;
@@ -282,8 +288,8 @@ void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_row
   if (by_cols && !by_rows && !part) {
     const long long tiles = ((rows + kTile - 1ll) / kTile) * ((cols + kHalf - 1ll) / kHalf);
     if (tiles > INT32_MAX) throw std::invalid_argument("a matrix is too large");
-    split_transposed_kernel<<<static_cast<unsigned>(tiles), 256, 0, s>>>(src, rows, cols, *by_cols);
-    check_cuda(cudaGetLastError(), "split");
+    launch_next("split", split_transposed_kernel<Source>, dim3(static_cast<unsigned>(tiles)), 256, 0, 1, s, src, rows, cols,
+                *by_cols);
     return;
   }
   auto kern = split_kernel<Source>;
@@ -297,9 +303,8 @@ void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_row
   const long long tiles = ((rows + kTile - 1ll) / kTile) * ((cols + kTile - 1ll) / kTile);
   if (tiles > INT32_MAX) throw std::invalid_argument("a matrix is too large");
   const SplitCopy none{};
-  kern<<<static_cast<unsigned>(tiles), 256, by_cols ? kSplitSmem : kSplitSums, s>>>(
-      src, rows, cols, by_rows ? *by_rows : none, by_cols ? *by_cols : none, part);
-  check_cuda(cudaGetLastError(), "split");
+  launch_next("split", kern, dim3(static_cast<unsigned>(tiles)), 256, by_cols ? kSplitSmem : kSplitSums, 1, s, src, rows,
+              cols, by_rows ? *by_rows : none, by_cols ? *by_cols : none, part);
 }
 
 // ------------------------------------------------------------------ products
@@ -462,6 +467,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
+  let_next();
+  after_previous();
   const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
 
   if (warp < P_SUM_WARP) {
@@ -565,16 +572,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         // the columns' through the staging tile (idle until the epilogue).
         const float* pa = inv_a + w.cb * ld_ia + wrow0 + lane;
         const float4* pb = reinterpret_cast<const float4*>(inv_b + w.cb * ld_ib + wcol0) + lane;
-        float ia = __ldg(pa);
-        stage_tile[lane] = __ldg(pb);
+        float ia = *pa;
+        stage_tile[lane] = *pb;
         __syncwarp();
         for (int c = w.cb; c < w.ce; ++c) {
           const float4* ib = stage_tile + 32 * ((c - w.cb) & 1);
           const bool more = c + 1 < w.ce;
           pa += ld_ia;
           pb += ld_ib / 4;
-          const float ia_next = more ? __ldg(pa) : 0.0f;
-          const float4 ib_next = more ? __ldg(pb) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float ia_next = more ? *pa : 0.0f;
+          const float4 ib_next = more ? *pb : make_float4(0.f, 0.f, 0.f, 0.f);
           ok = wait_acc(&acc);
           if (!ok) break;
 #pragma unroll
@@ -712,6 +719,8 @@ struct LinearPair {
 
 // The split tiles: parts summed in order, then the epilogue. Four rows of a tile per block.
 __global__ void __launch_bounds__(256) reduce_kernel(const PairWork work, const LinearEpilogue e, int M, int N) {
+  let_next();
+  after_previous();
   const int tm = (M + 2 * BM - 1) / (2 * BM), tn = (N + PN - 1) / PN;
   int mt, nt;
   pair_tile(work.full + static_cast<int>(blockIdx.x), tm, tn, mt, nt);
@@ -828,6 +837,8 @@ struct LossPair {
 // taken off. A warp per row.
 __global__ void __launch_bounds__(256) loss_scales_kernel(SplitCopy g, const float2* part, const float2* stat,
                                                           const int32_t* targets, int vocab, float grad_scale) {
+  let_next();
+  after_previous();
   const int row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   if (row >= g.rows) return;
   const int chunks = static_cast<int>(g.chunks());
@@ -919,9 +930,8 @@ int launch_pair(const PairInput& in, const Epi& epi, const PairWork& work, int* 
   }
   const long long tiles = tiles_of(in.M, in.N), units = work.full + (tiles - work.full) * work.splits;
   const int grid = 2 * static_cast<int>(std::min<long long>(units, std::min(kPairs, sm_count() / 2)));
-  kern<<<grid, P_THREADS, P_SMEM, s>>>(in.a, in.b, in.inv_a, in.ld_ia, in.inv_b, in.ld_ib, epi, in.M, in.N, in.steps,
-                                       in.boxes, static_cast<int>(units), work, d_err);
-  check_cuda(cudaGetLastError(), "linear");
+  launch_next("linear", kern, dim3(grid), P_THREADS, P_SMEM, 1, s, in.a, in.b, in.inv_a, in.ld_ia, in.inv_b, in.ld_ib, epi,
+              in.M, in.N, in.steps, in.boxes, static_cast<int>(units), work, d_err);
   return 0;
 }
 
@@ -991,8 +1001,7 @@ bool suits(int M, int N, int K, int steps, int worth, double least) {
 void reduce_parts(const PairInput& in, const PairWork& work, const LinearEpilogue& e, cudaStream_t s) {
   const long long tail = tiles_of(in.M, in.N) - work.full;
   if (!tail) return;
-  reduce_kernel<<<dim3(static_cast<unsigned>(tail), 2 * BM / 4), 256, 0, s>>>(work, e, in.M, in.N);
-  check_cuda(cudaGetLastError(), "linear");
+  launch_next("linear", reduce_kernel, dim3(static_cast<unsigned>(tail), 2 * BM / 4), 256, 0, 1, s, work, e, in.M, in.N);
 }
 
 long long copy_data_bytes(int rows, int k) { return rows * ((k + 127ll) / 128) * 512; }
@@ -1023,8 +1032,8 @@ void split(const SplitBackward& src, int rows, int cols, const SplitCopy* by_row
 void loss_scales(const SplitCopy& g, const float2* part, const float2* stat, const int32_t* targets, int vocab,
                  float grad_scale, cudaStream_t s) {
   if (g.rows <= 0) return;
-  loss_scales_kernel<<<(g.rows + 7) / 8, 256, 0, s>>>(g, part, stat, targets, vocab, grad_scale);
-  check_cuda(cudaGetLastError(), "loss gradient");
+  launch_next("loss gradient", loss_scales_kernel, dim3((g.rows + 7) / 8), 256, 0, 1, s, g, part, stat, targets, vocab,
+              grad_scale);
 }
 
 void split_transposed(const SplitCopy& src, const SplitCopy& by_cols, cudaStream_t s) {
@@ -1049,9 +1058,8 @@ void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_
   }
   const long long n = tiles(x_rows, x_cols) + tiles(y_rows, y_cols);
   if (n > INT32_MAX) throw std::invalid_argument("a matrix is too large");
-  split_two_kernel<<<static_cast<unsigned>(n), 256, smem, s>>>(job(x, x_rows, x_cols, x_by_rows, x_by_cols),
-                                                               job(y, y_rows, y_cols, y_by_rows, y_by_cols));
-  check_cuda(cudaGetLastError(), "split");
+  launch_next("split", split_two_kernel, dim3(static_cast<unsigned>(n)), 256, smem, 1, s,
+              job(x, x_rows, x_cols, x_by_rows, x_by_cols), job(y, y_rows, y_cols, y_by_rows, y_by_cols));
 }
 
 long long pair_ws_bytes(int M, int N, int K) { return parts_bytes(M, N, (K + 127) / 128, kWorthExact); }
