@@ -181,8 +181,9 @@ __global__ void __launch_bounds__(DirectTile<TERMS>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  const bool late = epi.late();
+  if (!late) after_previous();
   let_next();
-  after_previous();
   const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
   const uint32_t tmem_a = tmem_base + 2 * BN;  // three terms: A's stages
   float2* halves = reinterpret_cast<float2*>(smem + BM * BN * 4);  // behind the partial tile
@@ -372,11 +373,13 @@ __global__ void __launch_bounds__(DirectTile<TERMS>::THREADS, 1)
     tmem_dealloc(tmem_base, TL::TMEM_COLS);
   }
   __syncthreads();
+  if (late) after_previous();
 }
 
 struct LinearDirect {
   LinearEpilogue e;
   static constexpr bool kOwnSums = false;
+  __device__ __forceinline__ bool late() const { return e.late; }
   __device__ __forceinline__ LinearDirect slice(long long offset) const {
     LinearDirect d = *this;
     d.e.C += offset;
@@ -450,6 +453,7 @@ struct LinearDirect {
 struct LossDirect {
   LossEpilogue e;
   static constexpr bool kOwnSums = true;
+  __device__ __forceinline__ bool late() const { return false; }
   __device__ __forceinline__ LossDirect slice(long long) const { return *this; }
   // One part: the summing warps hold the row already, half of it each (lane = row): their
   // maximum and sum in registers, the halves joined through shared memory.
@@ -589,8 +593,8 @@ template <int MT, bool B_MN>
 __global__ void __launch_bounds__(256, few_blocks(MT))
     few_rows_kernel(const float* a, long long lda, const float* b, long long ldb, LinearEpilogue e, int M, int N, int K,
                     int splits, int slices, long long slice_stride) {
+  if (!e.late) after_previous();
   let_next();
-  after_previous();
   __shared__ __align__(16) float as[kFewPiece * MT];
   __shared__ __align__(16) float sums[(B_MN ? 8 : 1) * MT * kFewCols];  // [warps][MT][32], then [MT][32]
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -723,14 +727,15 @@ __global__ void __launch_bounds__(256, few_blocks(MT))
     linear_quad(e, e.act, drop, drop ? e.drop.rng[0] : 0, drop ? e.drop.rng[1] : 0, row, col, N, v, bias, r);
   }
   if (splits > 1) cluster_sync();  // a peer may still be reading this CTA's part
+  if (e.late) after_previous();
 }
 
 // ------------------------------------------------------------------ K slices
 // The slices' sums [slices][M, ld], in slice order, and the epilogue: a thread per quad.
 __global__ void __launch_bounds__(256) join_kernel(const float* parts, int slices, long long slice_stride,
                                                    long long ld, const LinearEpilogue e, int M, int N) {
-  let_next();
   after_previous();
+  let_next();
   const int quads = (N + 3) / 4;
   const long long i = blockIdx.x * 256ll + threadIdx.x, row = i / quads;
   const int col = 4 * static_cast<int>(i - row * quads);
@@ -760,8 +765,8 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long
                                                            long long ldz, int act, DropoutArgs drop, int rows,
                                                            int cols, int block_rows, float* dz, long long lddz,
                                                            float* part) {
-  let_next();
   after_previous();
+  let_next();
   __shared__ float4 sums[8][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int across = (cols + 127) / 128, band = static_cast<int>(blockIdx.x) / across;
@@ -808,8 +813,8 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const float* dc, long
 // 32 columns per block, eight rows of partials at a time, joined in a fixed order.
 __global__ void __launch_bounds__(256) sum_parts_kernel(const float* part, int parts, int cols, float* out,
                                                         int accumulate) {
-  let_next();
   after_previous();
+  let_next();
   __shared__ double sums[8][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, col = blockIdx.x * 32 + lane;
   double s = 0.0;
@@ -835,8 +840,8 @@ template <bool VEC, int U, class Index>
 __global__ void __launch_bounds__(256) dropout_kernel(const float* x, long long ldx, const float* r, long long ldr,
                                                       float* y, long long ldy, Index quads, int cols,
                                                       DropoutArgs drop) {
-  let_next();
   after_previous();
+  let_next();
   const uint64_t seed = drop.rng ? drop.rng[0] : 0, offset = drop.rng ? drop.rng[1] : 0;
   const Index step = static_cast<Index>(gridDim.x) * 256;
   for (long long first = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; first < quads; first += U * step) {
@@ -1010,6 +1015,7 @@ int direct_product(int M, int N, int K, GemmOperand A, GemmOperand B, const Line
   LinearEpilogue raw;  // a slice's sums as they are
   raw.C = static_cast<float*>(ws);
   raw.ldc = (N + 3ll) & ~3ll;
+  raw.late = e.late;
   const LinearEpilogue& out = cut.slices > 1 ? raw : e;
   if (M <= kFewRows && !A.mn_major) {
     if (M == 1) launch_few<1>(M, N, K, A, B, out, cut, s);

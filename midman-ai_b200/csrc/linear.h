@@ -28,6 +28,7 @@ struct LinearEpilogue {
   long long ldz = 0;
   float* C = nullptr;
   long long ldc = 0;
+  bool late = false;  // needs nothing of the launch before it: may run beside it (linear_epi.cuh)
 };
 
 // One 128-column tile's share of a row's softmax: the maximum of its logits and

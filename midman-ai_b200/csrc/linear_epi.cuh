@@ -16,10 +16,15 @@ namespace mm {
 // ends, so that its launch and its prologue are hidden (1 to 2 us a launch, of calls that
 // make four to eight short ones). Every thread of every kernel here waits for the one
 // before it to be complete and visible (`after_previous`) before it touches global
-// memory, so completion passes along the chain; kernels launched in any other way wait
-// for everything before them as ever. (So nothing is loaded as read-only for the
-// kernel's lifetime: that begins before the kernel that wrote it ends.) `let_next` comes once the CTA holds all that it
-// allocates, so a waiting CTA of the next kernel never holds what this one needs.
+// memory, then lets the next start (`let_next`); kernels launched in any other way wait
+// for everything before them as ever. So completion passes along the chain, and when a
+// kernel starts, everything before its predecessor is complete. (Nothing is loaded as
+// read-only for the kernel's lifetime, which begins before the one that wrote it ends.)
+//
+// A product that needs nothing of its predecessor, only of what came before that, may run
+// beside it (`late`): it lets the next start at once and waits at its end, when it holds
+// no tensor memory, so that its completion still means that of everything before it.
+// Several in a row may need what came before the last kernel that waits at its start.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -43,7 +43,8 @@ struct Plan {
   float* z;
   float* x;                                  // direct: the live rows of x
   SplitCopy w, wt, xr, xt, g, gt;            // pair: [vocab, dim], [dim, vocab], and of a block [n, dim], [dim, n],
-  void *xr_at, *xt_at, *g_at, *gt_at, *parts;  // [n, vocab], [vocab, n] (a block may be shorter)
+  void *xr_at, *xt_at, *g_at, *gt_at;        // [n, vocab], [vocab, n] (a block may be shorter)
+  void *parts_dx, *parts_dw;                 // of the gradients' products, which may run side by side
   long long bytes;
 };
 
@@ -99,26 +100,22 @@ Plan plan_of(int rows, int vocab, int dim, bool dx, bool dw, bool exact, void* w
       p.xt_at = at.take(split_copy_bytes(dim, p.rows));
       p.gt_at = at.take(split_copy_bytes(vocab, p.rows));
     }
-    // the last block may be shorter: its products may be cut into parts that the others are not
-    const int last = static_cast<int>(n - (blocks - 1) * p.rows);
-    long long parts = 0;
-    for (const int r : {p.rows, std::max(last, 1)}) {
-      if (dx) parts = std::max(parts, pair_ws_bytes(r, dim, vocab));
-      if (dw) parts = std::max({parts, pair_ws_bytes(vocab, dim, r), pair_ws_bytes(dim, vocab, r)});
-    }
-    p.parts = at.take(parts);
   } else {
     if (grad) p.z = static_cast<float*>(at.take(p.rows * p.ldz * 4));
     if (dw) p.x = static_cast<float*>(at.take(p.rows * p.ldx * 4));
-    const int last = static_cast<int>(n - (blocks - 1) * p.rows);
-    long long parts = 0;
-    for (const int r : {p.rows, std::max(last, 1)}) {
-      if (dx) parts = std::max(parts, plain_ws_bytes(r, dim, vocab, false, exact));
-      if (dw)
-        parts = std::max({parts, plain_ws_bytes(vocab, dim, r, true, exact), plain_ws_bytes(dim, vocab, r, true, exact)});
-    }
-    p.parts = at.take(parts);
   }
+  // the last block may be shorter: its products may be cut into parts that the others are not
+  const int last = static_cast<int>(n - (blocks - 1) * p.rows);
+  auto parts = [&](int M, int N, int K, bool a_mn_major) {
+    return p.pair ? pair_ws_bytes(M, N, K) : plain_ws_bytes(M, N, K, a_mn_major, exact);
+  };
+  long long most_dx = 0, most_dw = 0;
+  for (const int r : {p.rows, std::max(last, 1)}) {
+    if (dx) most_dx = std::max(most_dx, parts(r, dim, vocab, false));
+    if (dw) most_dw = std::max({most_dw, parts(vocab, dim, r, true), parts(dim, vocab, r, true)});
+  }
+  p.parts_dx = at.take(most_dx);
+  p.parts_dw = at.take(most_dw);
   p.bytes = at.at;
   return p;
 }
@@ -149,8 +146,8 @@ __device__ __forceinline__ float loss_of(MaxSum a, int t, int vocab, const float
 __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int tiles, const float* zt,
                                                        const int32_t* targets, int rows, int vocab,
                                                        float grad_scale, float* row_loss, float2* stat, int* err) {
-  let_next();
   after_previous();
+  let_next();
   const int r = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   if (r >= rows) return;
   MaxSum a{-INFINITY, 0.0f};
@@ -180,8 +177,8 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
                                                         float grad_scale, float* row_loss, const float* x,
                                                         long long ldx, int dim, float* live_x, long long ldl,
                                                         int* err) {
-  let_next();
   after_previous();
+  let_next();
   __shared__ MaxSum warps[8];
   const int r = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int t = targets[r];
@@ -230,8 +227,8 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
 // The mean over the rows that have a target (0 when none has), in f64.
 __global__ void __launch_bounds__(1024) mean_live_kernel(const float* row_loss, const int32_t* targets, int rows,
                                                          float* mean) {
-  let_next();
   after_previous();
+  let_next();
   __shared__ double sums[32];
   __shared__ int counts[32];
   double s = 0.0;
@@ -281,8 +278,13 @@ void copy_operands(const LinearLoss& a, const Plan& p, long long r0, int n, cons
     split_two(w, a.vocab, a.dim, &p.w, wt, x, n, a.dim, &p.xr, xt, s);
 }
 
-// One block of rows on copies.
-int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cudaStream_t s) {
+void mean_loss(const LinearLoss& a, cudaStream_t s) {
+  launch_next("mean loss", mean_live_kernel, dim3(1), 1024, 0, 1, s, a.row_loss, a.targets, a.rows, a.mean_loss);
+}
+
+// One block of rows on copies. The mean, once the last block's losses are there, and the
+// gradients' products need one another's results neither, so they run side by side.
+int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, bool mean, int* d_err, cudaStream_t s) {
   const int32_t* t = a.targets + r0;
   // For gradients x's rows without a target count as zeros: their logits are not used, but
   // their exponentials are multiplied by 0 for dx, and dw sums over all rows, and 0 times
@@ -311,12 +313,14 @@ int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cu
     p.gt = split_copy_at(p.gt_at, a.vocab, n);
     split_transposed(p.g, p.gt, s);
   }
+  if (mean) mean_loss(a, s);
   if (a.dx) {
     LinearEpilogue o;
     o.C = a.dx + r0 * a.lddx;
     o.R = a.accumulate ? o.C : nullptr;
     o.ldc = o.ldr = a.lddx;
-    rc = pair_product(p.g, p.wt, o, p.parts, d_err, s);
+    o.late = mean;
+    rc = pair_product(p.g, p.wt, o, p.parts_dx, d_err, s);
     if (rc) return rc;
   }
   if (a.dw) {
@@ -324,7 +328,9 @@ int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cu
     o.C = a.dw;
     o.R = a.accumulate || r0 > 0 ? a.dw : nullptr;
     o.ldc = o.ldr = a.lddw;
-    rc = a.w_mn_major ? pair_product(p.xt, p.gt, o, p.parts, d_err, s) : pair_product(p.gt, p.xt, o, p.parts, d_err, s);
+    o.late = mean || a.dx;
+    rc = a.w_mn_major ? pair_product(p.xt, p.gt, o, p.parts_dw, d_err, s)
+                      : pair_product(p.gt, p.xt, o, p.parts_dw, d_err, s);
   }
   return rc;
 }
@@ -332,7 +338,7 @@ int pair_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cu
 // One block of rows on direct products: G takes the logits' place. Where rows and classes
 // are many but the rows short, the logits have the tiles for a pair product and the
 // gradients do not.
-int direct_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, cudaStream_t s) {
+int direct_block(const LinearLoss& a, Plan& p, long long r0, int n, bool mean, int* d_err, cudaStream_t s) {
   const float* x = a.x + r0 * a.ldx;
   const int32_t* t = a.targets + r0;
   const LossEpilogue e{p.z, p.ldz, p.part, p.tiles, t, p.zt, nullptr, 0};
@@ -353,23 +359,26 @@ int direct_block(const LinearLoss& a, Plan& p, long long r0, int n, int* d_err, 
   const dim3 grid(n, static_cast<unsigned>((p.ldz + kSegment - 1) / kSegment));
   launch_next("loss gradient", loss_grad_kernel, grid, 256, 0, 1, s, p.z, p.ldz, p.part, p.tiles, p.zt, t, a.vocab,
               a.grad_scale, a.row_loss + r0, x, a.ldx, a.dim, a.dw ? p.x : nullptr, p.ldx, d_err);
-  if (a.dx) {
-    LinearEpilogue o;
-    o.C = a.dx + r0 * a.lddx;
-    o.R = a.accumulate ? o.C : nullptr;
-    o.ldc = o.ldr = a.lddx;
-    rc = plain_product(n, a.dim, a.vocab, {p.z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, p.parts, d_err,
-                       s);
-    if (rc) return rc;
-  }
+  if (mean) mean_loss(a, s);
   if (a.dw) {
     LinearEpilogue o;
     o.C = a.dw;
     o.R = a.accumulate || r0 > 0 ? a.dw : nullptr;
     o.ldc = o.ldr = a.lddw;
+    o.late = mean;
     const GemmOperand g{p.z, p.ldz, true}, xo{p.x, p.ldx, true};
-    rc = a.w_mn_major ? plain_product(a.dim, a.vocab, n, xo, g, o, a.exact, p.parts, d_err, s)
-                      : plain_product(a.vocab, a.dim, n, g, xo, o, a.exact, p.parts, d_err, s);
+    rc = a.w_mn_major ? plain_product(a.dim, a.vocab, n, xo, g, o, a.exact, p.parts_dw, d_err, s)
+                      : plain_product(a.vocab, a.dim, n, g, xo, o, a.exact, p.parts_dw, d_err, s);
+    if (rc) return rc;
+  }
+  if (a.dx) {
+    LinearEpilogue o;
+    o.C = a.dx + r0 * a.lddx;
+    o.R = a.accumulate ? o.C : nullptr;
+    o.ldc = o.ldr = a.lddx;
+    o.late = mean || a.dw;
+    rc = plain_product(n, a.dim, a.vocab, {p.z, p.ldz, false}, {a.w, a.ldw, !a.w_mn_major}, o, a.exact, p.parts_dx,
+                       d_err, s);
   }
   return rc;
 }
@@ -381,12 +390,11 @@ int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
   Plan p = plan_of(a.rows, a.vocab, a.dim, grad, grad, a.exact, ws);
   for (long long r0 = 0; r0 < a.rows; r0 += p.rows) {
     const int n = static_cast<int>(std::min<long long>(p.rows, a.rows - r0));
-    const int rc = p.pair ? pair_block(a, p, r0, n, d_err, s) : direct_block(a, p, r0, n, d_err, s);
+    const bool mean = a.mean_loss && grad && r0 + n == a.rows;
+    const int rc = p.pair ? pair_block(a, p, r0, n, mean, d_err, s) : direct_block(a, p, r0, n, mean, d_err, s);
     if (rc) return rc;
   }
-  if (a.mean_loss) {
-    launch_next("mean loss", mean_live_kernel, dim3(1), 1024, 0, 1, s, a.row_loss, a.targets, a.rows, a.mean_loss);
-  }
+  if (a.mean_loss && !grad) mean_loss(a, s);
   return 0;
 }
 

@@ -35,7 +35,7 @@ ForwardPlan forward_plan(int m, int n, int k, bool exact, void* ws) {
 struct BackwardPlan {
   bool pair;
   SplitCopy dz, dzt, at, b;  // [m, n], [n, m], [k, m], [k, n]
-  void* parts;               // of one product at a time
+  void *parts_da, *parts_db;  // of the products, which may run side by side
   float* dz_f32;
   float* sums;
   long long bytes;
@@ -49,11 +49,12 @@ BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
     p.dzt = at.copy(n, m);
     p.at = at.copy(k, m);
     p.b = at.copy(k, n);
-    p.parts = at.take(std::max(pair_ws_bytes(m, k, n), pair_ws_bytes(k, n, m)));
+    p.parts_da = at.take(pair_ws_bytes(m, k, n));
+    p.parts_db = at.take(std::max(pair_ws_bytes(k, n, m), pair_ws_bytes(n, k, m)));
   } else {
     p.dz_f32 = static_cast<float*>(at.take(m * round4(n) * 4));
-    p.parts = at.take(std::max({plain_ws_bytes(m, k, n, false, exact), plain_ws_bytes(k, n, m, true, exact),
-                                plain_ws_bytes(n, k, m, true, exact)}));
+    p.parts_da = at.take(plain_ws_bytes(m, k, n, false, exact));
+    p.parts_db = at.take(std::max(plain_ws_bytes(k, n, m, true, exact), plain_ws_bytes(n, k, m, true, exact)));
   }
   const long long parts = std::max(act_backward_parts(m, n), split_parts(m));
   p.sums = static_cast<float*>(at.take(parts * n * 4));
@@ -123,10 +124,11 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
       split(b, br, bc, b_rows, b_cols, s);
     else if (f.db)
       split(a, f.m, f.k, nullptr, &p.at, s);
-    if (f.da) rc = pair_product(p.dz, p.b, da, p.parts, d_err, s);
+    db.late = f.da;
+    if (f.da) rc = pair_product(p.dz, p.b, da, p.parts_da, d_err, s);
     if (f.db && !rc)
-      rc = f.b_mn_major ? pair_product(p.at, p.dzt, db, p.parts, d_err, s)
-                        : pair_product(p.dzt, p.at, db, p.parts, d_err, s);
+      rc = f.b_mn_major ? pair_product(p.at, p.dzt, db, p.parts_db, d_err, s)
+                        : pair_product(p.dzt, p.at, db, p.parts_db, d_err, s);
     return rc;
   }
   const bool plain = f.act == kActNone && !f.drop.rng;  // dz is dc
@@ -135,14 +137,17 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
     act_backward(f.dc, f.lddc, f.z, f.ldz, f.act, f.drop, f.m, f.n, plain ? nullptr : p.dz_f32, ldz,
                  f.dbias ? p.sums : nullptr, s);
   if (f.dbias) sum_parts(p.sums, act_backward_parts(f.m, f.n), f.n, f.dbias, f.accumulate, s);
+  // da beside the bias gradient's sums, db beside da
+  da.late = f.dbias != nullptr;
+  db.late = da.late || f.da;
   const float* g = plain ? f.dc : p.dz_f32;
   const long long ldg = plain ? f.lddc : ldz;
   if (f.da)
-    rc = plain_product(f.m, f.k, f.n, {g, ldg, false}, {f.b, f.ldb, !f.b_mn_major}, da, f.exact, p.parts, d_err, s);
+    rc = plain_product(f.m, f.k, f.n, {g, ldg, false}, {f.b, f.ldb, !f.b_mn_major}, da, f.exact, p.parts_da, d_err, s);
   if (f.db && !rc) {
     const GemmOperand ao{f.a, f.lda, true}, go{g, ldg, true};
-    rc = f.b_mn_major ? plain_product(f.k, f.n, f.m, ao, go, db, f.exact, p.parts, d_err, s)
-                      : plain_product(f.n, f.k, f.m, go, ao, db, f.exact, p.parts, d_err, s);
+    rc = f.b_mn_major ? plain_product(f.k, f.n, f.m, ao, go, db, f.exact, p.parts_db, d_err, s)
+                      : plain_product(f.n, f.k, f.m, go, ao, db, f.exact, p.parts_db, d_err, s);
   }
   return rc;
 }

@@ -225,8 +225,8 @@ __device__ __forceinline__ void split_tile(Source& src, int rows, int cols, cons
 template <class Source>
 __global__ void __launch_bounds__(256, 3) split_kernel(Source src, int rows, int cols, SplitCopy by_rows,
                                                        SplitCopy by_cols, float* part) {
-  let_next();
   after_previous();
+  let_next();
   const int tc = (cols + kTile - 1) / kTile, t = static_cast<int>(blockIdx.x);
   split_tile(src, rows, cols, by_rows, by_cols, part, t / tc, t % tc);
 }
@@ -238,8 +238,8 @@ __global__ void __launch_bounds__(256, 3) split_kernel(Source src, int rows, int
 constexpr int kHalf = 64;
 template <class Source>
 __global__ void __launch_bounds__(256, 6) split_transposed_kernel(Source src, int rows, int cols, SplitCopy by_cols) {
-  let_next();
   after_previous();
+  let_next();
   __shared__ __align__(16) float4 tile[kTile * kHalf / 4];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int tc = (cols + kHalf - 1) / kHalf, tile_r = static_cast<int>(blockIdx.x) / tc;
@@ -271,8 +271,8 @@ struct MatrixJob {
   SplitCopy by_rows, by_cols;
 };
 __global__ void __launch_bounds__(256, 3) split_two_kernel(MatrixJob x, MatrixJob y) {
-  let_next();
   after_previous();
+  let_next();
   const int tiles_x = ((x.rows + kTile - 1) / kTile) * ((x.cols + kTile - 1) / kTile);
   const bool first = static_cast<int>(blockIdx.x) < tiles_x;
   MatrixJob& job = first ? x : y;
@@ -467,8 +467,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
+  const bool late = epi.late();
+  if (!late) after_previous();
   let_next();
-  after_previous();
   const uint32_t tmem_base = *reinterpret_cast<uint32_t*>(tail);
 
   if (warp < P_SUM_WARP) {
@@ -637,6 +638,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 2 * PN);
   }
+  if (late) after_previous();
 }
 
 // A warp's 32 rows (lane = row) x 32 columns through its staging tile: 8 lanes per
@@ -650,6 +652,7 @@ __device__ __forceinline__ void stage_rows(const float* v, float4* stage_tile, i
 template <int ACT, bool DROP>
 struct LinearPair {
   LinearEpilogue e;
+  __device__ __forceinline__ bool late() const { return e.late; }
   // The residual's rows into L2 while the sums form (a row's 128 columns: four lines).
   __device__ __forceinline__ void prefetch(int wrow0, int n0, int M, int N, int lane) const {
     if (!e.R || wrow0 + lane >= M) return;
@@ -719,8 +722,8 @@ struct LinearPair {
 
 // The split tiles: parts summed in order, then the epilogue. Four rows of a tile per block.
 __global__ void __launch_bounds__(256) reduce_kernel(const PairWork work, const LinearEpilogue e, int M, int N) {
-  let_next();
   after_previous();
+  let_next();
   const int tm = (M + 2 * BM - 1) / (2 * BM), tn = (N + PN - 1) / PN;
   int mt, nt;
   pair_tile(work.full + static_cast<int>(blockIdx.x), tm, tn, mt, nt);
@@ -743,6 +746,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const PairWork work, const 
 
 struct LossPair {
   LossEpilogue e;
+  __device__ __forceinline__ bool late() const { return false; }
   __device__ __forceinline__ void prefetch(int, int, int, int, int) const {}
   __device__ __forceinline__ void tile(float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M, int N,
                                        int lane) const {
@@ -837,8 +841,8 @@ struct LossPair {
 // taken off. A warp per row.
 __global__ void __launch_bounds__(256) loss_scales_kernel(SplitCopy g, const float2* part, const float2* stat,
                                                           const int32_t* targets, int vocab, float grad_scale) {
-  let_next();
   after_previous();
+  let_next();
   const int row = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   if (row >= g.rows) return;
   const int chunks = static_cast<int>(g.chunks());

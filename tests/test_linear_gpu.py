@@ -531,6 +531,52 @@ def test_two_streams_at_once(mm, sizes):
 
 
 @pytest.mark.parametrize("sizes", SIZES)
+def test_calls_back_to_back_on_one_workspace(mm, sizes):
+    """Launches overlap: nothing of a call may start before what it reads is there, or write what is still read."""
+    pair = [tensors_for(mm, seed, *sizes) for seed in (1, 2)]
+    pair[1]["ws"] = pair[0]["ws"]
+    names = ("c", "z", "loss", "mean", "dc", "dw", "da", "db", "dbias", "y")
+    m, k, n, v = sizes[:4]
+    kw = dict(rows=m, vocab=v, dim=n, ldx=n, ldw=n, grad_scale=1 / m, precision=sizes[4], workspace=pair[0]["ws"])
+    # The loss without gradients joins a row's sums in another order than the loss with them: outputs of its own
+    names += ("alone", "mean alone")
+    want = []
+    for s in pair:
+        s["alone"], s["mean alone"] = torch.empty(m, device="cuda"), torch.empty(1, device="cuda")
+        all_of_them(mm, s)
+        torch.cuda.synchronize()
+        mm.linear_cross_entropy(s["c"], s["w"], s["t"], s["alone"], mean_loss=s["mean alone"], **kw)
+        torch.cuda.synchronize()
+        want.append([s[o].clone() for o in names])
+    one_by_one = []
+    for s in pair:  # a gradient alone, with the mean and without, the loss alone
+        for grads in (dict(dx="dc"), dict(dw="dw"), dict(dx="dc", dw="dw"), {}):
+            for mean in (True, False):
+                one_by_one.append((s, {a: s[t] for a, t in grads.items()}, mean))
+    for s in pair:
+        for o in names:
+            s[o].zero_()
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for s in pair:
+            all_of_them(mm, s)
+    for s, grads, mean in one_by_one:
+        mm.linear_cross_entropy(s["c"], s["w"], s["t"], s["loss"] if grads else s["alone"], **grads, lddx=n, lddw=n,
+                                mean_loss=(s["mean"] if grads else s["mean alone"]) if mean else None, **kw)
+        bw = dict(m=m, n=n, k=k, lda=k, ldb=n, lddc=n, activation=2, p=0.1, rng=s["rng"], z=s["z"], ldz=n, precision=sizes[4],
+                  workspace=pair[0]["ws"])
+        mm.linear_backward(s["a"], s["b"], s["dc"], da=s["da"], ldda=k, **bw)
+        mm.linear_backward(s["a"], s["b"], s["dc"], db=s["db"], lddb=n, dbias=s["dbias"], **bw)
+        mm.linear_backward(s["a"], s["b"], s["dc"], dbias=s["dbias"], **bw)
+        mm.dropout(s["da"], s["y"], rows=m, cols=k, ldx=k, ldy=k, p=0.1, rng=s["rng"])
+    torch.cuda.synchronize()
+    for s, w in zip(pair, want):
+        for o, x in zip(names, w):
+            assert torch.equal(s[o], x), o
+    mm.device_status()
+
+
+@pytest.mark.parametrize("sizes", SIZES)
 def test_captured_and_replayed(mm, sizes):
     s, other = tensors_for(mm, 1, *sizes), tensors_for(mm, 2, *sizes)
     all_of_them(mm, s)
