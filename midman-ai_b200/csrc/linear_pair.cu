@@ -18,8 +18,8 @@
 // rows, transposed, or both, so that every product reads K-major operands; the
 // loss's logits leave their product as a copy. The passes are bound by HBM: 4 bytes
 // read per value (8 for dz), 4 written per copy (8192 x 5632 and 5632 x 2048 in one
-// launch 82 us, 5.6 TB/s; dz of 8192 x 5632 by rows and transposed with the column sums
-// 158 us, 4.7 TB/s).
+// launch 77 us, 6.0 TB/s; dz of 8192 x 5632 by rows and transposed with the column sums
+// 148 us, 5.0 TB/s).
 //
 // Measured, copies aside: 8192 x 2048 x 5632 366 us (516 TFLOP/s of the product, 1,550 of
 // f16 executed; the 3xTF32 products of gemm.cu take 730 us), 8192 x 1024 -> 2816 with
@@ -46,7 +46,8 @@ namespace {
 
 // ------------------------------------------------------------------ split
 constexpr int kTile = 128;
-constexpr int kSplitSums = 8 * kTile * 4;  // the warps' column sums
+constexpr int kSplitWarps = 16;
+constexpr int kSplitSums = kSplitWarps * kTile * 4;  // the warps' column sums
 constexpr int kSplitSmem = kSplitSums + kTile * kTile * 4;
 
 // The power of two for a chunk whose largest magnitude has the bits m: [2^14, 2^15)
@@ -74,7 +75,6 @@ __device__ __forceinline__ void halves(float x, float y, uint32_t& hi, uint32_t&
 
 // Sources: begin once, then load of a row's four columns.
 struct MatrixSource {
-  static constexpr int ROWS = 4;
   SplitMatrix a;
   __device__ __forceinline__ void begin() {}
   __device__ __forceinline__ float4 load(long long row, int col, int cols) const {
@@ -87,7 +87,6 @@ struct MatrixSource {
   }
 };
 struct BackwardSource {
-  static constexpr int ROWS = 4;
   SplitBackward a;
   uint64_t seed, offset;
   __device__ __forceinline__ void begin() {
@@ -106,7 +105,6 @@ struct BackwardSource {
   }
 };
 struct CopySource {  // a copy's values again, scale and all
-  static constexpr int ROWS = 8;
   SplitCopy a;
   __device__ __forceinline__ void begin() {}
   __device__ __forceinline__ float4 load(long long row, int col, int) const {  // zeros past k, as the copy has
@@ -127,12 +125,12 @@ struct CopySource {  // a copy's values again, scale and all
 // r W / 4 + (q ^ (r / 8 & 7)): a warp takes a quad of columns, lane (c, j) column c and
 // rows 8 j.. of each 64 (eight j in eight different bank groups, so neither side has
 // conflicts), which are the 16 bytes of hi and of lo that it stores.
-template <int W>
+template <int W, int WARPS>
 __device__ __forceinline__ void split_columns(const float* tile, int cols, const SplitCopy& by_cols, int tile_r,
                                               int c0) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, c = lane & 3, j = lane >> 2;
 #pragma unroll 1
-  for (int q = warp; q < W / 4 && c0 + 4 * q < cols; q += 8) {
+  for (int q = warp; q < W / 4 && c0 + 4 * q < cols; q += WARPS) {
     const float* t = tile + 4 * (q ^ j) + c;
     float v[16];
     uint32_t m = 0;
@@ -160,31 +158,33 @@ __device__ __forceinline__ void split_columns(const float* tile, int cols, const
   }
 }
 
-// One 128 x 128 tile per block. By rows: a warp per row (16 each), a lane four columns.
-// By columns: through shared memory.
+// One 128 x 128 tile per block. By rows: a warp per row (8 each), a lane four columns. By
+// columns: through shared memory. Two blocks of 16 warps on an SM keep more loads in
+// flight than three of eight (8192 x 5632 with 5632 x 2048 by columns 77 us against 83, dz
+// by rows and columns 148 against 158; by rows alone 36.5 against 35.2).
 template <class Source>
 __device__ __forceinline__ void split_tile(Source& src, int rows, int cols, const SplitCopy& by_rows,
                                            const SplitCopy& by_cols, float* part, int tile_r, int tile_c) {
   extern __shared__ __align__(16) float split_smem[];
-  float* sums = split_smem;                                            // [8][128]
-  float4* tile = reinterpret_cast<float4*>(split_smem + 8 * kTile);    // where the columns are wanted
+  float* sums = split_smem;  // [warps][128]
+  float4* tile = reinterpret_cast<float4*>(split_smem + kSplitWarps * kTile);  // where the columns are wanted
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int r0 = tile_r * kTile, c0 = tile_c * kTile;
   const int col = c0 + 4 * lane;
   src.begin();
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  constexpr int U = Source::ROWS;  // rows of a warp in flight
+  constexpr int U = 4;  // rows of a warp in flight
 #pragma unroll 1
-  for (int i0 = 0; i0 < kTile / 8; i0 += U) {
+  for (int i0 = 0; i0 < kTile / kSplitWarps; i0 += U) {
     float4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long row = r0 + 8 * (i0 + u) + warp;
+      const long long row = r0 + kSplitWarps * (i0 + u) + warp;
       v[u] = row < rows && col < cols ? src.load(row, col, cols) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = 8 * (i0 + u) + warp;
+      const int r = kSplitWarps * (i0 + u) + warp;
       const long long row = r0 + r;
       if (by_cols.data) tile[r * 32 + (lane ^ ((r >> 3) & 7))] = v[u];
       if (part) {
@@ -213,17 +213,17 @@ __device__ __forceinline__ void split_tile(Source& src, int rows, int cols, cons
     __syncthreads();
     if (threadIdx.x < kTile && c0 + static_cast<int>(threadIdx.x) < cols) {
       float s = 0.0f;
-      for (int k = 0; k < 8; ++k) s += sums[k * kTile + threadIdx.x];
+      for (int k = 0; k < kSplitWarps; ++k) s += sums[k * kTile + threadIdx.x];
       part[static_cast<long long>(tile_r) * cols + c0 + threadIdx.x] = s;
     }
   }
   if (!by_cols.data) return;
   __syncthreads();
-  split_columns<kTile>(split_smem + 8 * kTile, cols, by_cols, tile_r, c0);
+  split_columns<kTile, kSplitWarps>(split_smem + kSplitWarps * kTile, cols, by_cols, tile_r, c0);
 }
 
 template <class Source>
-__global__ void __launch_bounds__(256, 3) split_kernel(Source src, int rows, int cols, SplitCopy by_rows,
+__global__ void __launch_bounds__(32 * kSplitWarps, 2) split_kernel(Source src, int rows, int cols, SplitCopy by_rows,
                                                        SplitCopy by_cols, float* part) {
   after_previous();
   let_next();
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(256, 6) split_transposed_kernel(Source src, in
     }
   }
   __syncthreads();
-  split_columns<kHalf>(reinterpret_cast<const float*>(tile), cols, by_cols, tile_r, c0);
+  split_columns<kHalf, 8>(reinterpret_cast<const float*>(tile), cols, by_cols, tile_r, c0);
 }
 
 // Two matrices in one launch (a product's operands): the first's tiles, then the second's.
@@ -270,7 +270,7 @@ struct MatrixJob {
   int rows, cols;
   SplitCopy by_rows, by_cols;
 };
-__global__ void __launch_bounds__(256, 3) split_two_kernel(MatrixJob x, MatrixJob y) {
+__global__ void __launch_bounds__(32 * kSplitWarps, 2) split_two_kernel(MatrixJob x, MatrixJob y) {
   after_previous();
   let_next();
   const int tiles_x = ((x.rows + kTile - 1) / kTile) * ((x.cols + kTile - 1) / kTile);
@@ -282,16 +282,19 @@ __global__ void __launch_bounds__(256, 3) split_two_kernel(MatrixJob x, MatrixJo
 }
 
 template <class Source>
+void launch_transposed(const Source& src, int rows, int cols, const SplitCopy& by_cols, cudaStream_t s) {
+  if (rows <= 0 || cols <= 0) return;
+  const long long tiles = ((rows + kTile - 1ll) / kTile) * ((cols + kHalf - 1ll) / kHalf);
+  if (tiles > INT32_MAX) throw std::invalid_argument("a matrix is too large");
+  launch_next("split", split_transposed_kernel<Source>, dim3(static_cast<unsigned>(tiles)), 256, 0, 1, s, src, rows,
+              cols, by_cols);
+}
+
+template <class Source>
 void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_rows, const SplitCopy* by_cols,
                   float* part, cudaStream_t s) {
   if (rows <= 0 || cols <= 0) return;
-  if (by_cols && !by_rows && !part) {
-    const long long tiles = ((rows + kTile - 1ll) / kTile) * ((cols + kHalf - 1ll) / kHalf);
-    if (tiles > INT32_MAX) throw std::invalid_argument("a matrix is too large");
-    launch_next("split", split_transposed_kernel<Source>, dim3(static_cast<unsigned>(tiles)), 256, 0, 1, s, src, rows, cols,
-                *by_cols);
-    return;
-  }
+  if (by_cols && !by_rows && !part) return launch_transposed(src, rows, cols, *by_cols, s);
   auto kern = split_kernel<Source>;
   static thread_local int configured_device = -1;
   int dev = 0;
@@ -303,8 +306,8 @@ void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_row
   const long long tiles = ((rows + kTile - 1ll) / kTile) * ((cols + kTile - 1ll) / kTile);
   if (tiles > INT32_MAX) throw std::invalid_argument("a matrix is too large");
   const SplitCopy none{};
-  launch_next("split", kern, dim3(static_cast<unsigned>(tiles)), 256, by_cols ? kSplitSmem : kSplitSums, 1, s, src, rows,
-              cols, by_rows ? *by_rows : none, by_cols ? *by_cols : none, part);
+  launch_next("split", kern, dim3(static_cast<unsigned>(tiles)), 32 * kSplitWarps, by_cols ? kSplitSmem : kSplitSums, 1,
+              s, src, rows, cols, by_rows ? *by_rows : none, by_cols ? *by_cols : none, part);
 }
 
 // ------------------------------------------------------------------ products
@@ -934,8 +937,8 @@ int launch_pair(const PairInput& in, const Epi& epi, const PairWork& work, int* 
   }
   const long long tiles = tiles_of(in.M, in.N), units = work.full + (tiles - work.full) * work.splits;
   const int grid = 2 * static_cast<int>(std::min<long long>(units, std::min(kPairs, sm_count() / 2)));
-  launch_next("linear", kern, dim3(grid), P_THREADS, P_SMEM, 1, s, in.a, in.b, in.inv_a, in.ld_ia, in.inv_b, in.ld_ib, epi,
-              in.M, in.N, in.steps, in.boxes, static_cast<int>(units), work, d_err);
+  launch_next("linear", kern, dim3(grid), P_THREADS, P_SMEM, 1, s, in.a, in.b, in.inv_a, in.ld_ia, in.inv_b, in.ld_ib,
+              epi, in.M, in.N, in.steps, in.boxes, static_cast<int>(units), work, d_err);
   return 0;
 }
 
@@ -1041,7 +1044,7 @@ void loss_scales(const SplitCopy& g, const float2* part, const float2* stat, con
 }
 
 void split_transposed(const SplitCopy& src, const SplitCopy& by_cols, cudaStream_t s) {
-  launch_split(CopySource{src}, src.rows, src.k, nullptr, &by_cols, nullptr, s);
+  launch_transposed(CopySource{src}, src.rows, src.k, by_cols, s);
 }
 
 void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_by_rows, const SplitCopy* x_by_cols,
@@ -1062,7 +1065,7 @@ void split_two(const SplitMatrix& x, int x_rows, int x_cols, const SplitCopy* x_
   }
   const long long n = tiles(x_rows, x_cols) + tiles(y_rows, y_cols);
   if (n > INT32_MAX) throw std::invalid_argument("a matrix is too large");
-  launch_next("split", split_two_kernel, dim3(static_cast<unsigned>(n)), 256, smem, 1, s,
+  launch_next("split", split_two_kernel, dim3(static_cast<unsigned>(n)), 32 * kSplitWarps, smem, 1, s,
               job(x, x_rows, x_cols, x_by_rows, x_by_cols), job(y, y_rows, y_cols, y_by_rows, y_by_cols));
 }
 
