@@ -908,13 +908,17 @@ Cut direct_cut(int M, int N, int K, bool sliced) {
   return best;
 }
 
-// Few rows: parts that all run at once, each at least 256 of K, then slices while one
-// has more than 2048 of it.
+// Few rows: parts that all run at once, each at least 128 of K, then slices while one
+// has more than 2048 of it. Parts by powers of two, which leave whole pieces of K (2048 ->
+// 5632 by [n, k], four rows: two parts 12.6 us, three 13.5), but six where five to eight
+// rows leave no room for eight (8 x 5632 -> 2048 16.6 us, 21.8 in four; 8 x 2048 -> 2048 9.7
+// and 10.2).
 Cut few_cut(int M, int N, int K) {
   const int fit = few_blocks(M <= 4 ? 4 : 8) * 148;
   const long long tiles = (N + kFewCols - 1) / kFewCols;
   Cut c;
-  while (c.splits < 8 && tiles * c.splits * 2 <= fit && K / (2 * c.splits) >= 256) c.splits *= 2;
+  while (c.splits < 8 && tiles * c.splits * 2 <= fit && K / (2 * c.splits) >= 128) c.splits *= 2;
+  if (M > 4 && c.splits == 4 && tiles * 6 <= fit && K / 6 >= 256) c.splits = 6;
   while (tiles * c.splits * c.slices * 2 <= fit && K / (c.splits * c.slices * 2) >= 1024) c.slices *= 2;
   return c;
 }
