@@ -594,6 +594,36 @@ def test_captured_and_replayed(mm, sizes):
     mm.device_status()
 
 
+def test_captured_on_streams_that_part_and_meet(mm):
+    """Overlapping launches beside event waits, copies and fills of a captured graph."""
+    pair = [tensors_for(mm, seed, 300, 96, 200, 1000, 1) for seed in (1, 2)]
+    mm.device_status()
+    want = [[t.clone() for t in all_of_them(mm, s)] for s in pair]
+    torch.cuda.synchronize()
+    kept_a = [s["a"].clone() for s in pair]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        pair[1]["a"].copy_(kept_a[1])
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            all_of_them(mm, pair[1])
+            pair[1]["y"].add_(0)
+        pair[0]["a"].copy_(kept_a[0])
+        all_of_them(mm, pair[0])
+        main.wait_stream(side)
+        mm.dropout(pair[1]["y"], pair[1]["y"], rows=300, cols=96, ldx=96, ldy=96, p=0.0)
+    for s in pair:
+        for o in ("c", "z", "dc", "dw", "da", "db", "y", "a"):
+            s[o].zero_()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for s, w in zip(pair, want):
+        assert all(torch.equal(s[o], x) for o, x in zip(("c", "z", "loss", "mean", "dc", "dw", "da", "db", "dbias", "y"), w))
+    mm.device_status()
+
+
 def test_linear_and_dropout_share_their_mask(mm):
     m, k, n = 50, 20, 70
     words = rng_words(3, 4)
