@@ -767,41 +767,43 @@ struct LossPair {
 #pragma unroll
     for (int i = 0; i < 128; ++i) top[i % 4] = live == 128 || i < live ? fmaxf(top[i % 4], sum[i]) : top[i % 4];
     const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    if (e.copy) {  // the exponentials take the logits' place
-#pragma unroll
-      for (int i = 0; i < 128; ++i) {
-        sum[i] = live == 128 || i < live ? loss_exp(sum[i] - m) : 0.0f;
-        all[i % 4] += sum[i];
-      }
+    if (e.copy) {
+      if (live == 128 && wrow0 + 32 <= M)
+        copy_slices<true>(sum, all, m, live, stage_tile, wrow0, n0, M, lane);
+      else
+        copy_slices<false>(sum, all, m, live, stage_tile, wrow0, n0, M, lane);
     } else {
 #pragma unroll
       for (int i = 0; i < 128; ++i) all[i % 4] += live == 128 || i < live ? loss_exp(sum[i] - m) : 0.0f;
     }
     if (my_row < M) e.part[my_row * e.tiles + n0 / 128] = make_float2(m, (all[0] + all[1]) + (all[2] + all[3]));
-    if (e.copy) {
-      if (wrow0 + 32 <= M)
-        store_copy<true>(sum, stage_tile, wrow0, n0, M, lane);
-      else
-        store_copy<false>(sum, stage_tile, wrow0, n0, M, lane);
-      return;
-    }
+    if (e.copy) return;
     if (!e.Z) return;
     if (wrow0 + 32 <= M && n0 + 128 <= N)
       store<true>(sum, stage_tile, wrow0, n0, M, N, lane);
     else
       store<false>(sum, stage_tile, wrow0, n0, M, N, lane);
   }
-  // The chunk's exponentials, in (0, 1], times 2^14 as hi and lo: the copy that dx's product
-  // reads once its scales (2^-14 exp(m - row maximum) grad_scale / row sum) are known.
+  // The chunk's exponentials, in (0, 1], added up and times 2^14 as hi and lo: the copy that
+  // dx's product reads once its scales (2^-14 exp(m - row maximum) grad_scale / row sum) are
+  // known. A rolled loop over slices of 32 columns, as in LinearPair.
   template <bool FULL>
-  __device__ __forceinline__ void store_copy(const float (&sum)[128], float4* stage_tile, int wrow0, int n0, int M,
-                                             int lane) const {
+  __device__ __forceinline__ void copy_slices(float (&sum)[128], float (&all)[4], float m, int live, float4* stage_tile,
+                                              int wrow0, int n0, int M, int lane) const {
     const int sub = lane & 7, rsub = lane >> 3;
-#pragma unroll
+    uint16_t* row = e.copy + (wrow0 + rsub) * e.copy_ld + (n0 / 128) * 256ll + 4 * sub;
+#pragma unroll 1
     for (int c = 0; c < 4; ++c) {
-      stage_rows(sum + 32 * c, stage_tile, lane);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        sum[i] = FULL || 32 * c + i < live ? loss_exp(sum[i] - m) : 0.0f;
+        all[i % 4] += sum[i];
+      }
+      stage_rows(sum, stage_tile, lane);
+#pragma unroll
+      for (int i = 0; i < 96; ++i) sum[i] = sum[i + 32];
       __syncwarp();
-      uint16_t* out = e.copy + (wrow0 + rsub) * e.copy_ld + (n0 / 128) * 256ll + (c / 2) * 128 + (c % 2) * 32 + 4 * sub;
+      uint16_t* out = row + (c / 2) * 128 + (c % 2) * 32;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int rr = 4 * i + rsub;
