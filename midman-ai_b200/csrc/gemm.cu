@@ -1601,6 +1601,15 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
         q == cudaDriverEntryPointSuccess)
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   });
+  // The encoder needs a current context, which a host thread has from its first runtime call on.
+  static thread_local bool bound = false;
+  if (!bound) {
+    int device = 0;
+    if (cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess)
+      bound = true;
+    else
+      cudaGetLastError();
+  }
   return fn;
 }
 

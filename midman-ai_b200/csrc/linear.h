@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <mutex>
 
 #include "dropout.cuh"
 #include "gemm.h"
@@ -165,6 +166,9 @@ int plain_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& 
                   void* ws, int* d_err, cudaStream_t s);
 int plain_loss_product(int M, int N, int K, const GemmOperand& A, const GemmOperand& B, const LossEpilogue& e,
                        bool exact, int* d_err, cudaStream_t s);
+
+// Held while a call with late products is enqueued (linear_epi.cuh).
+std::mutex& launch_order();
 
 struct LinearForward {
   int m, n, k;

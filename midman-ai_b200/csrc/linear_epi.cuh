@@ -25,6 +25,9 @@ namespace mm {
 // beside it (`late`): it lets the next start at once and waits at its end, when it holds
 // no tensor memory, so that its completion still means that of everything before it.
 // Several in a row may need what came before the last kernel that waits at its start.
+// Which kernels those are must not change between a call's launches, so calls with late
+// products are enqueued one at a time (`launch_order`): another thread's late product on
+// the same stream, put between a kernel and the one that counts on its end, would break it.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -388,6 +388,7 @@ int direct_block(const LinearLoss& a, Plan& p, long long r0, int n, bool mean, i
 int linear_loss(const LinearLoss& a, void* ws, int* d_err, cudaStream_t s) {
   const bool grad = a.dx || a.dw;
   Plan p = plan_of(a.rows, a.vocab, a.dim, grad, grad, a.exact, ws);
+  const std::lock_guard<std::mutex> lock(launch_order());
   for (long long r0 = 0; r0 < a.rows; r0 += p.rows) {
     const int n = static_cast<int>(std::min<long long>(p.rows, a.rows - r0));
     const bool mean = a.mean_loss && grad && r0 + n == a.rows;

@@ -64,6 +64,11 @@ BackwardPlan backward_plan(int m, int n, int k, bool exact, void* ws) {
 
 }  // namespace
 
+std::mutex& launch_order() {
+  static std::mutex m;
+  return m;
+}
+
 long long plain_ws_bytes(int M, int N, int K, bool a_mn_major, bool exact) {
   return !exact && tf32_pair_suits(M, N, K) ? tf32_pair_ws_bytes(M, N, K) : direct_ws_bytes(M, N, K, a_mn_major);
 }
@@ -100,6 +105,7 @@ long long linear_backward_ws_bytes(int m, int n, int k, bool exact) {
 int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t s) {
   if (f.m <= 0) return 0;
   const BackwardPlan p = backward_plan(f.m, f.n, f.k, f.exact, ws);
+  const std::lock_guard<std::mutex> lock(launch_order());
   LinearEpilogue da, db;
   da.C = f.da;
   da.R = f.accumulate ? f.da : nullptr;

@@ -11,6 +11,8 @@ absolute products):
 An activation passes an error on with its slope (at most 1.13) and adds its own: a few ulp of |z| + 1. Dropout multiplies by
 1 / (1 - p), rounded (2^-24) twice.
 """
+import threading
+
 import numpy as np
 import pytest
 
@@ -591,6 +593,51 @@ def test_captured_and_replayed(mm, sizes):
         graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(outs, want))
+    mm.device_status()
+
+
+@pytest.mark.parametrize("m,k,n,precision", [(4, 64, 40, 1), (40, 96, 72, 1), (40, 96, 72, 0), (2304, 512, 2304, 1), (2304, 512, 2304, 0)])
+def test_a_host_thread_whose_first_call_it_is(mm, m, k, n, precision):
+    a, b = torch.randn(m, k, device="cuda"), torch.randn(k, n, device="cuda")
+    c, d = torch.empty(m, n, device="cuda"), torch.empty(m, n, device="cuda")
+    ws = torch.empty(mm.linear_workspace(m, n, k, precision=precision) + 256, dtype=torch.uint8, device="cuda")
+    stream, failed = torch.cuda.current_stream().cuda_stream, []
+    call = [m, n, k, a.data_ptr(), k, b.data_ptr(), n, 1, None, 0, 0.0, None, None, 0, None, 0]
+    end = [n, precision, ws.data_ptr(), ws.numel(), stream]
+    assert mm.load().mm_gpu_linear_forward(*call, c.data_ptr(), *end) == 0
+    thread = threading.Thread(target=lambda: failed.append(mm.load().mm_gpu_linear_forward(*call, d.data_ptr(), *end)))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert failed == [0] and torch.equal(c, d)
+    mm.device_status()
+
+
+@pytest.mark.parametrize("sizes", SIZES)
+def test_two_host_threads_on_one_stream(mm, sizes):
+    pair = [tensors_for(mm, seed, *sizes) for seed in (1, 2)]
+    want = [[t.clone() for t in all_of_them(mm, s)] for s in pair]
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream().cuda_stream
+    start, failed = threading.Barrier(2), []
+
+    def work(s, w):
+        start.wait()
+        try:
+            for _ in range(20):
+                all_of_them(mm, s, stream)
+        except Exception as e:  # noqa: BLE001 - shown by the assertion
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=p) for p in zip(pair, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for s, w in zip(pair, want):
+        assert all(torch.equal(s[o], x) for o, x in zip(("c", "z", "loss", "mean", "dc", "dw", "da", "db", "dbias", "y"), w))
     mm.device_status()
 
 
