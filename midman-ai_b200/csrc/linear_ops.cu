@@ -103,7 +103,7 @@ long long linear_backward_ws_bytes(int m, int n, int k, bool exact) {
 }
 
 int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t s) {
-  if (f.m <= 0) return 0;
+  if (f.m <= 0 || !(f.da || f.db || f.dbias)) return 0;
   const BackwardPlan p = backward_plan(f.m, f.n, f.k, f.exact, ws);
   const std::lock_guard<std::mutex> lock(launch_order());
   LinearEpilogue da, db;
@@ -116,9 +116,8 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
   int rc = 0;
   if (p.pair) {
     // dz goes from dc and z straight into its copies
-    if (f.da || f.db || f.dbias)
-      split(SplitBackward{f.dc, f.lddc, f.z, f.ldz, f.act, f.drop}, f.m, f.n, f.da ? &p.dz : nullptr,
-            f.db ? &p.dzt : nullptr, f.dbias ? p.sums : nullptr, s);
+    split(SplitBackward{f.dc, f.lddc, f.z, f.ldz, f.act, f.drop}, f.m, f.n, f.da ? &p.dz : nullptr,
+          f.db ? &p.dzt : nullptr, f.dbias ? p.sums : nullptr, s);
     if (f.dbias) sum_parts(p.sums, split_parts(f.m), f.n, f.dbias, f.accumulate, s);
     // b [k, n] by rows, or [n, k] by columns, for da; a by columns for db
     const SplitMatrix a{f.a, f.lda}, b{f.b, f.ldb};
@@ -138,9 +137,10 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
     return rc;
   }
   const bool plain = f.act == kActNone && !f.drop.rng;  // dz is dc
+  const bool own_dz = !plain && (f.da || f.db);          // the products read it
   const long long ldz = round4(f.n);
-  if (!plain || f.dbias)
-    act_backward(f.dc, f.lddc, f.z, f.ldz, f.act, f.drop, f.m, f.n, plain ? nullptr : p.dz_f32, ldz,
+  if (own_dz || f.dbias)
+    act_backward(f.dc, f.lddc, f.z, f.ldz, f.act, f.drop, f.m, f.n, own_dz ? p.dz_f32 : nullptr, ldz,
                  f.dbias ? p.sums : nullptr, s);
   if (f.dbias) sum_parts(p.sums, act_backward_parts(f.m, f.n), f.n, f.dbias, f.accumulate, s);
   // da beside the bias gradient's sums, db beside da

@@ -758,6 +758,7 @@ uint64_t mm_op_linear(uint32_t tape, uint64_t x_h, uint64_t w_h, int32_t w_trans
       g.da = grad_of(0);
       g.db = grad_of(1);
       g.dbias = at_bias ? grad_of(at_bias) : nullptr;
+      if (!g.da && !g.db && !g.dbias) return;  // only the residual tracks: no z was kept
       g.accumulate = true;
       g.exact = exact;
       Buf ws = workspace(*tpp, linear_backward_ws_bytes(im, in, ik, exact));

@@ -102,6 +102,24 @@ def test_constants_get_no_gradient(mm, tape):
         tape.backward(tape.linear_cross_entropy(x, w, np.zeros(8, np.int32)))
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 8, 12), (37, 64, 176), (2304, 256, 2304)])  # few rows, direct, pairs
+@pytest.mark.parametrize("act", range(4))
+@pytest.mark.parametrize("p", [0.0, 0.25])
+def test_only_the_residual_tracks(mm, tape, m, k, n, act, p):
+    """Constant input, weight and bias, as of a frozen layer: no z is kept, and the residual's gradient is dc."""
+    rs = np.random.default_rng(m + act)
+    x, w, b = tape.tensor(rs.standard_normal((m, k))), tape.tensor(rs.standard_normal((k, n)) * 0.1), tape.tensor(rs.standard_normal(n))
+    r, head = tape.tensor(rs.standard_normal((m, n)), requires_grad=True), tape.tensor(rs.standard_normal((n, 8)) * 0.1)
+    y = tape.linear(x, w, bias=b, activation=act, p=p, seed=3, offset=1, residual=r)
+    leaf = tape.tensor(tape.read(y), requires_grad=True)
+    targets = (np.arange(m) % 8).astype(np.int32)
+    tape.backward(tape.linear_cross_entropy(y, head, targets))
+    got = tape.grad(r)
+    tape.backward(tape.linear_cross_entropy(leaf, head, targets))
+    assert got.any() and np.array_equal(got, tape.grad(leaf))
+    assert not tape.grad(x).any() and not tape.grad(w).any() and not tape.grad(b).any()
+
+
 def test_refusals(mm, tape):
     x, w = tape.tensor(np.ones((4, 8))), tape.tensor(np.ones((8, 12)))
     odd = tape.tensor(np.ones((8, 6)))
