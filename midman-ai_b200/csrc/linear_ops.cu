@@ -105,6 +105,9 @@ long long linear_backward_ws_bytes(int m, int n, int k, bool exact) {
 int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t s) {
   if (f.m <= 0 || !(f.da || f.db || f.dbias)) return 0;
   const BackwardPlan p = backward_plan(f.m, f.n, f.k, f.exact, ws);
+  // A tensor that is both input and weight has one gradient buffer: then db's product reads
+  // what da's wrote, and waits for it.
+  const bool one_buffer = f.da == f.db;
   const std::lock_guard<std::mutex> lock(launch_order());
   LinearEpilogue da, db;
   da.C = f.da;
@@ -129,7 +132,7 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
       split(b, br, bc, b_rows, b_cols, s);
     else if (f.db)
       split(a, f.m, f.k, nullptr, &p.at, s);
-    db.late = f.da;
+    db.late = f.da && !one_buffer;
     if (f.da) rc = pair_product(p.dz, p.b, da, p.parts_da, d_err, s);
     if (f.db && !rc)
       rc = f.b_mn_major ? pair_product(p.at, p.dzt, db, p.parts_db, d_err, s)
@@ -145,7 +148,7 @@ int linear_backward(const LinearBackward& f, void* ws, int* d_err, cudaStream_t 
   if (f.dbias) sum_parts(p.sums, act_backward_parts(f.m, f.n), f.n, f.dbias, f.accumulate, s);
   // da beside the bias gradient's sums, db beside da
   da.late = f.dbias != nullptr;
-  db.late = da.late || f.da;
+  db.late = (da.late || f.da) && !one_buffer;
   const float* g = plain ? f.dc : p.dz_f32;
   const long long ldg = plain ? f.lddc : ldz;
   if (f.da)

@@ -91,6 +91,30 @@ def test_one_tensor_in_every_place(mm, tape):
     assert rel(tape.grad(x), t.grad) <= tape.tol
 
 
+@pytest.mark.parametrize("n", [64, 256, 1024, 2048])  # one direct tile a product, four, many, pairs
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("bias", [False, True])
+def test_one_tensor_as_input_and_weight(mm, tape, n, transposed, bias):
+    """x x and x x^T: both products add to the one gradient, in an order that does not change from run to run.
+
+    The tolerance is the tape's relative one for the sum of the two products, which are each within it."""
+    rs = np.random.default_rng(n)
+    v = rs.standard_normal((n, n)).astype(np.float32) * np.float32(n ** -0.5)
+    head, targets = rs.standard_normal((n, 8)).astype(np.float32), (np.arange(n) % 8).astype(np.int32)
+    b = np.zeros(n, np.float32)
+    x, w, bh = tape.tensor(v, requires_grad=True), tape.tensor(head), tape.tensor(b, requires_grad=True)
+    loss = tape.linear_cross_entropy(tape.linear(x, x, w_transposed=transposed, bias=bh if bias else 0, activation=mm.ACT_SILU), w, targets)
+    tape.backward(loss)
+    first = tape.grad(x)
+    for _ in range(10):
+        tape.backward(loss)
+        assert np.array_equal(tape.grad(x), first)
+    t = torch.tensor(v, dtype=torch.float64, requires_grad=True)
+    y = torch.nn.functional.silu(t @ (t.T if transposed else t))
+    torch.nn.functional.cross_entropy(y @ torch.tensor(head, dtype=torch.float64), torch.tensor(targets, dtype=torch.long)).backward()
+    assert rel(first, t.grad) <= tape.tol
+
+
 def test_constants_get_no_gradient(mm, tape):
     rs = np.random.default_rng(6)
     x, w = tape.tensor(rs.standard_normal((8, 8))), tape.tensor(rs.standard_normal((8, 8)))
