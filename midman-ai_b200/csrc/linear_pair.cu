@@ -419,6 +419,37 @@ struct Tf32Feed {
   }
 };
 
+// sum += an accumulation's 32 rows x 128 columns with both scales undone: `ia` is this
+// lane's row's inverse, `ib` the columns' (the same for every lane). A chunk's sum is at
+// most 2^37 (128 products of entries up to 2^15), so times a row's inverse it stays below
+// 2^128 up to kSafeInverse, entries of 2^104. WIDE, where a row of the warp has larger
+// ones: the smaller inverse first, so that nothing overflows which the other would bring
+// back (two more instructions a value). What the first factor loses to f32's smallest
+// numbers is at most 2^-24 of a scaled unit, far below the copies' own 2^-25 of one in
+// every entry times the other operand's 2^14.
+constexpr float kSafeInverse = 0x1p90f;
+template <bool WIDE>
+__device__ __forceinline__ void add_chunk(float (&sum)[128], uint32_t acc, float ia, const float4* ib) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(acc + q * 32, r);
+    auto add = [&](int e, float b) {
+      const float v = __uint_as_float(r[e]);
+      float& o = sum[q * 32 + e];
+      o = WIDE ? fmaf(v * fminf(ia, b), fmaxf(ia, b), o) : fmaf(v * ia, b, o);
+    };
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float4 b = ib[q * 8 + e];
+      add(4 * e, b.x);
+      add(4 * e + 1, b.y);
+      add(4 * e + 2, b.z);
+      add(4 * e + 3, b.w);
+    }
+  }
+}
+
 template <class Feed, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const float* inv_a,
@@ -586,22 +617,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
           pb += ld_ib / 4;
           const float ia_next = more ? *pa : 0.0f;
           const float4 ib_next = more ? *pb : make_float4(0.f, 0.f, 0.f, 0.f);
+          const bool wide = __any_sync(0xffffffffu, ia > kSafeInverse);
           ok = wait_acc(&acc);
           if (!ok) break;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(acc + q * 32, r);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 b = ib[q * 8 + e];  // the columns' inverse scales, the same for every lane
-              float* o = sum + q * 32 + 4 * e;
-              o[0] = fmaf(__uint_as_float(r[4 * e]) * ia, b.x, o[0]);
-              o[1] = fmaf(__uint_as_float(r[4 * e + 1]) * ia, b.y, o[1]);
-              o[2] = fmaf(__uint_as_float(r[4 * e + 2]) * ia, b.z, o[2]);
-              o[3] = fmaf(__uint_as_float(r[4 * e + 3]) * ia, b.w, o[3]);
-            }
-          }
+          if (wide)
+            add_chunk<true>(sum, acc, ia, ib);
+          else
+            add_chunk<false>(sum, acc, ia, ib);
           release_acc();
           ia = ia_next;
           stage_tile[32 * ((c + 1 - w.cb) & 1) + lane] = ib_next;

@@ -278,6 +278,63 @@ def test_entries_of_very_different_sizes(mm):
         check(c, want, product_tol(1, a.to(F).abs() @ b.to(F).abs(), k) + 2 * ULP * want.abs(), "c")
 
 
+@pytest.mark.parametrize("m,k,n", [(33, 200, 100), (2304, 256, 2304), (2304, 512, 2304)])  # direct, direct, pairs
+@pytest.mark.parametrize("large_side", ["a", "b"])
+def test_the_largest_entries_give_their_products(mm, m, k, n, large_side):
+    """Entries of 2^100 to 2^127 on one side, 2^-100 to 2^-20 on the other: the products are ordinary numbers, and
+    f32's order of multiplying a chunk's two scales must not lose them to infinity. A zero meets the largest too."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rows, cols = (m, n) if large_side == "a" else (n, m)
+    unit = lambda *s: torch.rand(*s, device="cuda", generator=g) * 0.5 + 0.5  # noqa: E731
+    big = unit(rows, k) * 2.0 ** torch.randint(100, 128, (rows, 1), device="cuda", generator=g)
+    big *= torch.randint(0, 2, (rows, k), device="cuda", generator=g) * 2 - 1
+    small = unit(cols, k) * 2.0 ** torch.randint(-100, -19, (cols, 1), device="cuda", generator=g)
+    big[:, 3], small[:, 4] = 0, 0
+    a, b = (big, small) if large_side == "a" else (small, big)
+    c = torch.empty(m, n, device="cuda")
+    mm.linear_forward(a, b, c, m=m, n=n, k=k, lda=k, ldb=k, ldc=n, b_mn_major=False, precision=1)
+    mm.device_status()
+    want = a.to(F) @ b.to(F).T
+    check(c, want, product_tol(1, a.to(F).abs() @ b.to(F).abs().T, k) + 2 * ULP * want.abs(), "c")
+
+
+@pytest.mark.parametrize("k", [256, 512])  # direct, pairs
+@pytest.mark.parametrize("large_side", ["a", "b"])
+def test_small_entries_against_large_ones(mm, large_side, k):
+    """The other end: rows of 2^-120 to 2^-100, whose inverse scales reach the smallest there are."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    m = n = 2304
+    big = torch.randn(m, k, device="cuda", generator=g) * 2.0 ** torch.randint(90, 111, (m, 1), device="cuda", generator=g)
+    small = torch.randn(n, k, device="cuda", generator=g) * 2.0 ** torch.randint(-120, -99, (n, 1), device="cuda", generator=g)
+    a, b = (big, small) if large_side == "a" else (small, big)
+    c = torch.empty(m, n, device="cuda")
+    mm.linear_forward(a, b, c, m=m, n=n, k=k, lda=k, ldb=k, ldc=n, b_mn_major=False, precision=1)
+    mm.device_status()
+    want = a.to(F) @ b.to(F).T
+    check(c, want, product_tol(1, a.to(F).abs() @ b.to(F).abs().T, k) + 2 * ULP * want.abs(), "c")
+
+
+@pytest.mark.parametrize("below", [10, 17, 24, 31, 38, 45])
+def test_small_entries_beside_a_large_one(mm, below):
+    """Entries 2^-below of the largest of their 128 along the sum, which meets a zero: large exact products lose what the
+    header says and no more (2^-39 of the largest an entry: lo's last bit is 2^-24 of a scaled unit, half of it 2^-25,
+    and the largest is 2^14 at least), smaller ones nothing."""
+    g = torch.Generator(device="cuda").manual_seed(below)
+    for m, k, n in ((33, 256, 100), (2304, 256, 2304), (2304, 512, 2304)):  # direct, direct, pairs
+        a, b = torch.randn(m, k, device="cuda", generator=g).clamp(-2, 2), torch.randn(k, n, device="cuda", generator=g)
+        a *= 2.0 ** -below / 2
+        a[:, ::128], b[::128] = 1, 0
+        c = torch.empty(m, n, device="cuda")
+        mm.linear_forward(a, b, c, m=m, n=n, k=k, lda=k, ldb=n, ldc=n, precision=1)
+        mm.device_status()
+        want = a.to(F) @ b.to(F)
+        tol = product_tol(1, a.to(F).abs() @ b.to(F).abs(), k) + 2 * ULP * want.abs()
+        if k == 512:
+            tol = tol + 2.0 ** -39 * b.to(F).abs().sum(0)
+            assert below < 45 or (c == 0).all()
+        check(c, want, tol, "c")
+
+
 # ------------------------------------------------------------------ dropout
 @pytest.mark.parametrize("rows,cols,ldx,shift", [(1, 1, 1, 0), (3, 5, 5, 1), (7, 8, 12, 0), (100, 1001, 1001, 3), (33, 4096, 4096, 0),
                                                  (5000, 7, 8, 0), (257, 1030, 1032, 0)])

@@ -126,7 +126,7 @@ def test_constants_get_no_gradient(mm, tape):
         tape.backward(tape.linear_cross_entropy(x, w, np.zeros(8, np.int32)))
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 8, 12), (37, 64, 176), (2304, 256, 2304)])  # few rows, direct, pairs
+@pytest.mark.parametrize("m,k,n", [(1, 8, 12), (37, 64, 176), (2304, 256, 2304), (2304, 512, 2304)])  # few rows, direct, pairs
 @pytest.mark.parametrize("act", range(4))
 @pytest.mark.parametrize("p", [0.0, 0.25])
 def test_only_the_residual_tracks(mm, tape, m, k, n, act, p):
