@@ -169,22 +169,24 @@ __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int t
 // One row's kSegment logits -> gradients, in place; every block of a row joins
 // the row's pairs itself (vocab / 128 of them, from L2), the first writes the loss and,
 // where dw is wanted, copies the row of x (zeros for a row without a target: dw sums
-// over all rows, and 0 times what such a row holds may be NaN).
+// over all rows, and 0 times what such a row holds may be NaN). Blocks lie along x, a
+// segment's rows side by side: a vocabulary may have more segments than a grid's y.
 constexpr int kSegment = 4096;
 
 __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz, const float2* part, int tiles,
-                                                        const float* zt, const int32_t* targets, int vocab,
+                                                        const float* zt, const int32_t* targets, int rows, int vocab,
                                                         float grad_scale, float* row_loss, const float* x,
                                                         long long ldx, int dim, float* live_x, long long ldl,
                                                         int* err) {
   after_previous();
   let_next();
   __shared__ MaxSum warps[8];
-  const int r = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int segment = static_cast<int>(blockIdx.x) / rows, r = static_cast<int>(blockIdx.x) - segment * rows;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int t = targets[r];
   const bool live = t >= 0 && t < vocab;
   float4* row = reinterpret_cast<float4*>(z + r * ldz);
-  const int q_end = static_cast<int>(ldz / 4), q0 = blockIdx.y * (kSegment / 4) + threadIdx.x;
+  const int q_end = static_cast<int>(ldz / 4), q0 = segment * (kSegment / 4) + threadIdx.x;
   float4 v[kSegment / 1024];  // on their way while the row's pairs are joined
 #pragma unroll
   for (int u = 0; u < kSegment / 1024; ++u)
@@ -199,8 +201,8 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
   __syncthreads();
   a = warps[0];
   for (int w = 1; w < 8; ++w) a = join(a, warps[w]);
-  if (blockIdx.y == 0 && threadIdx.x == 0) row_loss[r] = loss_of(a, t, vocab, zt + r, err);
-  if (blockIdx.y == 0 && live_x)
+  if (segment == 0 && threadIdx.x == 0) row_loss[r] = loss_of(a, t, vocab, zt + r, err);
+  if (segment == 0 && live_x)
     for (int c = 4 * threadIdx.x; c < dim; c += 1024)  // ldl is dim rounded up to 4
       *reinterpret_cast<float4*>(live_x + r * ldl + c) =
           live ? load_quad(x + r * ldx, c, dim) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -356,9 +358,10 @@ int direct_block(const LinearLoss& a, Plan& p, long long r0, int n, bool mean, i
                 a.row_loss + r0, nullptr, d_err);
     return 0;
   }
-  const dim3 grid(n, static_cast<unsigned>((p.ldz + kSegment - 1) / kSegment));
-  launch_next("loss gradient", loss_grad_kernel, grid, 256, 0, 1, s, p.z, p.ldz, p.part, p.tiles, p.zt, t, a.vocab,
-              a.grad_scale, a.row_loss + r0, x, a.ldx, a.dim, a.dw ? p.x : nullptr, p.ldx, d_err);
+  const long long blocks = n * ((p.ldz + kSegment - 1) / kSegment);  // a block's logits / 16 KB, or its rows
+  if (blocks > INT32_MAX) return kGemmBadArgument;
+  launch_next("loss gradient", loss_grad_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, 1, s, p.z, p.ldz, p.part,
+              p.tiles, p.zt, t, n, a.vocab, a.grad_scale, a.row_loss + r0, x, a.ldx, a.dim, a.dw ? p.x : nullptr, p.ldx, d_err);
   if (mean) mean_loss(a, s);
   if (a.dw) {
     LinearEpilogue o;

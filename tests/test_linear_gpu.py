@@ -502,6 +502,39 @@ def test_a_target_that_is_no_class(mm):
     assert (dx[[1, 4]] == 0).all() and torch.isfinite(dw).all()
 
 
+@pytest.mark.parametrize("precision", [1, 0])
+def test_a_vocabulary_of_more_segments_than_a_grid_has(mm, precision):
+    """65,536 segments of 4096 classes and four classes: 268 million of width 4, one row. Off the target every gradient is
+    softmax's share; the sums' tolerances are test_linear_cross_entropy's, with their S over this vocabulary."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    vocab, dim, scale = (65536 << 12) + 4, 4, 1.0
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x, w = torch.randn(1, dim, device="cuda", generator=g), torch.randn(vocab, dim, device="cuda", generator=g)
+    t = torch.tensor([vocab - 2], dtype=torch.int32, device="cuda")
+    row_loss, mean, dx, dw = torch.empty(1, device="cuda"), torch.empty(1, device="cuda"), torch.empty_like(x), torch.empty_like(w)
+    mm.linear_cross_entropy(x, w, t, row_loss, rows=1, vocab=vocab, dim=dim, ldx=dim, ldw=dim, grad_scale=scale, mean_loss=mean, dx=dx,
+                            lddx=dim, dw=dw, lddw=dim, precision=precision)
+    mm.device_status()
+    X, z = x.to(F)[0], w.to(F) @ x.to(F)[0]
+    lse = torch.logsumexp(z, 0)
+    tz = product_tol(precision, (w.abs().to(F) @ X.abs()).max(), dim)
+    # the sum of 2^28 exponentials: 128 at a time, then 2^21 pairs by 256 threads, 2^13 roundings each in f32
+    t_exp = 2 * tz + (8192 + 64 + 2 * (z.max() - z.min())) * ULP
+    check(row_loss, (lse - z[-2]).view(1), t_exp + 4 * ULP * (lse.abs() + z.abs().max()), "row_loss")
+    assert mean.item() == row_loss.item()
+    q = (z - lse).exp()
+    q[-2] -= 1
+    for part in (slice(0, 1 << 20), slice(vocab - (1 << 20), vocab)):  # the first segments and the last
+        want = q[part, None] * X
+        tol = (t_exp + 8 * ULP) * want.abs() + product_tol(precision, want.abs(), 1) + 4 * ULP * X.abs() * (q[part, None] < 0)
+        check(dw[part], want, tol, "dw")
+    assert (dw[:, 0] != 0).all()  # no segment was left out
+    # dx: up to eight rows are f32 multiply-adds, 2^28 of them by 512 blocks of 32 at a time: 2^14 roundings each
+    size = q.abs() @ w.abs().to(F)
+    check(dx[0], q @ w.to(F), (t_exp + (16384 + 1024) * ULP) * size, "dx")
+
+
 def test_no_row_has_a_target(mm):
     x, w, t = torch.randn(9, 8, device="cuda"), torch.randn(50, 8, device="cuda"), torch.full((9,), -1, dtype=torch.int32, device="cuda")
     row_loss, mean, dx, dw = torch.empty(9, device="cuda"), torch.empty(1, device="cuda"), torch.empty_like(x), torch.empty_like(w)
