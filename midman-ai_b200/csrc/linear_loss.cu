@@ -203,9 +203,9 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
   for (int w = 1; w < 8; ++w) a = join(a, warps[w]);
   if (segment == 0 && threadIdx.x == 0) row_loss[r] = loss_of(a, t, vocab, zt + r, err);
   if (segment == 0 && live_x)
-    for (int c = 4 * threadIdx.x; c < dim; c += 1024)  // ldl is dim rounded up to 4
+    for (long long c = 4 * threadIdx.x; c < dim; c += 1024)  // ldl is dim rounded up to 4
       *reinterpret_cast<float4*>(live_x + r * ldl + c) =
-          live ? load_quad(x + r * ldx, c, dim) : make_float4(0.f, 0.f, 0.f, 0.f);
+          live ? load_quad(x + r * ldx, static_cast<int>(c), dim) : make_float4(0.f, 0.f, 0.f, 0.f);
   const float coef = grad_scale / a.s;
 #pragma unroll
   for (int u = 0; u < kSegment / 1024; ++u) {
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(1024) mean_live_kernel(const float* row_loss, 
   __shared__ int counts[32];
   double s = 0.0;
   int n = 0;
-  for (int r = threadIdx.x; r < rows; r += 1024)
+  for (long long r = threadIdx.x; r < rows; r += 1024)  // rows + 1023 may pass 32 bits
     if (targets[r] != -1) {
       s += row_loss[r];
       ++n;

@@ -502,12 +502,22 @@ def test_a_target_that_is_no_class(mm):
     assert (dx[[1, 4]] == 0).all() and torch.isfinite(dw).all()
 
 
+@pytest.fixture
+def room():
+    """room(gb) skips a test where the device has less memory; what the test took is given back."""
+    def need(gb):
+        torch.cuda.empty_cache()
+        if torch.cuda.mem_get_info()[0] < gb << 30:
+            pytest.skip(f"needs {gb} GB of device memory")
+    yield need
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("precision", [1, 0])
-def test_a_vocabulary_of_more_segments_than_a_grid_has(mm, precision):
+def test_a_vocabulary_of_more_segments_than_a_grid_has(mm, room, precision):
     """65,536 segments of 4096 classes and four classes: 268 million of width 4, one row. Off the target every gradient is
     softmax's share; the sums' tolerances are test_linear_cross_entropy's, with their S over this vocabulary."""
-    if torch.cuda.mem_get_info()[0] < 40 << 30:
-        pytest.skip("needs 40 GB of device memory")
+    room(40)
     vocab, dim, scale = (65536 << 12) + 4, 4, 1.0
     g = torch.Generator(device="cuda").manual_seed(12)
     x, w = torch.randn(1, dim, device="cuda", generator=g), torch.randn(vocab, dim, device="cuda", generator=g)
@@ -533,6 +543,41 @@ def test_a_vocabulary_of_more_segments_than_a_grid_has(mm, precision):
     # dx: up to eight rows are f32 multiply-adds, 2^28 of them by 512 blocks of 32 at a time: 2^14 roundings each
     size = q.abs() @ w.abs().to(F)
     check(dx[0], q @ w.to(F), (t_exp + (16384 + 1024) * ULP) * size, "dx")
+
+
+LONGEST = 2 ** 31 - 512
+
+
+def test_the_mean_over_the_most_rows(mm, room):
+    """The rows' loop ends at the last row: a step past it is beyond 32 bits."""
+    room(80)
+    x, w = torch.zeros(LONGEST, 4, device="cuda"), torch.eye(4, device="cuda")
+    t = torch.full((LONGEST,), -1, dtype=torch.int32, device="cuda")
+    row_loss, mean = torch.empty(LONGEST, device="cuda"), torch.empty(1, device="cuda")
+    at = torch.tensor([0, 1023, 1 << 30, LONGEST - 1025, LONGEST - 1], device="cuda")
+    t[at], x[at, 1] = 1, torch.arange(1.0, 6.0, device="cuda")
+    mm.linear_cross_entropy(x, w, t, row_loss, rows=LONGEST, vocab=4, dim=4, ldx=4, ldw=4, mean_loss=mean, precision=0)
+    mm.device_status()
+    z = torch.arange(1.0, 6.0, device="cuda", dtype=F)
+    want = torch.log(z.exp() + 3) - z  # whole numbers pass a TF32 product as they are; a few ulp of the exponentials and of lse
+    check(row_loss[at], want, 16 * ULP * (z + 1), "row_loss")
+    check(mean, want.mean().view(1), 16 * ULP * (z + 1).mean() + 4 * ULP, "mean")
+    assert torch.count_nonzero(row_loss) == 5
+
+
+def test_the_gradient_of_the_widest_rows(mm, room):
+    """The copy of x for dw ends at the last column, likewise."""
+    room(120)
+    x, w, dw = torch.zeros(1, LONGEST, device="cuda"), torch.zeros(4, LONGEST, device="cuda"), torch.empty(4, LONGEST, device="cuda")
+    at = torch.tensor([0, 1023, 1024, 1 << 30, LONGEST - 1025, LONGEST - 1024, LONGEST - 1], device="cuda")
+    x[0, at] = torch.arange(1.0, 8.0, device="cuda")
+    t, row_loss = torch.tensor([2], dtype=torch.int32, device="cuda"), torch.empty(1, device="cuda")
+    mm.linear_cross_entropy(x, w, t, row_loss, rows=1, vocab=4, dim=LONGEST, ldx=LONGEST, ldw=LONGEST, dw=dw, lddw=LONGEST, precision=0)
+    mm.device_status()
+    want = torch.tensor([0.25, 0.25, -0.75, 0.25], device="cuda")[:, None] * torch.arange(1.0, 8.0, device="cuda")
+    assert torch.equal(dw[:, at], want)  # exact: quarters of whole numbers
+    assert torch.count_nonzero(dw) == 28
+    check(row_loss, torch.tensor([4.0], device="cuda", dtype=F).log(), 4 * ULP, "row_loss")
 
 
 def test_no_row_has_a_target(mm):
