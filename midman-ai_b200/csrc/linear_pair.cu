@@ -33,6 +33,7 @@
 #include <cmath>
 #include <cstdint>
 #include <stdexcept>
+#include <type_traits>
 
 #include "device.h"
 #include "gemm.h"
@@ -361,11 +362,12 @@ __device__ __forceinline__ PairUnit unit_of(int u, const PairWork& w, int steps)
 __device__ __forceinline__ void stage_rows(const float* v, float4* stage_tile, int lane);
 
 // How operands reach the UMMAs. A work step is what a unit's K range counts: `LOADS`
-// stages; EACH: every work step is an accumulation of its own, scaled and summed in
-// registers, otherwise a unit is one accumulation.
+// stages. An accumulation covers CHUNK work steps, then the summing warps add it to the
+// sums in registers (SCALED: with both operands' scales undone): the tensor core truncates
+// at every UMMA, always toward zero, so what one accumulation loses grows with its length.
 struct ExactFeed {  // split copies: hi and lo of A and B, 64 of K a stage, a chunk two
-  static constexpr int STAGE = 4 * P_TILE, LOADS = 2;
-  static constexpr bool EACH = true;
+  static constexpr int STAGE = 4 * P_TILE, LOADS = 2, CHUNK = 1;
+  static constexpr bool SCALED = true;
   static constexpr uint32_t IDESC = idesc_f16(2 * BM, PN);
   static __device__ __forceinline__ void load(uint32_t st, const CUtensorMap* a, const CUtensorMap* b, uint32_t bar,
                                               int i, int m0, int n0, int) {
@@ -384,12 +386,15 @@ struct ExactFeed {  // split copies: hi and lo of A and B, 64 of K a stage, a ch
     }
   }
 };
-// The f32 operands themselves, one TF32 pass: 32 of K a stage. Bits 1 and 2 of
-// `boxes`: an MN-major A, B loads its stage in one 3-D box, else in 32-wide ones.
+// The f32 operands themselves, one TF32 pass: 32 of K a stage, 2048 an accumulation (256
+// UMMAs; sums of one sign come out 1.4e-5 low whatever their length, 2.4e-4 for 32768 of K
+// and 9.7e-4 for 131072 in one accumulation. 8192 x 5632 -> 2048: 327 us, 326 in one
+// accumulation, 341 in steps of 1024, which the direct kernel has for half the error). Bits
+// 1 and 2 of `boxes`: an MN-major A, B loads its stage in one 3-D box, else in 32-wide ones.
 template <bool A_MN, bool B_MN>
 struct Tf32Feed {
-  static constexpr int STAGE = 2 * P_TILE, LOADS = 1;
-  static constexpr bool EACH = false;
+  static constexpr int STAGE = 2 * P_TILE, LOADS = 1, CHUNK = 64;
+  static constexpr bool SCALED = false;
   static constexpr uint32_t IDESC = idesc_tf32(2 * BM, PN, A_MN, B_MN);
   template <bool MN>
   static __device__ __forceinline__ void side(uint32_t at, const CUtensorMap* map, uint32_t bar, int k0, int mn0,
@@ -535,14 +540,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
       bool ok = true;
       for (int u = pair; u < units && ok; u += npairs) {
         const PairUnit w = unit_of(u, work, steps);
-        for (int c = w.cb; c < w.ce && ok; c = Feed::EACH ? c + 1 : w.ce) {
+        for (int c = w.cb; c < w.ce && ok; c += Feed::CHUNK) {
           const int buf = j & 1;
           if (j >= 2 && !mbar_wait(acc_empty(buf), ((j >> 1) - 1) & 1, err, kErrWaitAccum)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int loads = Feed::LOADS * (Feed::EACH ? 1 : w.ce - c);
+          const int loads = Feed::LOADS * min(Feed::CHUNK, w.ce - c);
           for (int h = 0; h < loads; ++h, ++it) {
             const int s = it % P_STAGES, round = it / P_STAGES;
             if (!mbar_wait(full_bar(s), round & 1, err, kErrWaitFull)) {
@@ -591,17 +596,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
         ++j;
       };
       uint32_t acc = 0;
-      if (!Feed::EACH) {
-        ok = wait_acc(&acc);
-        if (!ok) break;
+      if (!Feed::SCALED) {
+        // the first accumulation on its own: its values are the sums, with nothing added
+        auto take = [&](auto first) {
+          ok = wait_acc(&acc);
+          if (!ok) return;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(acc + q * 32, r);
+          for (int q = 0; q < 4; ++q) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(acc + q * 32, r);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) sum[q * 32 + e] = __uint_as_float(r[e]);
-        }
-        release_acc();
+            for (int e = 0; e < 32; ++e) {
+              const float v = __uint_as_float(r[e]);
+              sum[q * 32 + e] = first ? v : sum[q * 32 + e] + v;
+            }
+          }
+          release_acc();
+        };
+        take(std::true_type{});
+        for (int c = w.cb + Feed::CHUNK; c < w.ce && ok; c += Feed::CHUNK) take(std::false_type{});
       } else {
         // The chunks' inverse scales, one chunk ahead: this lane's row's in a register,
         // the columns' through the staging tile (idle until the epilogue).

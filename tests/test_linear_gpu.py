@@ -335,6 +335,30 @@ def test_small_entries_beside_a_large_one(mm, below):
         check(c, want, tol, "c")
 
 
+@pytest.mark.parametrize("m,n", [(128, 256), (2304, 2304)])  # direct, pairs
+@pytest.mark.parametrize("b_t", [False, True])
+def test_long_sums_of_one_sign_in_one_tf32_pass(mm, m, n, b_t):
+    """Operands of 11 bits, so nothing of them is cut: what is left is the sums' error. An accumulation is 2048 of K at most,
+    256 UMMAs that each cut less than 2^-23 of the sum so far: 2^-15. The accumulations are added in f32, at most K / 1024
+    roundings of 2^-24, and up to 64 parts of K likewise."""
+    k = 32768
+    g = torch.Generator(device="cuda").manual_seed(n)
+    eleven = lambda *s: ((torch.rand(*s, device="cuda", generator=g) + 1).view(torch.int32) & ~0x1FFF).view(torch.float32)  # noqa: E731
+    a, b = eleven(m, k), eleven(*((n, k) if b_t else (k, n)))
+    c = torch.empty(m, n, device="cuda")
+    mm.linear_forward(a, b, c, m=m, n=n, k=k, lda=k, ldb=b.stride(0), ldc=n, b_mn_major=not b_t, precision=0)
+    mm.device_status()
+    want = a.to(F) @ (b.T if b_t else b).to(F)
+    check(c, want, (2.0 ** -15 + (k / 1024 + 64) * ULP) * want, "c")
+    # and a weight's gradient, whose sum is over the rows: a^T [k, m] plays the input, c's place is [k, n]
+    db, dc = torch.empty(m, n, device="cuda"), eleven(k, n)
+    x = a.T.contiguous()
+    mm.linear_backward(x, None, dc, m=k, n=n, k=m, lda=m, ldb=n, lddc=n, db=db, lddb=n, precision=0)
+    mm.device_status()
+    want = a.to(F) @ dc.to(F)
+    check(db, want, (2.0 ** -15 + (k / 1024 + 64) * ULP) * want, "db")
+
+
 # ------------------------------------------------------------------ dropout
 @pytest.mark.parametrize("rows,cols,ldx,shift", [(1, 1, 1, 0), (3, 5, 5, 1), (7, 8, 12, 0), (100, 1001, 1001, 3), (33, 4096, 4096, 0),
                                                  (5000, 7, 8, 0), (257, 1030, 1032, 0)])
