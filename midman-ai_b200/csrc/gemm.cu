@@ -1592,24 +1592,27 @@ int launch_status() {
 
 PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static PFN_cuCtxGetCurrent_v4000 get_current = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    auto find = [](const char* name, unsigned version) -> void* {
+      void* p = nullptr;
+      cudaDriverEntryPointQueryResult q;
+      return cudaGetDriverEntryPointByVersion(name, &p, version, cudaEnableDefault, &q) == cudaSuccess &&
+                     q == cudaDriverEntryPointSuccess
+                 ? p
+                 : nullptr;
+    };
+    fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(find("cuTensorMapEncodeTiled", 12000));
+    get_current = reinterpret_cast<PFN_cuCtxGetCurrent_v4000>(find("cuCtxGetCurrent", 4000));
   });
-  // The encoder needs a current context, which a host thread has from its first runtime call on.
-  static thread_local bool bound = false;
-  if (!bound) {
-    int device = 0;
-    if (cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess)
-      bound = true;
-    else
-      cudaGetLastError();
-  }
+  // The encoder needs a current context, which a host thread has from its first runtime
+  // call on. One that the caller made current through the driver stays.
+  CUcontext current = nullptr;
+  int device = 0;
+  if (get_current && get_current(&current) == CUDA_SUCCESS && !current &&
+      (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess))
+    cudaGetLastError();
   return fn;
 }
 

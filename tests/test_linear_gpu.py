@@ -11,7 +11,10 @@ absolute products):
 An activation passes an error on with its slope (at most 1.13) and adds its own: a few ulp of |z| + 1. Dropout multiplies by
 1 / (1 - p), rounded (2^-24) twice.
 """
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -770,6 +773,40 @@ def test_a_host_thread_whose_first_call_it_is(mm, m, k, n, precision):
     torch.cuda.synchronize()
     assert failed == [0] and torch.equal(c, d)
     mm.device_status()
+
+
+def test_a_callers_context_stays_current():
+    """A product's tensor maps need a current context; one that the caller made is left in its place. The sizes pass the
+    checks and the maps, and are refused before anything is launched. In a process of its own, as contexts outlive tests."""
+    code = """
+import ctypes, sys, threading
+sys.path.insert(0, sys.argv[1])
+import torch, midman_b200 as mm
+cuda = ctypes.CDLL("libcuda.so.1")
+x = torch.zeros(64, device="cuda")
+mm.device_status()
+seen = []
+def work():
+    mine, now, dev = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_int()
+    assert cuda.cuDeviceGet(ctypes.byref(dev), 0) == 0
+    assert cuda.cuCtxCreate_v2(ctypes.byref(mine), 0, dev) == 0
+    n = 2 ** 31 - 512
+    rc = mm.load().mm_gpu_linear_forward(n, n, 4, x.data_ptr(), 4, x.data_ptr(), 4, 0, None, 0, 0.0, None, None, 0, None, 0,
+                                         x.data_ptr() + 128, n, 1, None, 0, None)
+    assert cuda.cuCtxGetCurrent(ctypes.byref(now)) == 0
+    seen.extend([rc, mine.value, now.value])
+    assert cuda.cuCtxDestroy_v2(mine) == 0
+t = threading.Thread(target=work)
+t.start()
+t.join()
+torch.cuda.synchronize()
+assert seen[0] == -1, seen
+assert seen[1] == seen[2], "another context was made current"
+print("stays")
+"""
+    run = subprocess.run([sys.executable, "-c", code, str(Path(__file__).resolve().parent.parent / "midman-ai_b200")], capture_output=True,
+                         text=True, timeout=120)
+    assert run.returncode == 0 and "stays" in run.stdout, run.stderr
 
 
 @pytest.mark.parametrize("sizes", SIZES)
