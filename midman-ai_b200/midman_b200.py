@@ -297,8 +297,9 @@ def cross_entropy(logits, targets, row_loss, *, rows, vocab, ld, grad_scale, mea
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = range(4)
 
 
-def _device_tensors(dtype_name, **tensors):
-    """Refuses tensors of another type, in host memory, or on another GPU than the current one."""
+def _device_tensors(dtype_name, rng=None, **tensors):
+    """Refuses tensors of another type, in host memory, or on another GPU than the current one; rng must hold the two
+    words {seed, offset} side by side."""
     import torch
     dtype, current = getattr(torch, dtype_name), torch.cuda.current_device()
     for name, t in tensors.items():
@@ -306,14 +307,23 @@ def _device_tensors(dtype_name, **tensors):
             if t.dtype is not dtype:
                 raise TypeError(f"{name} must be {dtype_name}, not {t.dtype}")
             raise ValueError(f"{name} is on {t.device}, and the current device is cuda:{current}")
+    if rng is not None and (rng.dtype is not torch.int64 or rng.get_device() != current or rng.numel() < 2
+                            or not rng.is_contiguous()):
+        if rng.dtype is not torch.int64:
+            raise TypeError(f"rng must be int64, not {rng.dtype}")
+        raise ValueError(f"rng must hold [seed, offset] side by side on cuda:{current}")
 
 
 def _workspace(bytes_needed, given, like):
     """The caller's workspace, or one from torch's allocator (stream-ordered on the current stream)."""
     need = check(bytes_needed)
-    if given is not None or need == 0:
-        return given
+    if given is None and need == 0:
+        return None
     import torch
+    if given is not None:
+        if given.get_device() != torch.cuda.current_device() or not given.is_contiguous():
+            raise ValueError(f"workspace must be one piece of the current device's memory, and it is on {given.device}")
+        return given
     return torch.empty(need, dtype=torch.uint8, device=like.device)
 
 
@@ -323,8 +333,7 @@ def _bytes(t):
 
 def dropout(x, y, *, rows, cols, ldx, ldy, p, rng=None, r=None, ldr=0, stream=None):
     """y = r + dropout(x); rng: a CUDA int64 tensor [seed, offset] (see include/midman_gpu.h)."""
-    _device_tensors("float32", x=x, y=y, r=r)
-    _device_tensors("int64", rng=rng)
+    _device_tensors("float32", rng, x=x, y=y, r=r)
     return check(load().mm_gpu_dropout(rows, cols, _ptr(x), ldx, _ptr(r), ldr, _ptr(y), ldy, p, _ptr(rng),
                                        _stream(stream)))
 
@@ -338,8 +347,7 @@ def linear_forward(a, b, c, *, m, n, k, lda, ldb, ldc, b_mn_major=True, bias=Non
                    r=None, ldr=0, z=None, ldz=0, precision=0, workspace=None, stream=None):
     """c = r + dropout(activation(a b + bias)), z = a b + bias where wanted. Without a workspace one is allocated,
     which needs `stream` to be the current one."""
-    _device_tensors("float32", a=a, b=b, c=c, bias=bias, r=r, z=z)
-    _device_tensors("int64", rng=rng)
+    _device_tensors("float32", rng, a=a, b=b, c=c, bias=bias, r=r, z=z)
     lib = load()
     ws = _workspace(lib.mm_gpu_linear_workspace(m, n, k, 0, precision), workspace, c)
     return check(lib.mm_gpu_linear_forward(m, n, k, _ptr(a), lda, _ptr(b), ldb, int(b_mn_major), _ptr(bias), activation,
@@ -351,8 +359,7 @@ def linear_backward(a, b, dc, *, m, n, k, lda, ldb, lddc, b_mn_major=True, activ
                     ldz=0, da=None, ldda=0, db=None, lddb=0, dbias=None, accumulate=False, precision=0, workspace=None,
                     stream=None):
     """The gradients da, db, dbias (those given) of linear_forward from dc and the z it kept."""
-    _device_tensors("float32", a=a, b=b, dc=dc, z=z, da=da, db=db, dbias=dbias)
-    _device_tensors("int64", rng=rng)
+    _device_tensors("float32", rng, a=a, b=b, dc=dc, z=z, da=da, db=db, dbias=dbias)
     lib = load()
     ws = _workspace(lib.mm_gpu_linear_workspace(m, n, k, 1, precision), workspace, dc)
     return check(lib.mm_gpu_linear_backward(m, n, k, _ptr(a), lda, _ptr(b), ldb, int(b_mn_major), activation, p, _ptr(rng),

@@ -891,3 +891,27 @@ def test_wrong_types_and_places_are_refused(mm):
         mm.linear_cross_entropy(x, x, torch.zeros(4, dtype=torch.int64, device="cuda"), x[:, 0], rows=4, vocab=4, dim=8, ldx=8, ldw=8)
     with pytest.raises(mm.MidmanGpuError, match="workspace"):
         mm.linear_backward(x, x, x, m=4, n=8, k=4, lda=8, ldb=8, lddc=8, da=x, ldda=8, workspace=torch.empty(256, dtype=torch.uint8, device="cuda")[:8])
+
+
+def test_workspaces_and_words_in_wrong_places_are_refused(mm):
+    """Host memory, pieces and a single word, each before anything is queued: the kernels would follow their addresses."""
+    m, k, n, v = 300, 96, 200, 1000
+    s = tensors_for(mm, 1, m, k, n, v, 1)
+    kw = dict(m=m, n=n, k=k, lda=k, ldb=n, precision=1)
+    forward = lambda **c: mm.linear_forward(s["a"], s["b"], s["c"], ldc=n, **kw, **c)  # noqa: E731
+    backward = lambda **c: mm.linear_backward(s["a"], s["b"], s["dc"], lddc=n, da=s["da"], ldda=k, **kw, **c)  # noqa: E731
+    loss = lambda **c: mm.linear_cross_entropy(s["c"], s["w"], s["t"], s["loss"], rows=m, vocab=v, dim=n, ldx=n, ldw=n, dx=s["dc"],  # noqa: E731
+                                               lddx=n, precision=1, **c)
+    dropout = lambda **c: mm.dropout(s["a"], s["y"], rows=m, cols=k, ldx=k, ldy=k, p=0.1, **c)  # noqa: E731
+    host = torch.empty(s["ws"].numel(), dtype=torch.uint8)
+    for call in (forward, backward, loss):
+        for ws in (host, host.pin_memory(), torch.empty(2 * s["ws"].numel(), dtype=torch.uint8, device="cuda")[::2]):
+            with pytest.raises(ValueError, match="workspace"):
+                call(workspace=ws)
+    words = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for call in (lambda **c: forward(p=0.1, **c), lambda **c: backward(p=0.1, **c), dropout):
+        for rng in (words[:1], words[::2], words.cpu()):
+            with pytest.raises(ValueError):
+                call(rng=rng)
+        call(rng=words[2:])
+    mm.device_status()
