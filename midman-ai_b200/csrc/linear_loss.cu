@@ -169,24 +169,26 @@ __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int t
 // One row's kSegment logits -> gradients, in place; every block of a row joins
 // the row's pairs itself (vocab / 128 of them, from L2), the first writes the loss and,
 // where dw is wanted, copies the row of x (zeros for a row without a target: dw sums
-// over all rows, and 0 times what such a row holds may be NaN). Blocks lie along x, a
-// segment's rows side by side: a vocabulary may have more segments than a grid's y.
+// over all rows, and 0 times what such a row holds may be NaN). A
+// vocabulary may have more segments than a grid's y: those past it lie along z.
 constexpr int kSegment = 4096;
+constexpr long long kGridY = 65535;
 
 __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz, const float2* part, int tiles,
-                                                        const float* zt, const int32_t* targets, int rows, int vocab,
+                                                        const float* zt, const int32_t* targets, int vocab,
                                                         float grad_scale, float* row_loss, const float* x,
                                                         long long ldx, int dim, float* live_x, long long ldl,
                                                         int* err) {
   after_previous();
   let_next();
   __shared__ MaxSum warps[8];
-  const int segment = static_cast<int>(blockIdx.x) / rows, r = static_cast<int>(blockIdx.x) - segment * rows;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int r = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int segment = static_cast<int>(blockIdx.y + gridDim.y * blockIdx.z);
   const int t = targets[r];
   const bool live = t >= 0 && t < vocab;
   float4* row = reinterpret_cast<float4*>(z + r * ldz);
   const int q_end = static_cast<int>(ldz / 4), q0 = segment * (kSegment / 4) + threadIdx.x;
+  if (segment * (kSegment / 4) >= q_end) return;  // of the last z
   float4 v[kSegment / 1024];  // on their way while the row's pairs are joined
 #pragma unroll
   for (int u = 0; u < kSegment / 1024; ++u)
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
   for (int w = 1; w < 8; ++w) a = join(a, warps[w]);
   if (segment == 0 && threadIdx.x == 0) row_loss[r] = loss_of(a, t, vocab, zt + r, err);
   if (segment == 0 && live_x)
-    for (long long c = 4 * threadIdx.x; c < dim; c += 1024)  // ldl is dim rounded up to 4
+    for (unsigned c = 4 * threadIdx.x; c < static_cast<unsigned>(dim); c += 1024)  // ldl is dim rounded up to 4
       *reinterpret_cast<float4*>(live_x + r * ldl + c) =
           live ? load_quad(x + r * ldx, static_cast<int>(c), dim) : make_float4(0.f, 0.f, 0.f, 0.f);
   const float coef = grad_scale / a.s;
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(1024) mean_live_kernel(const float* row_loss, 
   __shared__ int counts[32];
   double s = 0.0;
   int n = 0;
-  for (long long r = threadIdx.x; r < rows; r += 1024)  // rows + 1023 may pass 32 bits
+  for (unsigned r = threadIdx.x; r < static_cast<unsigned>(rows); r += 1024)  // its last step may pass 31 bits
     if (targets[r] != -1) {
       s += row_loss[r];
       ++n;
@@ -358,10 +360,11 @@ int direct_block(const LinearLoss& a, Plan& p, long long r0, int n, bool mean, i
                 a.row_loss + r0, nullptr, d_err);
     return 0;
   }
-  const long long blocks = n * ((p.ldz + kSegment - 1) / kSegment);  // a block's logits / 16 KB, or its rows
-  if (blocks > INT32_MAX) return kGemmBadArgument;
-  launch_next("loss gradient", loss_grad_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, 1, s, p.z, p.ldz, p.part,
-              p.tiles, p.zt, t, n, a.vocab, a.grad_scale, a.row_loss + r0, x, a.ldx, a.dim, a.dw ? p.x : nullptr, p.ldx, d_err);
+  const long long segments = (p.ldz + kSegment - 1) / kSegment;
+  const dim3 grid(n, static_cast<unsigned>(std::min(segments, kGridY)),
+                  static_cast<unsigned>((segments + kGridY - 1) / kGridY));
+  launch_next("loss gradient", loss_grad_kernel, grid, 256, 0, 1, s, p.z, p.ldz, p.part, p.tiles, p.zt, t, a.vocab,
+              a.grad_scale, a.row_loss + r0, x, a.ldx, a.dim, a.dw ? p.x : nullptr, p.ldx, d_err);
   if (mean) mean_loss(a, s);
   if (a.dw) {
     LinearEpilogue o;
