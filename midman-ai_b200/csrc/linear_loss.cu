@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(256) row_loss_kernel(const float2* part, int t
 // the row's pairs itself (vocab / 128 of them, from L2), the first writes the loss and,
 // where dw is wanted, copies the row of x (zeros for a row without a target: dw sums
 // over all rows, and 0 times what such a row holds may be NaN). A
-// vocabulary may have more segments than a grid's y: those past it lie along z.
+// vocabulary may have more segments than a grid's y: those past it lie along z (and what
+// the last z has beyond the last segment finds nothing to write).
 constexpr int kSegment = 4096;
 constexpr long long kGridY = 65535;
 
@@ -188,7 +189,6 @@ __global__ void __launch_bounds__(256) loss_grad_kernel(float* z, long long ldz,
   const bool live = t >= 0 && t < vocab;
   float4* row = reinterpret_cast<float4*>(z + r * ldz);
   const int q_end = static_cast<int>(ldz / 4), q0 = segment * (kSegment / 4) + threadIdx.x;
-  if (segment * (kSegment / 4) >= q_end) return;  // of the last z
   float4 v[kSegment / 1024];  // on their way while the row's pairs are joined
 #pragma unroll
   for (int u = 0; u < kSegment / 1024; ++u)
@@ -237,11 +237,14 @@ __global__ void __launch_bounds__(1024) mean_live_kernel(const float* row_loss, 
   __shared__ int counts[32];
   double s = 0.0;
   int n = 0;
-  for (unsigned r = threadIdx.x; r < static_cast<unsigned>(rows); r += 1024)  // its last step may pass 31 bits
-    if (targets[r] != -1) {
-      s += row_loss[r];
+  for (unsigned r = threadIdx.x; r < static_cast<unsigned>(rows); r += 1024) {  // its last step may pass 31 bits
+    const int t = targets[r];
+    const float loss = row_loss[r];  // beside the target's load
+    if (t != -1) {
+      s += loss;
       ++n;
     }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, o);
