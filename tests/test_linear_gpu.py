@@ -529,6 +529,41 @@ def test_a_target_that_is_no_class(mm):
     assert (dx[[1, 4]] == 0).all() and torch.isfinite(dw).all()
 
 
+# direct; direct gradients of logits on pairs; pairs; several blocks on pairs
+@pytest.mark.parametrize("precision", [1, 0])
+@pytest.mark.parametrize("rows,vocab,dim,tied", [(300, 1000, 64, True), (2304, 4096, 128, True), (2304, 2305, 512, False), (1100, 131073, 260, True)])
+def test_targets_that_are_no_class_leave_the_other_rows_alone(mm, rows, vocab, dim, tied, precision):
+    """Their rows' loss is NaN, their gradients are 0 and they have no share in dw, whatever x holds there; every other row's
+    outputs, and dw, are those of a call that leaves these rows out."""
+    g = torch.Generator(device="cuda").manual_seed(rows + dim)
+    x, w, t = loss_case(g, rows, vocab, dim, tied, 0)
+    bad = torch.tensor([0, 1, 129, rows // 2, rows - 1], device="cuda")
+    t[bad] = torch.tensor([vocab, -2, 2 ** 31 - 1, -2 ** 31, vocab + 127], dtype=torch.int32, device="cuda")
+    x[bad, :dim] = float("nan")
+    out = t.clone()
+    out[bad] = -1
+    kw = dict(rows=rows, vocab=vocab, dim=dim, ldx=x.stride(0), ldw=w.stride(0), w_mn_major=not tied, grad_scale=1 / rows, precision=precision)
+    got, want = ([torch.full((rows,), 777.0, device="cuda"), out_buffer(rows, dim, 0), out_buffer(*((vocab, dim) if tied else (dim, vocab)), 0),
+                  torch.empty(1, device="cuda")] for _ in range(2))
+    for outs, targets in ((got, t), (want, out)):
+        row_loss, dx, dw, mean = outs
+        mm.linear_cross_entropy(x, w, targets, row_loss, mean_loss=mean, dx=dx, lddx=dx.stride(0), dw=dw, lddw=dw.stride(0), **kw)
+        if targets is t:
+            with pytest.raises(mm.MidmanGpuError, match="outside"):
+                mm.device_status()
+    mm.device_status()
+    assert torch.isnan(got[0][bad]).all() and torch.isnan(got[3]).all() and (want[0][bad] == 0).all()
+    good = torch.ones(rows, dtype=torch.bool, device="cuda").index_fill(0, bad, False)
+    assert torch.equal(got[0][good], want[0][good]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+    assert (got[1][bad, :dim] == 0).all() and torch.isfinite(got[2]).all()
+    # the loss alone
+    mm.linear_cross_entropy(x, w, t, got[0], mean_loss=got[3], **kw)
+    mm.linear_cross_entropy(x, w, out, want[0], mean_loss=want[3], **kw)
+    with pytest.raises(mm.MidmanGpuError, match="outside"):
+        mm.device_status()
+    assert torch.isnan(got[0][bad]).all() and torch.isnan(got[3]).all() and torch.equal(got[0][good], want[0][good])
+
+
 @pytest.fixture
 def room():
     """room(gb) skips a test where the device has less memory; what the test took is given back."""
