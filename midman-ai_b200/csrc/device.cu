@@ -14,8 +14,9 @@ std::vector<DeviceContext> g_ctx;
 }  // namespace
 
 void check_cuda(cudaError_t e, const char* what) {
-  if (e != cudaSuccess)
-    throw std::runtime_error(std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")");
+  if (e == cudaSuccess) return;
+  cudaGetLastError();  // reported here, and not by the next launch's check
+  throw std::runtime_error(std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")");
 }
 
 DeviceContext& device_context() {

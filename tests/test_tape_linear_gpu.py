@@ -144,6 +144,20 @@ def test_only_the_residual_tracks(mm, tape, m, k, n, act, p):
     assert not tape.grad(x).any() and not tape.grad(w).any() and not tape.grad(b).any()
 
 
+def test_the_call_after_one_without_memory_is_unharmed(mm, tape):
+    """[2^20, 2^20] outputs do not fit; the error belongs to the call that met it."""
+    wide, tall = tape.tensor(np.ones((4, 1 << 20))), tape.tensor(np.ones((1 << 20, 4)))
+    a, c = torch.ones(256, 256, device="cuda"), torch.empty(256, 256, device="cuda")
+    for call in (lambda: tape.linear(tall, wide), lambda: tape.linear(tall, wide, activation=mm.ACT_GELU, p=0.5), lambda: tape.matmul(tall, wide)):
+        with pytest.raises(mm.MidmanGpuError, match="out of memory"):
+            call()
+        mm.gemm(a, a, c, m=256, n=256, k=256, lda=256, ldb=256, ldc=256, a_mn_major=False, b_mn_major=False)
+        assert (c == 256).all()
+        with pytest.raises(mm.MidmanGpuError, match="out of memory"):
+            call()
+        assert (tape.read(tape.linear(tape.tensor(np.ones((8, 8))), tape.tensor(np.ones((8, 8))))) == 8).all()
+
+
 def test_refusals(mm, tape):
     x, w = tape.tensor(np.ones((4, 8))), tape.tensor(np.ones((8, 12)))
     odd = tape.tensor(np.ones((8, 6)))
