@@ -135,6 +135,14 @@ def test_dimensions_whose_tiles_pass_32_bits_are_refused(mm, call, change):
     assert rc == SHAPE and "longer than" in message
 
 
+@pytest.mark.parametrize("change", [dict(rows=2 ** 62), dict(rows=2 ** 60, ldx=2 ** 4, ldy=2 ** 4), dict(rows=2 ** 40, ldx=2 ** 40),
+                                    dict(rows=2 ** 40, r=P, ldr=2 ** 40)])
+def test_more_rows_than_addresses_are_refused(mm, change):
+    """Their count of quads passes 64 bits: nothing would run, and the call would say that all is well."""
+    rc, message = dropout(mm, **change)
+    assert rc == SHAPE and "addresses" in message
+
+
 def test_workspaces_of_the_longest_dimensions(mm):
     longest = LONG - 1
     for sizes in ((longest, 4, 4), (4, longest, 4), (4, 4, longest)):
