@@ -113,16 +113,6 @@ __device__ __forceinline__ float lo_part(float x) {
   return __uint_as_float(r);
 }
 
-// Tiles in groups of 8 row blocks, the row block fastest inside a group: the
-// tiles at work at one time then share rows of A and columns of B in L2.
-__device__ __forceinline__ void tile_mn(int t, int tm, int tn, int& mt, int& nt) {
-  const int per_group = 8 * tn;
-  const int g = t / per_group, r = t - g * per_group;
-  const int rows = min(8, tm - g * 8);
-  mt = g * 8 + r % rows;
-  nt = r / rows;
-}
-
 template <int TERMS, bool A_MN, bool B_MN, class Epi>
 __global__ void __launch_bounds__(DirectTile<TERMS>::THREADS, 1)
     direct_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Epi epi,

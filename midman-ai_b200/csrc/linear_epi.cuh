@@ -1,5 +1,6 @@
-// Device code shared by the kernels of linear.cu and linear_pair.cu: activations
-// and their slopes, four-column loads and stores, and the linear epilogue.
+// Device code shared by the kernels of linear.cu and linear_pair.cu: overlapping launches,
+// activations and their slopes, the order of tiles, four-column loads and stores, and the
+// linear epilogue.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -110,6 +111,16 @@ __device__ __forceinline__ void activate_quads(float4 (&v)[U], int act) {
     case kActSilu: each([](float z) { return activate(z, kActSilu); }); break;
     default: break;
   }
+}
+
+// Tiles in groups of 8 row blocks, the row block fastest inside a group: the tiles at
+// work at one time then share rows of A and columns of B in L2.
+__device__ __forceinline__ void tile_mn(int t, int tm, int tn, int& mt, int& nt) {
+  const int per_group = 8 * tn;
+  const int g = t / per_group, r = t - g * per_group;
+  const int rows = min(8, tm - g * 8);
+  mt = g * 8 + r % rows;
+  nt = r / rows;
 }
 
 // Four columns of a row; those at n and past it are not touched.

@@ -333,16 +333,6 @@ constexpr int P_TILE = 16384;   // 128 rows of 128 bytes
 constexpr int P_SMEM = P_RING + 1024 + 256 + 8 * 32 * 32 * 4;
 static_assert(P_SMEM <= 232448, "shared memory of a CTA");
 
-// Tiles in groups of 8 row blocks, the row block fastest inside a group, so that the
-// pairs at work at one time share rows of A and columns of B in L2.
-__device__ __forceinline__ void pair_tile(int t, int tm, int tn, int& mt, int& nt) {
-  const int per_group = 8 * tn;
-  const int g = t / per_group, r = t - g * per_group;
-  const int rows = min(8, tm - g * 8);
-  mt = g * 8 + r % rows;
-  nt = r / rows;
-}
-
 // Work unit u. Tiles [0, full) are whole units; each of the rest (the last, partial
 // wave) is cut into `splits` parts of its chunks, whose sums go to workspace tiles
 // that reduce_kernel adds, in part order, before the epilogue.
@@ -520,7 +510,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
       for (int u = pair; u < units && ok; u += npairs) {
         const PairUnit w = unit_of(u, work, steps);
         int mt, nt;
-        pair_tile(w.tile, tm, tn, mt, nt);
+        tile_mn(w.tile, tm, tn, mt, nt);
         const int my_m0 = mt * 2 * BM + static_cast<int>(rank) * BM;
         const int my_n0 = nt * PN + static_cast<int>(rank) * (PN / 2);
         for (int i = Feed::LOADS * w.cb; i < Feed::LOADS * w.ce; ++i, ++it) {
@@ -575,7 +565,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
     for (int u = pair; u < units && ok; u += npairs) {
       const PairUnit w = unit_of(u, work, steps);
       int mt, nt;
-      pair_tile(w.tile, tm, tn, mt, nt);
+      tile_mn(w.tile, tm, tn, mt, nt);
       const int wrow0 = mt * 2 * BM + static_cast<int>(rank) * BM + quarter * 32, wcol0 = nt * PN + half * 128;
       float sum[128];
 #pragma unroll
@@ -764,7 +754,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const PairWork work, const 
   let_next();
   const int tm = (M + 2 * BM - 1) / (2 * BM), tn = (N + PN - 1) / PN;
   int mt, nt;
-  pair_tile(work.full + static_cast<int>(blockIdx.x), tm, tn, mt, nt);
+  tile_mn(work.full + static_cast<int>(blockIdx.x), tm, tn, mt, nt);
   const int r = blockIdx.y * 4 + threadIdx.x / 64, c = (threadIdx.x % 64) * 4;
   const long long row = mt * 2 * BM + r;
   const int col = nt * PN + c;
