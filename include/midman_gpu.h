@@ -48,7 +48,7 @@ extern "C" {
 /* Activations of mm_gpu_linear_*. */
 #define MM_GPU_ACT_NONE 0
 #define MM_GPU_ACT_RELU 1 /* max(z, 0), slope 0 at 0, NaN for NaN */
-#define MM_GPU_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2 */
+#define MM_GPU_ACT_GELU 2 /* z (1 + erf(z / sqrt 2)) / 2, the factor of z within 4e-7 */
 #define MM_GPU_ACT_SILU 3 /* z / (1 + exp(-z)) */
 
 /* Message of the last failing call on this thread (NUL-terminated, static until
@@ -184,7 +184,8 @@ MM_GPU_EXPORT int32_t mm_gpu_cross_entropy(int32_t rows, int32_t vocab, float *l
  * it NaN or infinite, no others; activations keep a NaN, dropout drops it as it drops
  * any element.
  *
- * Precision: MM_GPU_TF32 is one TF32 pass (up to eight rows: f32 multiply-adds).
+ * Precision: MM_GPU_TF32 is one TF32 pass (up to eight rows: f32 multiply-adds), summed
+ * in f32 at least every 2048 entries along the sum.
  * MM_GPU_3XTF32 is the exact mode, f32 accuracy: three products of 11-bit halves,
  * TF32 ones, or for large products f16 ones of operands scaled by a power of two for
  * every 128 entries along the sum (an entry more than 2^-17 below the largest of its

@@ -19,8 +19,10 @@
 // beside it in shared memory (elementwise, so the swizzled layout is kept). What bounds
 // a K step of 32 of a 128 x 128 tile is shared memory: 32 KB in by TMA, 48 KB through
 // the converters, 48 KB read by the UMMAs, 1,024 cycles at 128 bytes each; 1,140
-// measured (with A's parts in shared memory too 1,536 and 1,600; with four warps on B's
-// lo part instead of two nothing changed). The parts' sums meet in shared memory over
+// measured, 0.58 us at 1.965 GHz (with A's parts in shared memory too 1,536 and 1,600;
+// with four warps on B's lo part instead of two nothing changed). Where all SMs bring
+// tiles that no other takes, the L2 bounds it: 148 tiles of 128 rows 0.74 us a step, 6.5
+// TB/s; one TF32 term 0.28 to 0.32. The parts' sums meet in shared memory over
 // the cluster (each CTA sums 128 / splits rows of all parts, in part order:
 // bit-identical run to run) and go through the epilogue in whole rows.
 #include <cuda.h>
@@ -554,8 +556,10 @@ struct LossDirect {
 // takes 32 columns and a part of K, a cluster's parts meet in shared memory, in part
 // order. B [k, n]: eight lanes hold the 32 columns of a k, a warp four k at a time,
 // eight loads in flight; B [n, k]: a warp takes four columns, its lanes lie along k.
-// A's values of 512 k at a time are kept in shared memory. One row of 2048 x 5632 10.6 us
-// (4.4 TB/s of B), 4096 x 11264 35 us (5.2).
+// A's values of 512 k at a time are kept in shared memory. One row of 2048 x 5632 11.2 us
+// with twelve such weights in rotation (4.1 TB/s of B from HBM), 7.7 us with one, which
+// stays in the L2; 4096 x 11264, larger than the L2, 36 us (5.1). What the small one lacks
+// is loads in flight: a CTA's run dry at the end of each piece of 512.
 constexpr int kFewRows = 8;
 constexpr int kFewPiece = 512;
 constexpr int kFewCols = 32;
@@ -872,7 +876,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 // time from waves of clusters, steps of a part and a tile's fixed cost. A cluster lies
 // in one GPC, so fewer CTAs run at once in larger ones (the occupancy query's counts for
 // this kernel on a B200; a device with other GPCs runs the same plan in other waves). A
-// step takes 0.66 us, a tile's start and end 5.5, the parts' join 0.5, the slices' launch
+// step takes 0.66 us (a fit over whole calls, between the loop's own 0.58 and the 0.74 of
+// tiles that share nothing), a tile's start and end 5.5, the parts' join 0.5, the slices' launch
 // and their sums 3, some of it the host's (2048 x 4096 -> 128 in six parts takes 24.7 us, in
 // nine slices 21.4, in four parts of two slices 22.0; 128 x 2048 -> 2048 16.8, 16.0 and 16.1;
 // 4096 x 2048 -> 128 in four parts 20.0, in four slices 21.6; 64 x 32000 -> 512 in eight

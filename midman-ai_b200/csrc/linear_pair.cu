@@ -21,10 +21,14 @@
 // launch 77 us, 6.0 TB/s; dz of 8192 x 5632 by rows and transposed with the column sums
 // 148 us, 5.0 TB/s).
 //
-// Measured, copies aside: 8192 x 2048 x 5632 366 us (516 TFLOP/s of the product, 1,550 of
-// f16 executed; the 3xTF32 products of gemm.cu take 730 us), 8192 x 1024 -> 2816 with
-// GELU and z kept 124 us (381), tensor pipe 85% of active cycles at 1.5 GHz under the
-// power cap. The one-pass TF32 form (Tf32Feed) 8192 x 2048 x 5632 273 us.
+// Measured, copies aside: 8192 x 2048 x 5632 366 us by itself at 1.5 GHz (516 TFLOP/s of
+// the product, 1,550 of f16 executed; the 3xTF32 products of gemm.cu take 730 us), 429 us
+// in a loop of backward calls, where the power cap leaves 1.40 GHz (1,322 executed, 93% of
+// what the library's bf16 product sustains under the cap); 8192 x 1024 -> 2816 with GELU
+// and z kept 124 us by itself, 129 in a loop. The tensor pipe is busy 88 to 96% of the
+// cycles of a long product, 69% of the loss's logits of 1024 of K, whose epilogue is the
+// longest. The one-pass TF32 form (Tf32Feed) 8192 x 2048 x 5632 273 us by itself, 282 to
+// 290 in a loop.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -315,8 +319,8 @@ void launch_split(const Source& src, int rows, int cols, const SplitCopy* by_row
 // 256 x 256 tiles on CTA pairs (cta_group::2): CTA r of a pair holds rows 128 r..
 // of the tile's A and of its B; a stage is 64 of K: Ah, Al, Bh, Bl, 16 KB each, a
 // chunk two stages. Per stage a CTA takes in 64 KB and its tensor core reads 3 x
-// 48 KB in 1,536 cycles: 135 bytes a cycle of shared memory, so the tensor pipe
-// stays above 90% busy. Warp 0 TMA, warp 1 UMMA (the leader's), warps 4..11 the
+// 48 KB in 1,536 cycles: 135 bytes a cycle of shared memory, which feeds the tensor
+// pipe through a long sum (96% busy at 32,000 of K). Warp 0 TMA, warp 1 UMMA (the leader's), warps 4..11 the
 // running sums (TMEM lanes 32 (w % 4).., columns 128 ((w - 4) / 4)..) and the
 // epilogue; the chunks' two TMEM accumulators let the next tile's first two chunks
 // run beside it.
@@ -325,7 +329,8 @@ constexpr int P_THREADS = 384;
 constexpr int P_SUM_WARP = 4;  // the first of the eight warps that sum and write
 // Registers: a launch of 384 threads has 168 a thread; warps 0..3 (TMA, UMMA, two
 // idle) give up all but 40, and the summing warps take 232 (40 + 2 x 232 = 3 x 168),
-// which holds 128 sums, the residuals and the epilogue without spills.
+// which holds 128 sums, the residuals and the epilogue (of the 28 instances seven spill 16
+// bytes a thread).
 constexpr int P_REGS = 168, P_REGS_FEW = 40, P_REGS_SUM = 232;
 static_assert(P_REGS_FEW + 2 * P_REGS_SUM <= 3 * P_REGS, "setmaxnreg draws on the launch's registers");
 constexpr int P_RING = 196608;  // the stages' bytes
@@ -419,7 +424,8 @@ struct Tf32Feed {
 // most 2^37 (128 products of entries up to 2^15), so times a row's inverse it stays below
 // 2^128 up to kSafeInverse, entries of 2^104. WIDE, where a row of the warp has larger
 // ones: the smaller inverse first, so that nothing overflows which the other would bring
-// back (two more instructions a value). What the first factor loses to f32's smallest
+// back (two more instructions a value; the test for it costs up to 0.8% of a call, 333 x
+// 50001 x 516 with gradients 400 -> 402 us). What the first factor loses to f32's smallest
 // numbers is at most 2^-24 of a scaled unit, far below the copies' own 2^-25 of one in
 // every entry times the other operand's 2^14.
 constexpr float kSafeInverse = 0x1p90f;
