@@ -420,7 +420,8 @@ struct Tf32Feed {
 };
 
 // sum += an accumulation's 32 rows x 128 columns with both scales undone: `ia` is this
-// lane's row's inverse, `ib` the columns' (the same for every lane). A chunk's sum is at
+// lane's row's inverse (of the loss's gradient it has grad_scale's sign), `ib` the columns'
+// (the same for every lane). A chunk's sum is at
 // most 2^37 (128 products of entries up to 2^15), so times a row's inverse it stays below
 // 2^128 up to kSafeInverse, entries of 2^104. WIDE, where a row of the warp has larger
 // ones: the smaller inverse first, so that nothing overflows which the other would bring
@@ -438,7 +439,8 @@ __device__ __forceinline__ void add_chunk(float (&sum)[128], uint32_t acc, float
     auto add = [&](int e, float b) {
       const float v = __uint_as_float(r[e]);
       float& o = sum[q * 32 + e];
-      o = WIDE ? fmaf(v * fminf(ia, b), fmaxf(ia, b), o) : fmaf(v * ia, b, o);
+      const bool first = !WIDE || fabsf(ia) < b;
+      o = fmaf(v * (first ? ia : b), first ? b : ia, o);
     };
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -626,7 +628,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
           pb += ld_ib / 4;
           const float ia_next = more ? *pa : 0.0f;
           const float4 ib_next = more ? *pb : make_float4(0.f, 0.f, 0.f, 0.f);
-          const bool wide = __any_sync(0xffffffffu, ia > kSafeInverse);
+          const bool wide = __any_sync(0xffffffffu, fabsf(ia) > kSafeInverse);
           ok = wait_acc(&acc);
           if (!ok) break;
           if (wide)

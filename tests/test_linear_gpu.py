@@ -642,6 +642,31 @@ def test_the_gradient_of_the_widest_rows(mm, room):
     check(row_loss, torch.tensor([4.0], device="cuda", dtype=F).log(), 4 * ULP, "row_loss")
 
 
+@pytest.mark.parametrize("precision", [1, 0])
+@pytest.mark.parametrize("rows,vocab,dim,tied", [(300, 1000, 64, True), (2304, 4096, 128, False), (2304, 2305, 512, True), (2304, 2305, 512, False)])
+def test_gradients_scale_with_grad_scale(mm, rows, vocab, dim, tied, precision):
+    """A power of two changes nothing but the exponents, of either sign and near the largest: losses and dw bit for bit. dx too,
+    but on pairs, where a chunk of 128 classes takes softmax's factor (no power of two) and w's scale in the order that does not
+    overflow: factor first, it is rounded (2^-24 of the chunk's sum) before it is added, scale first, it is not; so the chunks'
+    sums and the running sums differ by 2^-24 of what they hold, twice a chunk."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x, w, t = loss_case(g, rows, vocab, dim, tied, 0)
+    t[::7] = -1
+    outs = []
+    for scale in (1.0, -(2.0 ** 120), 2.0 ** 120, -(2.0 ** -40)):
+        row_loss, dx, dw = torch.empty(rows, device="cuda"), torch.zeros_like(x), torch.zeros_like(w)
+        mm.linear_cross_entropy(x, w, t, row_loss, rows=rows, vocab=vocab, dim=dim, ldx=x.stride(0), ldw=w.stride(0), w_mn_major=not tied,
+                                grad_scale=scale, dx=dx, lddx=dx.stride(0), dw=dw, lddw=dw.stride(0), precision=precision)
+        mm.device_status()
+        outs.append([row_loss] + [o[:, :n].to(F) / scale for o, n in ((dx, dim), (dw, dim if tied else vocab))])
+    W = (w[:, :dim] if tied else w[:, :vocab].T).to(F)
+    gr = loss64(x[:, :dim], W, t, 1.0, t >= 0)[4]
+    tol = 2 * (-(-vocab // 128) + 1) * ULP * (gr.abs() @ W.abs()) if dim == 512 and precision == 1 else torch.zeros_like(x[:, :dim])
+    for other in outs[1:]:
+        assert torch.equal(outs[0][0], other[0]) and torch.equal(outs[0][2], other[2])
+        check(other[1], outs[0][1], tol, "dx")
+
+
 def test_no_row_has_a_target(mm):
     x, w, t = torch.randn(9, 8, device="cuda"), torch.randn(50, 8, device="cuda"), torch.full((9,), -1, dtype=torch.int32, device="cuda")
     row_loss, mean, dx, dw = torch.empty(9, device="cuda"), torch.empty(1, device="cuda"), torch.empty_like(x), torch.empty_like(w)
