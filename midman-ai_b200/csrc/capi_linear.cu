@@ -117,7 +117,7 @@ int32_t mm_gpu_dropout(int64_t rows, int32_t cols, const float* x, int64_t ldx, 
     if (rows > 0 && (!x || !y)) return fail(MM_GPU_ERR_ARGUMENT, "dropout: null pointer");
     if (ldx < cols || ldy < cols || (r && ldr < cols))
       return fail(MM_GPU_ERR_SHAPE, "dropout: a row stride is smaller than the row");
-    if (rows > INT64_MAX / 4 / std::max({ldx, ldy, r ? ldr : 0}))  // the last row's address, and the count of quads
+    if (rows - 1 > INT64_MAX / 4 / std::max({ldx, ldy, r ? ldr : 0}))  // the last row's address, and the count of quads
       return fail(MM_GPU_ERR_SHAPE, "dropout: more rows than there are addresses");
     if (rows > 0 && ((y == x && ldy != ldx) || (y == r && ldy != ldr)))
       return fail(MM_GPU_ERR_SHAPE, "dropout: y may be x or r only with its row stride");
